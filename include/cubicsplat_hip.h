@@ -695,6 +695,48 @@ int cs_adan_step(int32_t ntensors, float* const* params, const float* const* gra
                  float* const* neg_pre_grads, const int64_t* numels, const float* scalars,
                  const int32_t* flags, const float* clip, hipStream_t stream);
 
+/* AdamW (decoupled weight decay) over any number of tensors, each with fp32 or
+ * 8-bit states; new (the reference has no AdamW).  table is a host array of
+ * ntensors rows of eight int64:
+ *   [0] parameter     fp32, bf16 or fp16, updated in place
+ *   [1] gradient      of the parameter's type
+ *   [2] master        fp32 copy of a bf16 or fp16 parameter (0 for fp32); the
+ *                     update moves it and the parameter is it, rounded
+ *   [3] exp_avg       fp32, or the 8-bit codes of the first moment
+ *   [4] exp_avg_sq    fp32, or the 8-bit codes of the second moment's root
+ *   [5] element count (0: the row is skipped)
+ *   [6] type (0 fp32, 1 bf16, 2 fp16) | 16 for 8-bit states | set << 8
+ *   [7] the tensor's number, which the rounding's random numbers depend on
+ * All of a tensor's arrays lie in the same element order.  8-bit codes of n
+ * values: B = ceil(n / CS_ADAMW_BLOCK) blocks; B * CS_ADAMW_BLOCK code bytes,
+ * then B bytes with each block's exponent; 8-byte aligned.
+ * sets: nsets rows of eight floats: 1 - lr * weight_decay,
+ * lr / (1 - beta1^t), sqrt(1 - beta2^t), 1 - beta1, beta2, 1 - beta2, eps, 0;
+ * keys: nsets random words, a new one each step.  clip: device fp32 factor of
+ * the gradients, or NULL.  One launch for up to 56 tensors and 12 sets. */
+#define CS_ADAMW_BLOCK 128
+int cs_adamw_step(int32_t ntensors, const int64_t* table, int32_t nsets, const float* sets,
+                  const uint32_t* keys, const float* clip, hipStream_t stream);
+
+/* fp32 states to 8-bit ones, rounded to nearest: rows as above with [0] and
+ * [1] the codes written, [3] and [4] the fp32 moments read, [5] and type 0. */
+int cs_adamw_pack_state(int32_t ntensors, const int64_t* table, hipStream_t stream);
+
+/* The moments' values in out_dtype (0 fp32, 1 bf16, 2 fp16): rows as above
+ * with [0] and [1] the arrays written (first and second moment), [2] how many
+ * elements of them (at least [5]; those past [5] become 0), [3] and [4] the
+ * states read, [5], and [6] 16 for 8-bit states. */
+int cs_adamw_unpack_state(int32_t ntensors, const int64_t* table, int32_t out_dtype,
+                          hipStream_t stream);
+
+/* The 2-norm over all gradients of the table ([1], [5] and the type of [6];
+ * the rest is not read): out[0] = norm, out[1] = min(1, max_norm / (norm +
+ * 1e-6)), or 1 where max_norm is 0.  partials: device scratch of
+ * CS_GRAD_NORM_BLOCKS + ntensors doubles.  The sum's order is fixed. */
+#define CS_GRAD_NORM_BLOCKS 2048
+int cs_grad_norm(int32_t ntensors, const int64_t* table, double max_norm, double* partials,
+                 float* out, hipStream_t stream);
+
 /* ---------------- 2D Gaussian splats (GsRenderFunction) ---------------- */
 
 /* project_gaussians_2d_scale_rot_forward_kernel (ops/forward2d.py:14-164):

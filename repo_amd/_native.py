@@ -25,6 +25,8 @@ SEG_RECORD_INTS = 8      # 32-byte segment record
 PRIM_RECORD_FLOATS = 20  # 80-byte primitive record
 RASTER_LOG_BLOCK_BYTES = 2048  # log pool reserved per wave at a time
 EDGE_AUX_INTS = 4        # 16-byte (segment, t0, t1) record of the adaptive flattening
+ADAMW_BLOCK = 128        # values that share an exponent in the 8-bit optimizer states
+GRAD_NORM_BLOCKS = 2048  # partial sums of the gradients' norm (and one a tensor)
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -131,6 +133,10 @@ _SIGNATURES = {
                                                   _F, _P, _P, _I32, _P]),
     "cs_adam_step": (ctypes.c_int, [_I32, _P, _P, _P, _P, _P, _P, _P, _P, _D, _D, _D, _P]),
     "cs_adan_step": (ctypes.c_int, [_I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "cs_adamw_step": (ctypes.c_int, [_I32, _P, _I32, _P, _P, _P, _P]),
+    "cs_adamw_pack_state": (ctypes.c_int, [_I32, _P, _P]),
+    "cs_adamw_unpack_state": (ctypes.c_int, [_I32, _P, _I32, _P]),
+    "cs_grad_norm": (ctypes.c_int, [_I32, _P, _D, _P, _P, _P]),
     "cs_gs_project_forward": (ctypes.c_int, [_P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P,
                                              _P, _P, _P]),
     "cs_gs_bin_prepare": (ctypes.c_int, [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P,

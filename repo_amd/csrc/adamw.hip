@@ -1,0 +1,592 @@
+// AdamW over all tensors of a network, with fp32 or 8-bit states, and the
+// global norm of their gradients.
+//
+// Per element (decoupled weight decay; t the step of the tensor):
+//   g  = grad * clip
+//   p  = p * (1 - lr * weight_decay)
+//   m  = m + (1 - beta1) * (g - m)
+//   v  = v * beta2 + (1 - beta2) * g * g
+//   p -= lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+// in fp32.  A bf16 or fp16 parameter has an fp32 master copy, which is what
+// the update moves; the parameter is the master rounded to nearest.
+//
+// 8-bit states.  A byte holds m as sign, 4 exponent bits and 3 mantissa bits,
+// and a byte holds sqrt(v), not v, as 4 exponent and 4 mantissa bits: the root
+// is what the update divides by, has half of v's exponent range and no sign.
+// 128 consecutive values share one byte, the biased fp32 exponent E of the
+// largest finite |value|: a code's exponent field e and mantissa f stand for
+//   e > 0:  (1 + f / 2^M) 2^(e - 14) 2^(E - 127),   e = 0: f / 2^M 2^(-13) 2^(E - 127)
+// so the largest value lies in the binade e = 14, and rounding up ends at
+// e = 15, f = 0 at most.  The code with all exponent and mantissa bits set is
+// NaN (and what infinity becomes).  The scale is a power of two, so that
+// scaling is exact and the code is the scaled float's own top bits: the float
+// x 2^(14 - E) has e in its exponent field, subnormals included.
+//
+// Rounding is stochastic: with beta2 near 1 a step changes v by a fraction of
+// a code's spacing, and rounding to nearest would lose every such change (v
+// would stop where 1 - beta2 times g^2 falls under half a spacing).  A 16-bit
+// random number is added below the code's last bit before the lower bits are
+// cut, so the expected value is the value.  The numbers are a hash of (seed,
+// step, tensor, element), hence the same in every run and launch shape.  A
+// root that is not zero never becomes zero: the update divides by it.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/cubicsplat_hip.h"
+
+namespace cs {
+
+constexpr int kAwThreads = 256;
+constexpr int kAwMaxTensors = 56;  // one lane each, and 4 KB of kernel arguments
+constexpr int kAwMaxSets = 12;
+constexpr int kAwPass = kAwThreads * 8;  // elements of a chunk's unit: whole blocks of 128
+constexpr int kBlk = CS_ADAMW_BLOCK;
+
+enum { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+struct AwTensor {
+    void* param;
+    const void* grad;
+    float* master;
+    void* avg;
+    void* sq;
+    int64_t n;
+    uint32_t first_block;
+    uint32_t meta;  // dtype | eight << 4 | vector << 5 | set << 8
+    uint32_t key;
+    uint32_t pad;
+};
+
+struct AwSet {
+    float decay, step_size, bc2_sqrt, omb1, beta2, omb2, eps, pad;
+};
+
+struct AwArgs {
+    AwTensor t[kAwMaxTensors];
+    AwSet s[kAwMaxSets];
+    const float* clip;
+    int64_t chunk;
+    int32_t n;
+    int32_t out_dtype;
+};
+
+__host__ __device__ inline uint32_t aw_mix(uint32_t x) {
+    x ^= x >> 16;
+    x *= 0x9E3779B9u;
+    x ^= x >> 15;
+    x *= 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+
+__device__ inline uint32_t aw_random(uint32_t key, int64_t i) {
+    return aw_mix(key + (uint32_t)i + (uint32_t)(i >> 32) * 0x3C6EF372u);
+}
+
+// The tensor this workgroup works on: lane k holds tensor k's first block.
+__device__ inline int aw_find(const AwArgs& a) {
+    const int lane = threadIdx.x & 63;
+    const bool mine = lane < a.n && a.t[lane < a.n ? lane : 0].first_block <= blockIdx.x;
+    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1);
+}
+
+template <int DT> struct AwType;
+template <> struct AwType<kF32> { typedef float type; };
+template <> struct AwType<kBF16> { typedef __bf16 type; };
+template <> struct AwType<kF16> { typedef _Float16 type; };
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) AwVec { T v[N]; };
+
+// N consecutive elements at element i; elements past n are 0 and not stored.
+template <int N, typename T>
+__device__ inline void aw_load(const T* src, int64_t i, int64_t n, bool vec, float (&out)[N]) {
+    if (vec && i + N <= n) {
+        const AwVec<T, N> x = *reinterpret_cast<const AwVec<T, N>*>(src + i);
+#pragma unroll
+        for (int k = 0; k < N; ++k) out[k] = (float)x.v[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) out[k] = i + k < n ? (float)src[i + k] : 0.0f;
+    }
+}
+
+template <int N, typename T>
+__device__ inline void aw_store(T* dst, int64_t i, int64_t n, bool vec, const float (&in)[N]) {
+    if (vec && i + N <= n) {
+        AwVec<T, N> x;
+#pragma unroll
+        for (int k = 0; k < N; ++k) x.v[k] = (T)in[k];
+        *reinterpret_cast<AwVec<T, N>*>(dst + i) = x;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (i + k < n) dst[i + k] = (T)in[k];
+    }
+}
+
+__device__ inline void aw_update(const AwSet& s, float g, float& p, float& m, float& v,
+                                 float& root) {
+    p = p * s.decay;
+    m = m + s.omb1 * (g - m);
+    v = v * s.beta2 + s.omb2 * (g * g);
+    root = __builtin_sqrtf(v);
+    p = p - s.step_size * (m / (root / s.bc2_sqrt + s.eps));
+}
+
+// ---- 8-bit codes
+
+template <int MB>
+__device__ inline float aw_decode(uint32_t code, int e) {
+    const uint32_t mag = code & ((1u << (4 + MB)) - 1u);
+    const float x = __builtin_ldexpf(__uint_as_float(mag << (23 - MB)), e - 14);
+    const float y = mag == (1u << (4 + MB)) - 1u ? __builtin_nanf("") : x;
+    return MB == 3 && (code & 0x80u) ? -y : y;
+}
+
+template <int MB, bool FLOOR>
+__device__ inline uint32_t aw_encode(float x, int e, uint32_t r16) {
+    const uint32_t t = __float_as_uint(__builtin_ldexpf(x, 14 - e)) & 0x7FFFFFFFu;
+    uint32_t c = (t + (r16 << (7 - MB))) >> (23 - MB);
+    if (FLOOR) c = x > 0.0f && c == 0 ? 1u : c;
+    c = t >= 0x7F800000u ? (1u << (4 + MB)) - 1u : c;
+    if (MB == 3) c |= (__float_as_uint(x) >> 24) & 0x80u;
+    return c;
+}
+
+// The largest of the 16 lanes of a row.
+__device__ inline float aw_row_max(float x) {
+#define CS_ROW_MAX(ctrl)                                                                   \
+    x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(                               \
+                     0, __float_as_int(x), ctrl, 0xF, 0xF, true)))
+    CS_ROW_MAX(0x128);  // row_ror:8
+    CS_ROW_MAX(0x124);
+    CS_ROW_MAX(0x122);
+    CS_ROW_MAX(0x121);
+#undef CS_ROW_MAX
+    return x;
+}
+
+__device__ inline int aw_shared_exponent(const float (&x)[8]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float a = __builtin_fabsf(x[k]);
+        top = a < __builtin_inff() ? fmaxf(top, a) : top;
+    }
+    return (int)(__float_as_uint(aw_row_max(top)) >> 23);
+}
+
+// The 8 bytes of a lane; the code arrays are whole blocks, so all 8 exist
+// wherever the lane's first element does.
+__device__ inline void aw_load_codes(const uint8_t* src, int64_t i, bool in, uint32_t (&c)[8]) {
+    uint2 w = make_uint2(0u, 0u);
+    if (in) w = *reinterpret_cast<const uint2*>(src + i);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) c[k] = ((k < 4 ? w.x : w.y) >> (8 * (k & 3))) & 0xFFu;
+}
+
+__device__ inline void aw_store_codes(uint8_t* dst, int64_t i, bool in, const uint32_t (&c)[8]) {
+    uint2 w;
+    w.x = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+    w.y = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
+    if (in) *reinterpret_cast<uint2*>(dst + i) = w;
+}
+
+__device__ inline int64_t aw_blocks(int64_t n) { return (n + kBlk - 1) / kBlk; }
+
+// Encodes and stores a lane's 8 values of m and root; every lane of the wave
+// takes part.
+__device__ inline void aw_hold(uint8_t* avg, uint8_t* sq, int64_t i, int64_t n,
+                               const float (&m)[8], const float (&root)[8],
+                               const uint32_t (&r)[8]) {
+    const bool in = i < n;
+    const int em = aw_shared_exponent(m), er = aw_shared_exponent(root);
+    uint32_t cm[8], cr[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        cm[k] = aw_encode<3, false>(m[k], em, r[k] & 0xFFFFu);
+        cr[k] = aw_encode<4, true>(root[k], er, r[k] >> 16);
+    }
+    aw_store_codes(avg, i, in, cm);
+    aw_store_codes(sq, i, in, cr);
+    if (in && (threadIdx.x & 15) == 0) {
+        const int64_t b = aw_blocks(n) * kBlk + i / kBlk;
+        avg[b] = (uint8_t)em;
+        sq[b] = (uint8_t)er;
+    }
+}
+
+__device__ inline void aw_held(const uint8_t* avg, const uint8_t* sq, int64_t i, int64_t n,
+                               float (&m)[8], float (&root)[8]) {
+    const bool in = i < n;
+    const int64_t b = aw_blocks(n) * kBlk + i / kBlk;
+    const int em = in ? avg[b] : 0, er = in ? sq[b] : 0;
+    uint32_t cm[8], cr[8];
+    aw_load_codes(avg, i, in, cm);
+    aw_load_codes(sq, i, in, cr);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        m[k] = aw_decode<3>(cm[k], em);
+        root[k] = aw_decode<4>(cr[k], er);
+    }
+}
+
+// ---- the step
+
+template <int DT>
+__device__ inline void aw_step32(const AwTensor& t, const AwSet& s, float clip, int64_t begin,
+                                 int64_t end) {
+    typedef typename AwType<DT>::type T;
+    const bool vec = (t.meta >> 5) & 1;
+    float* main = DT == kF32 ? (float*)t.param : t.master;
+    for (int64_t i = begin + threadIdx.x * 4; i < end; i += kAwThreads * 4) {
+        float p[4], g[4], m[4], v[4], root;
+        aw_load<4>(main, i, end, vec, p);
+        aw_load<4>((const T*)t.grad, i, end, vec, g);
+        aw_load<4>((const float*)t.avg, i, end, vec, m);
+        aw_load<4>((const float*)t.sq, i, end, vec, v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) aw_update(s, g[k] * clip, p[k], m[k], v[k], root);
+        aw_store<4>(main, i, end, vec, p);
+        if (DT != kF32) aw_store<4>((T*)t.param, i, end, vec, p);
+        aw_store<4>((float*)t.avg, i, end, vec, m);
+        aw_store<4>((float*)t.sq, i, end, vec, v);
+    }
+}
+
+template <int DT>
+__device__ inline void aw_step8(const AwTensor& t, const AwSet& s, float clip, int64_t begin,
+                                int64_t end) {
+    typedef typename AwType<DT>::type T;
+    const bool vec = (t.meta >> 5) & 1;
+    float* main = DT == kF32 ? (float*)t.param : t.master;
+    for (int64_t base = begin; base < end; base += kAwPass) {
+        const int64_t i = base + threadIdx.x * 8;
+        float p[8], g[8], m[8], root[8];
+        uint32_t r[8];
+        aw_load<8>(main, i, t.n, vec, p);
+        aw_load<8>((const T*)t.grad, i, t.n, vec, g);
+        aw_held((const uint8_t*)t.avg, (const uint8_t*)t.sq, i, t.n, m, root);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float v = root[k] * root[k];
+            aw_update(s, g[k] * clip, p[k], m[k], v, root[k]);
+            r[k] = aw_random(t.key, i + k);
+            // Elements past the end do not set a block's exponent.
+            if (i + k >= t.n) m[k] = root[k] = 0.0f;
+        }
+        aw_store<8>(main, i, t.n, vec, p);
+        if (DT != kF32) aw_store<8>((T*)t.param, i, t.n, vec, p);
+        aw_hold((uint8_t*)t.avg, (uint8_t*)t.sq, i, t.n, m, root, r);
+    }
+}
+
+__global__ __launch_bounds__(kAwThreads) void k_adamw(AwArgs a) {
+    const int k = aw_find(a);
+    const AwTensor& t = a.t[k];
+    const AwSet& s = a.s[t.meta >> 8];
+    const float clip = a.clip ? *a.clip : 1.0f;
+    const int64_t begin = (int64_t)(blockIdx.x - t.first_block) * a.chunk;
+    const int64_t end = begin + a.chunk < t.n ? begin + a.chunk : t.n;
+    switch (t.meta & 0x1F) {
+        case kF32: aw_step32<kF32>(t, s, clip, begin, end); break;
+        case kBF16: aw_step32<kBF16>(t, s, clip, begin, end); break;
+        case kF16: aw_step32<kF16>(t, s, clip, begin, end); break;
+        case kF32 | 16: aw_step8<kF32>(t, s, clip, begin, end); break;
+        case kBF16 | 16: aw_step8<kBF16>(t, s, clip, begin, end); break;
+        case kF16 | 16: aw_step8<kF16>(t, s, clip, begin, end); break;
+    }
+}
+
+// ---- state conversions
+
+// fp32 m (avg) and v (sq) -> codes at param (m) and grad (root), to nearest.
+__global__ __launch_bounds__(kAwThreads) void k_adamw_pack(AwArgs a) {
+    const AwTensor& t = a.t[aw_find(a)];
+    const bool vec = (t.meta >> 5) & 1;
+    const int64_t begin = (int64_t)(blockIdx.x - t.first_block) * a.chunk;
+    const int64_t end = begin + a.chunk < t.n ? begin + a.chunk : t.n;
+    for (int64_t base = begin; base < end; base += kAwPass) {
+        const int64_t i = base + threadIdx.x * 8;
+        float m[8], root[8];
+        uint32_t r[8];
+        aw_load<8>((const float*)t.avg, i, t.n, vec, m);
+        aw_load<8>((const float*)t.sq, i, t.n, vec, root);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            root[k] = __builtin_sqrtf(root[k]);
+            r[k] = 0x80008000u;  // one half of a spacing: to nearest
+        }
+        aw_hold((uint8_t*)t.param, (uint8_t*)t.grad, i, t.n, m, root, r);
+    }
+}
+
+template <typename T>
+__device__ inline void aw_unpack(const AwTensor& t, int64_t begin, int64_t end) {
+    const bool vec = (t.meta >> 5) & 1, eight = (t.meta >> 4) & 1;
+    const int64_t n = (int64_t)(intptr_t)t.master;  // with what follows the values
+    for (int64_t i = begin + threadIdx.x * 8; i < end; i += kAwPass) {
+        float m[8], v[8];
+        if (eight) {
+            aw_held((const uint8_t*)t.avg, (const uint8_t*)t.sq, i, t.n, m, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const bool in = i + k < t.n;
+                m[k] = in ? m[k] : 0.0f;
+                v[k] = in ? v[k] * v[k] : 0.0f;
+            }
+        } else {
+            aw_load<8>((const float*)t.avg, i, t.n, vec, m);
+            aw_load<8>((const float*)t.sq, i, t.n, vec, v);
+        }
+        aw_store<8>((T*)t.param, i, n, vec, m);
+        aw_store<8>((T*)const_cast<void*>(t.grad), i, n, vec, v);
+    }
+}
+
+__global__ __launch_bounds__(kAwThreads) void k_adamw_unpack(AwArgs a) {
+    const AwTensor& t = a.t[aw_find(a)];
+    const int64_t n = (int64_t)(intptr_t)t.master;
+    const int64_t begin = (int64_t)(blockIdx.x - t.first_block) * a.chunk;
+    const int64_t end = begin + a.chunk < n ? begin + a.chunk : n;
+    switch (a.out_dtype) {
+        case kF32: aw_unpack<float>(t, begin, end); break;
+        case kBF16: aw_unpack<__bf16>(t, begin, end); break;
+        case kF16: aw_unpack<_Float16>(t, begin, end); break;
+    }
+}
+
+// ---- the gradients' norm
+
+struct NormTensor {
+    const void* grad;
+    int64_t n;
+    uint32_t first_block;
+    uint32_t meta;  // dtype | vector << 5
+};
+
+constexpr int kNormMaxTensors = 64;
+constexpr int kNormBlocks = CS_GRAD_NORM_BLOCKS;
+
+struct NormArgs {
+    NormTensor t[kNormMaxTensors];
+    double* partials;  // of this launch's blocks
+    int64_t chunk;
+    int32_t n;
+};
+
+template <int DT>
+__device__ inline float norm_squares(const NormTensor& t, int64_t begin, int64_t end) {
+    typedef typename AwType<DT>::type T;
+    const bool vec = (t.meta >> 5) & 1;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t i = begin + threadIdx.x * 8; i < end; i += kAwPass) {
+        float g[8];
+        aw_load<8>((const T*)t.grad, i, end, vec, g);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k & 3] = __builtin_fmaf(g[k], g[k], s[k & 3]);
+    }
+    return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+__device__ inline double block_sum(double x, double* lds) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+__global__ __launch_bounds__(kAwThreads) void k_grad_squares(NormArgs a) {
+    __shared__ double lds[4];
+    const int lane = threadIdx.x & 63;
+    const bool mine = lane < a.n && a.t[lane < a.n ? lane : 0].first_block <= blockIdx.x;
+    const NormTensor& t =
+        a.t[__builtin_amdgcn_readfirstlane(__popcll(__ballot(mine)) - 1)];
+    const int64_t begin = (int64_t)(blockIdx.x - t.first_block) * a.chunk;
+    const int64_t end = begin + a.chunk < t.n ? begin + a.chunk : t.n;
+    float s = 0.0f;
+    switch (t.meta & 0xF) {
+        case kF32: s = norm_squares<kF32>(t, begin, end); break;
+        case kBF16: s = norm_squares<kBF16>(t, begin, end); break;
+        case kF16: s = norm_squares<kF16>(t, begin, end); break;
+    }
+    const double sum = block_sum((double)s, lds);
+    if (threadIdx.x == 0) a.partials[blockIdx.x] = sum;
+}
+
+__global__ __launch_bounds__(kAwThreads) void k_grad_norm(const double* partials, int32_t n,
+                                                          float max_norm, float* out) {
+    __shared__ double lds[4];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < n; i += kAwThreads) s += partials[i];
+    s = block_sum(s, lds);
+    if (threadIdx.x == 0) {
+        const float norm = (float)__builtin_sqrt(s);
+        const float c = max_norm / (norm + 1e-6f);
+        out[0] = norm;
+        out[1] = max_norm > 0.0f && !(c > 1.0f) ? c : 1.0f;  // a NaN norm stays one
+    }
+}
+
+static bool aw_aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+// Elements of a chunk: whole passes, and about `blocks` of them over the total.
+static int64_t aw_chunk(int64_t total, int64_t blocks) {
+    const int64_t per = (total + blocks - 1) / blocks;
+    return (per + kAwPass - 1) / kAwPass * kAwPass;
+}
+
+}  // namespace cs
+
+using namespace cs;
+
+namespace {
+
+enum AwOp { kStep, kPack, kUnpack };
+
+// table: [n][8] = param, grad, master, exp_avg, exp_avg_sq, numel, dtype | eight << 4 |
+// set << 8, ordinal.
+int aw_run(AwOp op, int32_t ntensors, const int64_t* table, int32_t nsets, const float* sets,
+           const uint32_t* set_keys, const float* clip, int32_t out_dtype,
+           hipStream_t stream) {
+    if (ntensors < 0 || (ntensors > 0 && !table) || out_dtype < kF32 || out_dtype > kF16)
+        return CS_ERR_ARGS;
+    int64_t total = 0;
+    for (int k = 0; k < ntensors; ++k) {
+        const int64_t* row = table + 8 * (int64_t)k;
+        const int64_t n = row[5], meta = row[6];
+        const int dtype = (int)(meta & 0xF);
+        const bool eight = (meta >> 4) & 1;
+        if (n < 0 || n > (int64_t)1 << 48 || dtype > kF16 || (meta & ~(int64_t)0x7FFFFF1F))
+            return CS_ERR_ARGS;
+        if (n == 0) continue;
+        if (!row[0] || !row[1] || !row[3] || !row[4]) return CS_ERR_ARGS;
+        if (op == kUnpack && (row[2] < n || row[2] > (int64_t)1 << 48)) return CS_ERR_ARGS;
+        if (op == kStep) {
+            if ((meta >> 8) >= nsets || !sets || !set_keys) return CS_ERR_ARGS;
+            if (dtype != kF32 && !row[2]) return CS_ERR_ARGS;
+        }
+        // The codes are read and written eight at a time.
+        if ((op != kPack && eight &&
+             (!aw_aligned((void*)row[3], 8) || !aw_aligned((void*)row[4], 8))) ||
+            (op == kPack && (!aw_aligned((void*)row[0], 8) || !aw_aligned((void*)row[1], 8))))
+            return CS_ERR_ARGS;
+        total += op == kUnpack ? row[2] : n;
+    }
+    if (total == 0) return CS_OK;
+    const int64_t chunk = aw_chunk(total, 8192);
+    int k = 0;
+    while (k < ntensors) {
+        AwArgs a;
+        int set_of[kAwMaxSets], used = 0;
+        a.n = 0;
+        uint64_t blocks = 0;
+        for (; k < ntensors && a.n < kAwMaxTensors; ++k) {
+            const int64_t* row = table + 8 * (int64_t)k;
+            const int64_t n = row[5];
+            if (n == 0) continue;
+            const int dtype = (int)(row[6] & 0xF), set = (int)(row[6] >> 8);
+            const bool eight = (row[6] >> 4) & 1;
+            int at = 0;
+            if (op == kStep) {
+                while (at < used && set_of[at] != set) ++at;
+                if (at == used) {
+                    if (used == kAwMaxSets) break;
+                    set_of[used++] = set;
+                    const float* f = sets + 8 * (int64_t)set;
+                    a.s[at] = AwSet{f[0], f[1], f[2], f[3], f[4], f[5], f[6], 0.0f};
+                }
+            }
+            const uint64_t b = (uint64_t)(((op == kUnpack ? row[2] : n) + chunk - 1) / chunk);
+            bool vec = true;
+            for (int c = 0; c < 5; ++c)
+                if (c != 2 || op == kStep) vec = vec && aw_aligned((void*)row[c], 16);
+            AwTensor& t = a.t[a.n++];
+            t.param = (void*)row[0];
+            t.grad = (const void*)row[1];
+            t.master = (float*)row[2];
+            t.avg = (void*)row[3];
+            t.sq = (void*)row[4];
+            t.n = n;
+            t.first_block = (uint32_t)blocks;
+            t.meta = (uint32_t)(dtype | (eight ? 16 : 0) | (vec ? 32 : 0) | at << 8);
+            t.key = op == kStep ? aw_mix(set_keys[set] + (uint32_t)row[7]) : 0u;
+            t.pad = 0;
+            blocks += b;
+        }
+        if (a.n == 0) continue;
+        a.clip = clip;
+        a.chunk = chunk;
+        a.out_dtype = out_dtype;
+        const dim3 grid((unsigned)blocks), block(kAwThreads);
+        if (op == kStep)
+            hipLaunchKernelGGL(k_adamw, grid, block, 0, stream, a);
+        else if (op == kPack)
+            hipLaunchKernelGGL(k_adamw_pack, grid, block, 0, stream, a);
+        else
+            hipLaunchKernelGGL(k_adamw_unpack, grid, block, 0, stream, a);
+        if (hipGetLastError() != hipSuccess) return CS_ERR_HIP;
+    }
+    return CS_OK;
+}
+
+}  // namespace
+
+extern "C" int cs_adamw_step(int32_t ntensors, const int64_t* table, int32_t nsets,
+                             const float* sets, const uint32_t* keys, const float* clip,
+                             hipStream_t stream) {
+    return aw_run(kStep, ntensors, table, nsets, sets, keys, clip, kF32, stream);
+}
+
+extern "C" int cs_adamw_pack_state(int32_t ntensors, const int64_t* table, hipStream_t stream) {
+    return aw_run(kPack, ntensors, table, 0, nullptr, nullptr, nullptr, kF32, stream);
+}
+
+extern "C" int cs_adamw_unpack_state(int32_t ntensors, const int64_t* table, int32_t out_dtype,
+                                     hipStream_t stream) {
+    return aw_run(kUnpack, ntensors, table, 0, nullptr, nullptr, nullptr, out_dtype, stream);
+}
+
+extern "C" int cs_grad_norm(int32_t ntensors, const int64_t* table, double max_norm,
+                            double* partials, float* out, hipStream_t stream) {
+    if (ntensors < 0 || (ntensors > 0 && !table) || !partials || !out || !(max_norm >= 0.0))
+        return CS_ERR_ARGS;
+    int64_t total = 0;
+    for (int k = 0; k < ntensors; ++k) {
+        const int64_t* row = table + 8 * (int64_t)k;
+        if (row[5] < 0 || row[5] > (int64_t)1 << 48 || (row[6] & 0xF) > kF16 ||
+            (row[5] > 0 && !row[1]))
+            return CS_ERR_ARGS;
+        total += row[5];
+    }
+    // Each tensor ends with a part of a chunk, so the blocks are at most
+    // kNormBlocks and one a tensor.
+    const int64_t chunk = aw_chunk(total, kNormBlocks);
+    int k = 0;
+    int64_t done = 0;
+    while (k < ntensors) {
+        NormArgs a;
+        a.n = 0;
+        int64_t blocks = 0;
+        for (; k < ntensors && a.n < kNormMaxTensors; ++k) {
+            const int64_t* row = table + 8 * (int64_t)k;
+            if (row[5] == 0) continue;
+            NormTensor& t = a.t[a.n++];
+            t.grad = (const void*)row[1];
+            t.n = row[5];
+            t.first_block = (uint32_t)blocks;
+            t.meta = (uint32_t)(row[6] & 0xF) | (aw_aligned((void*)row[1], 16) ? 32u : 0u);
+            blocks += (row[5] + chunk - 1) / chunk;
+        }
+        if (a.n == 0) break;
+        a.partials = partials + done;
+        a.chunk = chunk;
+        hipLaunchKernelGGL(k_grad_squares, dim3((unsigned)blocks), dim3(kAwThreads), 0, stream, a);
+        if (hipGetLastError() != hipSuccess) return CS_ERR_HIP;
+        done += blocks;
+    }
+    hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(kAwThreads), 0, stream, partials, (int32_t)done,
+                       (float)max_norm, out);
+    return hipGetLastError() == hipSuccess ? CS_OK : CS_ERR_HIP;
+}

@@ -1,4 +1,4 @@
-"""Adam and Adan with the step in one HIP launch for up to 16 parameters.
+"""Adam, Adan and AdamW with the step in one HIP launch for many parameters.
 
 The reference optimizes its primitives with ``torch.optim.Adam`` over
 per-group learning rates (gaussian_trace/model.py:172-189).  ``Adam`` here is
@@ -14,6 +14,12 @@ around ``step`` is left out, since it costs more host time than the launch.
 of its training script) with the update of ops/optim.py:8-113 as one
 ``cs_adan_step`` launch per 16 tensors; ``adan_step_from_grad_tilelang`` is
 the reference's functional single-tensor form.
+
+``AdamW`` (new: the reference trains its primitives directly, without a
+network) is for the weights of a network in front of the renderer: decoupled
+weight decay, fp32, bf16 and fp16 parameters of any dense layout, a global-norm
+clip without a host read, states in 32 or 8 bits, one launch for up to 56
+tensors.  ``global_grad_norm`` is the norm by itself.
 """
 from __future__ import annotations
 
@@ -21,12 +27,39 @@ import ctypes
 import math
 from itertools import chain
 
+import numpy as np
 import torch
 from torch.optim import optimizer as _torch_optimizer
 
 from . import _native as N
 
 MAX_TENSORS_PER_LAUNCH = 16
+
+
+def _run_pre_hooks(opt, closure):
+    """torch's step pre-hooks (global and of the instance): the (args, kwargs)
+    of the step and its closure as they leave them."""
+    args, kwargs = (opt,), {"closure": closure} if closure is not None else {}
+    if _torch_optimizer._global_optimizer_pre_hooks or opt._optimizer_step_pre_hooks:
+        for pre_hook in chain(_torch_optimizer._global_optimizer_pre_hooks.values(),
+                              opt._optimizer_step_pre_hooks.values()):
+            result = pre_hook(opt, args, kwargs)
+            if result is not None:
+                if isinstance(result, tuple) and len(result) == 2:
+                    args, kwargs = result
+                else:
+                    raise RuntimeError(
+                        "optimizer step pre-hooks must return None or (args, kwargs), got "
+                        f"{result}")
+        closure = kwargs.get("closure", closure)
+    return args, kwargs, closure
+
+
+def _run_post_hooks(opt, args, kwargs):
+    if opt._optimizer_step_post_hooks or _torch_optimizer._global_optimizer_post_hooks:
+        for post_hook in chain(opt._optimizer_step_post_hooks.values(),
+                               _torch_optimizer._global_optimizer_post_hooks.values()):
+            post_hook(opt, args, kwargs)
 
 
 class _LaunchArgs:
@@ -102,19 +135,7 @@ class Adam(torch.optim.Optimizer):
         return float(arr)
 
     def step(self, closure=None):
-        args, kwargs = (self,), {"closure": closure} if closure is not None else {}
-        if _torch_optimizer._global_optimizer_pre_hooks or self._optimizer_step_pre_hooks:
-            for pre_hook in chain(_torch_optimizer._global_optimizer_pre_hooks.values(),
-                                  self._optimizer_step_pre_hooks.values()):
-                result = pre_hook(self, args, kwargs)
-                if result is not None:
-                    if isinstance(result, tuple) and len(result) == 2:
-                        args, kwargs = result
-                    else:
-                        raise RuntimeError(
-                            "optimizer step pre-hooks must return None or (args, kwargs), got "
-                            f"{result}")
-            closure = kwargs.get("closure", closure)
+        args, kwargs, closure = _run_pre_hooks(self, closure)
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -150,10 +171,7 @@ class Adam(torch.optim.Optimizer):
             for k in range(0, len(items), MAX_TENSORS_PER_LAUNCH):
                 self._launch(dev, items[k:k + MAX_TENSORS_PER_LAUNCH], beta1, beta2, eps)
         self._optimizer_step_code()
-        if self._optimizer_step_post_hooks or _torch_optimizer._global_optimizer_post_hooks:
-            for post_hook in chain(self._optimizer_step_post_hooks.values(),
-                                   _torch_optimizer._global_optimizer_post_hooks.values()):
-                post_hook(self, args, kwargs)
+        _run_post_hooks(self, args, kwargs)
         return loss
 
     # torch's Optimizer wraps `step` of each subclass in a profiler range unless
@@ -367,3 +385,463 @@ def adan_step_from_grad_tilelang(param, grad, exp_avg, exp_avg_sq, exp_avg_diff,
     _adan_launch(param.device.index,
                  [(param, g, exp_avg, exp_avg_sq, exp_avg_diff, neg_pre_grad, scalars,
                    int(step) == 1, bool(no_prox))], None)
+
+
+# ------------------------------------------------------------------- AdamW
+
+_ADAMW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_EIGHT = 16                 # the bit of a table row's type for 8-bit states
+_SET_SHIFT = 8
+_P, _G, _MASTER, _AVG, _SQ, _NUMEL, _META, _NUMBER = range(8)   # columns of the table
+_AVG8, _SQ8 = "exp_avg_8bit", "exp_avg_sq_8bit"
+
+
+def _mix32(x):
+    x &= 0xFFFFFFFF
+    x ^= x >> 16
+    x = (x * 0x9E3779B9) & 0xFFFFFFFF
+    x ^= x >> 15
+    x = (x * 0xBB67AE85) & 0xFFFFFFFF
+    return x ^ (x >> 16)
+
+
+def _is_dense(t):
+    """Whether t's elements fill one range of memory, each of them once."""
+    if t.is_contiguous():
+        return True
+    run = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != run:
+            return False
+        run *= size
+    return True
+
+
+def _same_layout(a, b):
+    """Whether two dense tensors of one shape lie in memory in the same order."""
+    if a.is_contiguous() and b.is_contiguous():
+        return True
+    return all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1)
+
+
+def _codes_numel(numel):
+    """Bytes of an 8-bit state: whole blocks of codes and a byte for each."""
+    return -(-numel // N.ADAMW_BLOCK) * (N.ADAMW_BLOCK + 1)
+
+
+class _AdamWEntry:
+    """What the launches need of one parameter; remade when a tensor of it is
+    another one."""
+    __slots__ = ("p", "st", "avg", "sq", "master", "step_t", "step", "row", "dtype", "contiguous")
+
+
+class _AdamWPlan:
+    """The table of one device's launches, reused while the same parameters take part."""
+
+    def __init__(self, entries):
+        self.entries = entries
+        self.table = np.array([e.row for e in entries], dtype=np.int64).reshape(-1, 8)
+        self.address = self.table.ctypes.data
+        self.grads = self.table[:, _G]
+        self.metas = self.table[:, _META]
+        self.one_set = True   # every row of the first set
+
+
+def _check_grad(g, dtype, device):
+    if g.layout is not torch.strided:
+        raise RuntimeError("AdamW does not support sparse gradients")
+    if g.dtype is not dtype or g.device != device:
+        raise ValueError(f"a gradient of {g.dtype} on {g.device} beside a parameter of {dtype} "
+                         f"on {device}")
+
+
+def global_grad_norm(grads):
+    """The 2-norm over all gradients together, as a 0-d fp32 device tensor:
+    squares summed in fp32 within a thread and in fp64 across them, in a fixed
+    order, without a host read.  grads: fp32, bf16 and fp16 tensors of one
+    device, of any strides; None entries are passed over."""
+    held = []
+    for g in grads:
+        if g is None:
+            continue
+        if g.layout is not torch.strided:
+            raise RuntimeError("global_grad_norm does not support sparse gradients")
+        if g.dtype not in _ADAMW_DTYPES:
+            raise ValueError(f"global_grad_norm takes float32, bfloat16 and float16, got {g.dtype}")
+        N.require_gpu(g, "a gradient of global_grad_norm")
+        if held and g.device != held[0].device:
+            raise ValueError("global_grad_norm takes gradients of one device")
+        held.append(g.detach() if _is_dense(g) else g.detach().contiguous())
+    if not held:
+        raise ValueError("global_grad_norm needs a gradient")
+    table = np.zeros((len(held), 8), dtype=np.int64)
+    table[:, _G] = [g.data_ptr() for g in held]
+    table[:, _NUMEL] = [g.numel() for g in held]
+    table[:, _META] = [_ADAMW_DTYPES[g.dtype] for g in held]
+    with torch.cuda.device(held[0].device):
+        return _norm_launch(table.ctypes.data, len(held), held[0].device, 0.0)[0]
+
+
+def _norm_launch(address, n, device, max_norm):
+    """Device (norm, clip factor) of the table's gradients."""
+    out = torch.empty(2, dtype=torch.float32, device=device)
+    partials = torch.empty(N.GRAD_NORM_BLOCKS + n, dtype=torch.float64, device=device)
+    with N.prof("optim.grad_norm"):
+        N.call("cs_grad_norm", n, address, max_norm, partials.data_ptr(), out.data_ptr(),
+               N.stream(device))
+    return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over all of a network's tensors (torch.optim.AdamW's update,
+    amsgrad and maximize off), for fp32, bf16 and fp16 device parameters of any
+    dense layout.
+
+    ``state`` holds ``step`` (a CPU tensor), ``exp_avg`` and ``exp_avg_sq`` in
+    fp32, as torch's does for fp32 parameters, so those checkpoints move between
+    the two.  A 16-bit parameter has an fp32 copy ``master`` in its state; the
+    update moves the copy, and the parameter is the copy rounded to nearest.
+    Whoever writes to such a parameter by hand deletes ``state[p]["master"]``;
+    the next step makes it anew.
+
+    ``state_bits=8`` keeps both moments of a tensor of at least
+    ``min_8bit_numel`` elements in a byte each (``exp_avg_8bit``,
+    ``exp_avg_sq_8bit``): 4 exponent bits below the largest of 128 neighbours'
+    and 3 (first moment, signed) or 4 (root of the second) mantissa bits, rounded
+    stochastically with numbers that depend on ``seed``, the step, the tensor's
+    place among the parameters and the element alone, so a run repeats bit for
+    bit.  load_state_dict takes states of either width and converts them.
+
+    ``max_grad_norm`` > 0 scales all gradients by min(1, max_grad_norm / (norm +
+    1e-6)) within the step, from the norm over all of them (``grad_norm``, a
+    device tensor); the gradients themselves stay as they are."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                 amsgrad=False, *, maximize=False, capturable=False, differentiable=False,
+                 foreach=None, fused=None, state_bits=32, min_8bit_numel=4096,
+                 max_grad_norm=0.0, seed=0):
+        if not 0.0 <= float(lr):
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not 0.0 <= float(eps):
+            raise ValueError(f"Invalid epsilon value: {eps}")
+        if not 0.0 <= betas[0] < 1.0:
+            raise ValueError(f"Invalid beta parameter at index 0: {betas[0]}")
+        if not 0.0 <= betas[1] < 1.0:
+            raise ValueError(f"Invalid beta parameter at index 1: {betas[1]}")
+        if not 0.0 <= weight_decay:
+            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        if amsgrad or maximize or capturable or differentiable:
+            raise NotImplementedError(
+                "repo_amd.optim.AdamW implements amsgrad=False, maximize=False, "
+                "capturable=False, differentiable=False")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not 0 <= min_8bit_numel:
+            raise ValueError(f"Invalid min_8bit_numel: {min_8bit_numel}")
+        if not 0.0 <= max_grad_norm:
+            raise ValueError(f"Invalid max_grad_norm: {max_grad_norm}")
+        self.state_bits, self.min_8bit_numel = int(state_bits), int(min_8bit_numel)
+        self.max_grad_norm, self.seed = float(max_grad_norm), int(seed)
+        self._reset()
+        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False,
+                        maximize=False, foreach=None, capturable=False, differentiable=False,
+                        fused=None)
+        super().__init__(params, defaults)
+
+    def _reset(self):
+        self._entries, self._plans, self._norm = {}, {}, None
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits,
+                "min_8bit_numel": self.min_8bit_numel, "max_grad_norm": self.max_grad_norm,
+                "seed": self.seed}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._reset()
+
+    zero_grad = Adam.zero_grad
+
+    @property
+    def grad_norm(self):
+        """The norm over all gradients before the last step's clip, a 0-d
+        device tensor (None without max_grad_norm or before the first step)."""
+        return None if self._norm is None else self._norm[0]
+
+    # ---- state
+
+    def _eight(self, numel):
+        return self.state_bits == 8 and numel >= self.min_8bit_numel
+
+    def _check_param(self, p):
+        if p.dtype not in _ADAMW_DTYPES or not p.is_cuda or p.layout is not torch.strided:
+            raise ValueError("repo_amd.optim.AdamW needs float32, bfloat16 or float16 CUDA (ROCm) "
+                             f"parameters, got {p.dtype} on {p.device}")
+        if not _is_dense(p):
+            raise ValueError("repo_amd.optim.AdamW needs parameters that fill their memory, got "
+                             f"shape {tuple(p.shape)} with strides {p.stride()}")
+
+    def _init_state(self, p, st):
+        if "step" not in st:
+            st["step"] = torch.tensor(0.0, dtype=torch.float32)
+        if self._eight(p.numel()):
+            for name in (_AVG8, _SQ8):
+                if name not in st:
+                    st[name] = torch.zeros(_codes_numel(p.numel()), dtype=torch.uint8,
+                                           device=p.device)
+        else:
+            for name in ("exp_avg", "exp_avg_sq"):
+                if name not in st:
+                    st[name] = torch.zeros_like(p, dtype=torch.float32,
+                                                memory_format=torch.preserve_format)
+        if p.dtype is not torch.float32 and "master" not in st:
+            st["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
+
+    def _entry(self, p, number):
+        self._check_param(p)
+        st = self.state[p]
+        eight = self._eight(p.numel())
+        self._init_state(p, st)
+        e = _AdamWEntry()
+        e.p, e.st, e.dtype, e.contiguous = p, st, p.dtype, p.is_contiguous()
+        e.avg, e.sq = (st[_AVG8], st[_SQ8]) if eight else (st["exp_avg"], st["exp_avg_sq"])
+        e.master = st.get("master") if p.dtype is not torch.float32 else None
+        for t in (e.avg, e.sq, e.master):
+            if t is None:
+                continue
+            if eight and t is not e.master:
+                good = (t.dtype is torch.uint8 and t.numel() == _codes_numel(p.numel())
+                        and t.is_contiguous())
+            else:
+                good = (t.dtype is torch.float32 and t.shape == p.shape and _is_dense(t)
+                        and _same_layout(t, p))
+            if not good or t.device != p.device:
+                raise ValueError("an AdamW state does not fit its parameter: "
+                                 f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on "
+                                 f"{t.device} beside {tuple(p.shape)} with strides {p.stride()} on "
+                                 f"{p.device}")
+        step = st["step"]
+        if not (isinstance(step, torch.Tensor) and step.device.type == "cpu"
+                and step.dtype is torch.float32 and step.numel() == 1):
+            step = st["step"] = torch.tensor(float(step), dtype=torch.float32)
+        e.step_t, e.step = step, ctypes.c_float.from_address(step.data_ptr())
+        e.row = [p.data_ptr(), 0, 0 if e.master is None else e.master.data_ptr(),
+                 e.avg.data_ptr(), e.sq.data_ptr(), p.numel(),
+                 _ADAMW_DTYPES[p.dtype] | (_EIGHT if eight else 0), number]
+        return e
+
+    def _current(self, p, number):
+        """p's entry, remade if anything of it has been replaced."""
+        e = self._entries.get(p)
+        if e is not None:
+            st, row = e.st, e.row
+            a, b = (_AVG8, _SQ8) if row[_META] & _EIGHT else ("exp_avg", "exp_avg_sq")
+            if (self.state.get(p) is st and row[_P] == p.data_ptr() and p.dtype is e.dtype
+                    and row[_NUMEL] == p.numel() and row[_NUMBER] == number
+                    and st.get(a) is e.avg and st.get(b) is e.sq
+                    and st.get("step") is e.step_t and st.get("master") is e.master):
+                return e
+        e = self._entries[p] = self._entry(p, number)
+        return e
+
+    # ---- the step
+
+    def step(self, closure=None):
+        args, kwargs, closure = _run_pre_hooks(self, closure)
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        self._step()
+        self._optimizer_step_code()
+        _run_post_hooks(self, args, kwargs)
+        return loss
+
+    step.hooked = True   # as Adam's: the hooks are called above
+
+    def _step(self):
+        # Gathered first: nothing is launched or counted if a tensor is refused.
+        work, number = {}, -1
+        for k, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                number += 1
+                g = p.grad
+                if g is None:
+                    continue
+                e = self._current(p, number)
+                if g.dtype is not e.dtype or g.layout is not torch.strided:
+                    _check_grad(g, e.dtype, p.device)
+                if not (e.contiguous and g.is_contiguous()) and not (
+                        _is_dense(g) and _same_layout(g, p)):
+                    g = torch.empty_like(p).copy_(g.detach())
+                w = work.get(p.device)
+                if w is None:
+                    w = work[p.device] = ([], [], [], [])
+                w[0].append(e)
+                w[1].append(g)
+                w[2].append(g.data_ptr())
+                w[3].append((k, e.step.value + 1.0))
+        if len(self._entries) > number + 1:   # parameters that have left the groups
+            kept = {p for group in self.param_groups for p in group["params"]}
+            self._entries = {p: e for p, e in self._entries.items() if p in kept}
+        if not work:
+            return
+        if self.max_grad_norm > 0 and len(work) > 1:
+            raise NotImplementedError("max_grad_norm needs all parameters on one device")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("an AdamW step counts on the host and cannot be captured")
+        for device, w in work.items():
+            if device.index == torch.cuda.current_device():
+                self._launch(device, *w)
+            else:
+                with torch.cuda.device(device):
+                    self._launch(device, *w)
+
+    def _launch(self, device, entries, grads, grad_ptrs, steps):
+        plan = self._plans.get(device)
+        if plan is None or plan.entries != entries:
+            plan = self._plans[device] = _AdamWPlan(entries)
+        numbers = {}
+        for s in steps:
+            if s not in numbers:
+                numbers[s] = len(numbers)
+        if len(numbers) > 1 or not plan.one_set:
+            plan.metas[:] = [e.row[_META] | numbers[s] << _SET_SHIFT
+                             for e, s in zip(entries, steps)]
+            plan.one_set = len(numbers) == 1
+        plan.grads[:] = grad_ptrs
+        sets = np.zeros((len(numbers), 8), dtype=np.float32)
+        keys = np.zeros(len(numbers), dtype=np.uint32)
+        for (k, step), i in numbers.items():
+            group = self.param_groups[k]
+            beta1, beta2 = group["betas"]
+            lr = float(group["lr"])
+            sets[i] = (1.0 - lr * group["weight_decay"], lr / (1.0 - beta1 ** step),
+                       math.sqrt(1.0 - beta2 ** step), 1.0 - beta1, beta2, 1.0 - beta2,
+                       group["eps"], 0.0)
+            keys[i] = _mix32(self.seed + int(step) * 0x3C6EF372)
+        clip = None
+        if self.max_grad_norm > 0:
+            self._norm = _norm_launch(plan.address, len(entries), device, self.max_grad_norm)
+            clip = self._norm.data_ptr() + 4
+        with N.prof("optim.adamw"):
+            N.call("cs_adamw_step", len(entries), plan.address, len(numbers), sets.ctypes.data,
+                   keys.ctypes.data, clip, N.stream(device))
+        for e, (_, step) in zip(entries, steps):
+            e.step.value = step
+
+    # ---- reading and loading
+
+    def flat_state(self, dtype=torch.float32, align=1):
+        """Both moments of all parameters, (exp_avg, exp_avg_sq), each as one
+        flat tensor of ``dtype``: the parameters one after the other in the order
+        of the groups, each in the order in which it lies in memory and beginning
+        at a multiple of ``align`` elements, with zeros between them and for
+        parameters that have taken no step.  8-bit states give the values that
+        they stand for."""
+        if dtype not in _ADAMW_DTYPES:
+            raise ValueError(f"flat_state gives float32, bfloat16 and float16, got {dtype}")
+        if align < 1:
+            raise ValueError(f"Invalid align: {align}")
+        rows, begins, at, bare, device = [], [], 0, False, None
+        number = -1
+        for group in self.param_groups:
+            for p in group["params"]:
+                number += 1
+                size = -(-p.numel() // align) * align
+                device = device or p.device
+                if p.device != device:
+                    raise NotImplementedError("flat_state needs all parameters on one device")
+                st = self.state.get(p)
+                if st and ("exp_avg" in st or _AVG8 in st):
+                    row = list(self._current(p, number).row)
+                    row[_MASTER] = size
+                    rows.append(row)
+                    begins.append(at)
+                else:
+                    bare = bare or size > 0
+                at += size
+        make = torch.zeros if bare else torch.empty
+        out = (make(at, dtype=dtype, device=device), make(at, dtype=dtype, device=device))
+        if rows:
+            table = np.array(rows, dtype=np.int64)
+            for col, t in ((_P, out[0]), (_G, out[1])):
+                table[:, col] = np.array(begins) * t.element_size() + t.data_ptr()
+            table[:, _META] &= _EIGHT
+            with torch.cuda.device(device):
+                N.call("cs_adamw_unpack_state", len(rows), table.ctypes.data,
+                       _ADAMW_DTYPES[dtype], N.stream(device))
+        return out
+
+    def load_state_dict(self, state_dict):
+        """Takes states of either width, and of bf16 or fp16 (as torch's
+        optimizers keep them beside 16-bit parameters), and holds them as this
+        optimizer does.  torch's own loading would cast every state to its
+        parameter's type, so only the groups and step counts go through it."""
+        pre, post = (self._optimizer_load_state_dict_pre_hooks,
+                     self._optimizer_load_state_dict_post_hooks)
+        state_dict = state_dict.copy()
+        for hook in pre.values():
+            got = hook(self, state_dict)
+            if got is not None:
+                state_dict = got
+        slim = {**state_dict, "state": {k: {"step": s["step"]} if "step" in s else {}
+                                        for k, s in state_dict["state"].items()}}
+        self._optimizer_load_state_dict_pre_hooks = type(pre)()
+        self._optimizer_load_state_dict_post_hooks = type(post)()
+        try:
+            super().load_state_dict(slim)
+        finally:
+            self._optimizer_load_state_dict_pre_hooks = pre
+            self._optimizer_load_state_dict_post_hooks = post
+        ids = [k for group in state_dict["param_groups"] for k in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for k, p in zip(ids, params):
+            if k in state_dict["state"]:
+                self._take_state(p, state_dict["state"][k])
+        for hook in post.values():
+            hook(self)
+
+    @torch.no_grad()
+    def _take_state(self, p, given):
+        self._check_param(p)
+        st = self.state[p]
+        eight = self._eight(p.numel())
+
+        def fp32(t):
+            return torch.empty_like(p, dtype=torch.float32,
+                                    memory_format=torch.preserve_format).copy_(t)
+
+        for name, value in given.items():
+            if name not in ("step", "exp_avg", "exp_avg_sq", _AVG8, _SQ8, "master"):
+                st[name] = value
+        if given.get("master") is not None and p.dtype is not torch.float32:
+            st["master"] = fp32(given["master"])
+        if _AVG8 in given:
+            codes = [given[name].to(p.device, copy=True) for name in (_AVG8, _SQ8)]
+            if any(c.dtype is not torch.uint8 or c.numel() != _codes_numel(p.numel())
+                   for c in codes):
+                raise ValueError("8-bit AdamW states of another size than the parameter's")
+            if eight:
+                st[_AVG8], st[_SQ8] = codes
+                return
+            self._init_state(p, st)
+            to = (st["exp_avg"], st["exp_avg_sq"])
+            row = [to[0].data_ptr(), to[1].data_ptr(), p.numel(), codes[0].data_ptr(),
+                   codes[1].data_ptr(), p.numel(), _EIGHT, 0]
+            self._convert("cs_adamw_unpack_state", p, row, 0)
+        elif "exp_avg" in given:
+            avg, sq = fp32(given["exp_avg"]), fp32(given["exp_avg_sq"])
+            if not eight:
+                st["exp_avg"], st["exp_avg_sq"] = avg, sq
+                return
+            self._init_state(p, st)
+            row = [st[_AVG8].data_ptr(), st[_SQ8].data_ptr(), 0, avg.data_ptr(), sq.data_ptr(),
+                   p.numel(), 0, 0]
+            self._convert("cs_adamw_pack_state", p, row)
+
+    @staticmethod
+    def _convert(name, p, row, *args):
+        table = np.array([row], dtype=np.int64)
+        with torch.cuda.device(p.device):
+            N.call(name, 1, table.ctypes.data, *args, N.stream(p.device))
