@@ -737,6 +737,30 @@ int cs_adamw_unpack_state(int32_t ntensors, const int64_t* table, int32_t out_dt
 int cs_grad_norm(int32_t ntensors, const int64_t* table, double max_norm, double* partials,
                  float* out, hipStream_t stream);
 
+/* ---------------- group norm ---------------- */
+
+/* Group norm with an activation over n samples of s rows of c channels, channels
+ * contiguous ([n, s, c]); new (the reference has no network layers).  dtype of
+ * x, y, dy and dx, param_dtype of weight, bias and their gradients: 0 fp32, 1
+ * bf16, 2 fp16.  act: 0 none, 1 relu, 2 silu, 3 gelu (erf).  weight and bias
+ * [c], each NULL for 1 and 0.  eps is added to the variance (biased).  The
+ * forward writes mean and rstd ([n, groups] fp32; both or neither NULL), which
+ * the backward reads; the backward writes those of dx, dweight and dbias that are
+ * not NULL.  workspace: cs_group_norm_workspace_elems floats, 8-byte aligned, of
+ * which nothing is kept between calls.  n * s * c is at most 2^44, and n at most
+ * 2^23 (fewer with more than 2048 channels). */
+size_t cs_group_norm_workspace_elems(int64_t n, int64_t s, int32_t c, int32_t groups,
+                                     int32_t dtype, int32_t backward);
+int cs_group_norm_forward(const void* x, int64_t n, int64_t s, int32_t c, int32_t groups,
+                          int32_t dtype, const void* weight, const void* bias,
+                          int32_t param_dtype, double eps, int32_t act, float* workspace,
+                          float* mean, float* rstd, void* y, hipStream_t stream);
+int cs_group_norm_backward(const void* x, const void* dy, int64_t n, int64_t s, int32_t c,
+                           int32_t groups, int32_t dtype, const void* weight, const void* bias,
+                           int32_t param_dtype, int32_t act, const float* mean,
+                           const float* rstd, float* workspace, void* dx, void* dweight,
+                           void* dbias, hipStream_t stream);
+
 /* ---------------- 2D Gaussian splats (GsRenderFunction) ---------------- */
 
 /* project_gaussians_2d_scale_rot_forward_kernel (ops/forward2d.py:14-164):

@@ -137,6 +137,11 @@ _SIGNATURES = {
     "cs_adamw_pack_state": (ctypes.c_int, [_I32, _P, _P]),
     "cs_adamw_unpack_state": (ctypes.c_int, [_I32, _P, _I32, _P]),
     "cs_grad_norm": (ctypes.c_int, [_I32, _P, _D, _P, _P, _P]),
+    "cs_group_norm_workspace_elems": (_SZ, [_I64, _I64, _I32, _I32, _I32, _I32]),
+    "cs_group_norm_forward": (ctypes.c_int, [_P, _I64, _I64, _I32, _I32, _I32, _P, _P, _I32, _D,
+                                             _I32, _P, _P, _P, _P, _P]),
+    "cs_group_norm_backward": (ctypes.c_int, [_P, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _I32,
+                                              _I32, _P, _P, _P, _P, _P, _P, _P]),
     "cs_gs_project_forward": (ctypes.c_int, [_P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P,
                                              _P, _P, _P]),
     "cs_gs_bin_prepare": (ctypes.c_int, [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P,

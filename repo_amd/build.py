@@ -26,7 +26,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcubicsplat_hip.so")
 SOURCES = ["binning.hip", "raster.hip", "metric.hip", "optim.hip", "rings.hip", "gaussian.hip",
-           "adamw.hip"]
+           "adamw.hip", "norm.hip"]
 ARCH = os.environ.get("CS_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

@@ -1,0 +1,694 @@
+// Group norm with an activation over channels-last images, and its gradient.
+//
+// x is [N, S, C] (S the spatial positions of a sample), a group g the channels
+// [g D, (g + 1) D) of one sample, M = D S values:
+//   mean = E[x], r = 1 / sqrt(E[(x - mean)^2] + eps), xh = (x - mean) r,
+//   z = xh w_c + b_c, y = act(z)
+//   dz = dy act'(z), db_c = sum dz, dw_c = sum dz xh,
+//   dx = r (w dz - E[w dz] - xh E[w dz xh])
+// Everything is computed in fp32 and rounded once on storing.
+//
+// Two launches a direction: one sums, one applies.  A workgroup takes a slice of
+// channels (whole groups, up to 256 vectors wide) over a chunk of rows (spatial
+// positions); a thread keeps the same vector of channels over all of its rows,
+// so what depends on the channel stays in its registers.  The sums of a chunk
+// are written out, and each workgroup of the second launch joins the ones that
+// it needs, in a fixed order.
+//
+// The variance is not formed from a sum of squares: each thread sums x and x^2
+// relative to its first value per channel, and (count, mean, sum of squared
+// deviations) are what is joined, so a mean far from zero costs nothing.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/cubicsplat_hip.h"
+
+namespace cs {
+
+constexpr int kGnThreads = 256;
+constexpr int kGnMaxVec = 8;
+
+enum { kGnF32 = 0, kGnBF16 = 1, kGnF16 = 2 };
+enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
+
+struct GnShape {
+    int64_t s;             // rows of a sample
+    int32_t c, groups, d;  // d = c / groups
+    int32_t gs;            // groups of a slice (1 where a group has several parts)
+    int32_t parts;         // slices of a group
+    int32_t cs;            // channels of a slice (the last may have fewer)
+    int32_t slices;
+    int32_t chunks;        // of a sample, in the summing launch
+    int64_t rows;          // of such a chunk
+    int32_t apply_chunks;
+    int64_t apply_rows;
+};
+
+struct GnArgs {
+    GnShape h;
+    const void* x;
+    const void* dy;
+    const void* weight;
+    const void* bias;
+    int32_t wdtype;
+    float eps;
+    float* partials;   // [n][chunk][group][part][2]
+    float* channels;   // backward: [n][chunk][channel][2]
+    float* mean;
+    float* rstd;
+    void* out;         // y or dx
+    void* dweight;
+    void* dbias;
+    int32_t n;
+    int32_t channel_blocks;  // of the backward's second launch, for dw and db
+};
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) GnVec { T v[V]; };
+
+template <int V, typename T>
+__device__ inline void gn_load(const T* p, float (&out)[V]) {
+    const GnVec<T, V> x = *reinterpret_cast<const GnVec<T, V>*>(p);
+#pragma unroll
+    for (int k = 0; k < V; ++k) out[k] = (float)x.v[k];
+}
+
+template <int V, typename T>
+__device__ inline void gn_store(T* p, const float (&in)[V]) {
+    GnVec<T, V> x;
+#pragma unroll
+    for (int k = 0; k < V; ++k) x.v[k] = (T)in[k];
+    *reinterpret_cast<GnVec<T, V>*>(p) = x;
+}
+
+__device__ inline float gn_param(const void* p, int dtype, int c, float none) {
+    if (!p) return none;
+    if (dtype == kGnF32) return ((const float*)p)[c];
+    if (dtype == kGnBF16) return (float)((const __bf16*)p)[c];
+    return (float)((const _Float16*)p)[c];
+}
+
+__device__ inline void gn_store_param(void* p, int dtype, int c, float v) {
+    if (dtype == kGnF32) ((float*)p)[c] = v;
+    else if (dtype == kGnBF16) ((__bf16*)p)[c] = (__bf16)v;
+    else ((_Float16*)p)[c] = (_Float16)v;
+}
+
+__device__ inline float gn_sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+}
+
+template <int ACT>
+__device__ inline float gn_act(float z) {
+    if (ACT == kActRelu) return z < 0.0f ? 0.0f : z;  // NaN stays
+    if (ACT == kActSilu) return z * gn_sigmoid(z);
+    if (ACT == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+    return z;
+}
+
+template <int ACT>
+__device__ inline float gn_slope(float z) {
+    if (ACT == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
+    if (ACT == kActSilu) {
+        const float p = gn_sigmoid(z);
+        return p * __builtin_fmaf(z, 1.0f - p, 1.0f);
+    }
+    if (ACT == kActGelu) {
+        const float p = 0.5f * (1.0f + erff(z * 0.70710678f));
+        return __builtin_fmaf(z * 0.39894228f, __expf(-0.5f * z * z), p);
+    }
+    return 1.0f;
+}
+
+// A workgroup's place: its slice's first channel and width, its thread's first
+// channel and row, and the rows of a pass.
+struct GnPlace {
+    int c0, cs, vecs, passrows, row, chan;
+    int g0, ng;  // the slice's groups
+    int part;
+    bool live;
+};
+
+template <int V>
+__device__ inline GnPlace gn_place(const GnShape& h, int slice) {
+    GnPlace q;
+    const int group = h.parts > 1 ? slice / h.parts : slice * h.gs;
+    q.part = h.parts > 1 ? slice - group * h.parts : 0;
+    q.g0 = group;
+    q.c0 = group * h.d + q.part * h.cs;
+    const int end = h.parts > 1 ? (group + 1) * h.d : h.c;
+    q.cs = q.c0 + h.cs < end ? h.cs : end - q.c0;
+    q.ng = h.parts > 1 ? 1 : q.cs / h.d;
+    q.vecs = q.cs / V;
+    q.passrows = kGnThreads / q.vecs;
+    q.row = threadIdx.x / q.vecs;
+    q.chan = (threadIdx.x - q.row * q.vecs) * V;
+    q.live = q.row < q.passrows;
+    return q;
+}
+
+struct GnWhere { int n, chunk, slice; };
+
+__device__ inline GnWhere gn_where(const GnShape& h, uint32_t block, int chunks) {
+    GnWhere w;
+    const uint32_t per = (uint32_t)h.slices * chunks;
+    w.n = block / per;
+    const uint32_t rest = block - w.n * per;
+    w.chunk = rest / h.slices;
+    w.slice = rest - w.chunk * h.slices;
+    return w;
+}
+
+// Sums the threads' values of each channel over the rows of a pass, and leaves
+// the slice's channel sums in buf[0 .. cs).
+template <int V>
+__device__ inline void gn_rows_sum(float* buf, const GnPlace& q, const float (&v)[V]) {
+    __syncthreads();
+    if (q.live) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) buf[q.row * q.cs + q.chan + k] = v[k];
+    }
+    int n = q.passrows;
+    while (n > 1) {
+        const int half = (n + 1) >> 1;
+        __syncthreads();
+        for (int i = threadIdx.x; i < (n - half) * q.cs; i += kGnThreads)
+            buf[i] += buf[i + half * q.cs];
+        n = half;
+    }
+    __syncthreads();
+}
+
+// Lanes that work on one group together: a power of two.
+__device__ inline int gn_lanes(int ng) {
+    int t = 64;
+    while (t > 1 && t * ng > kGnThreads) t >>= 1;
+    return t;
+}
+
+__device__ inline float gn_lanes_sum(float x, int t) {
+    for (int m = t >> 1; m > 0; m >>= 1) x += __shfl_xor(x, m);
+    return x;
+}
+
+// Group sums of buf[0 .. cs) into out[0 .. ng).
+__device__ inline void gn_groups_sum(const float* buf, float* out, const GnPlace& q, int d) {
+    const int t = gn_lanes(q.ng), lane = threadIdx.x & (t - 1);
+    const int width = q.ng == 1 ? q.cs : d;
+    for (int g = threadIdx.x / t; g < (q.ng + kGnThreads / t - 1) / (kGnThreads / t) * (kGnThreads / t);
+         g += kGnThreads / t) {
+        float s = 0.0f;
+        if (g < q.ng)
+            for (int k = lane; k < width; k += t) s += buf[g * width + k];
+        s = gn_lanes_sum(s, t);
+        if (g < q.ng && lane == 0) out[g] = s;
+    }
+    __syncthreads();
+}
+
+// ---- forward
+
+template <typename T, int V>
+__global__ __launch_bounds__(kGnThreads) void k_gn_stats(GnArgs a) {
+    __shared__ float buf[kGnThreads * V];
+    __shared__ float gsum[kGnThreads * V], gmean[kGnThreads * V];
+    const GnShape& h = a.h;
+    const GnWhere at_block = gn_where(h, blockIdx.x, h.chunks);
+    const int n = at_block.n, chunk = at_block.chunk;
+    const GnPlace q = gn_place<V>(h, at_block.slice);
+    const int64_t begin = chunk * h.rows, end = begin + h.rows < h.s ? begin + h.rows : h.s;
+    const T* x = (const T*)a.x + ((int64_t)n * h.s) * h.c + q.c0 + q.chan;
+    float k0[V], s1[V], s2[V], cnt = 0.0f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) k0[k] = s1[k] = s2[k] = 0.0f;
+    if (q.live && begin + q.row < end) {
+        gn_load<V>(x + (begin + q.row) * h.c, k0);
+        for (int64_t r = begin + q.row; r < end; r += q.passrows) {
+            float v[V];
+            gn_load<V>(x + r * h.c, v);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float e = v[k] - k0[k];
+                s1[k] += e;
+                s2[k] = __builtin_fmaf(e, e, s2[k]);
+            }
+            cnt += 1.0f;
+        }
+    }
+    // The thread's mean and squared deviations per channel.
+    float mean[V], m2[V], w[V];
+    const float inv = cnt > 0.0f ? 1.0f / cnt : 0.0f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const float e = s1[k] * inv;
+        mean[k] = k0[k] + e;
+        m2[k] = fmaxf(__builtin_fmaf(-s1[k], e, s2[k]), 0.0f);
+        w[k] = cnt * mean[k];
+    }
+    gn_rows_sum<V>(buf, q, w);
+    gn_groups_sum(buf, gsum, q, h.d);
+    const int width = q.ng == 1 ? q.cs : h.d;
+    const float total = (float)(end - begin) * (float)width;
+    for (int g = threadIdx.x; g < q.ng; g += kGnThreads) gmean[g] = gsum[g] / total;
+    __syncthreads();
+    if (q.live) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float e = mean[k] - gmean[q.ng == 1 ? 0 : (q.chan + k) / h.d];
+            w[k] = __builtin_fmaf(cnt * e, e, m2[k]);
+        }
+    }
+    gn_rows_sum<V>(buf, q, w);
+    gn_groups_sum(buf, gsum, q, h.d);
+    for (int g = threadIdx.x; g < q.ng; g += kGnThreads) {
+        float* o = a.partials +
+                   ((((int64_t)n * h.chunks + chunk) * h.groups + q.g0 + g) * h.parts + q.part) * 2;
+        o[0] = gmean[g];
+        o[1] = gsum[g];
+    }
+}
+
+// Joins a slice's partial means and deviations: mean and 1 / sqrt(var + eps)
+// of its groups into LDS.
+__device__ inline void gn_join_stats(const GnArgs& a, const GnPlace& q, int n, float* mean,
+                                     float* rstd) {
+    const GnShape& h = a.h;
+    const int t = gn_lanes(q.ng), lane = threadIdx.x & (t - 1), step = kGnThreads / t;
+    const int entries = h.chunks * h.parts;
+    for (int base = 0; base < q.ng; base += step) {
+        const int g = base + threadIdx.x / t;
+        float sw = 0.0f, swm = 0.0f;
+        const float* p = a.partials + ((int64_t)n * h.chunks * h.groups + q.g0 + g) * h.parts * 2;
+        if (g < q.ng)
+            for (int i = lane; i < entries; i += t) {
+                const int chunk = i / h.parts, part = i - chunk * h.parts;
+                const int64_t left = h.s - chunk * h.rows;
+                const int width = h.d - part * h.cs < h.cs ? h.d - part * h.cs : h.cs;
+                const float w = (float)(left < h.rows ? left : h.rows) *
+                                (float)(h.parts > 1 ? width : h.d);
+                const float m = p[((int64_t)chunk * h.groups * h.parts + part) * 2];
+                sw += w;
+                swm = __builtin_fmaf(w, m, swm);
+            }
+        sw = gn_lanes_sum(sw, t);
+        const float mu = gn_lanes_sum(swm, t) / sw;
+        float m2 = 0.0f;
+        if (g < q.ng)
+            for (int i = lane; i < entries; i += t) {
+                const int chunk = i / h.parts, part = i - chunk * h.parts;
+                const int64_t left = h.s - chunk * h.rows;
+                const int width = h.d - part * h.cs < h.cs ? h.d - part * h.cs : h.cs;
+                const float w = (float)(left < h.rows ? left : h.rows) *
+                                (float)(h.parts > 1 ? width : h.d);
+                const float* e = p + ((int64_t)chunk * h.groups * h.parts + part) * 2;
+                const float dm = e[0] - mu;
+                m2 += __builtin_fmaf(w * dm, dm, e[1]);
+            }
+        m2 = gn_lanes_sum(m2, t);
+        if (g < q.ng && lane == 0) {
+            mean[g] = mu;
+            rstd[g] = 1.0f / __builtin_sqrtf(m2 / sw + a.eps);
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(kGnThreads) void k_gn_apply(GnArgs a) {
+    __shared__ float gmean[kGnThreads * V], grstd[kGnThreads * V];
+    const GnShape& h = a.h;
+    const GnWhere w = gn_where(h, blockIdx.x, h.apply_chunks);
+    const int n = w.n, chunk = w.chunk;
+    const GnPlace q = gn_place<V>(h, w.slice);
+    gn_join_stats(a, q, n, gmean, grstd);
+    if (a.mean && chunk == 0 && q.part == 0)
+        for (int g = threadIdx.x; g < q.ng; g += kGnThreads) {
+            a.mean[(int64_t)n * h.groups + q.g0 + g] = gmean[g];
+            a.rstd[(int64_t)n * h.groups + q.g0 + g] = grstd[g];
+        }
+    if (!q.live) return;
+    float mean[V], scale[V], bias[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int g = q.ng == 1 ? 0 : (q.chan + k) / h.d;
+        mean[k] = gmean[g];
+        scale[k] = grstd[g] * gn_param(a.weight, a.wdtype, q.c0 + q.chan + k, 1.0f);
+        bias[k] = gn_param(a.bias, a.wdtype, q.c0 + q.chan + k, 0.0f);
+    }
+    const int64_t begin = chunk * h.apply_rows;
+    const int64_t end = begin + h.apply_rows < h.s ? begin + h.apply_rows : h.s;
+    const int64_t at = ((int64_t)n * h.s) * h.c + q.c0 + q.chan;
+    const T* x = (const T*)a.x + at;
+    T* y = (T*)a.out + at;
+    for (int64_t r = begin + q.row; r < end; r += q.passrows) {
+        float v[V];
+        gn_load<V>(x + r * h.c, v);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            v[k] = gn_act<ACT>(__builtin_fmaf(v[k] - mean[k], scale[k], bias[k]));
+        gn_store<V>(y + r * h.c, v);
+    }
+}
+
+// ---- backward
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(kGnThreads) void k_gn_bwd_sums(GnArgs a) {
+    __shared__ float buf[kGnThreads * V], chan_sums[2][kGnThreads * V], gsum[kGnThreads * V];
+    const GnShape& h = a.h;
+    const GnWhere at_block = gn_where(h, blockIdx.x, h.chunks);
+    const int n = at_block.n, chunk = at_block.chunk;
+    const GnPlace q = gn_place<V>(h, at_block.slice);
+    const int64_t begin = chunk * h.rows, end = begin + h.rows < h.s ? begin + h.rows : h.s;
+    const int64_t at = ((int64_t)n * h.s) * h.c + q.c0 + q.chan;
+    const T* x = (const T*)a.x + at;
+    const T* dy = (const T*)a.dy + at;
+    float mean[V], rstd[V], weight[V], bias[V], sa[V], sb[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        sa[k] = sb[k] = 0.0f;
+        if (q.live) {
+            const int64_t g = (int64_t)n * h.groups + (q.c0 + q.chan + k) / h.d;
+            mean[k] = a.mean[g];
+            rstd[k] = a.rstd[g];
+            weight[k] = gn_param(a.weight, a.wdtype, q.c0 + q.chan + k, 1.0f);
+            bias[k] = gn_param(a.bias, a.wdtype, q.c0 + q.chan + k, 0.0f);
+        }
+    }
+    if (q.live)
+        for (int64_t r = begin + q.row; r < end; r += q.passrows) {
+            float v[V], t[V];
+            gn_load<V>(x + r * h.c, v);
+            gn_load<V>(dy + r * h.c, t);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float xh = (v[k] - mean[k]) * rstd[k];
+                const float dz = t[k] * gn_slope<ACT>(__builtin_fmaf(xh, weight[k], bias[k]));
+                sa[k] += dz;
+                sb[k] = __builtin_fmaf(dz, xh, sb[k]);
+            }
+        }
+    for (int w = 0; w < 2; ++w) {
+        gn_rows_sum<V>(buf, q, w ? sb : sa);
+        for (int c = threadIdx.x; c < q.cs; c += kGnThreads) {
+            const float s = buf[c];
+            chan_sums[w][c] = s;
+            buf[c] = s * gn_param(a.weight, a.wdtype, q.c0 + c, 1.0f);
+        }
+        __syncthreads();
+        gn_groups_sum(buf, gsum, q, h.d);
+        for (int g = threadIdx.x; g < q.ng; g += kGnThreads)
+            a.partials[((((int64_t)n * h.chunks + chunk) * h.groups + q.g0 + g) * h.parts +
+                        q.part) * 2 + w] = gsum[g];
+    }
+    if (a.channels)
+        for (int c = threadIdx.x; c < q.cs; c += kGnThreads) {
+            float2* o = (float2*)a.channels + ((int64_t)n * h.chunks + chunk) * h.c + q.c0 + c;
+            *o = make_float2(chan_sums[0][c], chan_sums[1][c]);
+        }
+}
+
+// dw and db of 16 channels: 16 threads a channel over the samples' chunks.
+__device__ inline void gn_channel_grads(const GnArgs& a, int block) {
+    __shared__ double sums[2][16][17];
+    const GnShape& h = a.h;
+    const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, c = block * 16 + lane;
+    double sa = 0.0, sb = 0.0;
+    if (c < h.c)
+        for (int64_t i = row; i < (int64_t)a.n * h.chunks; i += 16) {
+            const float2 v = ((const float2*)a.channels)[i * h.c + c];
+            sa += v.x;
+            sb += v.y;
+        }
+    sums[0][row][lane] = sa;
+    sums[1][row][lane] = sb;
+    __syncthreads();
+    if (row < 2 && c < h.c) {
+        double s = 0.0;
+        for (int k = 0; k < 16; ++k) s += sums[row][k][lane];
+        void* to = row ? a.dweight : a.dbias;
+        if (to) gn_store_param(to, a.wdtype, c, (float)s);
+    }
+}
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(kGnThreads) void k_gn_bwd_apply(GnArgs a) {
+    __shared__ float g1[kGnThreads * V], g2[kGnThreads * V];
+    const GnShape& h = a.h;
+    if ((int)blockIdx.x < a.channel_blocks) {
+        gn_channel_grads(a, blockIdx.x);
+        return;
+    }
+    const GnWhere at_block = gn_where(h, blockIdx.x - a.channel_blocks, h.apply_chunks);
+    const int n = at_block.n, chunk = at_block.chunk;
+    const GnPlace q = gn_place<V>(h, at_block.slice);
+    {  // E[w dz] and E[w dz xh] of the slice's groups
+        const int t = gn_lanes(q.ng), lane = threadIdx.x & (t - 1), step = kGnThreads / t;
+        const int entries = h.chunks * h.parts;
+        const float inv = 1.0f / ((float)h.s * (float)h.d);
+        for (int base = 0; base < q.ng; base += step) {
+            const int g = base + threadIdx.x / t;
+            float sa = 0.0f, sb = 0.0f;
+            const float2* p = (const float2*)a.partials +
+                              ((int64_t)n * h.chunks * h.groups + q.g0 + g) * h.parts;
+            if (g < q.ng)
+                for (int i = lane; i < entries; i += t) {
+                    const int ch = i / h.parts, part = i - ch * h.parts;
+                    const float2 v = p[(int64_t)ch * h.groups * h.parts + part];
+                    sa += v.x;
+                    sb += v.y;
+                }
+            sa = gn_lanes_sum(sa, t);
+            sb = gn_lanes_sum(sb, t);
+            if (g < q.ng && lane == 0) {
+                g1[g] = sa * inv;
+                g2[g] = sb * inv;
+            }
+        }
+        __syncthreads();
+    }
+    if (!q.live) return;
+    float mean[V], rstd[V], weight[V], bias[V], e1[V], e2[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int gl = q.ng == 1 ? 0 : (q.chan + k) / h.d;
+        const int64_t g = (int64_t)n * h.groups + q.g0 + gl;
+        mean[k] = a.mean[g];
+        rstd[k] = a.rstd[g];
+        weight[k] = gn_param(a.weight, a.wdtype, q.c0 + q.chan + k, 1.0f);
+        bias[k] = gn_param(a.bias, a.wdtype, q.c0 + q.chan + k, 0.0f);
+        e1[k] = g1[gl];
+        e2[k] = g2[gl];
+    }
+    const int64_t begin = chunk * h.apply_rows;
+    const int64_t end = begin + h.apply_rows < h.s ? begin + h.apply_rows : h.s;
+    const int64_t at = ((int64_t)n * h.s) * h.c + q.c0 + q.chan;
+    const T* x = (const T*)a.x + at;
+    const T* dy = (const T*)a.dy + at;
+    T* dx = (T*)a.out + at;
+    for (int64_t r = begin + q.row; r < end; r += q.passrows) {
+        float v[V], t[V];
+        gn_load<V>(x + r * h.c, v);
+        gn_load<V>(dy + r * h.c, t);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float xh = (v[k] - mean[k]) * rstd[k];
+            const float dz = t[k] * gn_slope<ACT>(__builtin_fmaf(xh, weight[k], bias[k]));
+            v[k] = rstd[k] * (__builtin_fmaf(-xh, e2[k], weight[k] * dz) - e1[k]);
+        }
+        gn_store<V>(dx + r * h.c, v);
+    }
+}
+
+// ---- host
+
+static int gn_gcd(int a, int b) { return b ? gn_gcd(b, a % b) : a; }
+
+// How n samples of s rows and c channels are cut, with vectors of `vec` channels
+// (1 where no slice of whole groups and whole vectors fits 256 of them).
+static GnShape gn_shape(int64_t n, int64_t s, int32_t c, int32_t groups, int* vec) {
+    GnShape h;
+    h.s = s;
+    h.c = c;
+    h.groups = groups;
+    h.d = c / groups;
+    h.parts = 1;
+    int unit = *vec / gn_gcd(h.d, *vec);
+    if (unit > 1 && (int64_t)unit * h.d > (int64_t)kGnThreads * *vec) *vec = unit = 1;
+    const int most = kGnThreads * *vec;
+    if (h.d > most) {
+        h.gs = 1;
+        h.parts = (h.d + most - 1) / most;
+        h.cs = (h.d + h.parts - 1) / h.parts;
+        h.cs = (h.cs + *vec - 1) / *vec * *vec;
+        h.parts = (h.d + h.cs - 1) / h.cs;
+        h.slices = groups * h.parts;
+    } else {
+        h.gs = most / h.d / unit * unit;
+        if (h.gs > groups) h.gs = groups;
+        h.cs = h.gs * h.d;
+        h.slices = (groups + h.gs - 1) / h.gs;
+    }
+    const int64_t passrows = kGnThreads / (h.cs / *vec);
+    auto cut = [&](int64_t blocks, int64_t passes, int64_t* rows) {
+        int64_t chunks = (blocks + n * h.slices - 1) / (n * h.slices);
+        const int64_t most_chunks = (s + passrows * passes - 1) / (passrows * passes);
+        if (chunks > most_chunks) chunks = most_chunks;
+        *rows = (s + chunks - 1) / chunks;
+        return (int32_t)((s + *rows - 1) / *rows);
+    };
+    h.chunks = cut(1024, 4, &h.rows);
+    h.apply_chunks = cut(4096, 4, &h.apply_rows);
+    return h;
+}
+
+static int gn_widest(int dtype) { return dtype == kGnF32 ? 4 : kGnMaxVec; }
+
+static bool gn_valid(int64_t n, int64_t s, int32_t c, int32_t groups, int32_t dtype) {
+    return n > 0 && s > 0 && c > 0 && groups > 0 && c % groups == 0 && dtype >= kGnF32 &&
+           dtype <= kGnF16 && s <= ((int64_t)1 << 40) / c &&
+           n <= ((int64_t)1 << 44) / (s * c);
+}
+
+// A launch has fewer than 2^24 workgroups of 256 threads.
+static bool gn_fits(int64_t n, const GnShape& h) {
+    const int64_t chunks = h.chunks > h.apply_chunks ? h.chunks : h.apply_chunks;
+    return n <= ((int64_t)1 << 23) / (h.slices * chunks);
+}
+
+static bool gn_aligned(const void* p, int to) { return ((uintptr_t)p % to) == 0; }
+
+}  // namespace cs
+
+using namespace cs;
+
+extern "C" size_t cs_group_norm_workspace_elems(int64_t n, int64_t s, int32_t c, int32_t groups,
+                                                int32_t dtype, int32_t backward) {
+    if (!gn_valid(n, s, c, groups, dtype)) return 0;
+    size_t most = 0;
+    for (int vec : {gn_widest(dtype), 1}) {
+        if (c % vec) continue;
+        const GnShape h = gn_shape(n, s, c, groups, &vec);
+        size_t e = (size_t)n * h.chunks * groups * h.parts * 2;
+        if (backward) e += (size_t)n * h.chunks * c * 2;
+        most = e > most ? e : most;
+    }
+    return most;
+}
+
+namespace {
+
+template <typename T, int V>
+int gn_forward(const GnArgs& a, int act, hipStream_t stream) {
+    const GnShape& h = a.h;
+    const dim3 sums((unsigned)(a.n * h.slices * h.chunks));
+    const dim3 apply((unsigned)(a.n * h.slices * h.apply_chunks)), block(kGnThreads);
+    hipLaunchKernelGGL((k_gn_stats<T, V>), sums, block, 0, stream, a);
+    switch (act) {
+        case kActNone: hipLaunchKernelGGL((k_gn_apply<T, V, kActNone>), apply, block, 0, stream, a); break;
+        case kActRelu: hipLaunchKernelGGL((k_gn_apply<T, V, kActRelu>), apply, block, 0, stream, a); break;
+        case kActSilu: hipLaunchKernelGGL((k_gn_apply<T, V, kActSilu>), apply, block, 0, stream, a); break;
+        case kActGelu: hipLaunchKernelGGL((k_gn_apply<T, V, kActGelu>), apply, block, 0, stream, a); break;
+    }
+    return hipGetLastError() == hipSuccess ? CS_OK : CS_ERR_HIP;
+}
+
+template <typename T, int V, int ACT>
+int gn_backward_act(const GnArgs& a, hipStream_t stream) {
+    const GnShape& h = a.h;
+    const dim3 sums((unsigned)(a.n * h.slices * h.chunks)), block(kGnThreads);
+    hipLaunchKernelGGL((k_gn_bwd_sums<T, V, ACT>), sums, block, 0, stream, a);
+    const int64_t blocks =
+        a.channel_blocks + (a.out ? a.n * h.slices * h.apply_chunks : 0);
+    if (blocks > 0)
+        hipLaunchKernelGGL((k_gn_bwd_apply<T, V, ACT>), dim3((unsigned)blocks), block, 0, stream, a);
+    return hipGetLastError() == hipSuccess ? CS_OK : CS_ERR_HIP;
+}
+
+template <typename T, int V>
+int gn_backward(const GnArgs& a, int act, hipStream_t stream) {
+    switch (act) {
+        case kActNone: return gn_backward_act<T, V, kActNone>(a, stream);
+        case kActRelu: return gn_backward_act<T, V, kActRelu>(a, stream);
+        case kActSilu: return gn_backward_act<T, V, kActSilu>(a, stream);
+        default: return gn_backward_act<T, V, kActGelu>(a, stream);
+    }
+}
+
+}  // namespace
+
+extern "C" int cs_group_norm_forward(const void* x, int64_t n, int64_t s, int32_t c,
+                                     int32_t groups, int32_t dtype, const void* weight,
+                                     const void* bias, int32_t param_dtype, double eps,
+                                     int32_t act, float* workspace, float* mean, float* rstd,
+                                     void* y, hipStream_t stream) {
+    if (!gn_valid(n, s, c, groups, dtype) || param_dtype < kGnF32 || param_dtype > kGnF16 ||
+        act < kActNone || act > kActGelu || !(eps >= 0.0) || !x || !y || !workspace ||
+        !mean != !rstd)
+        return CS_ERR_ARGS;
+    int vec = gn_widest(dtype);
+    if (c % vec || !gn_aligned(x, 16) || !gn_aligned(y, 16)) vec = 1;
+    GnArgs a{};
+    a.h = gn_shape(n, s, c, groups, &vec);
+    if (!gn_fits(n, a.h)) return CS_ERR_ARGS;
+    a.x = x;
+    a.weight = weight;
+    a.bias = bias;
+    a.wdtype = param_dtype;
+    a.eps = (float)eps;
+    a.partials = workspace;
+    a.mean = mean;
+    a.rstd = rstd;
+    a.out = y;
+    a.n = (int32_t)n;
+    if (dtype == kGnF32)
+        return vec > 1 ? gn_forward<float, 4>(a, act, stream) : gn_forward<float, 1>(a, act, stream);
+    if (dtype == kGnBF16)
+        return vec > 1 ? gn_forward<__bf16, 8>(a, act, stream)
+                       : gn_forward<__bf16, 1>(a, act, stream);
+    return vec > 1 ? gn_forward<_Float16, 8>(a, act, stream)
+                   : gn_forward<_Float16, 1>(a, act, stream);
+}
+
+extern "C" int cs_group_norm_backward(const void* x, const void* dy, int64_t n, int64_t s,
+                                      int32_t c, int32_t groups, int32_t dtype,
+                                      const void* weight, const void* bias, int32_t param_dtype,
+                                      int32_t act, const float* mean, const float* rstd,
+                                      float* workspace, void* dx, void* dweight, void* dbias,
+                                      hipStream_t stream) {
+    if (!gn_valid(n, s, c, groups, dtype) || param_dtype < kGnF32 || param_dtype > kGnF16 ||
+        act < kActNone || act > kActGelu || !x || !dy || !mean || !rstd || !workspace ||
+        !gn_aligned(workspace, 8))
+        return CS_ERR_ARGS;
+    if (!dx && !dweight && !dbias) return CS_OK;
+    int vec = gn_widest(dtype);
+    if (c % vec || !gn_aligned(x, 16) || !gn_aligned(dy, 16) || (dx && !gn_aligned(dx, 16))) vec = 1;
+    GnArgs a{};
+    a.h = gn_shape(n, s, c, groups, &vec);
+    if (!gn_fits(n, a.h)) return CS_ERR_ARGS;
+    a.x = x;
+    a.dy = dy;
+    a.weight = weight;
+    a.bias = bias;
+    a.wdtype = param_dtype;
+    a.partials = workspace;
+    a.mean = const_cast<float*>(mean);
+    a.rstd = const_cast<float*>(rstd);
+    a.out = dx;
+    a.dweight = dweight;
+    a.dbias = dbias;
+    a.n = (int32_t)n;
+    if (dweight || dbias) {
+        a.channels = workspace + (size_t)n * a.h.chunks * groups * a.h.parts * 2;
+        a.channel_blocks = (c + 15) / 16;
+    }
+    if (dtype == kGnF32)
+        return vec > 1 ? gn_backward<float, 4>(a, act, stream)
+                       : gn_backward<float, 1>(a, act, stream);
+    if (dtype == kGnBF16)
+        return vec > 1 ? gn_backward<__bf16, 8>(a, act, stream)
+                       : gn_backward<__bf16, 1>(a, act, stream);
+    return vec > 1 ? gn_backward<_Float16, 8>(a, act, stream)
+                   : gn_backward<_Float16, 1>(a, act, stream);
+}
