@@ -61,32 +61,86 @@ struct GnArgs {
     void* dweight;
     void* dbias;
     int32_t n;
-    int32_t channel_blocks;  // of the backward's second launch, for dw and db
+    int32_t channel_blocks;  // of the backward's second (or third) launch, for dw and db
+    int32_t joined;          // a launch in between has joined the sums
+    float* groups_out;       // backward, joined: [n][group] E[w dz], E[w dz xh]
+    int32_t past_in, past_out;  // whether the second launch reads and stores past the caches
 };
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) GnVec { T v[V]; };
 
 template <int V, typename T>
+__device__ inline GnVec<T, V> gn_raw(const T* p) {
+    return *reinterpret_cast<const GnVec<T, V>*>(p);
+}
+
+// The same past the caches, for what is not read again.
+typedef float GnFour __attribute__((ext_vector_type(4)));
+
+template <int V, typename T>
+__device__ inline GnVec<T, V> gn_raw(const T* p, bool past) {
+    if constexpr (sizeof(GnVec<T, V>) == sizeof(GnFour)) {
+        if (past) {
+            const GnFour v = __builtin_nontemporal_load(reinterpret_cast<const GnFour*>(p));
+            return __builtin_bit_cast(GnVec<T, V>, v);
+        }
+    }
+    return gn_raw<V>(p);
+}
+
+template <int V, typename T>
 __device__ inline void gn_load(const T* p, float (&out)[V]) {
-    const GnVec<T, V> x = *reinterpret_cast<const GnVec<T, V>*>(p);
+    const GnVec<T, V> x = gn_raw<V>(p);
 #pragma unroll
     for (int k = 0; k < V; ++k) out[k] = (float)x.v[k];
 }
 
 template <int V, typename T>
-__device__ inline void gn_store(T* p, const float (&in)[V]) {
+__device__ inline void gn_store(T* p, const float (&in)[V], bool past) {
     GnVec<T, V> x;
 #pragma unroll
     for (int k = 0; k < V; ++k) x.v[k] = (T)in[k];
+    if constexpr (sizeof(x) == sizeof(GnFour)) {
+        if (past) {
+            __builtin_nontemporal_store(__builtin_bit_cast(GnFour, x),
+                                        reinterpret_cast<GnFour*>(p));
+            return;
+        }
+    }
     *reinterpret_cast<GnVec<T, V>*>(p) = x;
 }
 
-__device__ inline float gn_param(const void* p, int dtype, int c, float none) {
-    if (!p) return none;
-    if (dtype == kGnF32) return ((const float*)p)[c];
-    if (dtype == kGnBF16) return (float)((const __bf16*)p)[c];
-    return (float)((const _Float16*)p)[c];
+// V parameters from channel c on (none: the value where there are none).  The type
+// is asked for once, so that the loads go out together.
+template <int V>
+__device__ inline void gn_params(const void* p, int dtype, int c, float none, float (&out)[V]) {
+    if (!p) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) out[k] = none;
+    } else if (dtype == kGnF32) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) out[k] = ((const float*)p)[c + k];
+    } else if (dtype == kGnBF16) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) out[k] = (float)((const __bf16*)p)[c + k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) out[k] = (float)((const _Float16*)p)[c + k];
+    }
+}
+
+// The groups of V consecutive channels, relative to the slice's first.
+template <int V>
+__device__ inline void gn_group_of(int chan, int d, int (&g)[V]) {
+    int at = chan / d, left = d - (chan - at * d);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        g[k] = at;
+        --left;
+        at += left == 0;
+        left = left == 0 ? d : left;
+    }
 }
 
 __device__ inline void gn_store_param(void* p, int dtype, int c, float v) {
@@ -112,7 +166,7 @@ __device__ inline float gn_slope(float z) {
     if (ACT == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
     if (ACT == kActSilu) {
         const float p = gn_sigmoid(z);
-        return p * __builtin_fmaf(z, 1.0f - p, 1.0f);
+        return __builtin_fmaf(p, __builtin_fmaf(-z, p, z), p);
     }
     if (ACT == kActGelu) {
         const float p = 0.5f * (1.0f + erff(z * 0.70710678f));
@@ -148,6 +202,21 @@ __device__ inline GnPlace gn_place(const GnShape& h, int slice) {
     return q;
 }
 
+// A thread's rows from r on, a pass apart: f(A, offset) takes A of them at once
+// (`stride` elements apart), so that their loads are in flight together.
+constexpr int kGnAhead = 4;
+
+template <int N> struct GnInt { static constexpr int value = N; };
+
+template <int A, typename F>
+__device__ inline void gn_rows(int64_t r, int64_t end, int passrows, int64_t stride, int c,
+                               F&& f) {
+    int64_t at = r * c;
+    int left = r < end ? (int)((end - r + passrows - 1) / passrows) : 0;
+    for (; left >= A; left -= A, at += A * stride) f(GnInt<A>(), at);
+    for (; left > 0; --left, at += stride) f(GnInt<1>(), at);
+}
+
 struct GnWhere { int n, chunk, slice; };
 
 __device__ inline GnWhere gn_where(const GnShape& h, uint32_t block, int chunks) {
@@ -169,13 +238,17 @@ __device__ inline void gn_rows_sum(float* buf, const GnPlace& q, const float (&v
 #pragma unroll
         for (int k = 0; k < V; ++k) buf[q.row * q.cs + q.chan + k] = v[k];
     }
-    int n = q.passrows;
-    while (n > 1) {
-        const int half = (n + 1) >> 1;
+    // Eight rows to one a step: a barrier costs more than the additions.
+    int n = q.passrows * q.cs;
+    while (n > q.cs) {
+        const int m = (n / q.cs + 7) / 8 * q.cs;
         __syncthreads();
-        for (int i = threadIdx.x; i < (n - half) * q.cs; i += kGnThreads)
-            buf[i] += buf[i + half * q.cs];
-        n = half;
+        for (int i = threadIdx.x; i < m; i += blockDim.x) {
+            float s = buf[i];
+            for (int j = i + m; j < n; j += m) s += buf[j];
+            buf[i] = s;
+        }
+        n = m;
     }
     __syncthreads();
 }
@@ -219,22 +292,27 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_stats(GnArgs a) {
     const GnPlace q = gn_place<V>(h, at_block.slice);
     const int64_t begin = chunk * h.rows, end = begin + h.rows < h.s ? begin + h.rows : h.s;
     const T* x = (const T*)a.x + ((int64_t)n * h.s) * h.c + q.c0 + q.chan;
+    const int64_t stride = (int64_t)q.passrows * h.c;
     float k0[V], s1[V], s2[V], cnt = 0.0f;
 #pragma unroll
     for (int k = 0; k < V; ++k) k0[k] = s1[k] = s2[k] = 0.0f;
     if (q.live && begin + q.row < end) {
         gn_load<V>(x + (begin + q.row) * h.c, k0);
-        for (int64_t r = begin + q.row; r < end; r += q.passrows) {
-            float v[V];
-            gn_load<V>(x + r * h.c, v);
+        gn_rows<kGnAhead>(begin + q.row, end, q.passrows, stride, h.c, [&](auto ahead, int64_t r) {
+            constexpr int A = decltype(ahead)::value;
+            GnVec<T, V> v[A];
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float e = v[k] - k0[k];
-                s1[k] += e;
-                s2[k] = __builtin_fmaf(e, e, s2[k]);
-            }
-            cnt += 1.0f;
-        }
+            for (int u = 0; u < A; ++u) v[u] = gn_raw<V>(x + r + u * stride);
+#pragma unroll
+            for (int u = 0; u < A; ++u)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float e = (float)v[u].v[k] - k0[k];
+                    s1[k] += e;
+                    s2[k] = __builtin_fmaf(e, e, s2[k]);
+                }
+            cnt += (float)A;
+        });
     }
     // The thread's mean and squared deviations per channel.
     float mean[V], m2[V], w[V];
@@ -253,9 +331,11 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_stats(GnArgs a) {
     for (int g = threadIdx.x; g < q.ng; g += kGnThreads) gmean[g] = gsum[g] / total;
     __syncthreads();
     if (q.live) {
+        int group[V];
+        gn_group_of<V>(q.ng == 1 ? 0 : q.chan, q.ng == 1 ? V + 1 : h.d, group);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const float e = mean[k] - gmean[q.ng == 1 ? 0 : (q.chan + k) / h.d];
+            const float e = mean[k] - gmean[group[k]];
             w[k] = __builtin_fmaf(cnt * e, e, m2[k]);
         }
     }
@@ -314,6 +394,29 @@ __device__ inline void gn_join_stats(const GnArgs& a, const GnPlace& q, int n, f
     __syncthreads();
 }
 
+// The joining as a launch of its own: four groups a workgroup, a wave each.
+constexpr int kGnJoin = kGnThreads / 64;
+
+__device__ inline GnPlace gn_join_place(const GnShape& h, uint32_t block, int* n) {
+    const uint32_t per = (h.groups + kGnJoin - 1) / kGnJoin;
+    GnPlace q;
+    *n = block / per;
+    q.g0 = (block - *n * per) * kGnJoin;
+    q.ng = h.groups - q.g0 < kGnJoin ? h.groups - q.g0 : kGnJoin;
+    return q;
+}
+
+__global__ __launch_bounds__(kGnThreads) void k_gn_join_stats(GnArgs a) {
+    __shared__ float gmean[kGnThreads], grstd[kGnThreads];
+    int n;
+    const GnPlace q = gn_join_place(a.h, blockIdx.x, &n);
+    gn_join_stats(a, q, n, gmean, grstd);
+    for (int g = threadIdx.x; g < q.ng; g += kGnThreads) {
+        a.mean[(int64_t)n * a.h.groups + q.g0 + g] = gmean[g];
+        a.rstd[(int64_t)n * a.h.groups + q.g0 + g] = grstd[g];
+    }
+}
+
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kGnThreads) void k_gn_apply(GnArgs a) {
     __shared__ float gmean[kGnThreads * V], grstd[kGnThreads * V];
@@ -321,34 +424,55 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_apply(GnArgs a) {
     const GnWhere w = gn_where(h, blockIdx.x, h.apply_chunks);
     const int n = w.n, chunk = w.chunk;
     const GnPlace q = gn_place<V>(h, w.slice);
-    gn_join_stats(a, q, n, gmean, grstd);
-    if (a.mean && chunk == 0 && q.part == 0)
+    float scale[V], bias[V];
+    if (q.live) {
+        gn_params<V>(a.weight, a.wdtype, q.c0 + q.chan, 1.0f, scale);
+        gn_params<V>(a.bias, a.wdtype, q.c0 + q.chan, 0.0f, bias);
+    }
+    if (a.joined) {
+        for (int g = threadIdx.x; g < q.ng; g += kGnThreads) {
+            gmean[g] = a.mean[(int64_t)n * h.groups + q.g0 + g];
+            grstd[g] = a.rstd[(int64_t)n * h.groups + q.g0 + g];
+        }
+        __syncthreads();
+    } else {
+        gn_join_stats(a, q, n, gmean, grstd);
+    }
+    if (a.mean && !a.joined && chunk == 0 && q.part == 0)
         for (int g = threadIdx.x; g < q.ng; g += kGnThreads) {
             a.mean[(int64_t)n * h.groups + q.g0 + g] = gmean[g];
             a.rstd[(int64_t)n * h.groups + q.g0 + g] = grstd[g];
         }
     if (!q.live) return;
-    float mean[V], scale[V], bias[V];
+    float mean[V];
+    int group[V];
+    gn_group_of<V>(q.ng == 1 ? 0 : q.chan, q.ng == 1 ? V + 1 : h.d, group);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        const int g = q.ng == 1 ? 0 : (q.chan + k) / h.d;
-        mean[k] = gmean[g];
-        scale[k] = grstd[g] * gn_param(a.weight, a.wdtype, q.c0 + q.chan + k, 1.0f);
-        bias[k] = gn_param(a.bias, a.wdtype, q.c0 + q.chan + k, 0.0f);
+        mean[k] = gmean[group[k]];
+        scale[k] *= grstd[group[k]];
     }
     const int64_t begin = chunk * h.apply_rows;
     const int64_t end = begin + h.apply_rows < h.s ? begin + h.apply_rows : h.s;
     const int64_t at = ((int64_t)n * h.s) * h.c + q.c0 + q.chan;
+    const int64_t stride = (int64_t)q.passrows * h.c;
     const T* x = (const T*)a.x + at;
     T* y = (T*)a.out + at;
-    for (int64_t r = begin + q.row; r < end; r += q.passrows) {
-        float v[V];
-        gn_load<V>(x + r * h.c, v);
+    gn_rows<kGnAhead>(begin + q.row, end, q.passrows, stride, h.c, [&](auto ahead, int64_t r) {
+        constexpr int A = decltype(ahead)::value;
+        GnVec<T, V> raw[A];
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-            v[k] = gn_act<ACT>(__builtin_fmaf(v[k] - mean[k], scale[k], bias[k]));
-        gn_store<V>(y + r * h.c, v);
-    }
+        for (int u = 0; u < A; ++u) raw[u] = gn_raw<V>(x + r + u * stride, a.past_in);
+#pragma unroll
+        for (int u = 0; u < A; ++u) {
+            float v[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                v[k] = gn_act<ACT>(
+                    __builtin_fmaf((float)raw[u].v[k] - mean[k], scale[k], bias[k]));
+            gn_store<V>(y + r + u * stride, v, a.past_out);
+        }
+    });
 }
 
 // ---- backward
@@ -362,39 +486,56 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_sums(GnArgs a) {
     const GnPlace q = gn_place<V>(h, at_block.slice);
     const int64_t begin = chunk * h.rows, end = begin + h.rows < h.s ? begin + h.rows : h.s;
     const int64_t at = ((int64_t)n * h.s) * h.c + q.c0 + q.chan;
+    const int64_t stride = (int64_t)q.passrows * h.c;
     const T* x = (const T*)a.x + at;
     const T* dy = (const T*)a.dy + at;
-    float mean[V], rstd[V], weight[V], bias[V], sa[V], sb[V];
+    // The sums are of dz and dz (x - mean); 1 / deviation is a factor of the latter.
+    float mean[V], rstd[V], scale[V], bias[V], sa[V], sb[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        sa[k] = sb[k] = 0.0f;
-        if (q.live) {
-            const int64_t g = (int64_t)n * h.groups + (q.c0 + q.chan + k) / h.d;
-            mean[k] = a.mean[g];
-            rstd[k] = a.rstd[g];
-            weight[k] = gn_param(a.weight, a.wdtype, q.c0 + q.chan + k, 1.0f);
-            bias[k] = gn_param(a.bias, a.wdtype, q.c0 + q.chan + k, 0.0f);
+    for (int k = 0; k < V; ++k) sa[k] = sb[k] = rstd[k] = 0.0f;
+    if (q.live) {
+        gn_params<V>(a.weight, a.wdtype, q.c0 + q.chan, 1.0f, scale);
+        gn_params<V>(a.bias, a.wdtype, q.c0 + q.chan, 0.0f, bias);
+        int group[V];
+        gn_group_of<V>(q.ng == 1 ? 0 : q.chan, q.ng == 1 ? V + 1 : h.d, group);
+        const int64_t g0 = (int64_t)n * h.groups + q.g0;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            mean[k] = a.mean[g0 + group[k]];
+            rstd[k] = a.rstd[g0 + group[k]];
         }
+#pragma unroll
+        for (int k = 0; k < V; ++k) scale[k] *= rstd[k];
     }
     if (q.live)
-        for (int64_t r = begin + q.row; r < end; r += q.passrows) {
-            float v[V], t[V];
-            gn_load<V>(x + r * h.c, v);
-            gn_load<V>(dy + r * h.c, t);
+        gn_rows<kGnAhead>(begin + q.row, end, q.passrows, stride, h.c, [&](auto ahead, int64_t r) {
+            constexpr int A = decltype(ahead)::value;
+            GnVec<T, V> v[A], t[A];
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float xh = (v[k] - mean[k]) * rstd[k];
-                const float dz = t[k] * gn_slope<ACT>(__builtin_fmaf(xh, weight[k], bias[k]));
-                sa[k] += dz;
-                sb[k] = __builtin_fmaf(dz, xh, sb[k]);
+            for (int u = 0; u < A; ++u) {
+                v[u] = gn_raw<V>(x + r + u * stride);
+                t[u] = gn_raw<V>(dy + r + u * stride);
             }
-        }
+#pragma unroll
+            for (int u = 0; u < A; ++u)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float e = (float)v[u].v[k] - mean[k];
+                    const float dz =
+                        (float)t[u].v[k] * gn_slope<ACT>(__builtin_fmaf(e, scale[k], bias[k]));
+                    sa[k] += dz;
+                    sb[k] = __builtin_fmaf(dz, e, sb[k]);
+                }
+        });
+#pragma unroll
+    for (int k = 0; k < V; ++k) sb[k] *= rstd[k];
     for (int w = 0; w < 2; ++w) {
         gn_rows_sum<V>(buf, q, w ? sb : sa);
         for (int c = threadIdx.x; c < q.cs; c += kGnThreads) {
-            const float s = buf[c];
+            float s = buf[c], weight[1];
+            gn_params<1>(a.weight, a.wdtype, q.c0 + c, 1.0f, weight);
             chan_sums[w][c] = s;
-            buf[c] = s * gn_param(a.weight, a.wdtype, q.c0 + c, 1.0f);
+            buf[c] = s * weight[0];
         }
         __syncthreads();
         gn_groups_sum(buf, gsum, q, h.d);
@@ -409,27 +550,86 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_sums(GnArgs a) {
         }
 }
 
-// dw and db of 16 channels: 16 threads a channel over the samples' chunks.
+// dw and db of kGnChans channels: 32 threads a channel over the samples' chunks,
+// eight loads in flight each.
+constexpr int kGnChans = kGnThreads / 32;
+
 __device__ inline void gn_channel_grads(const GnArgs& a, int block) {
-    __shared__ double sums[2][16][17];
+    __shared__ double sums[2][32][kGnChans + 1];
     const GnShape& h = a.h;
-    const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, c = block * 16 + lane;
+    const int lane = threadIdx.x % kGnChans, row = threadIdx.x / kGnChans;
+    const int c = block * kGnChans + lane, entries = a.n * h.chunks;
     double sa = 0.0, sb = 0.0;
-    if (c < h.c)
-        for (int64_t i = row; i < (int64_t)a.n * h.chunks; i += 16) {
-            const float2 v = ((const float2*)a.channels)[i * h.c + c];
+    if (c < h.c) {
+        const float2* p = (const float2*)a.channels + c;
+        int i = row;
+        for (; i + 7 * 32 < entries; i += 8 * 32) {
+            float2 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = p[(int64_t)(i + k * 32) * h.c];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                sa += v[k].x;
+                sb += v[k].y;
+            }
+        }
+        for (; i < entries; i += 32) {
+            const float2 v = p[(int64_t)i * h.c];
             sa += v.x;
             sb += v.y;
         }
+    }
     sums[0][row][lane] = sa;
     sums[1][row][lane] = sb;
     __syncthreads();
     if (row < 2 && c < h.c) {
         double s = 0.0;
-        for (int k = 0; k < 16; ++k) s += sums[row][k][lane];
+        for (int k = 0; k < 32; ++k) s += sums[row][k][lane];
         void* to = row ? a.dweight : a.dbias;
         if (to) gn_store_param(to, a.wdtype, c, (float)s);
     }
+}
+
+// E[w dz] and E[w dz xh] of a slice's groups.
+__device__ inline void gn_join_sums(const GnArgs& a, const GnPlace& q, int n, float* g1,
+                                    float* g2) {
+    const GnShape& h = a.h;
+    const int t = gn_lanes(q.ng), lane = threadIdx.x & (t - 1), step = kGnThreads / t;
+    const int entries = h.chunks * h.parts;
+    const float inv = 1.0f / ((float)h.s * (float)h.d);
+    for (int base = 0; base < q.ng; base += step) {
+        const int g = base + threadIdx.x / t;
+        float sa = 0.0f, sb = 0.0f;
+        const float2* p = (const float2*)a.partials +
+                          ((int64_t)n * h.chunks * h.groups + q.g0 + g) * h.parts;
+        if (g < q.ng)
+            for (int i = lane; i < entries; i += t) {
+                const int ch = i / h.parts, part = i - ch * h.parts;
+                const float2 v = p[(int64_t)ch * h.groups * h.parts + part];
+                sa += v.x;
+                sb += v.y;
+            }
+        sa = gn_lanes_sum(sa, t);
+        sb = gn_lanes_sum(sb, t);
+        if (g < q.ng && lane == 0) {
+            g1[g] = sa * inv;
+            g2[g] = sb * inv;
+        }
+    }
+    __syncthreads();
+}
+
+__global__ __launch_bounds__(kGnThreads) void k_gn_join_sums(GnArgs a) {
+    __shared__ float g1[kGnThreads], g2[kGnThreads];
+    if ((int)blockIdx.x < a.channel_blocks) {
+        gn_channel_grads(a, blockIdx.x);
+        return;
+    }
+    int n;
+    const GnPlace q = gn_join_place(a.h, blockIdx.x - a.channel_blocks, &n);
+    gn_join_sums(a, q, n, g1, g2);
+    for (int g = threadIdx.x; g < q.ng; g += kGnThreads)
+        ((float2*)a.groups_out)[(int64_t)n * a.h.groups + q.g0 + g] = make_float2(g1[g], g2[g]);
 }
 
 template <typename T, int V, int ACT>
@@ -443,62 +643,63 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_apply(GnArgs a) {
     const GnWhere at_block = gn_where(h, blockIdx.x - a.channel_blocks, h.apply_chunks);
     const int n = at_block.n, chunk = at_block.chunk;
     const GnPlace q = gn_place<V>(h, at_block.slice);
-    {  // E[w dz] and E[w dz xh] of the slice's groups
-        const int t = gn_lanes(q.ng), lane = threadIdx.x & (t - 1), step = kGnThreads / t;
-        const int entries = h.chunks * h.parts;
-        const float inv = 1.0f / ((float)h.s * (float)h.d);
-        for (int base = 0; base < q.ng; base += step) {
-            const int g = base + threadIdx.x / t;
-            float sa = 0.0f, sb = 0.0f;
-            const float2* p = (const float2*)a.partials +
-                              ((int64_t)n * h.chunks * h.groups + q.g0 + g) * h.parts;
-            if (g < q.ng)
-                for (int i = lane; i < entries; i += t) {
-                    const int ch = i / h.parts, part = i - ch * h.parts;
-                    const float2 v = p[(int64_t)ch * h.groups * h.parts + part];
-                    sa += v.x;
-                    sb += v.y;
-                }
-            sa = gn_lanes_sum(sa, t);
-            sb = gn_lanes_sum(sb, t);
-            if (g < q.ng && lane == 0) {
-                g1[g] = sa * inv;
-                g2[g] = sb * inv;
-            }
+    if (a.joined) {
+        for (int g = threadIdx.x; g < q.ng; g += kGnThreads) {
+            const float2 v = ((const float2*)a.groups_out)[(int64_t)n * h.groups + q.g0 + g];
+            g1[g] = v.x;
+            g2[g] = v.y;
         }
         __syncthreads();
+    } else {
+        gn_join_sums(a, q, n, g1, g2);
     }
     if (!q.live) return;
-    float mean[V], rstd[V], weight[V], bias[V], e1[V], e2[V];
+    // dx = (r w) dz - r E[w dz] - (x - mean) r^2 E[w dz xh]
+    float mean[V], rstd[V], scale[V], bias[V], e1[V], e2[V];
+    gn_params<V>(a.weight, a.wdtype, q.c0 + q.chan, 1.0f, scale);
+    gn_params<V>(a.bias, a.wdtype, q.c0 + q.chan, 0.0f, bias);
+    int group[V];
+    gn_group_of<V>(q.ng == 1 ? 0 : q.chan, q.ng == 1 ? V + 1 : h.d, group);
+    const int64_t g0 = (int64_t)n * h.groups + q.g0;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        const int gl = q.ng == 1 ? 0 : (q.chan + k) / h.d;
-        const int64_t g = (int64_t)n * h.groups + q.g0 + gl;
-        mean[k] = a.mean[g];
-        rstd[k] = a.rstd[g];
-        weight[k] = gn_param(a.weight, a.wdtype, q.c0 + q.chan + k, 1.0f);
-        bias[k] = gn_param(a.bias, a.wdtype, q.c0 + q.chan + k, 0.0f);
-        e1[k] = g1[gl];
-        e2[k] = g2[gl];
+        mean[k] = a.mean[g0 + group[k]];
+        rstd[k] = a.rstd[g0 + group[k]];
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        scale[k] *= rstd[k];
+        e1[k] = -rstd[k] * g1[group[k]];
+        e2[k] = -rstd[k] * (rstd[k] * g2[group[k]]);
     }
     const int64_t begin = chunk * h.apply_rows;
     const int64_t end = begin + h.apply_rows < h.s ? begin + h.apply_rows : h.s;
     const int64_t at = ((int64_t)n * h.s) * h.c + q.c0 + q.chan;
+    const int64_t stride = (int64_t)q.passrows * h.c;
     const T* x = (const T*)a.x + at;
     const T* dy = (const T*)a.dy + at;
     T* dx = (T*)a.out + at;
-    for (int64_t r = begin + q.row; r < end; r += q.passrows) {
-        float v[V], t[V];
-        gn_load<V>(x + r * h.c, v);
-        gn_load<V>(dy + r * h.c, t);
+    gn_rows<kGnAhead>(begin + q.row, end, q.passrows, stride, h.c, [&](auto ahead, int64_t r) {
+        constexpr int A = decltype(ahead)::value;
+        GnVec<T, V> v[A], t[A];
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float xh = (v[k] - mean[k]) * rstd[k];
-            const float dz = t[k] * gn_slope<ACT>(__builtin_fmaf(xh, weight[k], bias[k]));
-            v[k] = rstd[k] * (__builtin_fmaf(-xh, e2[k], weight[k] * dz) - e1[k]);
+        for (int u = 0; u < A; ++u) {
+            v[u] = gn_raw<V>(x + r + u * stride, a.past_in);
+            t[u] = gn_raw<V>(dy + r + u * stride, a.past_in);
         }
-        gn_store<V>(dx + r * h.c, v);
-    }
+#pragma unroll
+        for (int u = 0; u < A; ++u) {
+            float o[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float e = (float)v[u].v[k] - mean[k];
+                const float dz =
+                    (float)t[u].v[k] * gn_slope<ACT>(__builtin_fmaf(e, scale[k], bias[k]));
+                o[k] = __builtin_fmaf(dz, scale[k], __builtin_fmaf(e, e2[k], e1[k]));
+            }
+            gn_store<V>(dx + r + u * stride, o, a.past_out);
+        }
+    });
 }
 
 // ---- host
@@ -532,15 +733,31 @@ static GnShape gn_shape(int64_t n, int64_t s, int32_t c, int32_t groups, int* ve
     }
     const int64_t passrows = kGnThreads / (h.cs / *vec);
     auto cut = [&](int64_t blocks, int64_t passes, int64_t* rows) {
-        int64_t chunks = (blocks + n * h.slices - 1) / (n * h.slices);
+        int64_t chunks = blocks / (n * h.slices);
+        if (chunks < 1) chunks = 1;
         const int64_t most_chunks = (s + passrows * passes - 1) / (passrows * passes);
         if (chunks > most_chunks) chunks = most_chunks;
         *rows = (s + chunks - 1) / chunks;
         return (int32_t)((s + *rows - 1) / *rows);
     };
-    h.chunks = cut(1024, 4, &h.rows);
+    // Summing: three workgroups a CU, all resident at once (one more than fit
+    // would run by itself; 24x24576x128 bf16 backward: 1032 of them 151 us, 768 of
+    // them 135).  Applying: as many as keep every CU busy to the end.
+    h.chunks = cut(768, 4, &h.rows);
     h.apply_chunks = cut(4096, 4, &h.apply_rows);
     return h;
+}
+
+// Whether the sums are joined by a launch of their own: where a workgroup of the
+// second launch would read more of them than this.
+constexpr int64_t kGnInline = 1024;
+
+static bool gn_joined(const GnShape& h) {
+    return (int64_t)h.chunks * h.parts * h.gs > kGnInline;
+}
+
+static uint32_t gn_join_blocks(const GnArgs& a) {
+    return (uint32_t)a.n * ((a.h.groups + kGnJoin - 1) / kGnJoin);
 }
 
 static int gn_widest(int dtype) { return dtype == kGnF32 ? 4 : kGnMaxVec; }
@@ -557,6 +774,16 @@ static bool gn_fits(int64_t n, const GnShape& h) {
     return n <= ((int64_t)1 << 23) / (h.slices * chunks);
 }
 
+// Stores go past the caches where the tensor is larger than the L2s together, the
+// second reading of the inputs where they are too large to have stayed in the
+// memory-side cache (bf16, 128 channels, forward/backward in us, plain and so:
+// 48 MB 37.0/62.5 and 35.7/54.4 with stores, 144 MB 101/162 and 81/134 with both;
+// 96 MB forward 58.0 with stores, 58.9 with both, backward 105 and 96).
+static void gn_past(GnArgs& a, int64_t bytes, bool backward) {
+    a.past_out = bytes > (int64_t)32 << 20;
+    a.past_in = bytes > (int64_t)(backward ? 64 : 128) << 20;
+}
+
 static bool gn_aligned(const void* p, int to) { return ((uintptr_t)p % to) == 0; }
 
 }  // namespace cs
@@ -571,6 +798,7 @@ extern "C" size_t cs_group_norm_workspace_elems(int64_t n, int64_t s, int32_t c,
         if (c % vec) continue;
         const GnShape h = gn_shape(n, s, c, groups, &vec);
         size_t e = (size_t)n * h.chunks * groups * h.parts * 2;
+        if (gn_joined(h)) e += (size_t)n * groups * 2;
         if (backward) e += (size_t)n * h.chunks * c * 2;
         most = e > most ? e : most;
     }
@@ -585,6 +813,8 @@ int gn_forward(const GnArgs& a, int act, hipStream_t stream) {
     const dim3 sums((unsigned)(a.n * h.slices * h.chunks));
     const dim3 apply((unsigned)(a.n * h.slices * h.apply_chunks)), block(kGnThreads);
     hipLaunchKernelGGL((k_gn_stats<T, V>), sums, block, 0, stream, a);
+    if (a.joined)
+        hipLaunchKernelGGL(k_gn_join_stats, dim3(gn_join_blocks(a)), block, 0, stream, a);
     switch (act) {
         case kActNone: hipLaunchKernelGGL((k_gn_apply<T, V, kActNone>), apply, block, 0, stream, a); break;
         case kActRelu: hipLaunchKernelGGL((k_gn_apply<T, V, kActRelu>), apply, block, 0, stream, a); break;
@@ -595,10 +825,16 @@ int gn_forward(const GnArgs& a, int act, hipStream_t stream) {
 }
 
 template <typename T, int V, int ACT>
-int gn_backward_act(const GnArgs& a, hipStream_t stream) {
+int gn_backward_act(GnArgs a, hipStream_t stream) {
     const GnShape& h = a.h;
     const dim3 sums((unsigned)(a.n * h.slices * h.chunks)), block(kGnThreads);
     hipLaunchKernelGGL((k_gn_bwd_sums<T, V, ACT>), sums, block, 0, stream, a);
+    if (a.joined) {
+        hipLaunchKernelGGL(k_gn_join_sums,
+                           dim3(a.channel_blocks + (a.out ? gn_join_blocks(a) : 0)), block, 0,
+                           stream, a);
+        a.channel_blocks = 0;
+    }
     const int64_t blocks =
         a.channel_blocks + (a.out ? a.n * h.slices * h.apply_chunks : 0);
     if (blocks > 0)
@@ -642,6 +878,12 @@ extern "C" int cs_group_norm_forward(const void* x, int64_t n, int64_t s, int32_
     a.rstd = rstd;
     a.out = y;
     a.n = (int32_t)n;
+    gn_past(a, n * s * c * (dtype == kGnF32 ? 4 : 2), false);
+    a.joined = gn_joined(a.h);
+    if (a.joined && !mean) {
+        a.mean = workspace + (size_t)n * a.h.chunks * groups * a.h.parts * 2;
+        a.rstd = a.mean + (size_t)n * groups;
+    }
     if (dtype == kGnF32)
         return vec > 1 ? gn_forward<float, 4>(a, act, stream) : gn_forward<float, 1>(a, act, stream);
     if (dtype == kGnBF16)
@@ -679,9 +921,16 @@ extern "C" int cs_group_norm_backward(const void* x, const void* dy, int64_t n, 
     a.dweight = dweight;
     a.dbias = dbias;
     a.n = (int32_t)n;
+    gn_past(a, n * s * c * (dtype == kGnF32 ? 4 : 2), true);
+    a.joined = gn_joined(a.h);
+    float* rest = workspace + (size_t)n * a.h.chunks * groups * a.h.parts * 2;
+    if (a.joined) {
+        a.groups_out = rest;
+        rest += (size_t)n * groups * 2;
+    }
     if (dweight || dbias) {
-        a.channels = workspace + (size_t)n * a.h.chunks * groups * a.h.parts * 2;
-        a.channel_blocks = (c + 15) / 16;
+        a.channels = rest;
+        a.channel_blocks = (c + kGnChans - 1) / kGnChans;
     }
     if (dtype == kGnF32)
         return vec > 1 ? gn_backward<float, 4>(a, act, stream)
