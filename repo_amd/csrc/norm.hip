@@ -64,7 +64,7 @@ struct GnArgs {
     int32_t channel_blocks;  // of the backward's second (or third) launch, for dw and db
     int32_t joined;          // a launch in between has joined the sums
     float* groups_out;       // backward, joined: [n][group] E[w dz], E[w dz xh]
-    int32_t past_in, past_out;  // whether the second launch reads and stores past the caches
+    int32_t past;            // 1: the second launch stores past the caches, 2: it reads so too
 };
 
 template <typename T, int V>
@@ -78,15 +78,14 @@ __device__ inline GnVec<T, V> gn_raw(const T* p) {
 // The same past the caches, for what is not read again.
 typedef float GnFour __attribute__((ext_vector_type(4)));
 
-template <int V, typename T>
-__device__ inline GnVec<T, V> gn_raw(const T* p, bool past) {
-    if constexpr (sizeof(GnVec<T, V>) == sizeof(GnFour)) {
-        if (past) {
-            const GnFour v = __builtin_nontemporal_load(reinterpret_cast<const GnFour*>(p));
-            return __builtin_bit_cast(GnVec<T, V>, v);
-        }
+template <int V, bool PAST, typename T>
+__device__ inline GnVec<T, V> gn_raw_past(const T* p) {
+    if constexpr (PAST && sizeof(GnVec<T, V>) == sizeof(GnFour)) {
+        const GnFour v = __builtin_nontemporal_load(reinterpret_cast<const GnFour*>(p));
+        return __builtin_bit_cast(GnVec<T, V>, v);
+    } else {
+        return gn_raw<V>(p);
     }
-    return gn_raw<V>(p);
 }
 
 template <int V, typename T>
@@ -96,19 +95,15 @@ __device__ inline void gn_load(const T* p, float (&out)[V]) {
     for (int k = 0; k < V; ++k) out[k] = (float)x.v[k];
 }
 
-template <int V, typename T>
-__device__ inline void gn_store(T* p, const float (&in)[V], bool past) {
+template <int V, bool PAST, typename T>
+__device__ inline void gn_store(T* p, const float (&in)[V]) {
     GnVec<T, V> x;
 #pragma unroll
     for (int k = 0; k < V; ++k) x.v[k] = (T)in[k];
-    if constexpr (sizeof(x) == sizeof(GnFour)) {
-        if (past) {
-            __builtin_nontemporal_store(__builtin_bit_cast(GnFour, x),
-                                        reinterpret_cast<GnFour*>(p));
-            return;
-        }
-    }
-    *reinterpret_cast<GnVec<T, V>*>(p) = x;
+    if constexpr (PAST && sizeof(x) == sizeof(GnFour))
+        __builtin_nontemporal_store(__builtin_bit_cast(GnFour, x), reinterpret_cast<GnFour*>(p));
+    else
+        *reinterpret_cast<GnVec<T, V>*>(p) = x;
 }
 
 // V parameters from channel c on (none: the value where there are none).  The type
@@ -417,7 +412,7 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_join_stats(GnArgs a) {
     }
 }
 
-template <typename T, int V, int ACT>
+template <typename T, int V, int ACT, int PAST>
 __global__ __launch_bounds__(kGnThreads) void k_gn_apply(GnArgs a) {
     __shared__ float gmean[kGnThreads * V], grstd[kGnThreads * V];
     const GnShape& h = a.h;
@@ -462,7 +457,7 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_apply(GnArgs a) {
         constexpr int A = decltype(ahead)::value;
         GnVec<T, V> raw[A];
 #pragma unroll
-        for (int u = 0; u < A; ++u) raw[u] = gn_raw<V>(x + r + u * stride, a.past_in);
+        for (int u = 0; u < A; ++u) raw[u] = gn_raw_past<V, PAST == 2>(x + r + u * stride);
 #pragma unroll
         for (int u = 0; u < A; ++u) {
             float v[V];
@@ -470,7 +465,7 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_apply(GnArgs a) {
             for (int k = 0; k < V; ++k)
                 v[k] = gn_act<ACT>(
                     __builtin_fmaf((float)raw[u].v[k] - mean[k], scale[k], bias[k]));
-            gn_store<V>(y + r + u * stride, v, a.past_out);
+            gn_store<V, PAST != 0>(y + r + u * stride, v);
         }
     });
 }
@@ -632,7 +627,7 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_join_sums(GnArgs a) {
         ((float2*)a.groups_out)[(int64_t)n * a.h.groups + q.g0 + g] = make_float2(g1[g], g2[g]);
 }
 
-template <typename T, int V, int ACT>
+template <typename T, int V, int ACT, int PAST>
 __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_apply(GnArgs a) {
     __shared__ float g1[kGnThreads * V], g2[kGnThreads * V];
     const GnShape& h = a.h;
@@ -684,8 +679,8 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_apply(GnArgs a) {
         GnVec<T, V> v[A], t[A];
 #pragma unroll
         for (int u = 0; u < A; ++u) {
-            v[u] = gn_raw<V>(x + r + u * stride, a.past_in);
-            t[u] = gn_raw<V>(dy + r + u * stride, a.past_in);
+            v[u] = gn_raw_past<V, PAST == 2>(x + r + u * stride);
+            t[u] = gn_raw_past<V, PAST == 2>(dy + r + u * stride);
         }
 #pragma unroll
         for (int u = 0; u < A; ++u) {
@@ -697,7 +692,7 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_apply(GnArgs a) {
                     (float)t[u].v[k] * gn_slope<ACT>(__builtin_fmaf(e, scale[k], bias[k]));
                 o[k] = __builtin_fmaf(dz, scale[k], __builtin_fmaf(e, e2[k], e1[k]));
             }
-            gn_store<V>(dx + r + u * stride, o, a.past_out);
+            gn_store<V, PAST != 0>(dx + r + u * stride, o);
         }
     });
 }
@@ -779,9 +774,9 @@ static bool gn_fits(int64_t n, const GnShape& h) {
 // memory-side cache (bf16, 128 channels, forward/backward in us, plain and so:
 // 48 MB 37.0/62.5 and 35.7/54.4 with stores, 144 MB 101/162 and 81/134 with both;
 // 96 MB forward 58.0 with stores, 58.9 with both, backward 105 and 96).
-static void gn_past(GnArgs& a, int64_t bytes, bool backward) {
-    a.past_out = bytes > (int64_t)32 << 20;
-    a.past_in = bytes > (int64_t)(backward ? 64 : 128) << 20;
+static int gn_past(int64_t bytes, bool backward) {
+    if (bytes > (int64_t)(backward ? 64 : 128) << 20) return 2;
+    return bytes > (int64_t)32 << 20;
 }
 
 static bool gn_aligned(const void* p, int to) { return ((uintptr_t)p % to) == 0; }
@@ -807,20 +802,20 @@ extern "C" size_t cs_group_norm_workspace_elems(int64_t n, int64_t s, int32_t c,
 
 namespace {
 
-template <typename T, int V>
-int gn_forward(const GnArgs& a, int act, hipStream_t stream) {
+template <typename T, int V, int ACT>
+int gn_forward_act(const GnArgs& a, hipStream_t stream) {
     const GnShape& h = a.h;
     const dim3 sums((unsigned)(a.n * h.slices * h.chunks));
     const dim3 apply((unsigned)(a.n * h.slices * h.apply_chunks)), block(kGnThreads);
     hipLaunchKernelGGL((k_gn_stats<T, V>), sums, block, 0, stream, a);
     if (a.joined)
         hipLaunchKernelGGL(k_gn_join_stats, dim3(gn_join_blocks(a)), block, 0, stream, a);
-    switch (act) {
-        case kActNone: hipLaunchKernelGGL((k_gn_apply<T, V, kActNone>), apply, block, 0, stream, a); break;
-        case kActRelu: hipLaunchKernelGGL((k_gn_apply<T, V, kActRelu>), apply, block, 0, stream, a); break;
-        case kActSilu: hipLaunchKernelGGL((k_gn_apply<T, V, kActSilu>), apply, block, 0, stream, a); break;
-        case kActGelu: hipLaunchKernelGGL((k_gn_apply<T, V, kActGelu>), apply, block, 0, stream, a); break;
-    }
+    if (V > 1 && a.past == 2)
+        hipLaunchKernelGGL((k_gn_apply<T, V, ACT, (V > 1 ? 2 : 0)>), apply, block, 0, stream, a);
+    else if (V > 1 && a.past == 1)
+        hipLaunchKernelGGL((k_gn_apply<T, V, ACT, (V > 1 ? 1 : 0)>), apply, block, 0, stream, a);
+    else
+        hipLaunchKernelGGL((k_gn_apply<T, V, ACT, 0>), apply, block, 0, stream, a);
     return hipGetLastError() == hipSuccess ? CS_OK : CS_ERR_HIP;
 }
 
@@ -835,21 +830,49 @@ int gn_backward_act(GnArgs a, hipStream_t stream) {
                            stream, a);
         a.channel_blocks = 0;
     }
-    const int64_t blocks =
-        a.channel_blocks + (a.out ? a.n * h.slices * h.apply_chunks : 0);
-    if (blocks > 0)
-        hipLaunchKernelGGL((k_gn_bwd_apply<T, V, ACT>), dim3((unsigned)blocks), block, 0, stream, a);
+    const dim3 apply(
+        (unsigned)(a.channel_blocks + (a.out ? a.n * h.slices * h.apply_chunks : 0)));
+    if (apply.x == 0) {
+    } else if (V > 1 && a.past == 2) {
+        hipLaunchKernelGGL((k_gn_bwd_apply<T, V, ACT, (V > 1 ? 2 : 0)>), apply, block, 0, stream,
+                           a);
+    } else if (V > 1 && a.past == 1) {
+        hipLaunchKernelGGL((k_gn_bwd_apply<T, V, ACT, (V > 1 ? 1 : 0)>), apply, block, 0, stream,
+                           a);
+    } else {
+        hipLaunchKernelGGL((k_gn_bwd_apply<T, V, ACT, 0>), apply, block, 0, stream, a);
+    }
     return hipGetLastError() == hipSuccess ? CS_OK : CS_ERR_HIP;
 }
 
-template <typename T, int V>
-int gn_backward(const GnArgs& a, int act, hipStream_t stream) {
+template <typename T, int V, bool BACKWARD>
+int gn_run(const GnArgs& a, int act, hipStream_t stream) {
     switch (act) {
-        case kActNone: return gn_backward_act<T, V, kActNone>(a, stream);
-        case kActRelu: return gn_backward_act<T, V, kActRelu>(a, stream);
-        case kActSilu: return gn_backward_act<T, V, kActSilu>(a, stream);
-        default: return gn_backward_act<T, V, kActGelu>(a, stream);
+        case kActNone:
+            return BACKWARD ? gn_backward_act<T, V, kActNone>(a, stream)
+                            : gn_forward_act<T, V, kActNone>(a, stream);
+        case kActRelu:
+            return BACKWARD ? gn_backward_act<T, V, kActRelu>(a, stream)
+                            : gn_forward_act<T, V, kActRelu>(a, stream);
+        case kActSilu:
+            return BACKWARD ? gn_backward_act<T, V, kActSilu>(a, stream)
+                            : gn_forward_act<T, V, kActSilu>(a, stream);
+        default:
+            return BACKWARD ? gn_backward_act<T, V, kActGelu>(a, stream)
+                            : gn_forward_act<T, V, kActGelu>(a, stream);
     }
+}
+
+template <bool BACKWARD>
+int gn_dispatch(const GnArgs& a, int dtype, int vec, int act, hipStream_t stream) {
+    if (dtype == kGnF32)
+        return vec > 1 ? gn_run<float, 4, BACKWARD>(a, act, stream)
+                       : gn_run<float, 1, BACKWARD>(a, act, stream);
+    if (dtype == kGnBF16)
+        return vec > 1 ? gn_run<__bf16, 8, BACKWARD>(a, act, stream)
+                       : gn_run<__bf16, 1, BACKWARD>(a, act, stream);
+    return vec > 1 ? gn_run<_Float16, 8, BACKWARD>(a, act, stream)
+                   : gn_run<_Float16, 1, BACKWARD>(a, act, stream);
 }
 
 }  // namespace
@@ -878,19 +901,13 @@ extern "C" int cs_group_norm_forward(const void* x, int64_t n, int64_t s, int32_
     a.rstd = rstd;
     a.out = y;
     a.n = (int32_t)n;
-    gn_past(a, n * s * c * (dtype == kGnF32 ? 4 : 2), false);
+    a.past = gn_past(n * s * c * (dtype == kGnF32 ? 4 : 2), false);
     a.joined = gn_joined(a.h);
     if (a.joined && !mean) {
         a.mean = workspace + (size_t)n * a.h.chunks * groups * a.h.parts * 2;
         a.rstd = a.mean + (size_t)n * groups;
     }
-    if (dtype == kGnF32)
-        return vec > 1 ? gn_forward<float, 4>(a, act, stream) : gn_forward<float, 1>(a, act, stream);
-    if (dtype == kGnBF16)
-        return vec > 1 ? gn_forward<__bf16, 8>(a, act, stream)
-                       : gn_forward<__bf16, 1>(a, act, stream);
-    return vec > 1 ? gn_forward<_Float16, 8>(a, act, stream)
-                   : gn_forward<_Float16, 1>(a, act, stream);
+    return gn_dispatch<false>(a, dtype, vec, act, stream);
 }
 
 extern "C" int cs_group_norm_backward(const void* x, const void* dy, int64_t n, int64_t s,
@@ -921,7 +938,7 @@ extern "C" int cs_group_norm_backward(const void* x, const void* dy, int64_t n, 
     a.dweight = dweight;
     a.dbias = dbias;
     a.n = (int32_t)n;
-    gn_past(a, n * s * c * (dtype == kGnF32 ? 4 : 2), true);
+    a.past = gn_past(n * s * c * (dtype == kGnF32 ? 4 : 2), true);
     a.joined = gn_joined(a.h);
     float* rest = workspace + (size_t)n * a.h.chunks * groups * a.h.parts * 2;
     if (a.joined) {
@@ -932,12 +949,5 @@ extern "C" int cs_group_norm_backward(const void* x, const void* dy, int64_t n, 
         a.channels = rest;
         a.channel_blocks = (c + kGnChans - 1) / kGnChans;
     }
-    if (dtype == kGnF32)
-        return vec > 1 ? gn_backward<float, 4>(a, act, stream)
-                       : gn_backward<float, 1>(a, act, stream);
-    if (dtype == kGnBF16)
-        return vec > 1 ? gn_backward<__bf16, 8>(a, act, stream)
-                       : gn_backward<__bf16, 1>(a, act, stream);
-    return vec > 1 ? gn_backward<_Float16, 8>(a, act, stream)
-                   : gn_backward<_Float16, 1>(a, act, stream);
+    return gn_dispatch<true>(a, dtype, vec, act, stream);
 }
