@@ -64,6 +64,7 @@ struct GnArgs {
     int32_t channel_blocks;  // of the backward's second (or third) launch, for dw and db
     int32_t joined;          // a launch in between has joined the sums
     float* groups_out;       // backward, joined: [n][group] E[w dz], E[w dz xh]
+    int32_t act;             // of the one-launch kernels
     int32_t past;            // 1: the second launch stores past the caches, 2: it reads so too
 };
 
@@ -180,7 +181,7 @@ struct GnPlace {
 };
 
 template <int V>
-__device__ inline GnPlace gn_place(const GnShape& h, int slice) {
+__device__ inline GnPlace gn_place(const GnShape& h, int slice, int threads = kGnThreads) {
     GnPlace q;
     const int group = h.parts > 1 ? slice / h.parts : slice * h.gs;
     q.part = h.parts > 1 ? slice - group * h.parts : 0;
@@ -190,7 +191,7 @@ __device__ inline GnPlace gn_place(const GnShape& h, int slice) {
     q.cs = q.c0 + h.cs < end ? h.cs : end - q.c0;
     q.ng = h.parts > 1 ? 1 : q.cs / h.d;
     q.vecs = q.cs / V;
-    q.passrows = kGnThreads / q.vecs;
+    q.passrows = threads / q.vecs;
     q.row = threadIdx.x / q.vecs;
     q.chan = (threadIdx.x - q.row * q.vecs) * V;
     q.live = q.row < q.passrows;
@@ -262,10 +263,10 @@ __device__ inline float gn_lanes_sum(float x, int t) {
 
 // Group sums of buf[0 .. cs) into out[0 .. ng).
 __device__ inline void gn_groups_sum(const float* buf, float* out, const GnPlace& q, int d) {
-    const int t = gn_lanes(q.ng), lane = threadIdx.x & (t - 1);
+    const int t = gn_lanes(q.ng), lane = threadIdx.x & (t - 1), step = blockDim.x / t;
     const int width = q.ng == 1 ? q.cs : d;
-    for (int g = threadIdx.x / t; g < (q.ng + kGnThreads / t - 1) / (kGnThreads / t) * (kGnThreads / t);
-         g += kGnThreads / t) {
+    for (int base = 0; base < q.ng; base += step) {
+        const int g = base + threadIdx.x / t;
         float s = 0.0f;
         if (g < q.ng)
             for (int k = lane; k < width; k += t) s += buf[g * width + k];
@@ -697,6 +698,215 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_apply(GnArgs a) {
     });
 }
 
+// ---- one launch: a workgroup keeps its slice of a sample in registers
+
+// At most kGnWholeThreads threads with P vectors each; a is read once.
+constexpr int kGnWholeThreads = 1024;
+
+extern __shared__ float gn_lds[];
+
+__device__ inline float gn_act_of(int act, float z) {
+    switch (act) {
+        case kActRelu: return gn_act<kActRelu>(z);
+        case kActSilu: return gn_act<kActSilu>(z);
+        case kActGelu: return gn_act<kActGelu>(z);
+    }
+    return z;
+}
+
+__device__ inline float gn_slope_of(int act, float z) {
+    switch (act) {
+        case kActRelu: return gn_slope<kActRelu>(z);
+        case kActSilu: return gn_slope<kActSilu>(z);
+        case kActGelu: return gn_slope<kActGelu>(z);
+    }
+    return 1.0f;
+}
+
+// Workgroups go to the eight XCDs in turn; each XCD takes a run of consecutive
+// slices, so that the slices of a row, which share cache lines, share an L2.
+constexpr int kGnXcds = 8;
+
+__device__ inline int gn_by_xcd(int total) {
+    const int per = gridDim.x / kGnXcds;
+    const int id = (blockIdx.x % kGnXcds) * per + blockIdx.x / kGnXcds;
+    return id < total ? id : -1;
+}
+
+template <typename T, int V, int P>
+__global__ __launch_bounds__(kGnWholeThreads) void k_gn_whole(GnArgs a) {
+    const GnShape& h = a.h;
+    const int id = gn_by_xcd(a.n * h.slices);
+    if (id < 0) return;
+    const int n = id / h.slices, slice = id - n * h.slices;
+    const GnPlace q = gn_place<V>(h, slice, blockDim.x);
+    float* buf = gn_lds;
+    float* gmean = buf + blockDim.x * V;
+    float* grstd = gmean + q.cs;
+    const int64_t at = (int64_t)n * h.s * h.c + (int64_t)q.row * h.c + q.c0 + q.chan;
+    const int64_t stride = (int64_t)q.passrows * h.c;
+    const T* x = (const T*)a.x + at;
+    T* y = (T*)a.out + at;
+    const int mine = q.live && q.row < h.s ? (int)((h.s - q.row + q.passrows - 1) / q.passrows) : 0;
+    GnVec<T, V> raw[P];
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+        if (u < mine) raw[u] = gn_raw<V>(x + u * stride);
+    float scale[V], bias[V], w[V], mean[V];
+    if (q.live) {
+        gn_params<V>(a.weight, a.wdtype, q.c0 + q.chan, 1.0f, scale);
+        gn_params<V>(a.bias, a.wdtype, q.c0 + q.chan, 0.0f, bias);
+    }
+    int group[V];
+    gn_group_of<V>(q.ng == 1 ? 0 : q.chan, q.ng == 1 ? V + 1 : h.d, group);
+#pragma unroll
+    for (int k = 0; k < V; ++k) w[k] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+        if (u < mine) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) w[k] += (float)raw[u].v[k];
+        }
+    gn_rows_sum<V>(buf, q, w);
+    gn_groups_sum(buf, gmean, q, h.d);
+    const float inv = 1.0f / ((float)h.s * (float)h.d);
+    if (q.live) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) mean[k] = gmean[group[k]] * inv;
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) w[k] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+        if (u < mine) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float e = (float)raw[u].v[k] - mean[k];
+                w[k] = __builtin_fmaf(e, e, w[k]);
+            }
+        }
+    gn_rows_sum<V>(buf, q, w);
+    gn_groups_sum(buf, grstd, q, h.d);
+    for (int g = threadIdx.x; g < q.ng; g += blockDim.x) {
+        const float r = 1.0f / __builtin_sqrtf(grstd[g] * inv + a.eps);
+        grstd[g] = r;
+        if (a.mean) {
+            a.mean[(int64_t)n * h.groups + q.g0 + g] = gmean[g] * inv;
+            a.rstd[(int64_t)n * h.groups + q.g0 + g] = r;
+        }
+    }
+    __syncthreads();
+    if (!q.live) return;
+#pragma unroll
+    for (int k = 0; k < V; ++k) scale[k] *= grstd[group[k]];
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+        if (u < mine) {
+            float v[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                v[k] = gn_act_of(
+                    a.act, __builtin_fmaf((float)raw[u].v[k] - mean[k], scale[k], bias[k]));
+            gn_store<V, false>(y + u * stride, v);
+        }
+}
+
+template <typename T, int V, int P>
+__global__ __launch_bounds__(kGnWholeThreads) void k_gn_bwd_whole(GnArgs a) {
+    const GnShape& h = a.h;
+    const int id = gn_by_xcd(a.n * h.slices);
+    if (id < 0) return;
+    const int n = id / h.slices, slice = id - n * h.slices;
+    const GnPlace q = gn_place<V>(h, slice, blockDim.x);
+    float* buf = gn_lds;
+    float* g1 = buf + blockDim.x * V;
+    float* g2 = g1 + q.cs;
+    float* chan = g2 + q.cs;
+    const int64_t at = (int64_t)n * h.s * h.c + (int64_t)q.row * h.c + q.c0 + q.chan;
+    const int64_t stride = (int64_t)q.passrows * h.c;
+    const T* x = (const T*)a.x + at;
+    const T* dy = (const T*)a.dy + at;
+    const int mine = q.live && q.row < h.s ? (int)((h.s - q.row + q.passrows - 1) / q.passrows) : 0;
+    GnVec<T, V> v[P], t[P];
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+        if (u < mine) {
+            v[u] = gn_raw<V>(x + u * stride);
+            t[u] = gn_raw<V>(dy + u * stride);
+        }
+    float mean[V], rstd[V], scale[V], bias[V], sa[V], sb[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) sa[k] = sb[k] = rstd[k] = 0.0f;
+    int group[V];
+    gn_group_of<V>(q.ng == 1 ? 0 : q.chan, q.ng == 1 ? V + 1 : h.d, group);
+    if (q.live) {
+        gn_params<V>(a.weight, a.wdtype, q.c0 + q.chan, 1.0f, scale);
+        gn_params<V>(a.bias, a.wdtype, q.c0 + q.chan, 0.0f, bias);
+        const int64_t g0 = (int64_t)n * h.groups + q.g0;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            mean[k] = a.mean[g0 + group[k]];
+            rstd[k] = a.rstd[g0 + group[k]];
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) scale[k] *= rstd[k];
+    }
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+        if (u < mine) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float e = (float)v[u].v[k] - mean[k];
+                const float dz = (float)t[u].v[k] *
+                                 gn_slope_of(a.act, __builtin_fmaf(e, scale[k], bias[k]));
+                sa[k] += dz;
+                sb[k] = __builtin_fmaf(dz, e, sb[k]);
+            }
+        }
+#pragma unroll
+    for (int k = 0; k < V; ++k) sb[k] *= rstd[k];
+    for (int w = 0; w < 2; ++w) {
+        gn_rows_sum<V>(buf, q, w ? sb : sa);
+        for (int c = threadIdx.x; c < q.cs; c += blockDim.x) {
+            float s = buf[c], weight[1];
+            gn_params<1>(a.weight, a.wdtype, q.c0 + c, 1.0f, weight);
+            buf[c] = s * weight[0];
+            if (w == 0) {
+                chan[c] = s;
+            } else if (a.channels) {
+                ((float2*)a.channels)[(int64_t)n * h.c + q.c0 + c] = make_float2(chan[c], s);
+            } else {  // one sample: the sums are the gradients
+                if (a.dbias) gn_store_param(a.dbias, a.wdtype, q.c0 + c, chan[c]);
+                if (a.dweight) gn_store_param(a.dweight, a.wdtype, q.c0 + c, s);
+            }
+        }
+        __syncthreads();
+        gn_groups_sum(buf, w ? g2 : g1, q, h.d);
+    }
+    if (!q.live || !a.out) return;
+    const float inv = 1.0f / ((float)h.s * (float)h.d);
+    float e1[V], e2[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        e1[k] = -rstd[k] * (g1[group[k]] * inv);
+        e2[k] = -rstd[k] * (rstd[k] * (g2[group[k]] * inv));
+    }
+    T* dx = (T*)a.out + at;
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+        if (u < mine) {
+            float o[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float e = (float)v[u].v[k] - mean[k];
+                const float dz = (float)t[u].v[k] *
+                                 gn_slope_of(a.act, __builtin_fmaf(e, scale[k], bias[k]));
+                o[k] = __builtin_fmaf(dz, scale[k], __builtin_fmaf(e, e2[k], e1[k]));
+            }
+            gn_store<V, false>(dx + u * stride, o);
+        }
+}
+
 // ---- host
 
 static int gn_gcd(int a, int b) { return b ? gn_gcd(b, a % b) : a; }
@@ -763,6 +973,52 @@ static bool gn_valid(int64_t n, int64_t s, int32_t c, int32_t groups, int32_t dt
            n <= ((int64_t)1 << 44) / (s * c);
 }
 
+// Four channels a vector, of 16 bits too: eight would not leave registers for 16
+// vectors, and narrower slices make more workgroups.
+constexpr int kGnWholeVec = 4;
+
+// The one-launch form, where a slice of a sample fits a workgroup's registers
+// (`most` vectors a thread): the slice is the narrowest of whole groups and whole
+// vectors that gives a workgroup 256 vectors.  Threads of a workgroup, or 0.
+//
+// A slice of few channels is a few bytes of each row, which the two-launch form
+// reads whole: this form is for samples of few rows and tensors of a few MB (bf16,
+// us of this form and the other: 1x384x512 9.1 and 13.3 forward, 10.9 and 14.6
+// backward; 4x1536x128 10.0 and 13.3, 14.8 and 14.6; 4x6144x128 18.6 and 17.9, 29.8
+// and 20.8; 24x1536x512, 36 MB, 39.3 and 34.0, 69.0 and 44.4).
+constexpr int64_t kGnWholeBytes = (int64_t)24 << 20;
+constexpr int64_t kGnWholeRowsForward = 2048, kGnWholeRowsBackward = 1024;
+
+static int gn_whole(int64_t n, int64_t s, int32_t c, int32_t groups, int vec, int most,
+                    int64_t rows, int size, GnShape* shape) {
+    if (s > rows || n * s * c * size > kGnWholeBytes) return 0;
+    GnShape h{};
+    h.s = s;
+    h.c = c;
+    h.groups = groups;
+    h.d = c / groups;
+    h.parts = 1;
+    h.chunks = 1;
+    h.rows = s;
+    const int unit = vec / gn_gcd(h.d, vec);
+    const int64_t row_vecs = (int64_t)unit * h.d / vec;
+    if (row_vecs > 256) return 0;
+    int64_t wide = (256 + s * row_vecs - 1) / (s * row_vecs);
+    if (wide * row_vecs > 256) wide = 256 / row_vecs;
+    h.gs = (int32_t)(wide * unit < groups ? wide * unit : groups);
+    h.cs = h.gs * h.d;
+    h.slices = (groups + h.gs - 1) / h.gs;
+    const int vecs = h.cs / vec;
+    // Four vectors a thread, more where that takes too many threads.
+    int64_t threads = (((s + 3) / 4) * vecs + 63) / 64 * 64;
+    if (threads < 256) threads = 256;
+    if (threads > kGnWholeThreads) threads = kGnWholeThreads;
+    if ((s + threads / vecs - 1) / (threads / vecs) > most) return 0;
+    if (n > ((int64_t)1 << 22) / h.slices) return 0;
+    *shape = h;
+    return (int)threads;
+}
+
 // A launch has fewer than 2^24 workgroups of 256 threads.
 static bool gn_fits(int64_t n, const GnShape& h) {
     const int64_t chunks = h.chunks > h.apply_chunks ? h.chunks : h.apply_chunks;
@@ -801,6 +1057,46 @@ extern "C" size_t cs_group_norm_workspace_elems(int64_t n, int64_t s, int32_t c,
 }
 
 namespace {
+
+constexpr int kGnWholeForward = 16, kGnWholeBackward = 8;  // vectors a thread at most
+
+template <typename T, int V, bool BACKWARD>
+int gn_run_whole(const GnArgs& a, int threads, hipStream_t stream) {
+    const GnShape& h = a.h;
+    const dim3 grid((unsigned)((a.n * h.slices + kGnXcds - 1) / kGnXcds * kGnXcds));
+    const dim3 block((unsigned)threads);
+    const size_t lds = ((size_t)threads * V + (size_t)h.cs * (BACKWARD ? 3 : 2)) * sizeof(float);
+    const int passrows = threads / (h.cs / V);
+    const bool few = h.s <= 4 * (int64_t)passrows;
+    if (!BACKWARD) {
+        if (few)
+            hipLaunchKernelGGL((k_gn_whole<T, V, 4>), grid, block, lds, stream, a);
+        else
+            hipLaunchKernelGGL((k_gn_whole<T, V, kGnWholeForward>), grid, block, lds, stream, a);
+    } else {
+        if (few)
+            hipLaunchKernelGGL((k_gn_bwd_whole<T, V, 4>), grid, block, lds, stream, a);
+        else
+            hipLaunchKernelGGL((k_gn_bwd_whole<T, V, kGnWholeBackward>), grid, block, lds, stream,
+                               a);
+        if (a.channels)
+            hipLaunchKernelGGL(k_gn_join_sums, dim3(a.channel_blocks), dim3(kGnThreads), 0, stream,
+                               a);
+    }
+    return hipGetLastError() == hipSuccess ? CS_OK : CS_ERR_HIP;
+}
+
+template <bool BACKWARD>
+int gn_dispatch_whole(const GnArgs& a, int dtype, int vec, int threads, hipStream_t stream) {
+    if (dtype == kGnF32)
+        return vec > 1 ? gn_run_whole<float, kGnWholeVec, BACKWARD>(a, threads, stream)
+                       : gn_run_whole<float, 1, BACKWARD>(a, threads, stream);
+    if (dtype == kGnBF16)
+        return vec > 1 ? gn_run_whole<__bf16, kGnWholeVec, BACKWARD>(a, threads, stream)
+                       : gn_run_whole<__bf16, 1, BACKWARD>(a, threads, stream);
+    return vec > 1 ? gn_run_whole<_Float16, kGnWholeVec, BACKWARD>(a, threads, stream)
+                   : gn_run_whole<_Float16, 1, BACKWARD>(a, threads, stream);
+}
 
 template <typename T, int V, int ACT>
 int gn_forward_act(const GnArgs& a, hipStream_t stream) {
@@ -889,8 +1185,14 @@ extern "C" int cs_group_norm_forward(const void* x, int64_t n, int64_t s, int32_
     int vec = gn_widest(dtype);
     if (c % vec || !gn_aligned(x, 16) || !gn_aligned(y, 16)) vec = 1;
     GnArgs a{};
-    a.h = gn_shape(n, s, c, groups, &vec);
-    if (!gn_fits(n, a.h)) return CS_ERR_ARGS;
+    const int whole_vec = vec > 1 || (c % kGnWholeVec == 0 && gn_aligned(x, 16) && gn_aligned(y, 16))
+                              ? kGnWholeVec : 1;
+    const int size = dtype == kGnF32 ? 4 : 2;
+    const int whole = gn_whole(n, s, c, groups, whole_vec, kGnWholeForward, kGnWholeRowsForward,
+                               size, &a.h);
+    if (!whole) a.h = gn_shape(n, s, c, groups, &vec);
+    if (!whole && !gn_fits(n, a.h)) return CS_ERR_ARGS;
+    a.act = act;
     a.x = x;
     a.weight = weight;
     a.bias = bias;
@@ -901,7 +1203,8 @@ extern "C" int cs_group_norm_forward(const void* x, int64_t n, int64_t s, int32_
     a.rstd = rstd;
     a.out = y;
     a.n = (int32_t)n;
-    a.past = gn_past(n * s * c * (dtype == kGnF32 ? 4 : 2), false);
+    if (whole) return gn_dispatch_whole<false>(a, dtype, whole_vec, whole, stream);
+    a.past = gn_past(n * s * c * size, false);
     a.joined = gn_joined(a.h);
     if (a.joined && !mean) {
         a.mean = workspace + (size_t)n * a.h.chunks * groups * a.h.parts * 2;
@@ -924,8 +1227,15 @@ extern "C" int cs_group_norm_backward(const void* x, const void* dy, int64_t n, 
     int vec = gn_widest(dtype);
     if (c % vec || !gn_aligned(x, 16) || !gn_aligned(dy, 16) || (dx && !gn_aligned(dx, 16))) vec = 1;
     GnArgs a{};
-    a.h = gn_shape(n, s, c, groups, &vec);
-    if (!gn_fits(n, a.h)) return CS_ERR_ARGS;
+    const int whole_vec = vec > 1 || (c % kGnWholeVec == 0 && gn_aligned(x, 16) &&
+                                      gn_aligned(dy, 16) && (!dx || gn_aligned(dx, 16)))
+                              ? kGnWholeVec : 1;
+    const int size = dtype == kGnF32 ? 4 : 2;
+    const int whole = gn_whole(n, s, c, groups, whole_vec, kGnWholeBackward, kGnWholeRowsBackward,
+                               size, &a.h);
+    if (!whole) a.h = gn_shape(n, s, c, groups, &vec);
+    if (!whole && !gn_fits(n, a.h)) return CS_ERR_ARGS;
+    a.act = act;
     a.x = x;
     a.dy = dy;
     a.weight = weight;
@@ -938,7 +1248,14 @@ extern "C" int cs_group_norm_backward(const void* x, const void* dy, int64_t n, 
     a.dweight = dweight;
     a.dbias = dbias;
     a.n = (int32_t)n;
-    a.past = gn_past(n * s * c * (dtype == kGnF32 ? 4 : 2), true);
+    if (whole) {
+        if (n > 1 && (dweight || dbias)) {
+            a.channels = workspace;
+            a.channel_blocks = (c + kGnChans - 1) / kGnChans;
+        }
+        return gn_dispatch_whole<true>(a, dtype, whole_vec, whole, stream);
+    }
+    a.past = gn_past(n * s * c * size, true);
     a.joined = gn_joined(a.h);
     float* rest = workspace + (size_t)n * a.h.chunks * groups * a.h.parts * 2;
     if (a.joined) {

@@ -32,6 +32,9 @@ SHAPES = [
     (70, 40, (), 8), (2, 10, (3, 4, 5), 5), (1, 2048, (9,), 1), (1, 4096, (7,), 1),
     (1, 2100, (11,), 1), (1, 600, (13, 1), 8), (1, 4094, (3,), 2), (1, 16376, (2,), 8),
     (300, 16, (2, 2), 4), (1, 8, (100, 101), 2), (4, 64, (37, 3), 64), (2, 36, (29, 31), 6),
+    # Forward in one launch and backward in two; either at its longest; three launches.
+    (3, 64, (45, 44), 16), (2, 16, (32, 32), 4), (2, 16, (25, 41), 4), (1, 16, (32, 64), 4),
+    (1, 16, (3, 683), 2), (1, 128, (64, 100), 32), (9, 20, (61, 61), 10), (2, 1024, (33, 1), 1),
 ]
 
 
