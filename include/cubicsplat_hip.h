@@ -711,7 +711,7 @@ int cs_adan_step(int32_t ntensors, float* const* params, const float* const* gra
  * values: B = ceil(n / CS_ADAMW_BLOCK) blocks; B * CS_ADAMW_BLOCK code bytes,
  * then B bytes with each block's exponent; 8-byte aligned.
  * sets: nsets rows of eight floats: 1 - lr * weight_decay,
- * lr / (1 - beta1^t), sqrt(1 - beta2^t), 1 - beta1, beta2, 1 - beta2, eps, 0;
+ * lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), 1 - beta1, beta2, 1 - beta2, eps, 0;
  * keys: nsets random words, a new one each step.  clip: device fp32 factor of
  * the gradients, or NULL.  One launch for up to 56 tensors and 12 sets. */
 #define CS_ADAMW_BLOCK 128

@@ -58,7 +58,7 @@ struct AwTensor {
 };
 
 struct AwSet {
-    float decay, step_size, bc2_sqrt, omb1, beta2, omb2, eps, pad;
+    float decay, step_size, inv_bc2_sqrt, omb1, beta2, omb2, eps, pad;
 };
 
 struct AwArgs {
@@ -78,8 +78,9 @@ __host__ __device__ inline uint32_t aw_mix(uint32_t x) {
     return x ^ (x >> 16);
 }
 
-__device__ inline uint32_t aw_random(uint32_t key, int64_t i) {
-    return aw_mix(key + (uint32_t)i + (uint32_t)(i >> 32) * 0x3C6EF372u);
+// The hash's argument for element i, a multiple of 8; the seven after it follow.
+__device__ inline uint32_t aw_key(uint32_t key, int64_t i) {
+    return key + (uint32_t)i + (uint32_t)(i >> 32) * 0x3C6EF372u;
 }
 
 // The tensor this workgroup works on: lane k holds tensor k's first block.
@@ -97,10 +98,11 @@ template <> struct AwType<kF16> { typedef _Float16 type; };
 template <typename T, int N>
 struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) AwVec { T v[N]; };
 
-// N consecutive elements at element i; elements past n are 0 and not stored.
-template <int N, typename T>
-__device__ inline void aw_load(const T* src, int64_t i, int64_t n, bool vec, float (&out)[N]) {
-    if (vec && i + N <= n) {
+// N consecutive elements at element i.  FULL: all of them are there, aligned;
+// otherwise elements past n are 0 and not stored.
+template <int N, bool FULL, typename T>
+__device__ inline void aw_load(const T* src, int64_t i, int64_t n, float (&out)[N]) {
+    if constexpr (FULL) {
         const AwVec<T, N> x = *reinterpret_cast<const AwVec<T, N>*>(src + i);
 #pragma unroll
         for (int k = 0; k < N; ++k) out[k] = (float)x.v[k];
@@ -110,9 +112,9 @@ __device__ inline void aw_load(const T* src, int64_t i, int64_t n, bool vec, flo
     }
 }
 
-template <int N, typename T>
-__device__ inline void aw_store(T* dst, int64_t i, int64_t n, bool vec, const float (&in)[N]) {
-    if (vec && i + N <= n) {
+template <int N, bool FULL, typename T>
+__device__ inline void aw_store(T* dst, int64_t i, int64_t n, const float (&in)[N]) {
+    if constexpr (FULL) {
         AwVec<T, N> x;
 #pragma unroll
         for (int k = 0; k < N; ++k) x.v[k] = (T)in[k];
@@ -124,13 +126,29 @@ __device__ inline void aw_store(T* dst, int64_t i, int64_t n, bool vec, const fl
     }
 }
 
+// The passes of [begin, end): f(FULL, first element) by the whole workgroup, full
+// where all of the pass's elements are there and `vec` (a uniform choice, as the
+// lanes of a block work together).
+template <bool B> struct AwBool { static constexpr bool value = B; };
+
+template <typename F>
+__device__ inline void aw_passes(int64_t begin, int64_t end, bool vec, F&& f) {
+    int64_t base = begin;
+    if (vec)
+        for (; base + kAwPass <= end; base += kAwPass) f(AwBool<true>(), base);
+    for (; base < end; base += kAwPass) f(AwBool<false>(), base);
+}
+
 __device__ inline void aw_update(const AwSet& s, float g, float& p, float& m, float& v,
                                  float& root) {
     p = p * s.decay;
     m = m + s.omb1 * (g - m);
     v = v * s.beta2 + s.omb2 * (g * g);
     root = __builtin_sqrtf(v);
-    p = p - s.step_size * (m / (root / s.bc2_sqrt + s.eps));
+    // The hardware's reciprocal (1 ulp): the quotient is a few roundings off, the
+    // sequence of a rounded division would double the kernel's instructions.
+    const float inv = __builtin_amdgcn_rcpf(__builtin_fmaf(root, s.inv_bc2_sqrt, s.eps));
+    p = p - s.step_size * (m * inv);
 }
 
 // ---- 8-bit codes
@@ -196,10 +214,11 @@ __device__ inline int64_t aw_blocks(int64_t n) { return (n + kBlk - 1) / kBlk; }
 
 // Encodes and stores a lane's 8 values of m and root; every lane of the wave
 // takes part.
+template <bool FULL>
 __device__ inline void aw_hold(uint8_t* avg, uint8_t* sq, int64_t i, int64_t n,
                                const float (&m)[8], const float (&root)[8],
                                const uint32_t (&r)[8]) {
-    const bool in = i < n;
+    const bool in = FULL || i < n;
     const int em = aw_shared_exponent(m), er = aw_shared_exponent(root);
     uint32_t cm[8], cr[8];
 #pragma unroll
@@ -216,9 +235,10 @@ __device__ inline void aw_hold(uint8_t* avg, uint8_t* sq, int64_t i, int64_t n,
     }
 }
 
+template <bool FULL>
 __device__ inline void aw_held(const uint8_t* avg, const uint8_t* sq, int64_t i, int64_t n,
                                float (&m)[8], float (&root)[8]) {
-    const bool in = i < n;
+    const bool in = FULL || i < n;
     const int64_t b = aw_blocks(n) * kBlk + i / kBlk;
     const int em = in ? avg[b] : 0, er = in ? sq[b] : 0;
     uint32_t cm[8], cr[8];
@@ -239,19 +259,30 @@ __device__ inline void aw_step32(const AwTensor& t, const AwSet& s, float clip, 
     typedef typename AwType<DT>::type T;
     const bool vec = (t.meta >> 5) & 1;
     float* main = DT == kF32 ? (float*)t.param : t.master;
-    for (int64_t i = begin + threadIdx.x * 4; i < end; i += kAwThreads * 4) {
-        float p[4], g[4], m[4], v[4], root;
-        aw_load<4>(main, i, end, vec, p);
-        aw_load<4>((const T*)t.grad, i, end, vec, g);
-        aw_load<4>((const float*)t.avg, i, end, vec, m);
-        aw_load<4>((const float*)t.sq, i, end, vec, v);
+    aw_passes(begin, end, vec, [&](auto full, int64_t base) {
+        constexpr bool F = decltype(full)::value;
+        // Two vectors a thread, their loads in flight together.
+        float p[2][4], g[2][4], m[2][4], v[2][4], root;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) aw_update(s, g[k] * clip, p[k], m[k], v[k], root);
-        aw_store<4>(main, i, end, vec, p);
-        if (DT != kF32) aw_store<4>((T*)t.param, i, end, vec, p);
-        aw_store<4>((float*)t.avg, i, end, vec, m);
-        aw_store<4>((float*)t.sq, i, end, vec, v);
-    }
+        for (int u = 0; u < 2; ++u) {
+            const int64_t i = base + (u * kAwThreads + threadIdx.x) * 4;
+            aw_load<4, F>(main, i, end, p[u]);
+            aw_load<4, F>((const T*)t.grad, i, end, g[u]);
+            aw_load<4, F>((const float*)t.avg, i, end, m[u]);
+            aw_load<4, F>((const float*)t.sq, i, end, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int64_t i = base + (u * kAwThreads + threadIdx.x) * 4;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                aw_update(s, g[u][k] * clip, p[u][k], m[u][k], v[u][k], root);
+            aw_store<4, F>(main, i, end, p[u]);
+            if (DT != kF32) aw_store<4, F>((T*)t.param, i, end, p[u]);
+            aw_store<4, F>((float*)t.avg, i, end, m[u]);
+            aw_store<4, F>((float*)t.sq, i, end, v[u]);
+        }
+    });
 }
 
 template <int DT>
@@ -260,25 +291,27 @@ __device__ inline void aw_step8(const AwTensor& t, const AwSet& s, float clip, i
     typedef typename AwType<DT>::type T;
     const bool vec = (t.meta >> 5) & 1;
     float* main = DT == kF32 ? (float*)t.param : t.master;
-    for (int64_t base = begin; base < end; base += kAwPass) {
+    aw_passes(begin, end, vec, [&](auto full, int64_t base) {
+        constexpr bool F = decltype(full)::value;
         const int64_t i = base + threadIdx.x * 8;
         float p[8], g[8], m[8], root[8];
         uint32_t r[8];
-        aw_load<8>(main, i, t.n, vec, p);
-        aw_load<8>((const T*)t.grad, i, t.n, vec, g);
-        aw_held((const uint8_t*)t.avg, (const uint8_t*)t.sq, i, t.n, m, root);
+        aw_load<8, F>(main, i, t.n, p);
+        aw_load<8, F>((const T*)t.grad, i, t.n, g);
+        aw_held<F>((const uint8_t*)t.avg, (const uint8_t*)t.sq, i, t.n, m, root);
+        const uint32_t key = aw_key(t.key, i);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             float v = root[k] * root[k];
             aw_update(s, g[k] * clip, p[k], m[k], v, root[k]);
-            r[k] = aw_random(t.key, i + k);
+            r[k] = aw_mix(key + k);
             // Elements past the end do not set a block's exponent.
-            if (i + k >= t.n) m[k] = root[k] = 0.0f;
+            if (!F && i + k >= t.n) m[k] = root[k] = 0.0f;
         }
-        aw_store<8>(main, i, t.n, vec, p);
-        if (DT != kF32) aw_store<8>((T*)t.param, i, t.n, vec, p);
-        aw_hold((uint8_t*)t.avg, (uint8_t*)t.sq, i, t.n, m, root, r);
-    }
+        aw_store<8, F>(main, i, t.n, p);
+        if (DT != kF32) aw_store<8, F>((T*)t.param, i, t.n, p);
+        aw_hold<F>((uint8_t*)t.avg, (uint8_t*)t.sq, i, t.n, m, root, r);
+    });
 }
 
 __global__ __launch_bounds__(kAwThreads) void k_adamw(AwArgs a) {
@@ -306,42 +339,49 @@ __global__ __launch_bounds__(kAwThreads) void k_adamw_pack(AwArgs a) {
     const bool vec = (t.meta >> 5) & 1;
     const int64_t begin = (int64_t)(blockIdx.x - t.first_block) * a.chunk;
     const int64_t end = begin + a.chunk < t.n ? begin + a.chunk : t.n;
-    for (int64_t base = begin; base < end; base += kAwPass) {
+    aw_passes(begin, end, vec, [&](auto full, int64_t base) {
+        constexpr bool F = decltype(full)::value;
         const int64_t i = base + threadIdx.x * 8;
         float m[8], root[8];
         uint32_t r[8];
-        aw_load<8>((const float*)t.avg, i, t.n, vec, m);
-        aw_load<8>((const float*)t.sq, i, t.n, vec, root);
+        aw_load<8, F>((const float*)t.avg, i, t.n, m);
+        aw_load<8, F>((const float*)t.sq, i, t.n, root);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             root[k] = __builtin_sqrtf(root[k]);
             r[k] = 0x80008000u;  // one half of a spacing: to nearest
         }
-        aw_hold((uint8_t*)t.param, (uint8_t*)t.grad, i, t.n, m, root, r);
-    }
+        aw_hold<F>((uint8_t*)t.param, (uint8_t*)t.grad, i, t.n, m, root, r);
+    });
 }
 
 template <typename T>
 __device__ inline void aw_unpack(const AwTensor& t, int64_t begin, int64_t end) {
     const bool vec = (t.meta >> 5) & 1, eight = (t.meta >> 4) & 1;
     const int64_t n = (int64_t)(intptr_t)t.master;  // with what follows the values
-    for (int64_t i = begin + threadIdx.x * 8; i < end; i += kAwPass) {
+    // Full passes end with the values, not with what follows them.
+    const int64_t whole = t.n < end ? begin + (t.n - begin) / kAwPass * kAwPass : end;
+    const auto pass = [&](auto full, int64_t base) {
+        constexpr bool F = decltype(full)::value;
+        const int64_t i = base + threadIdx.x * 8;
         float m[8], v[8];
         if (eight) {
-            aw_held((const uint8_t*)t.avg, (const uint8_t*)t.sq, i, t.n, m, v);
+            aw_held<F>((const uint8_t*)t.avg, (const uint8_t*)t.sq, i, t.n, m, v);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const bool in = i + k < t.n;
+                const bool in = F || i + k < t.n;
                 m[k] = in ? m[k] : 0.0f;
                 v[k] = in ? v[k] * v[k] : 0.0f;
             }
         } else {
-            aw_load<8>((const float*)t.avg, i, t.n, vec, m);
-            aw_load<8>((const float*)t.sq, i, t.n, vec, v);
+            aw_load<8, F>((const float*)t.avg, i, t.n, m);
+            aw_load<8, F>((const float*)t.sq, i, t.n, v);
         }
-        aw_store<8>((T*)t.param, i, n, vec, m);
-        aw_store<8>((T*)const_cast<void*>(t.grad), i, n, vec, v);
-    }
+        aw_store<8, F>((T*)t.param, i, n, m);
+        aw_store<8, F>((T*)const_cast<void*>(t.grad), i, n, v);
+    };
+    if (whole > begin) aw_passes(begin, whole, vec, pass);
+    aw_passes(whole > begin ? whole : begin, end, false, pass);
 }
 
 __global__ __launch_bounds__(kAwThreads) void k_adamw_unpack(AwArgs a) {
@@ -380,12 +420,13 @@ __device__ inline float norm_squares(const NormTensor& t, int64_t begin, int64_t
     typedef typename AwType<DT>::type T;
     const bool vec = (t.meta >> 5) & 1;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t i = begin + threadIdx.x * 8; i < end; i += kAwPass) {
+    aw_passes(begin, end, vec, [&](auto full, int64_t base) {
+        constexpr bool F = decltype(full)::value;
         float g[8];
-        aw_load<8>((const T*)t.grad, i, end, vec, g);
+        aw_load<8, F>((const T*)t.grad, base + threadIdx.x * 8, end, g);
 #pragma unroll
         for (int k = 0; k < 8; ++k) s[k & 3] = __builtin_fmaf(g[k], g[k], s[k & 3]);
-    }
+    });
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
 

@@ -26,6 +26,7 @@ from __future__ import annotations
 import ctypes
 import math
 from itertools import chain
+from operator import is_
 
 import numpy as np
 import torch
@@ -429,22 +430,53 @@ def _codes_numel(numel):
     return -(-numel // N.ADAMW_BLOCK) * (N.ADAMW_BLOCK + 1)
 
 
+def _same(a, b):
+    """Whether two lists hold the same objects."""
+    return len(a) == len(b) and all(map(is_, a, b))
+
+
 class _AdamWEntry:
     """What the launches need of one parameter; remade when a tensor of it is
-    another one."""
-    __slots__ = ("p", "st", "avg", "sq", "master", "step_t", "step", "row", "dtype", "contiguous")
+    another one, or lies elsewhere."""
+    __slots__ = ("p", "st", "avg_key", "sq_key", "avg", "sq", "master", "step_t", "step", "row",
+                 "ptr", "numel", "dtype", "device", "stride", "contiguous", "place")
+
+    def fresh(self):
+        p, st = self.p, self.st
+        try:
+            return (p.data_ptr() == self.ptr and p.numel() == self.numel
+                    and p.dtype is self.dtype
+                    and (p.is_contiguous() if self.contiguous else p.stride() == self.stride)
+                    and st[self.avg_key] is self.avg and st[self.sq_key] is self.sq
+                    and st["step"] is self.step_t
+                    and (self.master is None or st["master"] is self.master))
+        except KeyError:
+            return False
 
 
 class _AdamWPlan:
-    """The table of one device's launches, reused while the same parameters take part."""
+    """The table of one device's launches, reused while the same parameters take
+    part.  Each group has a set of its own as long as its parameters' step counts
+    agree."""
 
-    def __init__(self, entries):
-        self.entries = entries
+    def __init__(self, version, entries, ngroups):
+        self.version, self.entries = version, entries
+        self.groups = [e.place[1] for e in entries]
         self.table = np.array([e.row for e in entries], dtype=np.int64).reshape(-1, 8)
+        self.table[:, _NUMBER] = [e.place[0] for e in entries]
         self.address = self.table.ctypes.data
         self.grads = self.table[:, _G]
         self.metas = self.table[:, _META]
-        self.one_set = True   # every row of the first set
+        self.types = self.metas.copy()
+        self.by_group = self.types | (np.array(self.groups, np.int64) << _SET_SHIFT)
+        self.metas[:] = self.by_group
+        self.regular = True   # the sets are the groups'
+        self.make_sets(ngroups)
+
+    def make_sets(self, n):
+        self.sets = np.zeros((n, 8), dtype=np.float32)
+        self.keys = np.zeros(n, dtype=np.uint32)
+        self.sets_address, self.keys_address = self.sets.ctypes.data, self.keys.ctypes.data
 
 
 def _check_grad(g, dtype, device):
@@ -549,7 +581,10 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, defaults)
 
     def _reset(self):
-        self._entries, self._plans, self._norm = {}, {}, None
+        # Entries in the parameters' order (None: no state yet), with the lists
+        # that they were made from, to notice a change of any.
+        self._order, self._params, self._sizes, self._keys, self._values = [], [], [], [], []
+        self._version, self._plans, self._flat, self._norm = 0, {}, None, None
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits,
@@ -597,14 +632,21 @@ class AdamW(torch.optim.Optimizer):
         if p.dtype is not torch.float32 and "master" not in st:
             st["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
 
-    def _entry(self, p, number):
+    def _entry(self, number, k):
+        """A new entry of parameter `number`, which is of group k."""
+        p = self._params[number]
+        self._version += 1
         self._check_param(p)
         st = self.state[p]
         eight = self._eight(p.numel())
         self._init_state(p, st)
         e = _AdamWEntry()
-        e.p, e.st, e.dtype, e.contiguous = p, st, p.dtype, p.is_contiguous()
-        e.avg, e.sq = (st[_AVG8], st[_SQ8]) if eight else (st["exp_avg"], st["exp_avg_sq"])
+        e.place = (number, k)
+        e.p, e.st, e.dtype, e.device = p, st, p.dtype, p.device
+        e.ptr, e.numel, e.stride, e.contiguous = (p.data_ptr(), p.numel(), p.stride(),
+                                                  p.is_contiguous())
+        e.avg_key, e.sq_key = (_AVG8, _SQ8) if eight else ("exp_avg", "exp_avg_sq")
+        e.avg, e.sq = st[e.avg_key], st[e.sq_key]
         e.master = st.get("master") if p.dtype is not torch.float32 else None
         for t in (e.avg, e.sq, e.master):
             if t is None:
@@ -627,22 +669,32 @@ class AdamW(torch.optim.Optimizer):
         e.step_t, e.step = step, ctypes.c_float.from_address(step.data_ptr())
         e.row = [p.data_ptr(), 0, 0 if e.master is None else e.master.data_ptr(),
                  e.avg.data_ptr(), e.sq.data_ptr(), p.numel(),
-                 _ADAMW_DTYPES[p.dtype] | (_EIGHT if eight else 0), number]
+                 _ADAMW_DTYPES[p.dtype] | (_EIGHT if eight else 0), 0]
+        self._order[number] = e
         return e
 
-    def _current(self, p, number):
-        """p's entry, remade if anything of it has been replaced."""
-        e = self._entries.get(p)
-        if e is not None:
-            st, row = e.st, e.row
-            a, b = (_AVG8, _SQ8) if row[_META] & _EIGHT else ("exp_avg", "exp_avg_sq")
-            if (self.state.get(p) is st and row[_P] == p.data_ptr() and p.dtype is e.dtype
-                    and row[_NUMEL] == p.numel() and row[_NUMBER] == number
-                    and st.get(a) is e.avg and st.get(b) is e.sq
-                    and st.get("step") is e.step_t and st.get("master") is e.master):
-                return e
-        e = self._entries[p] = self._entry(p, number)
-        return e
+    def _entries(self):
+        """The entries in the parameters' order, None where a parameter has none.
+        An entry that is there may still have to be remade (`fresh`)."""
+        groups = self.param_groups
+        params = [p for group in groups for p in group["params"]]
+        sizes = [len(group["params"]) for group in groups]
+        keys, values = list(self.state), list(self.state.values())
+        if not (sizes == self._sizes and _same(params, self._params) and _same(keys, self._keys)
+                and _same(values, self._values)):
+            old = {id(e.p): e for e in self._order if e is not None}
+            self._order = []
+            for k, group in enumerate(groups):
+                for p in group["params"]:
+                    e = old.get(id(p))
+                    if e is not None and e.st is self.state.get(p):
+                        e.place = (len(self._order), k)
+                    else:
+                        e = None
+                    self._order.append(e)
+            self._params, self._sizes, self._keys, self._values = params, sizes, keys, values
+            self._version += 1
+        return self._order
 
     # ---- the step
 
@@ -661,63 +713,78 @@ class AdamW(torch.optim.Optimizer):
 
     def _step(self):
         # Gathered first: nothing is launched or counted if a tensor is refused.
-        work, number = {}, -1
+        order = self._entries()
+        work, number, regular, strided = {}, -1, True, torch.strided
+        last, w = None, None
         for k, group in enumerate(self.param_groups):
+            first = None
             for p in group["params"]:
                 number += 1
                 g = p.grad
                 if g is None:
                     continue
-                e = self._current(p, number)
-                if g.dtype is not e.dtype or g.layout is not torch.strided:
+                e = order[number]
+                if e is None or not e.fresh():
+                    e = self._entry(number, k)
+                if g.dtype is not e.dtype or g.layout is not strided:
                     _check_grad(g, e.dtype, p.device)
                 if not (e.contiguous and g.is_contiguous()) and not (
                         _is_dense(g) and _same_layout(g, p)):
                     g = torch.empty_like(p).copy_(g.detach())
-                w = work.get(p.device)
-                if w is None:
-                    w = work[p.device] = ([], [], [], [])
+                step = e.step.value + 1.0
+                if step != first:
+                    regular = regular and first is None
+                    first = step
+                if e.device is not last:
+                    last = e.device
+                    w = work.setdefault(last, ([], [], []))
                 w[0].append(e)
                 w[1].append(g)
-                w[2].append(g.data_ptr())
-                w[3].append((k, e.step.value + 1.0))
-        if len(self._entries) > number + 1:   # parameters that have left the groups
-            kept = {p for group in self.param_groups for p in group["params"]}
-            self._entries = {p: e for p, e in self._entries.items() if p in kept}
+                w[2].append(step)
         if not work:
             return
+        if len(self.state) != len(self._keys):   # states made just now
+            self._keys, self._values = list(self.state), list(self.state.values())
         if self.max_grad_norm > 0 and len(work) > 1:
             raise NotImplementedError("max_grad_norm needs all parameters on one device")
-        if torch.cuda.is_current_stream_capturing():
+        if torch._C._cuda_isCurrentStreamCapturing():
             raise RuntimeError("an AdamW step counts on the host and cannot be captured")
         for device, w in work.items():
-            if device.index == torch.cuda.current_device():
-                self._launch(device, *w)
+            if device.index == torch._C._cuda_getDevice():
+                self._launch(device, regular, *w)
             else:
                 with torch.cuda.device(device):
-                    self._launch(device, *w)
+                    self._launch(device, regular, *w)
 
-    def _launch(self, device, entries, grads, grad_ptrs, steps):
+    def _launch(self, device, regular, entries, grads, steps):
+        groups = self.param_groups
         plan = self._plans.get(device)
-        if plan is None or plan.entries != entries:
-            plan = self._plans[device] = _AdamWPlan(entries)
-        numbers = {}
-        for s in steps:
-            if s not in numbers:
-                numbers[s] = len(numbers)
-        if len(numbers) > 1 or not plan.one_set:
-            plan.metas[:] = [e.row[_META] | numbers[s] << _SET_SHIFT
-                             for e, s in zip(entries, steps)]
-            plan.one_set = len(numbers) == 1
-        plan.grads[:] = grad_ptrs
-        sets = np.zeros((len(numbers), 8), dtype=np.float32)
-        keys = np.zeros(len(numbers), dtype=np.uint32)
-        for (k, step), i in numbers.items():
-            group = self.param_groups[k]
+        if plan is None or plan.version != self._version or not _same(plan.entries, entries):
+            plan = self._plans[device] = _AdamWPlan(self._version, entries, len(groups))
+        # Each set's (group, step).
+        if regular:
+            pairs = dict(zip(plan.groups, steps)).items()
+            if not plan.regular:
+                plan.metas[:] = plan.by_group
+                plan.make_sets(len(groups))
+        else:
+            numbers = {}
+            for pair in zip(plan.groups, steps):
+                numbers.setdefault(pair, len(numbers))
+            pairs = list(numbers)
+            plan.metas[:] = plan.types | np.array(
+                [numbers[pair] << _SET_SHIFT for pair in zip(plan.groups, steps)], np.int64)
+            plan.make_sets(len(pairs))
+        plan.regular = regular
+        plan.grads[:] = [g.data_ptr() for g in grads]
+        sets, keys = plan.sets, plan.keys
+        for i, (k, step) in enumerate(pairs):
+            group = groups[k]
             beta1, beta2 = group["betas"]
             lr = float(group["lr"])
+            i = k if regular else i
             sets[i] = (1.0 - lr * group["weight_decay"], lr / (1.0 - beta1 ** step),
-                       math.sqrt(1.0 - beta2 ** step), 1.0 - beta1, beta2, 1.0 - beta2,
+                       1.0 / math.sqrt(1.0 - beta2 ** step), 1.0 - beta1, beta2, 1.0 - beta2,
                        group["eps"], 0.0)
             keys[i] = _mix32(self.seed + int(step) * 0x3C6EF372)
         clip = None
@@ -725,9 +792,9 @@ class AdamW(torch.optim.Optimizer):
             self._norm = _norm_launch(plan.address, len(entries), device, self.max_grad_norm)
             clip = self._norm.data_ptr() + 4
         with N.prof("optim.adamw"):
-            N.call("cs_adamw_step", len(entries), plan.address, len(numbers), sets.ctypes.data,
-                   keys.ctypes.data, clip, N.stream(device))
-        for e, (_, step) in zip(entries, steps):
+            N.call("cs_adamw_step", len(entries), plan.address, len(keys), plan.sets_address,
+                   plan.keys_address, clip, N.stream(device))
+        for e, step in zip(entries, steps):
             e.step.value = step
 
     # ---- reading and loading
@@ -743,33 +810,45 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"flat_state gives float32, bfloat16 and float16, got {dtype}")
         if align < 1:
             raise ValueError(f"Invalid align: {align}")
-        rows, begins, at, bare, device = [], [], 0, False, None
-        number = -1
-        for group in self.param_groups:
-            for p in group["params"]:
-                number += 1
-                size = -(-p.numel() // align) * align
-                device = device or p.device
-                if p.device != device:
-                    raise NotImplementedError("flat_state needs all parameters on one device")
+        order, sizes = self._entries(), self._sizes
+        number, k, left = -1, 0, sizes[0]
+        for p in self._params:
+            number += 1
+            while left == 0:
+                k += 1
+                left = sizes[k]
+            left -= 1
+            e = order[number]
+            if e is None or not e.fresh():
                 st = self.state.get(p)
+                order[number] = None
                 if st and ("exp_avg" in st or _AVG8 in st):
-                    row = list(self._current(p, number).row)
-                    row[_MASTER] = size
-                    rows.append(row)
-                    begins.append(at)
-                else:
-                    bare = bare or size > 0
-                at += size
-        make = torch.zeros if bare else torch.empty
-        out = (make(at, dtype=dtype, device=device), make(at, dtype=dtype, device=device))
-        if rows:
-            table = np.array(rows, dtype=np.int64)
-            for col, t in ((_P, out[0]), (_G, out[1])):
-                table[:, col] = np.array(begins) * t.element_size() + t.data_ptr()
+                    self._entry(number, k)
+        flat = self._flat
+        key = (self._version, align,
+               [p.numel() for p, e in zip(self._params, order) if e is None])
+        if flat is None or flat[0] != key or not _same(flat[1], order):
+            device = self._params[0].device
+            if any(p.device != device for p in self._params):
+                raise NotImplementedError("flat_state needs all parameters on one device")
+            padded = [-(-p.numel() // align) * align for p in self._params]
+            begins = np.cumsum([0] + padded)
+            here = [i for i, e in enumerate(order) if e is not None]
+            table = np.array([order[i].row for i in here], dtype=np.int64).reshape(-1, 8)
             table[:, _META] &= _EIGHT
+            # Up to the alignment only: a parameter without a state may follow.
+            table[:, _MASTER] = [padded[i] for i in here]
+            flat = self._flat = (key, list(order), device, table, begins[here], int(begins[-1]),
+                                 any(n and e is None for n, e in zip(padded, order)))
+        _, _, device, table, begins, total, bare = flat
+        make = torch.zeros if bare else torch.empty
+        out = (make(total, dtype=dtype, device=device), make(total, dtype=dtype, device=device))
+        if len(table):
+            begins = begins * out[0].element_size()
+            for col, t in ((_P, out[0]), (_G, out[1])):
+                table[:, col] = begins + t.data_ptr()
             with torch.cuda.device(device):
-                N.call("cs_adamw_unpack_state", len(rows), table.ctypes.data,
+                N.call("cs_adamw_unpack_state", len(table), table.ctypes.data,
                        _ADAMW_DTYPES[dtype], N.stream(device))
         return out
 
