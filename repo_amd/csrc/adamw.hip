@@ -98,12 +98,38 @@ template <> struct AwType<kF16> { typedef _Float16 type; };
 template <typename T, int N>
 struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) AwVec { T v[N]; };
 
+typedef float AwFour __attribute__((ext_vector_type(4)));
+typedef float AwTwo __attribute__((ext_vector_type(2)));
+
+// One vector of at most 16 bytes; PAST: past the caches.
+template <bool PAST, typename T, int N>
+__device__ inline AwVec<T, N> aw_get(const T* p) {
+    if constexpr (PAST && sizeof(AwVec<T, N>) == sizeof(AwFour))
+        return __builtin_bit_cast(AwVec<T, N>,
+                                  __builtin_nontemporal_load(reinterpret_cast<const AwFour*>(p)));
+    else if constexpr (PAST && sizeof(AwVec<T, N>) == sizeof(AwTwo))
+        return __builtin_bit_cast(AwVec<T, N>,
+                                  __builtin_nontemporal_load(reinterpret_cast<const AwTwo*>(p)));
+    else
+        return *reinterpret_cast<const AwVec<T, N>*>(p);
+}
+
+template <bool PAST, typename T, int N>
+__device__ inline void aw_put(T* p, const AwVec<T, N>& x) {
+    if constexpr (PAST && sizeof(x) == sizeof(AwFour))
+        __builtin_nontemporal_store(__builtin_bit_cast(AwFour, x), reinterpret_cast<AwFour*>(p));
+    else if constexpr (PAST && sizeof(x) == sizeof(AwTwo))
+        __builtin_nontemporal_store(__builtin_bit_cast(AwTwo, x), reinterpret_cast<AwTwo*>(p));
+    else
+        *reinterpret_cast<AwVec<T, N>*>(p) = x;
+}
+
 // N consecutive elements at element i.  FULL: all of them are there, aligned;
 // otherwise elements past n are 0 and not stored.
-template <int N, bool FULL, typename T>
+template <int N, bool FULL, bool PAST = false, typename T>
 __device__ inline void aw_load(const T* src, int64_t i, int64_t n, float (&out)[N]) {
     if constexpr (FULL) {
-        const AwVec<T, N> x = *reinterpret_cast<const AwVec<T, N>*>(src + i);
+        const AwVec<T, N> x = aw_get<PAST, T, N>(src + i);
 #pragma unroll
         for (int k = 0; k < N; ++k) out[k] = (float)x.v[k];
     } else {
@@ -112,13 +138,13 @@ __device__ inline void aw_load(const T* src, int64_t i, int64_t n, float (&out)[
     }
 }
 
-template <int N, bool FULL, typename T>
+template <int N, bool FULL, bool PAST = false, typename T>
 __device__ inline void aw_store(T* dst, int64_t i, int64_t n, const float (&in)[N]) {
     if constexpr (FULL) {
         AwVec<T, N> x;
 #pragma unroll
         for (int k = 0; k < N; ++k) x.v[k] = (T)in[k];
-        *reinterpret_cast<AwVec<T, N>*>(dst + i) = x;
+        aw_put<PAST>(dst + i, x);
     } else {
 #pragma unroll
         for (int k = 0; k < N; ++k)
@@ -253,7 +279,7 @@ __device__ inline void aw_held(const uint8_t* avg, const uint8_t* sq, int64_t i,
 
 // ---- the step
 
-template <int DT>
+template <int DT, int PAST>
 __device__ inline void aw_step32(const AwTensor& t, const AwSet& s, float clip, int64_t begin,
                                  int64_t end) {
     typedef typename AwType<DT>::type T;
@@ -266,10 +292,10 @@ __device__ inline void aw_step32(const AwTensor& t, const AwSet& s, float clip, 
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int64_t i = base + (u * kAwThreads + threadIdx.x) * 4;
-            aw_load<4, F>(main, i, end, p[u]);
-            aw_load<4, F>((const T*)t.grad, i, end, g[u]);
-            aw_load<4, F>((const float*)t.avg, i, end, m[u]);
-            aw_load<4, F>((const float*)t.sq, i, end, v[u]);
+            aw_load<4, F, PAST == 2>(main, i, end, p[u]);
+            aw_load<4, F, PAST == 2>((const T*)t.grad, i, end, g[u]);
+            aw_load<4, F, PAST != 0>((const float*)t.avg, i, end, m[u]);
+            aw_load<4, F, PAST != 0>((const float*)t.sq, i, end, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -277,10 +303,10 @@ __device__ inline void aw_step32(const AwTensor& t, const AwSet& s, float clip, 
 #pragma unroll
             for (int k = 0; k < 4; ++k)
                 aw_update(s, g[u][k] * clip, p[u][k], m[u][k], v[u][k], root);
-            aw_store<4, F>(main, i, end, p[u]);
-            if (DT != kF32) aw_store<4, F>((T*)t.param, i, end, p[u]);
-            aw_store<4, F>((float*)t.avg, i, end, m[u]);
-            aw_store<4, F>((float*)t.sq, i, end, v[u]);
+            aw_store<4, F, PAST == 2>(main, i, end, p[u]);
+            if (DT != kF32) aw_store<4, F, PAST == 2>((T*)t.param, i, end, p[u]);
+            aw_store<4, F, PAST != 0>((float*)t.avg, i, end, m[u]);
+            aw_store<4, F, PAST != 0>((float*)t.sq, i, end, v[u]);
         }
     });
 }
@@ -314,6 +340,9 @@ __device__ inline void aw_step8(const AwTensor& t, const AwSet& s, float clip, i
     });
 }
 
+// PAST: 1 the moments of 32 bits, which nothing reads before the next step, go past
+// the caches; 2 all of a tensor with them does.
+template <int PAST>
 __global__ __launch_bounds__(kAwThreads) void k_adamw(AwArgs a) {
     const int k = aw_find(a);
     const AwTensor& t = a.t[k];
@@ -322,9 +351,9 @@ __global__ __launch_bounds__(kAwThreads) void k_adamw(AwArgs a) {
     const int64_t begin = (int64_t)(blockIdx.x - t.first_block) * a.chunk;
     const int64_t end = begin + a.chunk < t.n ? begin + a.chunk : t.n;
     switch (t.meta & 0x1F) {
-        case kF32: aw_step32<kF32>(t, s, clip, begin, end); break;
-        case kBF16: aw_step32<kBF16>(t, s, clip, begin, end); break;
-        case kF16: aw_step32<kF16>(t, s, clip, begin, end); break;
+        case kF32: aw_step32<kF32, PAST>(t, s, clip, begin, end); break;
+        case kBF16: aw_step32<kBF16, PAST>(t, s, clip, begin, end); break;
+        case kF16: aw_step32<kF16, PAST>(t, s, clip, begin, end); break;
         case kF32 | 16: aw_step8<kF32>(t, s, clip, begin, end); break;
         case kBF16 | 16: aw_step8<kBF16>(t, s, clip, begin, end); break;
         case kF16 | 16: aw_step8<kF16>(t, s, clip, begin, end); break;
@@ -415,18 +444,37 @@ struct NormArgs {
     int32_t n;
 };
 
+// Vectors of 16 bytes, kNormAhead of them in flight a thread.
+constexpr int kNormAhead = 4;
+
 template <int DT>
 __device__ inline float norm_squares(const NormTensor& t, int64_t begin, int64_t end) {
     typedef typename AwType<DT>::type T;
-    const bool vec = (t.meta >> 5) & 1;
+    constexpr int N = 16 / sizeof(T);
+    constexpr int64_t step = (int64_t)kAwThreads * N;
+    const T* src = (const T*)t.grad;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    aw_passes(begin, end, vec, [&](auto full, int64_t base) {
-        constexpr bool F = decltype(full)::value;
-        float g[8];
-        aw_load<8, F>((const T*)t.grad, base + threadIdx.x * 8, end, g);
+    int64_t i = begin + threadIdx.x * N;
+    if ((t.meta >> 5) & 1)
+        for (; i + (kNormAhead - 1) * step + N <= end; i += kNormAhead * step) {
+            AwVec<T, N> g[kNormAhead];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s[k & 3] = __builtin_fmaf(g[k], g[k], s[k & 3]);
-    });
+            for (int u = 0; u < kNormAhead; ++u)
+                g[u] = *reinterpret_cast<const AwVec<T, N>*>(src + i + u * step);
+#pragma unroll
+            for (int u = 0; u < kNormAhead; ++u)
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const float x = (float)g[u].v[k];
+                    s[k & 3] = __builtin_fmaf(x, x, s[k & 3]);
+                }
+        }
+    for (; i < end; i += step) {
+        float g[N];
+        aw_load<N, false>(src, i, end, g);
+#pragma unroll
+        for (int k = 0; k < N; ++k) s[k & 3] = __builtin_fmaf(g[k], g[k], s[k & 3]);
+    }
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
@@ -486,6 +534,18 @@ namespace {
 
 enum AwOp { kStep, kPack, kUnpack };
 
+// One pass a workgroup (bf16, 197M weights, 8-bit states: 8192 workgroups of many
+// passes 660 us, one pass each 617), more only beyond 2^32 elements.
+constexpr int64_t kAwBlocks = (int64_t)1 << 21;
+
+// The moments go past the caches where a step moves more than the memory-side cache
+// holds (fp32, us with and without: 10.1M weights, 283 MB, 43.8 and 47.6; 6.4M, 179
+// MB, 29.8 and 28.4); the weights and gradients too where they alone are more than
+// it holds (bf16, 197M, us: nothing 1027, the moments 1010, all 920; fp32, 16.3M:
+// 87, 68, 75).
+constexpr int64_t kAwPastBytes = (int64_t)224 << 20;
+constexpr int64_t kAwPastWeights = (int64_t)256 << 20;
+
 // table: [n][8] = param, grad, master, exp_avg, exp_avg_sq, numel, dtype | eight << 4 |
 // set << 8, ordinal.
 int aw_run(AwOp op, int32_t ntensors, const int64_t* table, int32_t nsets, const float* sets,
@@ -493,7 +553,7 @@ int aw_run(AwOp op, int32_t ntensors, const int64_t* table, int32_t nsets, const
            hipStream_t stream) {
     if (ntensors < 0 || (ntensors > 0 && !table) || out_dtype < kF32 || out_dtype > kF16)
         return CS_ERR_ARGS;
-    int64_t total = 0;
+    int64_t total = 0, bytes = 0, weights = 0;
     for (int k = 0; k < ntensors; ++k) {
         const int64_t* row = table + 8 * (int64_t)k;
         const int64_t n = row[5], meta = row[6];
@@ -514,9 +574,12 @@ int aw_run(AwOp op, int32_t ntensors, const int64_t* table, int32_t nsets, const
             (op == kPack && (!aw_aligned((void*)row[0], 8) || !aw_aligned((void*)row[1], 8))))
             return CS_ERR_ARGS;
         total += op == kUnpack ? row[2] : n;
+        bytes += n * (eight ? 16 : 28);
+        weights += n * 8;
     }
     if (total == 0) return CS_OK;
-    const int64_t chunk = aw_chunk(total, 8192);
+    const int64_t chunk = aw_chunk(total, kAwBlocks);
+    const int past = weights > kAwPastWeights ? 2 : bytes > kAwPastBytes;
     int k = 0;
     while (k < ntensors) {
         AwArgs a;
@@ -561,8 +624,12 @@ int aw_run(AwOp op, int32_t ntensors, const int64_t* table, int32_t nsets, const
         a.chunk = chunk;
         a.out_dtype = out_dtype;
         const dim3 grid((unsigned)blocks), block(kAwThreads);
-        if (op == kStep)
-            hipLaunchKernelGGL(k_adamw, grid, block, 0, stream, a);
+        if (op == kStep && past == 2)
+            hipLaunchKernelGGL((k_adamw<2>), grid, block, 0, stream, a);
+        else if (op == kStep && past == 1)
+            hipLaunchKernelGGL((k_adamw<1>), grid, block, 0, stream, a);
+        else if (op == kStep)
+            hipLaunchKernelGGL((k_adamw<0>), grid, block, 0, stream, a);
         else if (op == kPack)
             hipLaunchKernelGGL(k_adamw_pack, grid, block, 0, stream, a);
         else
