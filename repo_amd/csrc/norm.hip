@@ -19,7 +19,6 @@
 // relative to its first value per channel, and (count, mean, sum of squared
 // deviations) are what is joined, so a mean far from zero costs nothing.
 #include <hip/hip_runtime.h>
-#include <math.h>
 #include <stdint.h>
 
 #include "../../include/cubicsplat_hip.h"
@@ -149,11 +148,28 @@ __device__ inline float gn_sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
 }
 
+// The normal distribution's tail below -|z| and e = exp(-z^2 / 2): erfc(x) = t P(t)
+// exp(-x^2), t = 1 / (1 + p x), Abramowitz and Stegun 7.1.26, within 1.5e-7.
+__device__ inline float gn_tail(float z, float* e) {
+    const float x = __builtin_fabsf(z);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(x, 0.3275911f * 0.70710678f, 1.0f));
+    *e = __expf(-0.5f * z * z);
+    float q = __builtin_fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+    q = __builtin_fmaf(t, q, 0.5f * 1.421413741f);
+    q = __builtin_fmaf(t, q, 0.5f * -0.284496736f);
+    q = __builtin_fmaf(t, q, 0.5f * 0.254829592f);
+    return q * t * *e;
+}
+
 template <int ACT>
 __device__ inline float gn_act(float z) {
     if (ACT == kActRelu) return z < 0.0f ? 0.0f : z;  // NaN stays
     if (ACT == kActSilu) return z * gn_sigmoid(z);
-    if (ACT == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+    if (ACT == kActGelu) {
+        float e;
+        const float q = z * gn_tail(z, &e);
+        return z > 0.0f ? z - q : q;
+    }
     return z;
 }
 
@@ -165,8 +181,9 @@ __device__ inline float gn_slope(float z) {
         return __builtin_fmaf(p, __builtin_fmaf(-z, p, z), p);
     }
     if (ACT == kActGelu) {
-        const float p = 0.5f * (1.0f + erff(z * 0.70710678f));
-        return __builtin_fmaf(z * 0.39894228f, __expf(-0.5f * z * z), p);
+        float e;
+        const float q = gn_tail(z, &e);
+        return __builtin_fmaf(z * 0.39894228f, e, z > 0.0f ? 1.0f - q : q);
     }
     return 1.0f;
 }

@@ -9,6 +9,7 @@ libcubicsplat_hip.so, in fp32 whatever the images' type.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -37,6 +38,11 @@ def _empty_channels_last(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t.movedim(1, -1), memory_format=torch.contiguous_format).movedim(-1, 1)
 
 
+@lru_cache(maxsize=1024)
+def _workspace_elems(n, s, c, groups, dtype, backward):
+    return int(N.lib().cs_group_norm_workspace_elems(n, s, c, groups, dtype, backward))
+
+
 def _param_ptr(p):
     return None if p is None else p.data_ptr()
 
@@ -48,8 +54,8 @@ def _forward(x, groups, weight, bias, eps, act, stats):
     s = x.numel() // (n * c)
     y = _empty_channels_last(x)
     dtype = _DTYPES[x.dtype]
-    work = torch.empty(N.lib().cs_group_norm_workspace_elems(n, s, c, groups, dtype, 0),
-                       dtype=torch.float32, device=x.device)
+    work = torch.empty(_workspace_elems(n, s, c, groups, dtype, 0), dtype=torch.float32,
+                       device=x.device)
     saved, mean, rstd = None, None, None
     if stats:
         saved = torch.empty((2, n, groups), dtype=torch.float32, device=x.device)
@@ -84,8 +90,8 @@ class _GroupNorm(torch.autograd.Function):
         dx = _empty_channels_last(x) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty_like(bias) if need_b else None
-        work = torch.empty(N.lib().cs_group_norm_workspace_elems(n, s, c, groups, dtype, 1),
-                           dtype=torch.float32, device=x.device)
+        work = torch.empty(_workspace_elems(n, s, c, groups, dtype, 1), dtype=torch.float32,
+                           device=x.device)
         affine = weight if weight is not None else bias
         mean = saved.data_ptr()
         with N.prof("norm.bwd"):
