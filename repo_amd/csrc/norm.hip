@@ -362,44 +362,69 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_stats(GnArgs a) {
     }
 }
 
+// The values that one partial result of a group stands for.
+__device__ inline float gn_weight(const GnShape& h, int chunk, int part) {
+    const int64_t left = h.s - chunk * h.rows;
+    const int width = h.d - part * h.cs < h.cs ? h.d - part * h.cs : h.cs;
+    return (float)(left < h.rows ? left : h.rows) * (float)(h.parts > 1 ? width : h.d);
+}
+
 // Joins a slice's partial means and deviations: mean and 1 / sqrt(var + eps)
-// of its groups into LDS.
+// of its groups into LDS.  A lane holds HELD of them, so that they are loaded
+// together and once; what is beyond is read twice.
+constexpr int kGnHeld = 12, kGnHeldInline = 4;  // as many as there are, mostly
+
+template <int HELD>
 __device__ inline void gn_join_stats(const GnArgs& a, const GnPlace& q, int n, float* mean,
                                      float* rstd) {
     const GnShape& h = a.h;
     const int t = gn_lanes(q.ng), lane = threadIdx.x & (t - 1), step = kGnThreads / t;
     const int entries = h.chunks * h.parts;
+    const float2* all = (const float2*)a.partials + (int64_t)n * h.chunks * h.groups * h.parts;
+    const int64_t row = (int64_t)h.groups * h.parts;
     for (int base = 0; base < q.ng; base += step) {
         const int g = base + threadIdx.x / t;
-        float sw = 0.0f, swm = 0.0f;
-        const float* p = a.partials + ((int64_t)n * h.chunks * h.groups + q.g0 + g) * h.parts * 2;
-        if (g < q.ng)
-            for (int i = lane; i < entries; i += t) {
-                const int chunk = i / h.parts, part = i - chunk * h.parts;
-                const int64_t left = h.s - chunk * h.rows;
-                const int width = h.d - part * h.cs < h.cs ? h.d - part * h.cs : h.cs;
-                const float w = (float)(left < h.rows ? left : h.rows) *
-                                (float)(h.parts > 1 ? width : h.d);
-                const float m = p[((int64_t)chunk * h.groups * h.parts + part) * 2];
-                sw += w;
-                swm = __builtin_fmaf(w, m, swm);
+        const bool in = g < q.ng;
+        const float2* p = all + (int64_t)(q.g0 + g) * h.parts;
+        float2 v[HELD];
+        float w[HELD], sw = 0.0f, swm = 0.0f;
+#pragma unroll
+        for (int u = 0; u < HELD; ++u) {
+            const int i = lane + u * t, chunk = i / h.parts, part = i - chunk * h.parts;
+            v[u] = make_float2(0.0f, 0.0f);
+            w[u] = 0.0f;
+            if (in && i < entries) {
+                v[u] = p[chunk * row + part];
+                w[u] = gn_weight(h, chunk, part);
             }
+        }
+#pragma unroll
+        for (int u = 0; u < HELD; ++u) {
+            sw += w[u];
+            swm = __builtin_fmaf(w[u], v[u].x, swm);
+        }
+        for (int i = lane + HELD * t; in && i < entries; i += t) {
+            const int chunk = i / h.parts, part = i - chunk * h.parts;
+            const float m = gn_weight(h, chunk, part);
+            sw += m;
+            swm = __builtin_fmaf(m, p[chunk * row + part].x, swm);
+        }
         sw = gn_lanes_sum(sw, t);
         const float mu = gn_lanes_sum(swm, t) / sw;
         float m2 = 0.0f;
-        if (g < q.ng)
-            for (int i = lane; i < entries; i += t) {
-                const int chunk = i / h.parts, part = i - chunk * h.parts;
-                const int64_t left = h.s - chunk * h.rows;
-                const int width = h.d - part * h.cs < h.cs ? h.d - part * h.cs : h.cs;
-                const float w = (float)(left < h.rows ? left : h.rows) *
-                                (float)(h.parts > 1 ? width : h.d);
-                const float* e = p + ((int64_t)chunk * h.groups * h.parts + part) * 2;
-                const float dm = e[0] - mu;
-                m2 += __builtin_fmaf(w * dm, dm, e[1]);
-            }
+#pragma unroll
+        for (int u = 0; u < HELD; ++u) {
+            const float dm = v[u].x - mu;
+            m2 += __builtin_fmaf(w[u] * dm, dm, v[u].y);
+        }
+        for (int i = lane + HELD * t; in && i < entries; i += t) {
+            const int chunk = i / h.parts, part = i - chunk * h.parts;
+            const float2 e = p[chunk * row + part];
+            const float dm = e.x - mu;
+            m2 += __builtin_fmaf(gn_weight(h, chunk, part) * dm, dm, e.y);
+        }
         m2 = gn_lanes_sum(m2, t);
-        if (g < q.ng && lane == 0) {
+        if (in && lane == 0) {
             mean[g] = mu;
             rstd[g] = 1.0f / __builtin_sqrtf(m2 / sw + a.eps);
         }
@@ -423,7 +448,7 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_join_stats(GnArgs a) {
     __shared__ float gmean[kGnThreads], grstd[kGnThreads];
     int n;
     const GnPlace q = gn_join_place(a.h, blockIdx.x, &n);
-    gn_join_stats(a, q, n, gmean, grstd);
+    gn_join_stats<kGnHeld>(a, q, n, gmean, grstd);
     for (int g = threadIdx.x; g < q.ng; g += kGnThreads) {
         a.mean[(int64_t)n * a.h.groups + q.g0 + g] = gmean[g];
         a.rstd[(int64_t)n * a.h.groups + q.g0 + g] = grstd[g];
@@ -449,7 +474,7 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_apply(GnArgs a) {
         }
         __syncthreads();
     } else {
-        gn_join_stats(a, q, n, gmean, grstd);
+        gn_join_stats<kGnHeldInline>(a, q, n, gmean, grstd);
     }
     if (a.mean && !a.joined && chunk == 0 && q.part == 0)
         for (int g = threadIdx.x; g < q.ng; g += kGnThreads) {
@@ -604,6 +629,7 @@ __device__ inline void gn_channel_grads(const GnArgs& a, int block) {
 }
 
 // E[w dz] and E[w dz xh] of a slice's groups.
+template <int HELD>
 __device__ inline void gn_join_sums(const GnArgs& a, const GnPlace& q, int n, float* g1,
                                     float* g2) {
     const GnShape& h = a.h;
@@ -615,13 +641,21 @@ __device__ inline void gn_join_sums(const GnArgs& a, const GnPlace& q, int n, fl
         float sa = 0.0f, sb = 0.0f;
         const float2* p = (const float2*)a.partials +
                           ((int64_t)n * h.chunks * h.groups + q.g0 + g) * h.parts;
-        if (g < q.ng)
-            for (int i = lane; i < entries; i += t) {
-                const int ch = i / h.parts, part = i - ch * h.parts;
-                const float2 v = p[(int64_t)ch * h.groups * h.parts + part];
-                sa += v.x;
-                sb += v.y;
+        const int64_t row = (int64_t)h.groups * h.parts;
+        for (int first = lane; g < q.ng && first < entries; first += HELD * t) {
+            float2 v[HELD];
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) {
+                const int i = first + u * t, ch = i / h.parts, part = i - ch * h.parts;
+                v[u] = make_float2(0.0f, 0.0f);
+                if (i < entries) v[u] = p[ch * row + part];
             }
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) {
+                sa += v[u].x;
+                sb += v[u].y;
+            }
+        }
         sa = gn_lanes_sum(sa, t);
         sb = gn_lanes_sum(sb, t);
         if (g < q.ng && lane == 0) {
@@ -640,7 +674,7 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_join_sums(GnArgs a) {
     }
     int n;
     const GnPlace q = gn_join_place(a.h, blockIdx.x - a.channel_blocks, &n);
-    gn_join_sums(a, q, n, g1, g2);
+    gn_join_sums<kGnHeld>(a, q, n, g1, g2);
     for (int g = threadIdx.x; g < q.ng; g += kGnThreads)
         ((float2*)a.groups_out)[(int64_t)n * a.h.groups + q.g0 + g] = make_float2(g1[g], g2[g]);
 }
@@ -664,7 +698,7 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_apply(GnArgs a) {
         }
         __syncthreads();
     } else {
-        gn_join_sums(a, q, n, g1, g2);
+        gn_join_sums<kGnHeldInline>(a, q, n, g1, g2);
     }
     if (!q.live) return;
     // dx = (r w) dz - r E[w dz] - (x - mean) r^2 E[w dz xh]
