@@ -78,7 +78,7 @@ __host__ __device__ inline uint32_t aw_mix(uint32_t x) {
     return x ^ (x >> 16);
 }
 
-// The hash's argument for element i, a multiple of 8; the seven after it follow.
+// The hash's argument for element i, a multiple of 4; the three after it follow.
 __device__ inline uint32_t aw_key(uint32_t key, int64_t i) {
     return key + (uint32_t)i + (uint32_t)(i >> 32) * 0x3C6EF372u;
 }
@@ -197,8 +197,8 @@ __device__ inline uint32_t aw_encode(float x, int e, uint32_t r16) {
     return c;
 }
 
-// The largest of the 16 lanes of a row.
-__device__ inline float aw_row_max(float x) {
+// The largest of the 32 lanes that hold a block.
+__device__ inline float aw_block_max(float x) {
 #define CS_ROW_MAX(ctrl)                                                                   \
     x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(                               \
                      0, __float_as_int(x), ctrl, 0xF, 0xF, true)))
@@ -207,71 +207,74 @@ __device__ inline float aw_row_max(float x) {
     CS_ROW_MAX(0x122);
     CS_ROW_MAX(0x121);
 #undef CS_ROW_MAX
-    return x;
+    // Both rows of 16 have their own; the odd rows of one copy change places with the
+    // even rows of the other.
+    const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x),
+                                                       false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
 }
 
-__device__ inline int aw_shared_exponent(const float (&x)[8]) {
+__device__ inline int aw_shared_exponent(const float (&x)[4]) {
     float top = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 4; ++k) {
         const float a = __builtin_fabsf(x[k]);
         top = a < __builtin_inff() ? fmaxf(top, a) : top;
     }
-    return (int)(__float_as_uint(aw_row_max(top)) >> 23);
+    return (int)(__float_as_uint(aw_block_max(top)) >> 23);
 }
 
-// The 8 bytes of a lane; the code arrays are whole blocks, so all 8 exist
+// The four or eight bytes of a lane; the code arrays are whole blocks, so all exist
 // wherever the lane's first element does.
-__device__ inline void aw_load_codes(const uint8_t* src, int64_t i, bool in, uint32_t (&c)[8]) {
-    uint2 w = make_uint2(0u, 0u);
-    if (in) w = *reinterpret_cast<const uint2*>(src + i);
+template <int N>
+__device__ inline void aw_load_codes(const uint8_t* src, int64_t i, bool in, uint32_t (&c)[N]) {
+    uint32_t w[N / 4] = {};
+    if (in) __builtin_memcpy(w, __builtin_assume_aligned(src + i, N), N);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) c[k] = ((k < 4 ? w.x : w.y) >> (8 * (k & 3))) & 0xFFu;
+    for (int k = 0; k < N; ++k) c[k] = (w[k / 4] >> (8 * (k & 3))) & 0xFFu;
 }
 
-__device__ inline void aw_store_codes(uint8_t* dst, int64_t i, bool in, const uint32_t (&c)[8]) {
-    uint2 w;
-    w.x = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-    w.y = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
-    if (in) *reinterpret_cast<uint2*>(dst + i) = w;
+__device__ inline void aw_store_codes(uint8_t* dst, int64_t i, bool in, const uint32_t (&c)[4]) {
+    if (in)
+        *reinterpret_cast<uint32_t*>(dst + i) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
 }
 
 __device__ inline int64_t aw_blocks(int64_t n) { return (n + kBlk - 1) / kBlk; }
 
-// Encodes and stores a lane's 8 values of m and root; every lane of the wave
+// Encodes and stores a lane's four values of m and root; every lane of the wave
 // takes part.
 template <bool FULL>
 __device__ inline void aw_hold(uint8_t* avg, uint8_t* sq, int64_t i, int64_t n,
-                               const float (&m)[8], const float (&root)[8],
-                               const uint32_t (&r)[8]) {
+                               const float (&m)[4], const float (&root)[4],
+                               const uint32_t (&r)[4]) {
     const bool in = FULL || i < n;
     const int em = aw_shared_exponent(m), er = aw_shared_exponent(root);
-    uint32_t cm[8], cr[8];
+    uint32_t cm[4], cr[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 4; ++k) {
         cm[k] = aw_encode<3, false>(m[k], em, r[k] & 0xFFFFu);
         cr[k] = aw_encode<4, true>(root[k], er, r[k] >> 16);
     }
     aw_store_codes(avg, i, in, cm);
     aw_store_codes(sq, i, in, cr);
-    if (in && (threadIdx.x & 15) == 0) {
+    if (in && (threadIdx.x & 31) == 0) {
         const int64_t b = aw_blocks(n) * kBlk + i / kBlk;
         avg[b] = (uint8_t)em;
         sq[b] = (uint8_t)er;
     }
 }
 
-template <bool FULL>
+template <bool FULL, int N>
 __device__ inline void aw_held(const uint8_t* avg, const uint8_t* sq, int64_t i, int64_t n,
-                               float (&m)[8], float (&root)[8]) {
+                               float (&m)[N], float (&root)[N]) {
     const bool in = FULL || i < n;
     const int64_t b = aw_blocks(n) * kBlk + i / kBlk;
     const int em = in ? avg[b] : 0, er = in ? sq[b] : 0;
-    uint32_t cm[8], cr[8];
+    uint32_t cm[N], cr[N];
     aw_load_codes(avg, i, in, cm);
     aw_load_codes(sq, i, in, cr);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < N; ++k) {
         m[k] = aw_decode<3>(cm[k], em);
         root[k] = aw_decode<4>(cr[k], er);
     }
@@ -311,7 +314,7 @@ __device__ inline void aw_step32(const AwTensor& t, const AwSet& s, float clip, 
     });
 }
 
-template <int DT>
+template <int DT, int PAST>
 __device__ inline void aw_step8(const AwTensor& t, const AwSet& s, float clip, int64_t begin,
                                 int64_t end) {
     typedef typename AwType<DT>::type T;
@@ -319,29 +322,38 @@ __device__ inline void aw_step8(const AwTensor& t, const AwSet& s, float clip, i
     float* main = DT == kF32 ? (float*)t.param : t.master;
     aw_passes(begin, end, vec, [&](auto full, int64_t base) {
         constexpr bool F = decltype(full)::value;
-        const int64_t i = base + threadIdx.x * 8;
-        float p[8], g[8], m[8], root[8];
-        uint32_t r[8];
-        aw_load<8, F>(main, i, t.n, p);
-        aw_load<8, F>((const T*)t.grad, i, t.n, g);
-        aw_held<F>((const uint8_t*)t.avg, (const uint8_t*)t.sq, i, t.n, m, root);
-        const uint32_t key = aw_key(t.key, i);
+        // Two vectors of four a thread, their loads in flight together.
+        float p[2][4], g[2][4], m[2][4], root[2][4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            float v = root[k] * root[k];
-            aw_update(s, g[k] * clip, p[k], m[k], v, root[k]);
-            r[k] = aw_mix(key + k);
-            // Elements past the end do not set a block's exponent.
-            if (!F && i + k >= t.n) m[k] = root[k] = 0.0f;
+        for (int u = 0; u < 2; ++u) {
+            const int64_t i = base + (u * kAwThreads + threadIdx.x) * 4;
+            aw_load<4, F, PAST != 0>(main, i, t.n, p[u]);
+            aw_load<4, F, PAST != 0>((const T*)t.grad, i, t.n, g[u]);
+            aw_held<F, 4>((const uint8_t*)t.avg, (const uint8_t*)t.sq, i, t.n, m[u], root[u]);
         }
-        aw_store<8, F>(main, i, t.n, p);
-        if (DT != kF32) aw_store<8, F>((T*)t.param, i, t.n, p);
-        aw_hold<F>((uint8_t*)t.avg, (uint8_t*)t.sq, i, t.n, m, root, r);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int64_t i = base + (u * kAwThreads + threadIdx.x) * 4;
+            const uint32_t key = aw_key(t.key, i);
+            uint32_t r[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float v = root[u][k] * root[u][k];
+                aw_update(s, g[u][k] * clip, p[u][k], m[u][k], v, root[u][k]);
+                r[k] = aw_mix(key + k);
+                // Elements past the end do not set a block's exponent.
+                if (!F && i + k >= t.n) m[u][k] = root[u][k] = 0.0f;
+            }
+            aw_store<4, F, PAST != 0>(main, i, t.n, p[u]);
+            if (DT != kF32) aw_store<4, F, PAST != 0>((T*)t.param, i, t.n, p[u]);
+            aw_hold<F>((uint8_t*)t.avg, (uint8_t*)t.sq, i, t.n, m[u], root[u], r);
+        }
     });
 }
 
 // PAST: 1 the moments of 32 bits, which nothing reads before the next step, go past
-// the caches; 2 all of a tensor with them does.
+// the caches, and the weights and gradients of tensors with 8-bit ones, whose codes
+// are the smaller part; 2 the weights and gradients of all.
 template <int PAST>
 __global__ __launch_bounds__(kAwThreads) void k_adamw(AwArgs a) {
     const int k = aw_find(a);
@@ -354,9 +366,9 @@ __global__ __launch_bounds__(kAwThreads) void k_adamw(AwArgs a) {
         case kF32: aw_step32<kF32, PAST>(t, s, clip, begin, end); break;
         case kBF16: aw_step32<kBF16, PAST>(t, s, clip, begin, end); break;
         case kF16: aw_step32<kF16, PAST>(t, s, clip, begin, end); break;
-        case kF32 | 16: aw_step8<kF32>(t, s, clip, begin, end); break;
-        case kBF16 | 16: aw_step8<kBF16>(t, s, clip, begin, end); break;
-        case kF16 | 16: aw_step8<kF16>(t, s, clip, begin, end); break;
+        case kF32 | 16: aw_step8<kF32, PAST>(t, s, clip, begin, end); break;
+        case kBF16 | 16: aw_step8<kBF16, PAST>(t, s, clip, begin, end); break;
+        case kF16 | 16: aw_step8<kF16, PAST>(t, s, clip, begin, end); break;
     }
 }
 
@@ -370,21 +382,26 @@ __global__ __launch_bounds__(kAwThreads) void k_adamw_pack(AwArgs a) {
     const int64_t end = begin + a.chunk < t.n ? begin + a.chunk : t.n;
     aw_passes(begin, end, vec, [&](auto full, int64_t base) {
         constexpr bool F = decltype(full)::value;
-        const int64_t i = base + threadIdx.x * 8;
-        float m[8], root[8];
-        uint32_t r[8];
-        aw_load<8, F>((const float*)t.avg, i, t.n, m);
-        aw_load<8, F>((const float*)t.sq, i, t.n, root);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            root[k] = __builtin_sqrtf(root[k]);
-            r[k] = 0x80008000u;  // one half of a spacing: to nearest
+        for (int u = 0; u < 2; ++u) {
+            const int64_t i = base + (u * kAwThreads + threadIdx.x) * 4;
+            float m[4], root[4];
+            uint32_t r[4];
+            aw_load<4, F>((const float*)t.avg, i, t.n, m);
+            aw_load<4, F>((const float*)t.sq, i, t.n, root);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                root[k] = __builtin_sqrtf(root[k]);
+                r[k] = 0x80008000u;  // one half of a spacing: to nearest
+            }
+            aw_hold<F>((uint8_t*)t.param, (uint8_t*)t.grad, i, t.n, m, root, r);
         }
-        aw_hold<F>((uint8_t*)t.param, (uint8_t*)t.grad, i, t.n, m, root, r);
     });
 }
 
-template <typename T>
+// PAST: 16-bit values go past the caches (bf16, 54.5M values of each moment, 63 and
+// 50 us; fp32 values lie 32 bytes a lane, in two stores that only the cache joins).
+template <typename T, bool PAST>
 __device__ inline void aw_unpack(const AwTensor& t, int64_t begin, int64_t end) {
     const bool vec = (t.meta >> 5) & 1, eight = (t.meta >> 4) & 1;
     const int64_t n = (int64_t)(intptr_t)t.master;  // with what follows the values
@@ -395,7 +412,7 @@ __device__ inline void aw_unpack(const AwTensor& t, int64_t begin, int64_t end) 
         const int64_t i = base + threadIdx.x * 8;
         float m[8], v[8];
         if (eight) {
-            aw_held<F>((const uint8_t*)t.avg, (const uint8_t*)t.sq, i, t.n, m, v);
+            aw_held<F, 8>((const uint8_t*)t.avg, (const uint8_t*)t.sq, i, t.n, m, v);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const bool in = F || i + k < t.n;
@@ -406,22 +423,23 @@ __device__ inline void aw_unpack(const AwTensor& t, int64_t begin, int64_t end) 
             aw_load<8, F>((const float*)t.avg, i, t.n, m);
             aw_load<8, F>((const float*)t.sq, i, t.n, v);
         }
-        aw_store<8, F>((T*)t.param, i, n, m);
-        aw_store<8, F>((T*)const_cast<void*>(t.grad), i, n, v);
+        aw_store<8, F, PAST && sizeof(T) == 2>((T*)t.param, i, n, m);
+        aw_store<8, F, PAST && sizeof(T) == 2>((T*)const_cast<void*>(t.grad), i, n, v);
     };
     if (whole > begin) aw_passes(begin, whole, vec, pass);
     aw_passes(whole > begin ? whole : begin, end, false, pass);
 }
 
+template <bool PAST>
 __global__ __launch_bounds__(kAwThreads) void k_adamw_unpack(AwArgs a) {
     const AwTensor& t = a.t[aw_find(a)];
     const int64_t n = (int64_t)(intptr_t)t.master;
     const int64_t begin = (int64_t)(blockIdx.x - t.first_block) * a.chunk;
     const int64_t end = begin + a.chunk < n ? begin + a.chunk : n;
     switch (a.out_dtype) {
-        case kF32: aw_unpack<float>(t, begin, end); break;
-        case kBF16: aw_unpack<__bf16>(t, begin, end); break;
-        case kF16: aw_unpack<_Float16>(t, begin, end); break;
+        case kF32: aw_unpack<float, PAST>(t, begin, end); break;
+        case kBF16: aw_unpack<__bf16, PAST>(t, begin, end); break;
+        case kF16: aw_unpack<_Float16, PAST>(t, begin, end); break;
     }
 }
 
@@ -542,9 +560,11 @@ constexpr int64_t kAwBlocks = (int64_t)1 << 21;
 // holds (fp32, us with and without: 10.1M weights, 283 MB, 43.8 and 47.6; 6.4M, 179
 // MB, 29.8 and 28.4); the weights and gradients too where they alone are more than
 // it holds (bf16, 197M, us: nothing 1027, the moments 1010, all 920; fp32, 16.3M:
-// 87, 68, 75).
+// 87, 68, 75).  With 8-bit states the weights and gradients: 197M 580 and 539, 16.3M
+// (261 MB) 49.7 and 46.4, 6.4M (102 MB) 21.4 and 21.8.
 constexpr int64_t kAwPastBytes = (int64_t)224 << 20;
 constexpr int64_t kAwPastWeights = (int64_t)256 << 20;
+constexpr int64_t kAwPastValues = (int64_t)64 << 20;
 
 // table: [n][8] = param, grad, master, exp_avg, exp_avg_sq, numel, dtype | eight << 4 |
 // set << 8, ordinal.
@@ -632,8 +652,10 @@ int aw_run(AwOp op, int32_t ntensors, const int64_t* table, int32_t nsets, const
             hipLaunchKernelGGL((k_adamw<0>), grid, block, 0, stream, a);
         else if (op == kPack)
             hipLaunchKernelGGL(k_adamw_pack, grid, block, 0, stream, a);
+        else if (total * 4 > kAwPastValues)
+            hipLaunchKernelGGL((k_adamw_unpack<true>), grid, block, 0, stream, a);
         else
-            hipLaunchKernelGGL(k_adamw_unpack, grid, block, 0, stream, a);
+            hipLaunchKernelGGL((k_adamw_unpack<false>), grid, block, 0, stream, a);
         if (hipGetLastError() != hipSuccess) return CS_ERR_HIP;
     }
     return CS_OK;
