@@ -70,6 +70,8 @@ struct AwArgs {
     int32_t out_dtype;
 };
 
+static_assert(sizeof(AwArgs) <= 4096, "kernel arguments");
+
 __host__ __device__ inline uint32_t aw_mix(uint32_t x) {
     x ^= x >> 16;
     x *= 0x9E3779B9u;

@@ -145,6 +145,9 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
         weight = weight.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
+    if x.device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(x.device):
+            return group_norm(x, num_groups, weight, bias, eps, activation)
     x = _channels_last(x)
     act = _ACTIVATIONS[activation]
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
