@@ -61,6 +61,11 @@ def build(verbose: bool = False) -> str:
         # The compiled binding is an optional speed-up: without it the host
         # path calls the same library through ctypes.
         warnings.warn(f"the compiled binding _cs_fast was not built ({e}); using ctypes")
+    from . import torchcall
+    try:
+        torchcall.build(LIB, verbose=verbose)
+    except (OSError, subprocess.CalledProcessError) as e:
+        warnings.warn(f"the extension _cs_torch was not built ({e}); its work is done in Python")
     return LIB
 
 

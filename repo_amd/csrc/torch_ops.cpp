@@ -1,0 +1,257 @@
+// `_cs_torch`, a CPython extension on torch's C++ tensors, for what costs the host
+// most in Python: the autograd node of group norm (its backward then runs in the
+// engine's thread without the interpreter), and the checks that an AdamW step
+// makes of every parameter and gradient.  The kernels are reached through the C
+// ABI of libcubicsplat_hip.so, as everywhere.
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <ATen/ATen.h>
+#include <c10/hip/HIPStream.h>
+
+#include <Python.h>
+#include <optional>
+
+#include "../../include/cubicsplat_hip.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void check(int rc, const char* what) {
+    TORCH_CHECK(rc == CS_OK, what, ": ",
+                rc == CS_ERR_ARGS ? "invalid arguments" : "HIP launch failure", " (status ", rc,
+                ")");
+}
+
+int type_code(const Tensor& t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return 0;
+        case at::kBFloat16: return 1;
+        case at::kHalf: return 2;
+        default: return -1;
+    }
+}
+
+void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+struct Sizes {
+    int64_t n, s;
+    int32_t c;
+    explicit Sizes(const Tensor& x)
+        : n(x.size(0)), s(x.numel() / (x.size(0) * x.size(1))), c((int32_t)x.size(1)) {}
+};
+
+Tensor workspace(const Tensor& x, const Sizes& z, int64_t groups, int backward) {
+    const size_t elems = cs_group_norm_workspace_elems(z.n, z.s, z.c, (int32_t)groups,
+                                                       type_code(x), backward);
+    return at::empty({(int64_t)elems}, x.options().dtype(at::kFloat));
+}
+
+hipStream_t stream(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.device().index()); }
+
+// t if its channels lie together without gaps, else a copy that does.
+Tensor channels_last(const Tensor& t) {
+    const Tensor last = t.movedim(1, -1);
+    return last.is_contiguous() ? t : last.contiguous().movedim(-1, 1);
+}
+
+int affine_code(const Tensor& weight, const Tensor& bias) {
+    return weight.defined() ? type_code(weight) : bias.defined() ? type_code(bias) : 0;
+}
+
+Tensor forward(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups,
+               double eps, int64_t act, Tensor* stats) {
+    const Sizes z(x);
+    Tensor y = at::empty_like(x);
+    const Tensor work = workspace(x, z, groups, 0);
+    float *mean = nullptr, *rstd = nullptr;
+    if (stats) {
+        *stats = at::empty({2, z.n, groups}, x.options().dtype(at::kFloat));
+        mean = stats->data_ptr<float>();
+        rstd = mean + z.n * groups;
+    }
+    check(cs_group_norm_forward(x.data_ptr(), z.n, z.s, z.c, (int32_t)groups, type_code(x),
+                                pointer(weight), pointer(bias), affine_code(weight, bias), eps,
+                                (int32_t)act, work.data_ptr<float>(), mean, rstd, y.data_ptr(),
+                                stream(x)),
+          "cs_group_norm_forward");
+    return y;
+}
+
+struct GroupNorm : torch::autograd::Function<GroupNorm> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x,
+                          const std::optional<Tensor>& given_weight,
+                          const std::optional<Tensor>& given_bias, int64_t groups, double eps,
+                          int64_t act) {
+        const Tensor weight = given_weight.value_or(Tensor()), bias = given_bias.value_or(Tensor());
+        Tensor stats;
+        Tensor y = ::forward(x, weight, bias, groups, eps, act, &stats);
+        ctx->save_for_backward({x, weight, bias, stats});
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["act"] = act;
+        return y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
+        const int64_t groups = ctx->saved_data["groups"].toInt();
+        const Sizes z(x);
+        variable_list out(6);
+        {
+            at::AutoGradMode off(false);
+            const Tensor dy = channels_last(grads[0]);
+            // The node's edges are those of the tensors that there are.
+            if (ctx->needs_input_grad(0)) out[0] = at::empty_like(x);
+            if (weight.defined() && ctx->needs_input_grad(1)) out[1] = at::empty_like(weight);
+            if (bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1))
+                out[2] = at::empty_like(bias);
+            const Tensor work = workspace(x, z, groups, 1);
+            const float* mean = stats.data_ptr<float>();
+            check(cs_group_norm_backward(
+                      x.data_ptr(), dy.data_ptr(), z.n, z.s, z.c, (int32_t)groups, type_code(x),
+                      pointer(weight), pointer(bias), affine_code(weight, bias),
+                      (int32_t)ctx->saved_data["act"].toInt(), mean, mean + z.n * groups,
+                      work.data_ptr<float>(), pointer(out[0]), pointer(out[1]), pointer(out[2]),
+                      stream(x)),
+                  "cs_group_norm_backward");
+        }
+        if (at::GradMode::is_enabled()) {
+            // Under create_graph the gradients get a node that refuses to be
+            // differentiated, rather than none.
+            variable_list given;
+            for (int k = 0; k < 3; ++k)
+                if (out[k].defined()) given.push_back(out[k].detach().set_requires_grad(true));
+            auto refuse = std::make_shared<torch::autograd::DelayedError>(
+                "group_norm is differentiable once", (int)given.size());
+            variable_list refused = (*refuse)(std::move(given));
+            for (int k = 0, j = 0; k < 3; ++k)
+                if (out[k].defined()) out[k] = refused[j++];
+        }
+        return out;
+    }
+};
+
+std::optional<Tensor> optional_tensor(PyObject* o) {
+    if (o == Py_None) return std::nullopt;
+    return THPVariable_Unpack(o);
+}
+
+// group_norm(x, weight | None, bias | None, groups, eps, act): x channels last
+// without gaps, all arguments checked by the caller.
+PyObject* py_group_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(nargs == 6, "group_norm: expected 6 arguments");
+    TORCH_CHECK_TYPE(THPVariable_Check(args[0]), "group_norm: x must be a tensor");
+    for (int k = 1; k < 3; ++k)
+        TORCH_CHECK_TYPE(args[k] == Py_None || THPVariable_Check(args[k]),
+                         "group_norm: weight and bias must be tensors or None");
+    const Tensor& x = THPVariable_Unpack(args[0]);
+    const std::optional<Tensor> weight = optional_tensor(args[1]), bias = optional_tensor(args[2]);
+    const int64_t groups = PyLong_AsLongLong(args[3]), act = PyLong_AsLongLong(args[5]);
+    const double eps = PyFloat_AsDouble(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    TORCH_CHECK_VALUE(x.is_cuda() && type_code(x) >= 0 && x.dim() >= 2 && x.numel() > 0 &&
+                          x.movedim(1, -1).is_contiguous(),
+                      "group_norm: x must be on the GPU, channels last without gaps");
+    for (const auto& p : {weight, bias})
+        TORCH_CHECK_VALUE(!p || (p->device() == x.device() && p->numel() == x.size(1) &&
+                                 type_code(*p) >= 0 && p->is_contiguous()),
+                          "group_norm: weight and bias must lie beside x");
+    const bool grad = at::GradMode::is_enabled() &&
+                      (x.requires_grad() || (weight && weight->requires_grad()) ||
+                       (bias && bias->requires_grad()));
+    Tensor y = grad ? GroupNorm::apply(x, weight, bias, groups, eps, act)
+                    : forward(x, weight.value_or(Tensor()), bias.value_or(Tensor()), groups, eps,
+                              act, nullptr);
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// adamw_current(params, states, keys, tensors, table, steps, gradients): whether
+// each parameter still is what its row of the table (int64 [n][8], by address)
+// says, and each states[i][keys[i][j]] the object tensors[i][j]; with `gradients`,
+// whether each parameter has a gradient that can be read as it is, whose address
+// goes into the row, and whether all step counts (float pointers, by the address of
+// their array) agree.  The count with `gradients`, else 0; -1 where anything is not
+// so.
+PyObject* py_adamw_current(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(nargs == 7, "adamw_current: expected 7 arguments");
+    for (int k = 0; k < 4; ++k)
+        TORCH_CHECK_TYPE(PyList_Check(args[k]) &&
+                             PyList_GET_SIZE(args[k]) == PyList_GET_SIZE(args[0]),
+                         "adamw_current: expected lists of one length");
+    int64_t* table = (int64_t*)PyLong_AsVoidPtr(args[4]);
+    float* const* steps = (float* const*)PyLong_AsVoidPtr(args[5]);
+    const int gradients = PyObject_IsTrue(args[6]);
+    if (PyErr_Occurred()) return nullptr;
+    const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+    double step = 0.0;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject* po = PyList_GET_ITEM(args[0], i);
+        PyObject* state = PyList_GET_ITEM(args[1], i);
+        PyObject* keys = PyList_GET_ITEM(args[2], i);
+        PyObject* tensors = PyList_GET_ITEM(args[3], i);
+        TORCH_CHECK_TYPE(THPVariable_Check(po) && PyDict_Check(state) && PyTuple_Check(keys) &&
+                             PyTuple_Check(tensors) &&
+                             PyTuple_GET_SIZE(keys) == PyTuple_GET_SIZE(tensors),
+                         "adamw_current: expected tensors, dicts and tuples");
+        for (Py_ssize_t j = 0; j < PyTuple_GET_SIZE(keys); ++j) {
+            PyObject* held = PyDict_GetItemWithError(state, PyTuple_GET_ITEM(keys, j));
+            if (!held && PyErr_Occurred()) return nullptr;
+            if (held != PyTuple_GET_ITEM(tensors, j)) return PyFloat_FromDouble(-1.0);
+        }
+        const Tensor& p = THPVariable_Unpack(po);
+        int64_t* row = table + 8 * i;
+        if ((int64_t)p.data_ptr() != row[0] || p.numel() != row[5] ||
+            type_code(p) != (int)(row[6] & 0xF) || !p.is_contiguous())
+            return PyFloat_FromDouble(-1.0);
+        if (!gradients) continue;
+        const Tensor& g = p.grad();
+        if (!g.defined() || g.layout() != at::kStrided || g.scalar_type() != p.scalar_type() ||
+            g.device() != p.device() || g.numel() != p.numel() || !g.is_contiguous())
+            return PyFloat_FromDouble(-1.0);
+        row[1] = (int64_t)g.data_ptr();
+        if (i == 0) step = *steps[0];
+        if (*steps[i] != step) return PyFloat_FromDouble(-1.0);
+    }
+    return PyFloat_FromDouble(step);
+    END_HANDLE_TH_ERRORS
+}
+
+// adamw_count(steps, n, value): sets the n step counts.
+PyObject* py_adamw_count(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(nargs == 3, "adamw_count: expected 3 arguments");
+    float* const* steps = (float* const*)PyLong_AsVoidPtr(args[0]);
+    const Py_ssize_t n = PyLong_AsSsize_t(args[1]);
+    const double value = PyFloat_AsDouble(args[2]);
+    if (PyErr_Occurred()) return nullptr;
+    for (Py_ssize_t i = 0; i < n; ++i) *steps[i] = (float)value;
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_signature_hash(PyObject*, PyObject*) {
+    return PyUnicode_FromString(CS_SIGNATURE_HASH);
+}
+
+PyMethodDef methods[] = {
+    {"group_norm", (PyCFunction)(void (*)(void))py_group_norm, METH_FASTCALL, nullptr},
+    {"adamw_current", (PyCFunction)(void (*)(void))py_adamw_current, METH_FASTCALL, nullptr},
+    {"adamw_count", (PyCFunction)(void (*)(void))py_adamw_count, METH_FASTCALL, nullptr},
+    {"signature_hash", py_signature_hash, METH_NOARGS, nullptr},
+    {nullptr, nullptr, 0, nullptr},
+};
+
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_cs_torch", nullptr, -1, methods};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__cs_torch(void) { return PyModule_Create(&module); }

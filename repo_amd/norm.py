@@ -15,6 +15,7 @@ from typing import Optional
 import torch
 
 from . import _native as N
+from . import torchcall
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3}
@@ -150,6 +151,10 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
             return group_norm(x, num_groups, weight, bias, eps, activation)
     x = _channels_last(x)
     act = _ACTIVATIONS[activation]
+    ext = torchcall.module()
+    if ext is not None and N._PROFILE_CTX_FACTORY is None:
+        return ext.group_norm(x, weight, bias, int(num_groups), float(eps), act)
+    # Without the extension, or where each launch is bracketed by a context manager.
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _GroupNorm.apply(x, weight, bias, int(num_groups), float(eps), act)
