@@ -29,6 +29,14 @@
 // cut, so the expected value is the value.  The numbers are a hash of (seed,
 // step, tensor, element), hence the same in every run and launch shape.  A
 // root that is not zero never becomes zero: the update divides by it.
+//
+// Bound: HBM at 28 bytes an element with fp32 states and 16 with 8-bit ones (some 90
+// VALU slots an element there, of about 100 that the bandwidth leaves).  A launch
+// takes up to 56 tensors, whose pointers travel in its arguments, so nothing of the
+// step is uploaded; a workgroup takes one pass of 2048 elements of one tensor, found
+// by one ballot over the tensors' first workgroups, and its loads go out together.
+// Measured: fp32 states 870 us of 197M bf16 weights (6.3 TB/s), 67 us of 16.3M fp32
+// (6.8 TB/s); 8-bit states 520 us (6.1 TB/s) and 44 us (5.9 TB/s).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -376,7 +384,8 @@ __global__ __launch_bounds__(kAwThreads) void k_adamw(AwArgs a) {
 
 // ---- state conversions
 
-// fp32 m (avg) and v (sq) -> codes at param (m) and grad (root), to nearest.
+// fp32 m (avg) and v (sq) -> codes at param (m) and grad (root), to nearest.  Bound:
+// HBM, 10 bytes an element; taken when a checkpoint is loaded.
 __global__ __launch_bounds__(kAwThreads) void k_adamw_pack(AwArgs a) {
     const AwTensor& t = a.t[aw_find(a)];
     const bool vec = (t.meta >> 5) & 1;
@@ -401,7 +410,8 @@ __global__ __launch_bounds__(kAwThreads) void k_adamw_pack(AwArgs a) {
     });
 }
 
-// PAST: 16-bit values go past the caches (bf16, 54.5M values of each moment, 63 and
+// What the states stand for, in T.  Bound: HBM, 6 bytes an element from 8 bits to
+// bf16: 217 us of 197M (5.4 TB/s).  PAST: 16-bit values go past the caches (bf16, 54.5M values of each moment, 63 and
 // 50 us; fp32 values lie 32 bytes a lane, in two stores that only the cache joins).
 template <typename T, bool PAST>
 __device__ inline void aw_unpack(const AwTensor& t, int64_t begin, int64_t end) {
@@ -447,6 +457,9 @@ __global__ __launch_bounds__(kAwThreads) void k_adamw_unpack(AwArgs a) {
 
 // ---- the gradients' norm
 
+// One launch sums squares, up to 2048 workgroups over all tensors, and a workgroup
+// of its own joins them in fp64.  Bound: HBM, reads the gradients: 73 us of 197M bf16
+// (5.4 TB/s), 12 us of 16.3M fp32 (5.4 TB/s), and 4 us for the joining launch.
 struct NormTensor {
     const void* grad;
     int64_t n;
