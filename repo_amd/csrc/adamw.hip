@@ -30,13 +30,14 @@
 // step, tensor, element), hence the same in every run and launch shape.  A
 // root that is not zero never becomes zero: the update divides by it.
 //
-// Bound: HBM at 28 bytes an element with fp32 states and 16 with 8-bit ones (some 90
-// VALU slots an element there, of about 100 that the bandwidth leaves).  A launch
-// takes up to 56 tensors, whose pointers travel in its arguments, so nothing of the
-// step is uploaded; a workgroup takes one pass of 2048 elements of one tensor, found
-// by one ballot over the tensors' first workgroups, and its loads go out together.
-// Measured: fp32 states 870 us of 197M bf16 weights (6.3 TB/s), 67 us of 16.3M fp32
-// (6.8 TB/s); 8-bit states 520 us (6.1 TB/s) and 44 us (5.9 TB/s).
+// Bound: HBM at 28 bytes an element with fp32 states and 16 with 8-bit ones, whose
+// 80 or so VALU slots an element come near the hundred that the bandwidth leaves.  A
+// launch takes up to 56 tensors, whose pointers travel in its arguments, so nothing
+// of the step is uploaded; a workgroup takes one pass of 2048 elements of one tensor,
+// found by one ballot over the tensors' first workgroups, and its loads go out
+// together.  Measured: fp32 states 870 us of 197M bf16 weights (6.3 TB/s), 67 us of
+// 16.3M fp32 (6.8 TB/s); 8-bit states 139 us of 54.5M bf16 (6.3 TB/s), 45 us of 16.3M
+// fp32 (5.8 TB/s).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -175,16 +176,40 @@ __device__ inline void aw_passes(int64_t begin, int64_t end, bool vec, F&& f) {
     for (; base < end; base += kAwPass) f(AwBool<false>(), base);
 }
 
-__device__ inline void aw_update(const AwSet& s, float g, float& p, float& m, float& v,
-                                 float& root) {
-    p = p * s.decay;
+__device__ inline void aw_moments(const AwSet& s, float g, float& m, float& v) {
     m = m + s.omb1 * (g - m);
     v = v * s.beta2 + s.omb2 * (g * g);
-    root = __builtin_sqrtf(v);
-    // The hardware's reciprocal (1 ulp): the quotient is a few roundings off, the
-    // sequence of a rounded division would double the kernel's instructions.
+}
+
+// p after the step.  The hardware's reciprocal (1 ulp): the quotient is a few
+// roundings off, the sequence of a rounded division would double the instructions.
+__device__ inline float aw_move(const AwSet& s, float p, float m, float root) {
     const float inv = __builtin_amdgcn_rcpf(__builtin_fmaf(root, s.inv_bc2_sqrt, s.eps));
-    p = p - s.step_size * (m * inv);
+    return p * s.decay - s.step_size * (m * inv);
+}
+
+// Square roots of four second moments.  Where all of a wave's are ordinary numbers,
+// by a reciprocal root and one correction by its exact remainder, half the
+// instructions of the general sequence and the same roundings.
+__device__ inline void aw_roots(const float (&v)[4], float (&root)[4]) {
+    uint32_t low = ~0u, high = 0u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t b = __float_as_uint(v[k]);   // no sign: in the numbers' order
+        low = b < low ? b : low;
+        high = b > high ? b : high;
+    }
+    if (__all(low >= 0x0F800000u && high < 0x7F800000u)) {   // 2^-96, infinity
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float r = __builtin_amdgcn_rsqf(v[k]);
+            const float x = v[k] * r;
+            root[k] = __builtin_fmaf(__builtin_fmaf(-x, x, v[k]), 0.5f * r, x);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) root[k] = __builtin_sqrtf(v[k]);
+    }
 }
 
 // ---- 8-bit codes
@@ -201,17 +226,24 @@ template <int MB, bool FLOOR>
 __device__ inline uint32_t aw_encode(float x, int e, uint32_t r16) {
     const uint32_t t = __float_as_uint(__builtin_ldexpf(x, 14 - e)) & 0x7FFFFFFFu;
     uint32_t c = (t + (r16 << (7 - MB))) >> (23 - MB);
-    if (FLOOR) c = x > 0.0f && c == 0 ? 1u : c;
-    c = t >= 0x7F800000u ? (1u << (4 + MB)) - 1u : c;
+    if (FLOOR) {  // x has no sign: 1 where it is not zero
+        const uint32_t b = __float_as_uint(x), one = b < 1u ? b : 1u;
+        c = c < one ? one : c;
+    }
+    const uint32_t all = (1u << (4 + MB)) - 1u;   // infinity and NaN end above it
+    c = c < all ? c : all;
     if (MB == 3) c |= (__float_as_uint(x) >> 24) & 0x80u;
     return c;
 }
 
 // The largest of the 32 lanes that hold a block.
-__device__ inline float aw_block_max(float x) {
-#define CS_ROW_MAX(ctrl)                                                                   \
-    x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(                               \
-                     0, __float_as_int(x), ctrl, 0xF, 0xF, true)))
+__device__ inline uint32_t aw_block_max(uint32_t x) {
+#define CS_ROW_MAX(ctrl)                                                                    \
+    {                                                                                       \
+        const uint32_t o =                                                                  \
+            (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xF, 0xF, true);         \
+        x = x > o ? x : o;                                                                  \
+    }
     CS_ROW_MAX(0x128);  // row_ror:8
     CS_ROW_MAX(0x124);
     CS_ROW_MAX(0x122);
@@ -219,19 +251,31 @@ __device__ inline float aw_block_max(float x) {
 #undef CS_ROW_MAX
     // Both rows of 16 have their own; the odd rows of one copy change places with the
     // even rows of the other.
-    const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x),
-                                                       false, false);
-    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+    const auto both = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return both[0] > both[1] ? both[0] : both[1];
 }
 
+// The exponent field of a block's largest finite magnitude; every lane of the wave
+// takes part.  Magnitudes compare as their bits do; blocks with infinities or NaN
+// are looked at again without them.
 __device__ inline int aw_shared_exponent(const float (&x)[4]) {
-    float top = 0.0f;
+    uint32_t top = 0u;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const float a = __builtin_fabsf(x[k]);
-        top = a < __builtin_inff() ? fmaxf(top, a) : top;
+        const uint32_t a = __float_as_uint(x[k]) & 0x7FFFFFFFu;
+        top = a > top ? a : top;
     }
-    return (int)(__float_as_uint(aw_block_max(top)) >> 23);
+    top = aw_block_max(top);
+    if (__any(top >= 0x7F800000u)) {
+        top = 0u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t a = __float_as_uint(x[k]) & 0x7FFFFFFFu;
+            top = a > top && a < 0x7F800000u ? a : top;
+        }
+        top = aw_block_max(top);
+    }
+    return (int)(top >> 23);
 }
 
 // The four or eight bytes of a lane; the code arrays are whole blocks, so all exist
@@ -301,7 +345,7 @@ __device__ inline void aw_step32(const AwTensor& t, const AwSet& s, float clip, 
     aw_passes(begin, end, vec, [&](auto full, int64_t base) {
         constexpr bool F = decltype(full)::value;
         // Two vectors a thread, their loads in flight together.
-        float p[2][4], g[2][4], m[2][4], v[2][4], root;
+        float p[2][4], g[2][4], m[2][4], v[2][4];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int64_t i = base + (u * kAwThreads + threadIdx.x) * 4;
@@ -314,8 +358,10 @@ __device__ inline void aw_step32(const AwTensor& t, const AwSet& s, float clip, 
         for (int u = 0; u < 2; ++u) {
             const int64_t i = base + (u * kAwThreads + threadIdx.x) * 4;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                aw_update(s, g[u][k] * clip, p[u][k], m[u][k], v[u][k], root);
+            for (int k = 0; k < 4; ++k) {
+                aw_moments(s, g[u][k] * clip, m[u][k], v[u][k]);
+                p[u][k] = aw_move(s, p[u][k], m[u][k], __builtin_sqrtf(v[u][k]));
+            }
             aw_store<4, F, PAST == 2>(main, i, end, p[u]);
             if (DT != kF32) aw_store<4, F, PAST == 2>((T*)t.param, i, end, p[u]);
             aw_store<4, F, PAST != 0>((float*)t.avg, i, end, m[u]);
@@ -346,10 +392,16 @@ __device__ inline void aw_step8(const AwTensor& t, const AwSet& s, float clip, i
             const int64_t i = base + (u * kAwThreads + threadIdx.x) * 4;
             const uint32_t key = aw_key(t.key, i);
             uint32_t r[4];
+            float v[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                float v = root[u][k] * root[u][k];
-                aw_update(s, g[u][k] * clip, p[u][k], m[u][k], v, root[u][k]);
+                v[k] = root[u][k] * root[u][k];
+                aw_moments(s, g[u][k] * clip, m[u][k], v[k]);
+            }
+            aw_roots(v, root[u]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                p[u][k] = aw_move(s, p[u][k], m[u][k], root[u][k]);
                 r[k] = aw_mix(key + k);
                 // Elements past the end do not set a block's exponent.
                 if (!F && i + k >= t.n) m[u][k] = root[u][k] = 0.0f;
