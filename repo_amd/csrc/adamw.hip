@@ -222,18 +222,36 @@ __device__ inline float aw_decode(uint32_t code, int e) {
     return MB == 3 && (code & 0x80u) ? -y : y;
 }
 
+// The codes of a lane's four values; every lane of the wave takes part.  Scaled, a
+// number's bits begin with its code.  Below the lowest binade the scaling rounds to
+// nearest; there the bits are cut off instead, as the random number goes on top of
+// what is left: 3 values of 10,000 of a normal distribution, so that most waves skip it.
 template <int MB, bool FLOOR>
-__device__ inline uint32_t aw_encode(float x, int e, uint32_t r16) {
-    const uint32_t t = __float_as_uint(__builtin_ldexpf(x, 14 - e)) & 0x7FFFFFFFu;
-    uint32_t c = (t + (r16 << (7 - MB))) >> (23 - MB);
-    if (FLOOR) {  // x has no sign: 1 where it is not zero
-        const uint32_t b = __float_as_uint(x), one = b < 1u ? b : 1u;
-        c = c < one ? one : c;
+__device__ inline void aw_encode(const float (&x)[4], int e, const uint32_t (&r16)[4],
+                                 uint32_t (&c)[4]) {
+    uint32_t t[4], low = ~0u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        t[k] = __float_as_uint(__builtin_ldexpf(x[k], 14 - e)) & 0x7FFFFFFFu;
+        low = t[k] < low ? t[k] : low;
+    }
+    if (__any(low <= 0x00800000u)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (t[k] <= 0x00800000u)
+                t[k] = (uint32_t)__builtin_ldexpf(__builtin_fabsf(x[k]), 14 - e + 149);
     }
     const uint32_t all = (1u << (4 + MB)) - 1u;   // infinity and NaN end above it
-    c = c < all ? c : all;
-    if (MB == 3) c |= (__float_as_uint(x) >> 24) & 0x80u;
-    return c;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        c[k] = (t[k] + (r16[k] << (7 - MB))) >> (23 - MB);
+        if (FLOOR) {  // x has no sign: 1 where it is not zero
+            const uint32_t b = __float_as_uint(x[k]), one = b < 1u ? b : 1u;
+            c[k] = c[k] < one ? one : c[k];
+        }
+        c[k] = c[k] < all ? c[k] : all;
+        if (MB == 3) c[k] |= (__float_as_uint(x[k]) >> 24) & 0x80u;
+    }
 }
 
 // The largest of the 32 lanes that hold a block.
@@ -303,12 +321,14 @@ __device__ inline void aw_hold(uint8_t* avg, uint8_t* sq, int64_t i, int64_t n,
                                const uint32_t (&r)[4]) {
     const bool in = FULL || i < n;
     const int em = aw_shared_exponent(m), er = aw_shared_exponent(root);
-    uint32_t cm[4], cr[4];
+    uint32_t lo[4], hi[4], cm[4], cr[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        cm[k] = aw_encode<3, false>(m[k], em, r[k] & 0xFFFFu);
-        cr[k] = aw_encode<4, true>(root[k], er, r[k] >> 16);
+        lo[k] = r[k] & 0xFFFFu;
+        hi[k] = r[k] >> 16;
     }
+    aw_encode<3, false>(m, em, lo, cm);
+    aw_encode<4, true>(root, er, hi, cr);
     aw_store_codes(avg, i, in, cm);
     aw_store_codes(sq, i, in, cr);
     if (in && (threadIdx.x & 31) == 0) {

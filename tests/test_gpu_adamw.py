@@ -146,6 +146,32 @@ def test_8bit_states_are_the_models_bit_for_bit(dtype):
 
 
 @pytest.mark.gpu
+def test_8bit_rounds_the_smallest_by_all_their_bits():
+    """Below a block's lowest binade the spacing is fixed: gradients that are, or
+    just are not, as far above a code as the random number takes to the next."""
+    from repo_amd.optim import AdamW
+    n, hyper = 1 << 14, dict(lr=1e-3, betas=(0.0, 0.0), eps=1e-8, weight_decay=0.0)
+    r0, r1 = O.rounding_numbers(5, 1, 0, 2 * n)
+    r = np.where(np.arange(2 * n) < n, r0, r1).astype(np.float64)
+    mantissa = np.where(np.arange(2 * n) < n, 3, 4)
+    # In spacings: 1 or 2 and what the random number leaves to the next, less one last bit.
+    k = 1.0 + np.arange(2 * n) % 2
+    k = k + (65536.0 - r) / 65536.0
+    k = np.where(np.arange(2 * n) // 2 % 2 == 1, np.nextafter(k.astype(np.float32), np.float32(0)), k)
+    grad = (k * np.ldexp(1.0, -13 - mantissa)).astype(np.float32)
+    grad[::128] = 1.0
+    p = torch.zeros(2 * n, device="cuda", requires_grad=True)
+    opt = AdamW([p], state_bits=8, min_8bit_numel=0, seed=5, **hyper)
+    p.grad = torch.from_numpy(grad).cuda()
+    opt.step()
+    m, v = opt.flat_state(torch.float32)
+    rm, rr, _ = _model8(np.zeros(2 * n, np.float32), grad, np.zeros(2 * n, np.float32),
+                        np.zeros(2 * n, np.float32), step=1, seed=5, number=0, **hyper)
+    assert np.array_equal(_np(m), rm)
+    assert np.array_equal(_np(v), rr * rr)
+
+
+@pytest.mark.gpu
 def test_small_tensors_keep_fp32_states():
     from repo_amd.optim import AdamW
     ps, g = _make([(4095,), (4096,)], torch.float32, seed=3)
