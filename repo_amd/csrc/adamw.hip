@@ -483,9 +483,11 @@ __global__ __launch_bounds__(kAwThreads) void k_adamw_pack(AwArgs a) {
 }
 
 // What the states stand for, in T.  Bound: HBM, 6 bytes an element from 8 bits to
-// bf16: 217 us of 197M (5.4 TB/s).  PAST: 16-bit values go past the caches (bf16, 54.5M values of each moment, 63 and
-// 50 us; fp32 values lie 32 bytes a lane, in two stores that only the cache joins).
-template <typename T, bool PAST>
+// bf16: 206 us of 197M (5.7 TB/s).  16-bit values go past the caches (bf16, us
+// without and with: 54.5M values of each moment 63 and 50, 16.3M 21.9 and 16.9, 3.5M
+// 6.7 and 5.4); fp32 values lie 32 bytes a lane, in two stores that only the cache
+// joins.
+template <typename T>
 __device__ inline void aw_unpack(const AwTensor& t, int64_t begin, int64_t end) {
     const bool vec = (t.meta >> 5) & 1, eight = (t.meta >> 4) & 1;
     const int64_t n = (int64_t)(intptr_t)t.master;  // with what follows the values
@@ -507,23 +509,22 @@ __device__ inline void aw_unpack(const AwTensor& t, int64_t begin, int64_t end) 
             aw_load<8, F>((const float*)t.avg, i, t.n, m);
             aw_load<8, F>((const float*)t.sq, i, t.n, v);
         }
-        aw_store<8, F, PAST && sizeof(T) == 2>((T*)t.param, i, n, m);
-        aw_store<8, F, PAST && sizeof(T) == 2>((T*)const_cast<void*>(t.grad), i, n, v);
+        aw_store<8, F, sizeof(T) == 2>((T*)t.param, i, n, m);
+        aw_store<8, F, sizeof(T) == 2>((T*)const_cast<void*>(t.grad), i, n, v);
     };
     if (whole > begin) aw_passes(begin, whole, vec, pass);
     aw_passes(whole > begin ? whole : begin, end, false, pass);
 }
 
-template <bool PAST>
 __global__ __launch_bounds__(kAwThreads) void k_adamw_unpack(AwArgs a) {
     const AwTensor& t = a.t[aw_find(a)];
     const int64_t n = (int64_t)(intptr_t)t.master;
     const int64_t begin = (int64_t)(blockIdx.x - t.first_block) * a.chunk;
     const int64_t end = begin + a.chunk < n ? begin + a.chunk : n;
     switch (a.out_dtype) {
-        case kF32: aw_unpack<float, PAST>(t, begin, end); break;
-        case kBF16: aw_unpack<__bf16, PAST>(t, begin, end); break;
-        case kF16: aw_unpack<_Float16, PAST>(t, begin, end); break;
+        case kF32: aw_unpack<float>(t, begin, end); break;
+        case kBF16: aw_unpack<__bf16>(t, begin, end); break;
+        case kF16: aw_unpack<_Float16>(t, begin, end); break;
     }
 }
 
@@ -651,7 +652,6 @@ constexpr int64_t kAwBlocks = (int64_t)1 << 21;
 // (261 MB) 49.7 and 46.4, 6.4M (102 MB) 21.4 and 21.8.
 constexpr int64_t kAwPastBytes = (int64_t)224 << 20;
 constexpr int64_t kAwPastWeights = (int64_t)256 << 20;
-constexpr int64_t kAwPastValues = (int64_t)64 << 20;
 
 // table: [n][8] = param, grad, master, exp_avg, exp_avg_sq, numel, dtype | eight << 4 |
 // set << 8, ordinal.
@@ -739,10 +739,8 @@ int aw_run(AwOp op, int32_t ntensors, const int64_t* table, int32_t nsets, const
             hipLaunchKernelGGL((k_adamw<0>), grid, block, 0, stream, a);
         else if (op == kPack)
             hipLaunchKernelGGL(k_adamw_pack, grid, block, 0, stream, a);
-        else if (total * 4 > kAwPastValues)
-            hipLaunchKernelGGL((k_adamw_unpack<true>), grid, block, 0, stream, a);
         else
-            hipLaunchKernelGGL((k_adamw_unpack<false>), grid, block, 0, stream, a);
+            hipLaunchKernelGGL(k_adamw_unpack, grid, block, 0, stream, a);
         if (hipGetLastError() != hipSuccess) return CS_ERR_HIP;
     }
     return CS_OK;
