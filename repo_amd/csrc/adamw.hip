@@ -552,6 +552,9 @@ struct NormArgs {
 
 // Vectors of 16 bytes, kNormAhead of them in flight a thread.
 constexpr int kNormAhead = 4;
+// A chunk is whole rounds of them (bf16; 2048 elements, so that most of a chunk may
+// be less than a round: 5.4M weights 13.1 us for 9.6, 197M 78.7 for 71.5).
+constexpr int64_t kNormPass = (int64_t)kAwThreads * kNormAhead * 8;
 
 template <int DT>
 __device__ inline float norm_squares(const NormTensor& t, int64_t begin, int64_t end) {
@@ -574,6 +577,15 @@ __device__ inline float norm_squares(const NormTensor& t, int64_t begin, int64_t
                     const float x = (float)g[u].v[k];
                     s[k & 3] = __builtin_fmaf(x, x, s[k & 3]);
                 }
+        }
+    if ((t.meta >> 5) & 1)
+        for (; i + N <= end; i += step) {
+            const AwVec<T, N> g = *reinterpret_cast<const AwVec<T, N>*>(src + i);
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const float x = (float)g.v[k];
+                s[k & 3] = __builtin_fmaf(x, x, s[k & 3]);
+            }
         }
     for (; i < end; i += step) {
         float g[N];
@@ -626,10 +638,10 @@ __global__ __launch_bounds__(kAwThreads) void k_grad_norm(const double* partials
 
 static bool aw_aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
-// Elements of a chunk: whole passes, and about `blocks` of them over the total.
-static int64_t aw_chunk(int64_t total, int64_t blocks) {
+// Elements of a chunk: whole passes, and at most `blocks` of them over the total.
+static int64_t aw_chunk(int64_t total, int64_t blocks, int64_t pass) {
     const int64_t per = (total + blocks - 1) / blocks;
-    return (per + kAwPass - 1) / kAwPass * kAwPass;
+    return (per + pass - 1) / pass * pass;
 }
 
 }  // namespace cs
@@ -685,7 +697,7 @@ int aw_run(AwOp op, int32_t ntensors, const int64_t* table, int32_t nsets, const
         weights += n * 8;
     }
     if (total == 0) return CS_OK;
-    const int64_t chunk = aw_chunk(total, kAwBlocks);
+    const int64_t chunk = aw_chunk(total, kAwBlocks, kAwPass);
     const int past = weights > kAwPastWeights ? 2 : bytes > kAwPastBytes;
     int k = 0;
     while (k < ntensors) {
@@ -777,7 +789,7 @@ extern "C" int cs_grad_norm(int32_t ntensors, const int64_t* table, double max_n
     }
     // Each tensor ends with a part of a chunk, so the blocks are at most
     // kNormBlocks and one a tensor.
-    const int64_t chunk = aw_chunk(total, kNormBlocks);
+    const int64_t chunk = aw_chunk(total, kNormBlocks, kNormPass);
     int k = 0;
     int64_t done = 0;
     while (k < ntensors) {
