@@ -859,7 +859,7 @@ class AdamW(torch.optim.Optimizer):
         order, bulk = self._entries(), self._bulk
         if (bulk is None or bulk.version != self._version
                 or bulk.current(*bulk.args, False) < 0.0):
-            number = -1
+            number, bulk = -1, None
             for k, group in enumerate(self.param_groups):
                 for p in group["params"]:
                     number += 1
@@ -870,32 +870,40 @@ class AdamW(torch.optim.Optimizer):
                         if st and ("exp_avg" in st or _AVG8 in st):
                             self._entry(number, k)
         flat = self._flat
-        key = (self._version, align,
-               [p.numel() for p, e in zip(self._params, order) if e is None])
-        if flat is None or flat[0] != key or not _same(flat[1], order):
-            device = self._params[0].device
-            if any(p.device != device for p in self._params):
-                raise NotImplementedError("flat_state needs all parameters on one device")
-            padded = [-(-p.numel() // align) * align for p in self._params]
-            begins = np.cumsum([0] + padded)
-            here = [i for i, e in enumerate(order) if e is not None]
-            table = np.array([order[i].row for i in here], dtype=np.int64).reshape(-1, 8)
-            table[:, _META] &= _EIGHT
-            # Up to the alignment only: a parameter without a state may follow.
-            table[:, _MASTER] = [padded[i] for i in here]
-            flat = self._flat = (key, list(order), device, table, begins[here], int(begins[-1]),
-                                 any(n and e is None for n, e in zip(padded, order)))
-        _, _, device, table, begins, total, bare = flat
+        kind = (dtype, align, self._version, None if bulk is not None else
+                [p.numel() for p, e in zip(self._params, order) if e is None])
+        if flat is None or flat[0] != kind or not (
+                flat[1] is bulk if bulk is not None else _same(flat[2], order)):
+            flat = self._flat = (kind, bulk, list(order), *self._flat_table(order, dtype, align))
+        _, _, _, device, table, address, begins, total, bare = flat
         make = torch.zeros if bare else torch.empty
         out = (make(total, dtype=dtype, device=device), make(total, dtype=dtype, device=device))
         if len(table):
-            begins = begins * out[0].element_size()
-            for col, t in ((_P, out[0]), (_G, out[1])):
-                table[:, col] = begins + t.data_ptr()
-            with torch.cuda.device(device):
-                N.call("cs_adamw_unpack_state", len(table), table.ctypes.data,
-                       _ADAMW_DTYPES[dtype], N.stream(device))
+            np.add(begins, out[0].data_ptr(), out=table[:, _P])
+            np.add(begins, out[1].data_ptr(), out=table[:, _G])
+            args = ("cs_adamw_unpack_state", len(table), address, _ADAMW_DTYPES[dtype],
+                    N.stream(device))
+            if device.index == torch._C._cuda_getDevice():
+                N.call(*args)
+            else:
+                with torch.cuda.device(device):
+                    N.call(*args)
         return out
+
+    def _flat_table(self, order, dtype, align):
+        """Where flat_state's launch reads, and where in its outputs, in bytes, it writes."""
+        device = self._params[0].device
+        if any(p.device != device for p in self._params):
+            raise NotImplementedError("flat_state needs all parameters on one device")
+        padded = [-(-p.numel() // align) * align for p in self._params]
+        begins = np.cumsum([0] + padded)
+        here = [i for i, e in enumerate(order) if e is not None]
+        table = np.array([order[i].row for i in here], dtype=np.int64).reshape(-1, 8)
+        table[:, _META] &= _EIGHT
+        # Up to the alignment only: a parameter without a state may follow.
+        table[:, _MASTER] = [padded[i] for i in here]
+        return (device, table, table.ctypes.data, begins[here] * dtype.itemsize, int(begins[-1]),
+                any(n and e is None for n, e in zip(padded, order)))
 
     def load_state_dict(self, state_dict):
         """Takes states of either width, and of bf16 or fp16 (as torch's
