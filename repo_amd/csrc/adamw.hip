@@ -35,7 +35,7 @@
 // launch takes up to 56 tensors, whose pointers travel in its arguments, so nothing
 // of the step is uploaded; a workgroup takes one pass of 2048 elements of one tensor,
 // found by one ballot over the tensors' first workgroups, and its loads go out
-// together.  Measured: fp32 states 870 us of 197M bf16 weights (6.3 TB/s), 67 us of
+// together.  Measured: fp32 states 890 us of 197M bf16 weights (6.2 TB/s), 67 us of
 // 16.3M fp32 (6.8 TB/s); 8-bit states 139 us of 54.5M bf16 (6.3 TB/s), 45 us of 16.3M
 // fp32 (5.8 TB/s).
 #include <hip/hip_runtime.h>
@@ -531,8 +531,8 @@ __global__ __launch_bounds__(kAwThreads) void k_adamw_unpack(AwArgs a) {
 // ---- the gradients' norm
 
 // One launch sums squares, up to 2048 workgroups over all tensors, and a workgroup
-// of its own joins them in fp64.  Bound: HBM, reads the gradients: 73 us of 197M bf16
-// (5.4 TB/s), 12 us of 16.3M fp32 (5.4 TB/s), and 4 us for the joining launch.
+// of its own joins them in fp64.  Bound: HBM, reads the gradients: 69 us of 197M bf16
+// (5.7 TB/s), 14 us of 16.3M fp32 (4.6 TB/s), and 4 us for the joining launch.
 struct NormTensor {
     const void* grad;
     int64_t n;

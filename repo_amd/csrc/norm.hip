@@ -529,8 +529,8 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_apply(GnArgs a) {
 // ---- backward
 
 // Sums of dz and dz xh per channel and, weighted, per group over a chunk.  Reads x and
-// dy: 60 us of 24x24576x128 bf16 silu (5.0 TB/s; the VALU is busy for 40 of them),
-// 122 us of 2766240x32 fp32 (5.8 TB/s).
+// dy: 60 us of 24x24576x128 bf16 silu (5.0 TB/s; its arithmetic takes some 40 of
+// them at the VALU's full rate), 122 us of 2766240x32 fp32 (5.8 TB/s).
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_sums(GnArgs a) {
     __shared__ float buf[kGnThreads * V], chan_sums[2][kGnThreads * V], gsum[kGnThreads * V];
