@@ -173,9 +173,63 @@ PyObject* py_group_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// Where and how a tensor's elements lie: what a launch's table says of it as long as
+// all of this is unchanged.  order: 0 for the logical one, which the sizes do not
+// change; sizes of one have no stride.
+struct Place {
+    int64_t address, type, numel, order;
+    explicit Place(const Tensor& t)
+        : address((int64_t)t.data_ptr()),
+          type((int64_t)t.scalar_type() << 8 | (int64_t)t.layout()),
+          numel(t.numel()),
+          order(0) {
+        if (t.is_contiguous()) return;
+        uint64_t mix = (uint64_t)t.dim();
+        for (int64_t d = 0; d < t.dim(); ++d) {
+            const int64_t size = t.size(d);
+            mix = (mix ^ (uint64_t)size) * 0x9E3779B97F4A7C15u;
+            mix = (mix ^ (uint64_t)(size == 1 ? 0 : t.stride(d))) * 0xC2B2AE3D27D4EB4Fu;
+            mix ^= mix >> 29;
+        }
+        order = (int64_t)mix;
+    }
+};
+
+// adamw_place(tensors, places): writes each tensor's Place into the array by that
+// address; adamw_held(tensors, places): whether all still are what it holds.
+PyObject* with_places(PyObject* const* args, Py_ssize_t nargs, bool write) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(nargs == 2 && PyTuple_Check(args[0]), "expected a tuple and an address");
+    Place* places = (Place*)PyLong_AsVoidPtr(args[1]);
+    if (PyErr_Occurred()) return nullptr;
+    const Py_ssize_t n = PyTuple_GET_SIZE(args[0]);
+    bool same = true;
+    for (Py_ssize_t i = 0; i < n && same; ++i) {
+        PyObject* o = PyTuple_GET_ITEM(args[0], i);
+        TORCH_CHECK_TYPE(THPVariable_Check(o), "expected tensors");
+        const Place now(THPVariable_Unpack(o));
+        if (write)
+            places[i] = now;
+        else
+            same = now.address == places[i].address && now.type == places[i].type &&
+                   now.numel == places[i].numel && now.order == places[i].order;
+    }
+    return PyBool_FromLong(same);
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_adamw_place(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return with_places(args, nargs, true);
+}
+
+PyObject* py_adamw_held(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return with_places(args, nargs, false);
+}
+
 // adamw_current(params, states, keys, tensors, table, steps, gradients): whether
 // each parameter still is what its row of the table (int64 [n][8], by address)
-// says, and each states[i][keys[i][j]] the object tensors[i][j]; with `gradients`,
+// says, and each states[i][keys[i][j]] the object tensors[i][j] (whose place adamw_held
+// has found unchanged: the step counts are read by address); with `gradients`,
 // whether each parameter has a gradient that can be read as it is, whose address
 // goes into the row, and whether all step counts (float pointers, by the address of
 // their array) agree.  The count with `gradients`, else 0; -1 where anything is not
@@ -244,6 +298,8 @@ PyObject* py_signature_hash(PyObject*, PyObject*) {
 
 PyMethodDef methods[] = {
     {"group_norm", (PyCFunction)(void (*)(void))py_group_norm, METH_FASTCALL, nullptr},
+    {"adamw_place", (PyCFunction)(void (*)(void))py_adamw_place, METH_FASTCALL, nullptr},
+    {"adamw_held", (PyCFunction)(void (*)(void))py_adamw_held, METH_FASTCALL, nullptr},
     {"adamw_current", (PyCFunction)(void (*)(void))py_adamw_current, METH_FASTCALL, nullptr},
     {"adamw_count", (PyCFunction)(void (*)(void))py_adamw_count, METH_FASTCALL, nullptr},
     {"signature_hash", py_signature_hash, METH_NOARGS, nullptr},

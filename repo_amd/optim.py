@@ -436,11 +436,37 @@ def _same(a, b):
     return len(a) == len(b) and all(map(is_, a, b))
 
 
+class _Held:
+    """State tensors and where each lies: their storage may be replaced (t.data =
+    ..., as a program does that moves states off the GPU and back) while the
+    objects stay."""
+    __slots__ = ("tensors", "places", "address", "held")
+
+    def __init__(self, tensors):
+        self.tensors, ext = tuple(tensors), torchcall.module()
+        self.held = None if ext is None else ext.adamw_held
+        if ext is None:
+            self.places = [self.place(t) for t in self.tensors]
+        else:
+            self.places = np.empty((len(self.tensors), 4), dtype=np.int64)
+            self.address = self.places.ctypes.data
+            ext.adamw_place(self.tensors, self.address)
+
+    @staticmethod
+    def place(t):
+        return t.data_ptr(), t.dtype, t.layout, t.shape, t.stride()
+
+    def same(self):
+        if self.held is not None:
+            return self.held(self.tensors, self.address)
+        return [self.place(t) for t in self.tensors] == self.places
+
+
 class _AdamWEntry:
     """What the launches need of one parameter; remade when a tensor of it is
     another one, or lies elsewhere."""
     __slots__ = ("p", "st", "avg_key", "sq_key", "avg", "sq", "master", "step_t", "step", "row",
-                 "ptr", "numel", "dtype", "device", "stride", "contiguous", "place")
+                 "ptr", "numel", "dtype", "device", "stride", "contiguous", "place", "held")
 
     def fresh(self):
         p, st = self.p, self.st
@@ -450,7 +476,8 @@ class _AdamWEntry:
                     and (p.is_contiguous() if self.contiguous else p.stride() == self.stride)
                     and st[self.avg_key] is self.avg and st[self.sq_key] is self.sq
                     and st["step"] is self.step_t
-                    and (self.master is None or st["master"] is self.master))
+                    and (self.master is None or st["master"] is self.master)
+                    and self.held.same())
         except KeyError:
             return False
 
@@ -515,7 +542,13 @@ class _AdamWBulk:
         self.args = ([e.p for e in entries], [e.st for e in entries], keys,
                      [tuple(e.st[key] for key in ks) for e, ks in zip(entries, keys)],
                      self.plan.address, self.steps.ctypes.data)
-        self.current = torchcall.module().adamw_current
+        self._current = torchcall.module().adamw_current
+        self.held = _Held(chain.from_iterable(self.args[3]))
+
+    def current(self, gradients):
+        """The common step count, or 0 without gradients; -1 where anything changed.
+        The step counts are read by their addresses, so where they lie comes first."""
+        return self._current(*self.args, gradients) if self.held.same() else -1.0
 
     @staticmethod
     def of(version, order, ngroups):
@@ -716,6 +749,7 @@ class AdamW(torch.optim.Optimizer):
         e.row = [p.data_ptr(), 0, 0 if e.master is None else e.master.data_ptr(),
                  e.avg.data_ptr(), e.sq.data_ptr(), p.numel(),
                  _ADAMW_DTYPES[p.dtype] | (_EIGHT if eight else 0), 0]
+        e.held = _Held(t for t in (e.avg, e.sq, e.step_t, e.master) if t is not None)
         self._order[number] = e
         return e
 
@@ -762,7 +796,7 @@ class AdamW(torch.optim.Optimizer):
         order = self._entries()
         bulk = self._bulk
         if bulk is not None and bulk.version == self._version:
-            step = bulk.current(*bulk.args, True) + 1.0
+            step = bulk.current(True) + 1.0
             if step > 0.0:
                 self._on(bulk.device, self._launch, bulk.device, bulk.plan,
                          [(k, step) for k in bulk.groups])
@@ -858,7 +892,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"Invalid align: {align}")
         order, bulk = self._entries(), self._bulk
         if (bulk is None or bulk.version != self._version
-                or bulk.current(*bulk.args, False) < 0.0):
+                or bulk.current(False) < 0.0):
             number, bulk = -1, None
             for k, group in enumerate(self.param_groups):
                 for p in group["params"]:

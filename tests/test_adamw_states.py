@@ -1,0 +1,205 @@
+"""AdamW's states as a program may treat them between steps: storage that is replaced,
+another memory order, checkpoints that are shared, options that it does not have.
+
+On the CPU the launches are recorded instead of run: what they would read and write
+has to be the tensors that the states hold then."""
+from __future__ import annotations
+
+import ctypes
+from contextlib import nullcontext
+
+import numpy as np
+import pytest
+import torch
+
+EXTENSION = ["extension", "python"]
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """AdamW on host tensors; the (name, table) of each launch that it would make."""
+    from repo_amd import _native as N
+    from repo_amd.optim import AdamW
+    seen = []
+
+    def call(name, n, address, *args):
+        rows = np.ctypeslib.as_array((ctypes.c_int64 * (8 * n)).from_address(address))
+        seen.append((name, rows.reshape(n, 8).copy()))
+
+    monkeypatch.setattr(N, "call", call)
+    monkeypatch.setattr(N, "stream", lambda device=None: 0)
+    monkeypatch.setattr(AdamW, "_check_param", lambda self, p: None)
+    monkeypatch.setattr(AdamW, "_on", staticmethod(lambda device, launch, *args: launch(*args)))
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: None, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", lambda device: nullcontext())
+    return seen
+
+
+def _without_extension(monkeypatch, how):
+    from repo_amd import torchcall
+    if how == "python":
+        monkeypatch.setattr(torchcall, "_MODULE", None)
+    elif torchcall.module() is None:
+        pytest.skip("extension not built (run __graft_entry__.build())")
+
+
+def _moments(opt, p):
+    st = opt.state[p]
+    return [st["exp_avg_8bit" if "exp_avg_8bit" in st else "exp_avg"],
+            st["exp_avg_sq_8bit" if "exp_avg_sq_8bit" in st else "exp_avg_sq"]]
+
+
+def _expected(opt, ps):
+    """Parameter, gradient, master and moments of each row."""
+    return [[p.data_ptr(), p.grad.data_ptr(),
+             opt.state[p]["master"].data_ptr() if "master" in opt.state[p] else 0,
+             *(t.data_ptr() for t in _moments(opt, p))] for p in ps]
+
+
+def _move(t):
+    t.data = t.data.clone()
+
+
+@pytest.mark.parametrize("how", EXTENSION)
+@pytest.mark.parametrize("state_bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_launches_follow_states_that_moved(recorded, monkeypatch, how, state_bits, dtype):
+    """t.data = ... keeps the tensor object and frees its memory: the next step and
+    flat_state have to take the new address, of the step count too."""
+    from repo_amd.optim import AdamW
+    _without_extension(monkeypatch, how)
+    ps = [torch.randn(300).to(dtype).requires_grad_(True),
+          torch.randn(4, 8, 3, 3).to(dtype).requires_grad_(True)]
+    if state_bits == 32:  # one that is not contiguous leaves the path over all at once
+        ps.append(torch.randn(2, 4, 3, 3).to(dtype).contiguous(
+            memory_format=torch.channels_last).requires_grad_(True))
+    opt = AdamW(ps, state_bits=state_bits, min_8bit_numel=0)
+    kept = []   # the freed storages' stand-ins: no address comes back
+
+    def step(count):
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        del recorded[:]
+        opt.step()
+        assert [name for name, _ in recorded] == ["cs_adamw_step"]
+        assert recorded[0][1][:, :5].tolist() == _expected(opt, ps)
+        assert [float(opt.state[p]["step"]) for p in ps] == [count] * len(ps)
+        del recorded[:]
+        opt.flat_state()
+        assert recorded[0][1][:, 3:5].tolist() == [r[3:] for r in _expected(opt, ps)]
+
+    step(1)
+    step(2)
+    count = 2
+    for p in ps:
+        for name in list(opt.state[p]):
+            if not isinstance(opt.state[p][name], torch.Tensor):
+                continue
+            kept.append(opt.state[p][name].data)
+            _move(opt.state[p][name])
+            if name != "step":   # read first by flat_state, then by the step
+                del recorded[:]
+                opt.flat_state()
+                assert recorded[0][1][:, 3:5].tolist() == [r[3:] for r in _expected(opt, ps)]
+                kept.append(opt.state[p][name].data)
+                _move(opt.state[p][name])
+            count += 1
+            step(count)
+    for p in ps:   # all of them, as a program does that moves the states away and back
+        for t in opt.state[p].values():
+            if isinstance(t, torch.Tensor):
+                kept.append(t.data)
+                _move(t)
+    step(count + 1)
+
+
+@pytest.mark.parametrize("how", EXTENSION)
+def test_states_of_another_form_at_the_same_address_are_refused(recorded, monkeypatch, how):
+    """Storage that stays where it is but is looked at in another way."""
+    from repo_amd.optim import AdamW
+    _without_extension(monkeypatch, how)
+    changes = {
+        "type": lambda t: t.view(torch.int32),
+        "shape": lambda t: t[:2],
+        "order": lambda t: t.view(6, 4).t(),
+    }
+    for name, change in changes.items():
+        p = torch.zeros(4, 6, requires_grad=True)
+        opt = AdamW([p])
+        for _ in range(2):
+            p.grad = torch.ones(4, 6)
+            opt.step()
+        st = opt.state[p]["exp_avg"]
+        where = st.data_ptr()
+        st.data = change(st.data)
+        assert st.data_ptr() == where
+        del recorded[:]
+        with pytest.raises(ValueError, match="does not fit"):
+            opt.step()
+        assert not recorded and float(opt.state[p]["step"]) == 2.0, name
+
+
+def test_places_of_tensors():
+    """The extension's record of where tensors lie, and its refusals."""
+    from repo_amd import torchcall
+    ext = torchcall.module()
+    if ext is None:
+        pytest.skip("extension not built (run __graft_entry__.build())")
+    a, b = torch.zeros(4, 6), torch.tensor(3.0)
+    places = np.zeros((2, 4), np.int64)
+    where = places.ctypes.data
+    assert ext.adamw_place((a, b), where) is True
+    assert places[:, 0].tolist() == [a.data_ptr(), b.data_ptr()]
+    assert places[:, 2].tolist() == [24, 1]
+    assert ext.adamw_held((a, b), where) is True
+    assert ext.adamw_held((a.view(-1), b), where) is True         # another object, there
+    for other in (a.view(torch.int32), a[:2], a.view(6, 4).t(), a[1:], a.clone()):
+        assert ext.adamw_held((other, b), where) is False
+    assert ext.adamw_held((a, torch.tensor(3.0)), where) is False
+    one = torch.zeros(4, 1)
+    ext.adamw_place((one,), where)
+    assert ext.adamw_held((one.as_strided((4, 1), (1, 7)),), where) is True   # no stride of one
+    assert ext.adamw_held((), 0) is True
+    for bad in (((a,),), ([a], where), ((None,), where), ((a,), "0")):
+        with pytest.raises(TypeError):
+            ext.adamw_held(*bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", EXTENSION)
+@pytest.mark.parametrize("state_bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_states_moved_off_the_gpu_and_back(monkeypatch, how, state_bits, dtype):
+    """Two optimizers on equal parameters; the states of one are moved away and back
+    between the steps."""
+    from repo_amd.optim import AdamW
+    _without_extension(monkeypatch, how)
+    g = torch.Generator().manual_seed(1)
+    a = [torch.randn(s, generator=g).to(dtype).cuda().requires_grad_(True)
+         for s in ((5000,), (40, 30))]
+    b = [p.detach().clone().requires_grad_(True) for p in a]
+    x, y = (AdamW(ps, state_bits=state_bits, min_8bit_numel=0, seed=3) for ps in (a, b))
+    for step in range(5):
+        for p, q in zip(a, b):
+            p.grad = torch.randn(p.shape, generator=g).to(dtype).cuda()
+            q.grad = p.grad.clone()
+        x.step()
+        y.step()
+        tensors = [t for st in y.state.values() for t in st.values()
+                   if isinstance(t, torch.Tensor)]
+        for t in tensors:
+            device = t.device
+            t.data = t.data.cpu().clone()
+            t.data = t.data.to(device, copy=True)
+        assert all(torch.equal(p, q) for p, q in zip(x.flat_state(), y.flat_state()))
+        for p, q in zip(a, b):
+            assert torch.equal(p.detach(), q.detach())
+            assert float(x.state[p]["step"]) == float(y.state[q]["step"]) == step + 1
+            if dtype is not torch.float32:
+                assert torch.equal(x.state[p]["master"], y.state[q]["master"])
+    # Left on the host, they are refused.
+    for t in y.state[b[0]].values():
+        t.data = t.data.cpu()
+    b[0].grad = torch.ones_like(b[0])
+    with pytest.raises(ValueError, match="does not fit"):
+        y.step()
