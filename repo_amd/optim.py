@@ -395,7 +395,7 @@ _ADAMW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _EIGHT = 16                 # the bit of a table row's type for 8-bit states
 _SET_SHIFT = 8
 _P, _G, _MASTER, _AVG, _SQ, _NUMEL, _META, _NUMBER = range(8)   # columns of the table
-_AVG8, _SQ8 = "exp_avg_8bit", "exp_avg_sq_8bit"
+_AVG8, _SQ8, _ORDER8 = "exp_avg_8bit", "exp_avg_sq_8bit", "order_8bit"
 
 
 def _mix32(x):
@@ -424,6 +424,21 @@ def _same_layout(a, b):
     if a.is_contiguous() and b.is_contiguous():
         return True
     return all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1)
+
+
+def _memory_order(t):
+    """The dimensions of a dense tensor from the outermost in memory to the innermost,
+    without those of size one; () for the logical order."""
+    dims = [d for d in range(t.dim()) if t.shape[d] != 1]
+    order = sorted(dims, key=lambda d: -t.stride(d))
+    return () if t.numel() < 2 or order == dims else tuple(order)
+
+
+def _in_order(flat, shape, order):
+    """A flat tensor whose values lie in the memory order `order`, as one of `shape`."""
+    dims = [*order, *(d for d in range(len(shape)) if d not in order)]
+    return flat.view([shape[d] for d in dims]).permute(
+        sorted(range(len(dims)), key=dims.__getitem__))
 
 
 def _codes_numel(numel):
@@ -466,7 +481,7 @@ class _AdamWEntry:
     """What the launches need of one parameter; remade when a tensor of it is
     another one, or lies elsewhere."""
     __slots__ = ("p", "st", "avg_key", "sq_key", "avg", "sq", "master", "step_t", "step", "row",
-                 "ptr", "numel", "dtype", "device", "stride", "contiguous", "place", "held")
+                 "ptr", "numel", "dtype", "device", "shape", "stride", "contiguous", "place", "held")
 
     def fresh(self):
         p, st = self.p, self.st
@@ -621,7 +636,10 @@ class AdamW(torch.optim.Optimizer):
     and 3 (first moment, signed) or 4 (root of the second) mantissa bits, rounded
     stochastically with numbers that depend on ``seed``, the step, the tensor's
     place among the parameters and the element alone, so a run repeats bit for
-    bit.  load_state_dict takes states of either width and converts them.
+    bit.  The codes lie in the parameter's memory order, which stands beside them
+    (``order_8bit``, the dimensions from the outermost) where it is not the logical
+    one.  load_state_dict takes states of either width and converts them, also
+    those of a parameter that lies in another order.
 
     ``max_grad_norm`` > 0 scales all gradients by min(1, max_grad_norm / (norm +
     1e-6)) within the step, from the norm over all of them (``grad_norm``, a
@@ -699,6 +717,8 @@ class AdamW(torch.optim.Optimizer):
         if "step" not in st:
             st["step"] = torch.tensor(0.0, dtype=torch.float32)
         if self._eight(p.numel()):
+            if _AVG8 not in st and _SQ8 not in st:
+                self._set_order(p, st)
             for name in (_AVG8, _SQ8):
                 if name not in st:
                     st[name] = torch.zeros(_codes_numel(p.numel()), dtype=torch.uint8,
@@ -711,6 +731,16 @@ class AdamW(torch.optim.Optimizer):
         if p.dtype is not torch.float32 and "master" not in st:
             st["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
 
+    @staticmethod
+    def _set_order(p, st):
+        """Codes lie in their parameter's memory order, which they do not show: it
+        stands beside them, where it is not the logical one."""
+        order = _memory_order(p)
+        if order:
+            st[_ORDER8] = order
+        else:
+            st.pop(_ORDER8, None)
+
     def _entry(self, number, k):
         """A new entry of parameter `number`, which is of group k."""
         p = self._params[number]
@@ -722,8 +752,8 @@ class AdamW(torch.optim.Optimizer):
         e = _AdamWEntry()
         e.place = (number, k)
         e.p, e.st, e.dtype, e.device = p, st, p.dtype, p.device
-        e.ptr, e.numel, e.stride, e.contiguous = (p.data_ptr(), p.numel(), p.stride(),
-                                                  p.is_contiguous())
+        e.ptr, e.numel, e.contiguous = p.data_ptr(), p.numel(), p.is_contiguous()
+        e.shape, e.stride = p.shape, p.stride()
         e.avg_key, e.sq_key = (_AVG8, _SQ8) if eight else ("exp_avg", "exp_avg_sq")
         e.avg, e.sq = st[e.avg_key], st[e.sq_key]
         e.master = st.get("master") if p.dtype is not torch.float32 else None
@@ -741,6 +771,14 @@ class AdamW(torch.optim.Optimizer):
                                  f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on "
                                  f"{t.device} beside {tuple(p.shape)} with strides {p.stride()} on "
                                  f"{p.device}")
+        # Codes have no shape of their own: that of the parameter which they last were of.
+        old = self._order[number]
+        if eight and (tuple(st.get(_ORDER8, ())) != _memory_order(p) or (
+                old is not None and old.avg is e.avg and old.shape != p.shape)):
+            raise ValueError("an 8-bit AdamW state does not fit its parameter: it is of another "
+                             f"memory order or shape than {tuple(p.shape)} with strides "
+                             f"{p.stride()} (load_state_dict(state_dict()) brings it into a new "
+                             "order)")
         step = st["step"]
         if not (isinstance(step, torch.Tensor) and step.device.type == "cpu"
                 and step.dtype is torch.float32 and step.numel() == 1):
@@ -900,9 +938,10 @@ class AdamW(torch.optim.Optimizer):
                     e = order[number]
                     if e is None or not e.fresh():
                         st = self.state.get(p)
-                        order[number] = None
                         if st and ("exp_avg" in st or _AVG8 in st):
                             self._entry(number, k)
+                        else:
+                            order[number] = None
         flat = self._flat
         kind = (dtype, align, self._version, None if bulk is not None else
                 [p.numel() for p, e in zip(self._params, order) if e is None])
@@ -979,7 +1018,7 @@ class AdamW(torch.optim.Optimizer):
                                     memory_format=torch.preserve_format).copy_(t)
 
         for name, value in given.items():
-            if name not in ("step", "exp_avg", "exp_avg_sq", _AVG8, _SQ8, "master"):
+            if name not in ("step", "exp_avg", "exp_avg_sq", _AVG8, _SQ8, _ORDER8, "master"):
                 st[name] = value
         if given.get("master") is not None and p.dtype is not torch.float32:
             st["master"] = fp32(given["master"])
@@ -988,23 +1027,38 @@ class AdamW(torch.optim.Optimizer):
             if any(c.dtype is not torch.uint8 or c.numel() != _codes_numel(p.numel())
                    for c in codes):
                 raise ValueError("8-bit AdamW states of another size than the parameter's")
-            if eight:
+            order = given.get(_ORDER8, ())
+            if order and not (isinstance(order, (tuple, list)) and sorted(order) == [
+                    d for d in range(p.dim()) if p.shape[d] != 1]):
+                raise ValueError(f"8-bit AdamW states in an order {order} of the dimensions of "
+                                 f"{tuple(p.shape)}")
+            same = tuple(order) == _memory_order(p)
+            if eight and same:
                 st[_AVG8], st[_SQ8] = codes
+                self._set_order(p, st)
                 return
-            self._init_state(p, st)
-            to = (st["exp_avg"], st["exp_avg_sq"])
-            row = [to[0].data_ptr(), to[1].data_ptr(), p.numel(), codes[0].data_ptr(),
+            if same:
+                avg, sq = (torch.empty_like(p, dtype=torch.float32,
+                                            memory_format=torch.preserve_format) for _ in range(2))
+            else:
+                avg, sq = (torch.empty(p.numel(), dtype=torch.float32, device=p.device)
+                           for _ in range(2))
+            row = [avg.data_ptr(), sq.data_ptr(), p.numel(), codes[0].data_ptr(),
                    codes[1].data_ptr(), p.numel(), _EIGHT, 0]
             self._convert("cs_adamw_unpack_state", p, row, 0)
+            if not same:
+                avg, sq = (fp32(_in_order(t, p.shape, order)) for t in (avg, sq))
         elif "exp_avg" in given:
             avg, sq = fp32(given["exp_avg"]), fp32(given["exp_avg_sq"])
-            if not eight:
-                st["exp_avg"], st["exp_avg_sq"] = avg, sq
-                return
-            self._init_state(p, st)
-            row = [st[_AVG8].data_ptr(), st[_SQ8].data_ptr(), 0, avg.data_ptr(), sq.data_ptr(),
-                   p.numel(), 0, 0]
-            self._convert("cs_adamw_pack_state", p, row)
+        else:
+            return
+        if not eight:
+            st["exp_avg"], st["exp_avg_sq"] = avg, sq
+            return
+        self._init_state(p, st)
+        row = [st[_AVG8].data_ptr(), st[_SQ8].data_ptr(), 0, avg.data_ptr(), sq.data_ptr(),
+               p.numel(), 0, 0]
+        self._convert("cs_adamw_pack_state", p, row)
 
     @staticmethod
     def _convert(name, p, row, *args):
