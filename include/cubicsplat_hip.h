@@ -747,8 +747,9 @@ int cs_grad_norm(int32_t ntensors, const int64_t* table, double max_norm, double
  * forward writes mean and rstd ([n, groups] fp32; both or neither NULL), which
  * the backward reads; the backward writes those of dx, dweight and dbias that are
  * not NULL.  workspace: cs_group_norm_workspace_elems floats, 8-byte aligned, of
- * which nothing is kept between calls.  n * s * c is at most 2^44, and n at most
- * 2^23 (fewer with more than 2048 channels). */
+ * which nothing is kept between calls.  n * s * c is at most 2^44, n at most 2^23
+ * divided by the slices of up to 2048 (fp32: 1024; where channels or addresses are off
+ * 16 bytes: 256) channels, and c under 2^26 where dweight or dbias is written. */
 size_t cs_group_norm_workspace_elems(int64_t n, int64_t s, int32_t c, int32_t groups,
                                      int32_t dtype, int32_t backward);
 int cs_group_norm_forward(const void* x, int64_t n, int64_t s, int32_t c, int32_t groups,

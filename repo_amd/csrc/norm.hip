@@ -1026,11 +1026,11 @@ static GnShape gn_shape(int64_t n, int64_t s, int32_t c, int32_t groups, int* ve
 }
 
 // Whether the sums are joined by a launch of their own: where a workgroup of the
-// second launch would read more of them than this.
+// second launch would read more of them than this, and a group has more than one.
 constexpr int64_t kGnInline = 1024;
 
 static bool gn_joined(const GnShape& h) {
-    return (int64_t)h.chunks * h.parts * h.gs > kGnInline;
+    return (int64_t)h.chunks * h.parts > 1 && (int64_t)h.chunks * h.parts * h.gs > kGnInline;
 }
 
 static uint32_t gn_join_blocks(const GnArgs& a) {
@@ -1091,10 +1091,15 @@ static int gn_whole(int64_t n, int64_t s, int32_t c, int32_t groups, int vec, in
     return (int)threads;
 }
 
-// A launch has fewer than 2^24 workgroups of 256 threads.
-static bool gn_fits(int64_t n, const GnShape& h) {
+// A launch has fewer than 2^24 workgroups of 256 threads: those of the samples, 2^23 at
+// most, and where dw or db is asked for those of the channels' sums beside them.  No product
+// overflows, as n s c is at most 2^44.
+static bool gn_fits(int64_t n, const GnShape& h, bool sums) {
     const int64_t chunks = h.chunks > h.apply_chunks ? h.chunks : h.apply_chunks;
-    return n <= ((int64_t)1 << 23) / (h.slices * chunks);
+    const int64_t join = gn_joined(h) ? n * ((h.groups + kGnJoin - 1) / kGnJoin) : 0;
+    const int64_t blocks = n * h.slices * chunks > join ? n * h.slices * chunks : join;
+    const int64_t channels = sums ? (h.c + (int64_t)kGnChans - 1) / kGnChans : 0;
+    return blocks <= (int64_t)1 << 23 && blocks + channels < (int64_t)1 << 24;
 }
 
 // Stores go past the caches where the tensor is larger than the L2s together, the
@@ -1263,7 +1268,7 @@ extern "C" int cs_group_norm_forward(const void* x, int64_t n, int64_t s, int32_
     const int whole = gn_whole(n, s, c, groups, whole_vec, kGnWholeForward, kGnWholeRowsForward,
                                size, &a.h);
     if (!whole) a.h = gn_shape(n, s, c, groups, &vec);
-    if (!whole && !gn_fits(n, a.h)) return CS_ERR_ARGS;
+    if (!whole && !gn_fits(n, a.h, false)) return CS_ERR_ARGS;
     a.act = act;
     a.x = x;
     a.weight = weight;
@@ -1306,7 +1311,7 @@ extern "C" int cs_group_norm_backward(const void* x, const void* dy, int64_t n, 
     const int whole = gn_whole(n, s, c, groups, whole_vec, kGnWholeBackward, kGnWholeRowsBackward,
                                size, &a.h);
     if (!whole) a.h = gn_shape(n, s, c, groups, &vec);
-    if (!whole && !gn_fits(n, a.h)) return CS_ERR_ARGS;
+    if (!whole && !gn_fits(n, a.h, dweight || dbias)) return CS_ERR_ARGS;
     a.act = act;
     a.x = x;
     a.dy = dy;
