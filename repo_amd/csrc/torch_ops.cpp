@@ -142,6 +142,8 @@ std::optional<Tensor> optional_tensor(PyObject* o) {
     return THPVariable_Unpack(o);
 }
 
+bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+
 // group_norm(x, weight | None, bias | None, groups, eps, act): x channels last
 // without gaps, all arguments checked by the caller.
 PyObject* py_group_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -163,10 +165,13 @@ PyObject* py_group_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         TORCH_CHECK_VALUE(!p || (p->device() == x.device() && p->numel() == x.size(1) &&
                                  type_code(*p) >= 0 && p->is_contiguous()),
                           "group_norm: weight and bias must lie beside x");
-    const bool grad = at::GradMode::is_enabled() &&
-                      (x.requires_grad() || (weight && weight->requires_grad()) ||
-                       (bias && bias->requires_grad()));
-    Tensor y = grad ? GroupNorm::apply(x, weight, bias, groups, eps, act)
+    // A tangent of forward mode goes to the node too, which refuses it.
+    const bool node = (at::GradMode::is_enabled() &&
+                       (x.requires_grad() || (weight && weight->requires_grad()) ||
+                        (bias && bias->requires_grad()))) ||
+                      has_tangent(x) || (weight && has_tangent(*weight)) ||
+                      (bias && has_tangent(*bias));
+    Tensor y = node ? GroupNorm::apply(x, weight, bias, groups, eps, act)
                     : forward(x, weight.value_or(Tensor()), bias.value_or(Tensor()), groups, eps,
                               act, nullptr);
     return THPVariable_Wrap(std::move(y));

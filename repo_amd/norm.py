@@ -48,20 +48,18 @@ def _param_ptr(p):
     return None if p is None else p.data_ptr()
 
 
-def _forward(x, groups, weight, bias, eps, act, stats):
-    """y of x (channels last), and with stats the mean and 1/deviation of each
-    group ([2, N, groups] fp32)."""
+def _forward(x, groups, weight, bias, eps, act):
+    """y of x (channels last), and the mean and 1/deviation of each group
+    ([2, N, groups] fp32)."""
     n, c = x.shape[0], x.shape[1]
     s = x.numel() // (n * c)
     y = _empty_channels_last(x)
     dtype = _DTYPES[x.dtype]
     work = torch.empty(_workspace_elems(n, s, c, groups, dtype, 0), dtype=torch.float32,
                        device=x.device)
-    saved, mean, rstd = None, None, None
-    if stats:
-        saved = torch.empty((2, n, groups), dtype=torch.float32, device=x.device)
-        mean = saved.data_ptr()
-        rstd = mean + 4 * n * groups
+    saved = torch.empty((2, n, groups), dtype=torch.float32, device=x.device)
+    mean = saved.data_ptr()
+    rstd = mean + 4 * n * groups
     affine = weight if weight is not None else bias
     with N.prof("norm.fwd"):
         N.call("cs_group_norm_forward", x.data_ptr(), n, s, c, groups, dtype, _param_ptr(weight),
@@ -73,7 +71,7 @@ def _forward(x, groups, weight, bias, eps, act, stats):
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        y, saved = _forward(x, groups, weight, bias, eps, act, True)
+        y, saved = _forward(x, groups, weight, bias, eps, act)
         ctx.save_for_backward(x, weight, bias, saved)
         ctx.groups, ctx.act = groups, act
         return y
@@ -115,8 +113,8 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     channels last and of x's type.  weight and bias ([C], either may be absent)
     are of x's type or fp32.  activation: None, "relu", "silu" or "gelu" (erf).
     Mean, variance and everything that follows are computed in fp32 and rounded
-    once.  Differentiable (once) in x, weight and bias; gradient sums are taken in
-    a fixed order."""
+    once.  Differentiable (once, in reverse mode; forward-mode derivatives are
+    refused) in x, weight and bias; gradient sums are taken in a fixed order."""
     if x.dim() < 2:
         raise ValueError(f"expected [N, C, ...], got {tuple(x.shape)}")
     if x.dtype not in _DTYPES:
@@ -155,10 +153,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     if ext is not None and N._PROFILE_CTX_FACTORY is None:
         return ext.group_norm(x, weight, bias, int(num_groups), float(eps), act)
     # Without the extension, or where each launch is bracketed by a context manager.
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
-        return _GroupNorm.apply(x, weight, bias, int(num_groups), float(eps), act)
-    return _forward(x, int(num_groups), weight, bias, float(eps), act, False)[0]
+    return _GroupNorm.apply(x, weight, bias, int(num_groups), float(eps), act)
 
 
 def _empty(x, weight, bias):
