@@ -477,6 +477,14 @@ class _Held:
         return [self.place(t) for t in self.tensors] == self.places
 
 
+def _refuse_options(groups):
+    """Options of torch's AdamW that change its update, wherever a group has them from."""
+    for group in groups:
+        for option in ("amsgrad", "maximize", "differentiable"):
+            if group.get(option):
+                raise NotImplementedError(f"repo_amd.optim.AdamW implements {option}=False")
+
+
 class _AdamWEntry:
     """What the launches need of one parameter; remade when a tensor of it is
     another one, or lies elsewhere."""
@@ -694,6 +702,11 @@ class AdamW(torch.optim.Optimizer):
 
     zero_grad = Adam.zero_grad
 
+    def add_param_group(self, param_group):
+        if isinstance(param_group, dict):
+            _refuse_options([param_group])
+        super().add_param_group(param_group)
+
     @property
     def grad_norm(self):
         """The norm over all gradients before the last step's clip, a 0-d
@@ -831,6 +844,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _step(self):
         # Gathered first: nothing is launched or counted if a tensor is refused.
+        _refuse_options(self.param_groups)
         order = self._entries()
         bulk = self._bulk
         if bulk is not None and bulk.version == self._version:
@@ -990,6 +1004,7 @@ class AdamW(torch.optim.Optimizer):
             got = hook(self, state_dict)
             if got is not None:
                 state_dict = got
+        _refuse_options(state_dict["param_groups"])
         slim = {**state_dict, "state": {k: {"step": s["step"]} if "step" in s else {}
                                         for k, s in state_dict["state"].items()}}
         self._optimizer_load_state_dict_pre_hooks = type(pre)()

@@ -351,3 +351,54 @@ def test_8bit_states_loaded_into_another_order(dtype, shape):
         opt.load_state_dict(opt.state_dict())
         p.grad = torch.ones_like(p)
         opt.step()
+
+
+# ------------------------------------------------------- options it has not
+
+
+@pytest.mark.parametrize("option", ["amsgrad", "maximize", "differentiable"])
+def test_options_that_it_has_not_are_refused_wherever_they_come_from(recorded, option):
+    """In a checkpoint of torch's class, in a group's own options, and set later."""
+    from repo_amd.optim import AdamW
+    p = torch.ones(40, requires_grad=True)
+    theirs = torch.optim.AdamW([p], foreach=False)
+    p.grad = torch.ones(40)
+    theirs.step()
+    good = theirs.state_dict()
+    bad = {**good, "param_groups": [{**g, option: True} for g in good["param_groups"]]}
+    opt = AdamW([p])
+    opt.load_state_dict(good)
+    before = {k: v.clone() for k, v in opt.state[p].items()}
+    with pytest.raises(NotImplementedError, match=option):
+        opt.load_state_dict(bad)
+    # Nothing of the refused one was taken.
+    assert not opt.param_groups[0][option]
+    assert all(torch.equal(opt.state[p][k], v) for k, v in before.items())
+    opt.step()
+    assert float(opt.state[p]["step"]) == 2.0 and len(recorded) == 1
+    opt.param_groups[0][option] = True
+    for _ in range(2):
+        with pytest.raises(NotImplementedError, match=option):
+            opt.step()
+    assert float(opt.state[p]["step"]) == 2.0 and len(recorded) == 1
+    with pytest.raises(NotImplementedError, match=option):
+        AdamW([{"params": [p], option: True}])
+    more = AdamW([p])
+    with pytest.raises(NotImplementedError, match=option):
+        more.add_param_group({"params": [torch.ones(3, requires_grad=True)], option: True})
+    assert len(more.param_groups) == 1
+
+
+def test_a_torch_checkpoint_that_counts_on_the_device_is_taken(recorded):
+    """capturable says where torch counts; the update is the same, and so is fused's."""
+    from repo_amd.optim import AdamW
+    p = torch.ones(40, requires_grad=True)
+    theirs = torch.optim.AdamW([p], foreach=False)
+    p.grad = torch.ones(40)
+    theirs.step()
+    good = theirs.state_dict()
+    opt = AdamW([p])
+    opt.load_state_dict({**good, "param_groups": [{**g, "capturable": True, "fused": True}
+                                                  for g in good["param_groups"]]})
+    opt.step()
+    assert float(opt.state[p]["step"]) == 2.0
