@@ -477,6 +477,10 @@ class _Held:
         return [self.place(t) for t in self.tensors] == self.places
 
 
+def _copied(value):
+    return value.detach().clone() if isinstance(value, torch.Tensor) else value
+
+
 def _refuse_options(groups):
     """Options of torch's AdamW that change its update, wherever a group has them from."""
     for group in groups:
@@ -1005,7 +1009,8 @@ class AdamW(torch.optim.Optimizer):
             if got is not None:
                 state_dict = got
         _refuse_options(state_dict["param_groups"])
-        slim = {**state_dict, "state": {k: {"step": s["step"]} if "step" in s else {}
+        # torch's loading would keep the very tensors of the step counts.
+        slim = {**state_dict, "state": {k: {"step": _copied(s["step"])} if "step" in s else {}
                                         for k, s in state_dict["state"].items()}}
         self._optimizer_load_state_dict_pre_hooks = type(pre)()
         self._optimizer_load_state_dict_post_hooks = type(post)()

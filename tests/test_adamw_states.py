@@ -402,3 +402,35 @@ def test_a_torch_checkpoint_that_counts_on_the_device_is_taken(recorded):
                                                   for g in good["param_groups"]]})
     opt.step()
     assert float(opt.state[p]["step"]) == 2.0
+
+
+# --------------------------------------------- what a loaded state consists of
+
+
+@pytest.mark.parametrize("state_bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_loaded_state_is_the_optimizers_own(recorded, state_bits, dtype):
+    """Two optimizers loaded from one state_dict, and that of the first itself: each
+    counts its own steps and shares no tensor."""
+    from repo_amd.optim import AdamW
+    p = torch.ones(300).to(dtype).requires_grad_(True)
+    p.grad = torch.ones_like(p)
+    first = AdamW([p], state_bits=state_bits, min_8bit_numel=0)
+    first.step()
+    saved = first.state_dict()
+    twins = [AdamW([p], state_bits=state_bits, min_8bit_numel=0) for _ in range(2)]
+    for opt in twins:
+        opt.load_state_dict(saved)
+    twins[0].step()
+    twins[0].step()
+    counts = [float(opt.state[p]["step"]) for opt in (first, *twins)]
+    assert counts == [1.0, 3.0, 1.0] and float(saved["state"][0]["step"]) == 1.0
+    places = [t.data_ptr() for opt in (first, *twins) for t in opt.state[p].values()
+              if isinstance(t, torch.Tensor)]
+    assert len(set(places)) == len(places)
+    twins[0].load_state_dict(saved)   # back to the snapshot
+    assert float(twins[0].state[p]["step"]) == 1.0
+    for step in (2, 2.0, torch.tensor(2), torch.tensor(2.0, dtype=torch.float64)):
+        twins[1].load_state_dict({**saved, "state": {0: {**saved["state"][0], "step": step}}})
+        twins[1].step()
+        assert float(twins[1].state[p]["step"]) == 3.0 and float(step) == 2.0
