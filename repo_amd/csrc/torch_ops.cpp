@@ -297,6 +297,20 @@ PyObject* py_adamw_count(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// adamw_written(params): raises the version counters of the tensors that have one.
+PyObject* py_adamw_written(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(nargs == 1 && PyList_Check(args[0]), "adamw_written: expected a list");
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(args[0]); ++i) {
+        PyObject* o = PyList_GET_ITEM(args[0], i);
+        TORCH_CHECK_TYPE(THPVariable_Check(o), "adamw_written: expected tensors");
+        const Tensor& p = THPVariable_Unpack(o);
+        if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+    }
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_signature_hash(PyObject*, PyObject*) {
     return PyUnicode_FromString(CS_SIGNATURE_HASH);
 }
@@ -307,6 +321,7 @@ PyMethodDef methods[] = {
     {"adamw_held", (PyCFunction)(void (*)(void))py_adamw_held, METH_FASTCALL, nullptr},
     {"adamw_current", (PyCFunction)(void (*)(void))py_adamw_current, METH_FASTCALL, nullptr},
     {"adamw_count", (PyCFunction)(void (*)(void))py_adamw_count, METH_FASTCALL, nullptr},
+    {"adamw_written", (PyCFunction)(void (*)(void))py_adamw_written, METH_FASTCALL, nullptr},
     {"signature_hash", py_signature_hash, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

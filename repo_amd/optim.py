@@ -30,6 +30,7 @@ from operator import is_
 
 import numpy as np
 import torch
+from torch.autograd.graph import increment_version
 from torch.optim import optimizer as _torch_optimizer
 
 from . import _native as N
@@ -477,6 +478,15 @@ class _Held:
         return [self.place(t) for t in self.tensors] == self.places
 
 
+def _written(params):
+    """Tells autograd, which knows nothing of the launch, of a write in place."""
+    ext = torchcall.module()
+    if ext is None:
+        increment_version(params)
+    else:
+        ext.adamw_written(params)
+
+
 def _copied(value):
     return value.detach().clone() if isinstance(value, torch.Tensor) else value
 
@@ -857,6 +867,7 @@ class AdamW(torch.optim.Optimizer):
                 self._on(bulk.device, self._launch, bulk.device, bulk.plan,
                          [(k, step) for k in bulk.groups])
                 torchcall.module().adamw_count(bulk.args[-1], bulk.n, step)
+                _written(bulk.args[0])
                 return
         work, number, regular = {}, -1, True
         last, w = None, None
@@ -902,6 +913,7 @@ class AdamW(torch.optim.Optimizer):
             self._on(device, self._launch, device, plan, pairs)
             for e, step in zip(entries, steps):
                 e.step.value = step
+            _written([e.p for e in entries])
 
     @staticmethod
     def _on(device, launch, *args):

@@ -434,3 +434,59 @@ def test_a_loaded_state_is_the_optimizers_own(recorded, state_bits, dtype):
         twins[1].load_state_dict({**saved, "state": {0: {**saved["state"][0], "step": step}}})
         twins[1].step()
         assert float(twins[1].state[p]["step"]) == 3.0 and float(step) == 2.0
+
+
+# ------------------------------------------------------------ version counters
+
+
+@pytest.mark.parametrize("how", EXTENSION)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_step_counts_as_a_write_to_the_parameters(recorded, monkeypatch, how, dtype):
+    """A graph that saved a parameter before the step is refused after it."""
+    from repo_amd import torchcall
+    from repo_amd.optim import AdamW
+    _without_extension(monkeypatch, how)
+    ps = [torch.ones(4, 6).to(dtype).requires_grad_(True),
+          torch.ones(8).to(dtype).requires_grad_(True)]
+    opt = AdamW(ps)
+    for step in range(4):
+        out = (ps[0].square().sum() + ps[1].square().sum()).float()
+        out.backward(retain_graph=True)
+        if step == 2:
+            ps[1].grad = None
+        before = [p._version for p in ps]
+        opt.step()
+        live = [p.grad is not None for p in ps]
+        assert [p._version > v for p, v in zip(ps, before)] == live
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.backward()
+        opt.zero_grad()
+    if how == "extension":
+        for bad in ((), (tuple(ps),), ([None],)):
+            with pytest.raises(TypeError):
+                torchcall.module().adamw_written(*bad)
+    # A tensor made in inference mode has no counter.
+    with torch.inference_mode():
+        q = torch.ones(5)
+        opt = AdamW([q])
+        q.grad = torch.ones(5)
+    for _ in range(3):
+        opt.step()
+    assert float(opt.state[q]["step"]) == 3.0
+
+
+@pytest.mark.gpu
+def test_a_second_backward_through_a_kept_graph_is_refused_after_a_step():
+    from repo_amd.norm import GroupNorm
+    from repo_amd.optim import AdamW
+    net = torch.nn.Sequential(torch.nn.Conv2d(3, 8, 3), GroupNorm(2, 8, activation="silu")).cuda()
+    opt = AdamW(net.parameters())
+    x = torch.randn(2, 3, 9, 9, device="cuda")
+    for _ in range(3):
+        out = net(x).square().sum()
+        out.backward(retain_graph=True)
+        out.backward(retain_graph=True)   # nothing was written in between
+        opt.step()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.backward()
+        opt.zero_grad()
