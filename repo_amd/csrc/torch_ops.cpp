@@ -297,18 +297,40 @@ PyObject* py_adamw_count(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
-// adamw_written(params): raises the version counters of the tensors that have one.
-PyObject* py_adamw_written(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+// What autograd counts of a tensor's writes in place, for those that it counts.
+int64_t version_of(const Tensor& t) { return t.is_inference() ? 0 : (int64_t)t._version(); }
+
+// adamw_unwritten(params, versions): whether each 16-bit parameter's version counter
+// is the one in the array (int64, by address); adamw_written(params, versions): raises
+// all counters and puts them there.
+PyObject* with_versions(PyObject* const* args, Py_ssize_t nargs, bool write) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK_TYPE(nargs == 1 && PyList_Check(args[0]), "adamw_written: expected a list");
-    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(args[0]); ++i) {
+    TORCH_CHECK_TYPE(nargs == 2 && PyList_Check(args[0]), "expected a list and an address");
+    int64_t* versions = (int64_t*)PyLong_AsVoidPtr(args[1]);
+    if (PyErr_Occurred()) return nullptr;
+    const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+    bool same = true;
+    for (Py_ssize_t i = 0; i < n && same; ++i) {
         PyObject* o = PyList_GET_ITEM(args[0], i);
-        TORCH_CHECK_TYPE(THPVariable_Check(o), "adamw_written: expected tensors");
+        TORCH_CHECK_TYPE(THPVariable_Check(o), "expected tensors");
         const Tensor& p = THPVariable_Unpack(o);
-        if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+        if (write) {
+            if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+            versions[i] = version_of(p);
+        } else if (p.scalar_type() != at::kFloat) {
+            same = version_of(p) == versions[i];
+        }
     }
-    Py_RETURN_NONE;
+    return PyBool_FromLong(same);
     END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_adamw_unwritten(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return with_versions(args, nargs, false);
+}
+
+PyObject* py_adamw_written(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return with_versions(args, nargs, true);
 }
 
 PyObject* py_signature_hash(PyObject*, PyObject*) {
@@ -321,6 +343,7 @@ PyMethodDef methods[] = {
     {"adamw_held", (PyCFunction)(void (*)(void))py_adamw_held, METH_FASTCALL, nullptr},
     {"adamw_current", (PyCFunction)(void (*)(void))py_adamw_current, METH_FASTCALL, nullptr},
     {"adamw_count", (PyCFunction)(void (*)(void))py_adamw_count, METH_FASTCALL, nullptr},
+    {"adamw_unwritten", (PyCFunction)(void (*)(void))py_adamw_unwritten, METH_FASTCALL, nullptr},
     {"adamw_written", (PyCFunction)(void (*)(void))py_adamw_written, METH_FASTCALL, nullptr},
     {"signature_hash", py_signature_hash, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},

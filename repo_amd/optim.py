@@ -478,13 +478,33 @@ class _Held:
         return [self.place(t) for t in self.tensors] == self.places
 
 
-def _written(params):
-    """Tells autograd, which knows nothing of the launch, of a write in place."""
-    ext = torchcall.module()
-    if ext is None:
-        increment_version(params)
-    else:
-        ext.adamw_written(params)
+def _version_of(t):
+    """What autograd counts of t's writes in place; tensors of inference mode have no count."""
+    return 0 if t.is_inference() else t._version
+
+
+class _Versions:
+    """The version counters of the parameters when their masters last agreed with them."""
+
+    def __init__(self, params):
+        self.params = params
+        self.values = np.zeros(len(params), dtype=np.int64)
+        self.address, self.ext = self.values.ctypes.data, torchcall.module()
+
+    def unwritten(self):
+        """Whether no 16-bit parameter was written since."""
+        if self.ext is not None:
+            return self.ext.adamw_unwritten(self.params, self.address)
+        return all(p.dtype is torch.float32 or _version_of(p) == v
+                   for p, v in zip(self.params, self.values.tolist()))
+
+    def count(self, entries):
+        """A step has written the entries' parameters, which autograd does not know of."""
+        if self.ext is not None and len(entries) == len(self.params):
+            self.ext.adamw_written(self.params, self.address)
+        else:
+            increment_version([e.p for e in entries])
+            self.values[[e.place[0] for e in entries]] = [_version_of(e.p) for e in entries]
 
 
 def _copied(value):
@@ -648,9 +668,12 @@ class AdamW(torch.optim.Optimizer):
     ``state`` holds ``step`` (a CPU tensor), ``exp_avg`` and ``exp_avg_sq`` in
     fp32, as torch's does for fp32 parameters, so those checkpoints move between
     the two.  A 16-bit parameter has an fp32 copy ``master`` in its state; the
-    update moves the copy, and the parameter is the copy rounded to nearest.
-    Whoever writes to such a parameter by hand deletes ``state[p]["master"]``;
-    the next step makes it anew.
+    update moves the copy, and the parameter is the copy rounded to nearest.  A
+    parameter that is written in place between steps (``load_state_dict`` of the
+    model, for one) is noticed by its version counter: where it is not the copy
+    rounded, the copy takes its values.  Writes that leave the counter alone
+    (through ``p.data``) are not noticed; whoever makes such deletes
+    ``state[p]["master"]``, and the next step makes it anew.
 
     ``state_bits=8`` keeps both moments of a tensor of at least
     ``min_8bit_numel`` elements in a byte each (``exp_avg_8bit``,
@@ -704,6 +727,7 @@ class AdamW(torch.optim.Optimizer):
         # that they were made from, to notice a change of any.
         self._order, self._params, self._sizes, self._keys, self._values = [], [], [], [], []
         self._version, self._bulk, self._plans, self._flat, self._norm = 0, None, {}, None, None
+        self._versions = _Versions([])
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits,
@@ -798,8 +822,12 @@ class AdamW(torch.optim.Optimizer):
                                  f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on "
                                  f"{t.device} beside {tuple(p.shape)} with strides {p.stride()} on "
                                  f"{p.device}")
-        # Codes have no shape of their own: that of the parameter which they last were of.
         old = self._order[number]
+        if (e.master is not None and old is not None and old.master is e.master
+                and (old.ptr != e.ptr or self._versions.values[number] != _version_of(p))):
+            self._follow(e)
+        self._versions.values[number] = _version_of(p)
+        # Codes have no shape of their own: that of the parameter which they last were of.
         if eight and (tuple(st.get(_ORDER8, ())) != _memory_order(p) or (
                 old is not None and old.avg is e.avg and old.shape != p.shape)):
             raise ValueError("an 8-bit AdamW state does not fit its parameter: it is of another "
@@ -818,6 +846,14 @@ class AdamW(torch.optim.Optimizer):
         self._order[number] = e
         return e
 
+    @staticmethod
+    @torch.no_grad()
+    def _follow(e):
+        """Where a 16-bit parameter is not its master rounded it has been written since:
+        the master takes its values there."""
+        p = e.p.detach()
+        e.master.copy_(torch.where(e.master.to(p.dtype) == p, e.master, p.float()))
+
     def _entries(self):
         """The entries in the parameters' order, None where a parameter has none.
         An entry that is there may still have to be remade (`fresh`)."""
@@ -828,11 +864,13 @@ class AdamW(torch.optim.Optimizer):
         if not (sizes == self._sizes and _same(params, self._params) and _same(keys, self._keys)
                 and _same(values, self._values)):
             old = {id(e.p): e for e in self._order if e is not None}
-            self._order = []
+            versions = self._versions.values
+            self._order, self._versions = [], _Versions(params)
             for k, group in enumerate(groups):
                 for p in group["params"]:
                     e = old.get(id(p))
                     if e is not None and e.st is self.state.get(p):
+                        self._versions.values[len(self._order)] = versions[e.place[0]]
                         e.place = (len(self._order), k)
                     else:
                         e = None
@@ -863,13 +901,14 @@ class AdamW(torch.optim.Optimizer):
         bulk = self._bulk
         if bulk is not None and bulk.version == self._version:
             step = bulk.current(True) + 1.0
-            if step > 0.0:
+            if step > 0.0 and self._versions.unwritten():
                 self._on(bulk.device, self._launch, bulk.device, bulk.plan,
                          [(k, step) for k in bulk.groups])
                 torchcall.module().adamw_count(bulk.args[-1], bulk.n, step)
-                _written(bulk.args[0])
+                self._versions.count(bulk.plan.entries)
                 return
         work, number, regular = {}, -1, True
+        written = not self._versions.unwritten()
         last, w = None, None
         for k, group in enumerate(self.param_groups):
             first = None
@@ -881,6 +920,10 @@ class AdamW(torch.optim.Optimizer):
                 e = order[number]
                 if e is None or not e.fresh():
                     e = self._entry(number, k)
+                elif (written and e.master is not None
+                      and self._versions.values[number] != _version_of(p)):
+                    self._follow(e)
+                    self._versions.values[number] = _version_of(p)
                 _check_grad(g, p)
                 if not (e.contiguous and g.is_contiguous()) and not (
                         _is_dense(g) and _same_layout(g, p)):
@@ -913,7 +956,7 @@ class AdamW(torch.optim.Optimizer):
             self._on(device, self._launch, device, plan, pairs)
             for e, step in zip(entries, steps):
                 e.step.value = step
-            _written([e.p for e in entries])
+            self._versions.count(entries)
 
     @staticmethod
     def _on(device, launch, *args):
@@ -1036,6 +1079,14 @@ class AdamW(torch.optim.Optimizer):
         for k, p in zip(ids, params):
             if k in state_dict["state"]:
                 self._take_state(p, state_dict["state"][k])
+        # From here on writes to a parameter are told from what its master was loaded for.
+        self._entries()
+        number = -1
+        for k, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                number += 1
+                if "master" in self.state.get(p, ()):
+                    self._entry(number, k)
         for hook in post.values():
             hook(self)
 
