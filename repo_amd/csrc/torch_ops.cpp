@@ -274,7 +274,7 @@ PyObject* py_adamw_current(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         if (!gradients) continue;
         const Tensor& g = p.grad();
         if (!g.defined() || g.layout() != at::kStrided || g.scalar_type() != p.scalar_type() ||
-            g.device() != p.device() || g.numel() != p.numel() || !g.is_contiguous())
+            g.device() != p.device() || g.sizes() != p.sizes() || !g.is_contiguous())
             return PyFloat_FromDouble(-1.0);
         row[1] = (int64_t)g.data_ptr();
         if (i == 0) step = *steps[0];

@@ -600,3 +600,29 @@ def test_weights_loaded_between_steps_are_trained_on(monkeypatch, how, state_bit
             for p, q in zip(net.parameters(), twin.parameters()):
                 assert torch.equal(p.detach(), q.detach())
                 assert torch.equal(opt.state[p]["master"], ref.state[q]["master"])
+
+
+# ---------------------------------------------------------------- refused shapes
+
+
+@pytest.mark.parametrize("how", EXTENSION)
+def test_gradients_of_another_shape_are_refused_in_every_step(recorded, monkeypatch, how):
+    """Also where they have the parameter's size and lie without gaps, and after steps
+    that all went well."""
+    from repo_amd.optim import AdamW
+    _without_extension(monkeypatch, how)
+    p, q = torch.ones(4, 6, requires_grad=True), torch.ones(3, requires_grad=True)
+    opt = AdamW([p, q])
+    for _ in range(3):
+        p.grad, q.grad = torch.ones(4, 6), torch.ones(3)
+        opt.step()
+    for shape in ((6, 4), (24,), (1, 4, 6)):
+        p.grad = torch.ones(4, 6)
+        p.grad.data = torch.ones(shape)
+        del recorded[:]
+        with pytest.raises(ValueError, match="a gradient of"):
+            opt.step()
+        assert not recorded and float(opt.state[p]["step"]) == float(opt.state[q]["step"]) == 3.0
+    p.grad = torch.ones(4, 6)
+    opt.step()
+    assert float(opt.state[p]["step"]) == 4.0
