@@ -1097,6 +1097,9 @@ class AdamW(torch.optim.Optimizer):
         eight = self._eight(p.numel())
 
         def fp32(t):
+            if t.shape != p.shape:   # copy_ would broadcast it
+                raise ValueError(f"an AdamW state does not fit its parameter: {tuple(t.shape)} "
+                                 f"beside {tuple(p.shape)}")
             return torch.empty_like(p, dtype=torch.float32,
                                     memory_format=torch.preserve_format).copy_(t)
 

@@ -626,3 +626,21 @@ def test_gradients_of_another_shape_are_refused_in_every_step(recorded, monkeypa
     p.grad = torch.ones(4, 6)
     opt.step()
     assert float(opt.state[p]["step"]) == 4.0
+
+
+@pytest.mark.parametrize("state_bits", [32, 8])
+@pytest.mark.parametrize("name", ["exp_avg", "exp_avg_sq", "master"])
+def test_loaded_states_of_another_shape_are_refused(recorded, state_bits, name):
+    """None is spread over its parameter because it happens to broadcast."""
+    from repo_amd.optim import AdamW
+    p = torch.ones(4, 6).bfloat16().requires_grad_(True)
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], min_8bit_numel=0)
+    opt.step()
+    saved = opt.state_dict()
+    for shape in ((), (1,), (6,), (4, 1), (6, 4), (24,), (1, 4, 6)):
+        to = AdamW([p], state_bits=state_bits, min_8bit_numel=0)
+        state = {**saved["state"][0], name: torch.zeros(shape)}
+        with pytest.raises(ValueError, match="does not fit"):
+            to.load_state_dict({**saved, "state": {0: state}})
+    to.load_state_dict(saved)
