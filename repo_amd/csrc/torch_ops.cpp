@@ -302,26 +302,27 @@ int64_t version_of(const Tensor& t) { return t.is_inference() ? 0 : (int64_t)t._
 
 // adamw_unwritten(params, versions): whether each 16-bit parameter's version counter
 // is the one in the array (int64, by address); adamw_written(params, versions): raises
-// all counters and puts them there.
+// all counters and then puts them there (views of one buffer share theirs).
 PyObject* with_versions(PyObject* const* args, Py_ssize_t nargs, bool write) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(nargs == 2 && PyList_Check(args[0]), "expected a list and an address");
     int64_t* versions = (int64_t*)PyLong_AsVoidPtr(args[1]);
     if (PyErr_Occurred()) return nullptr;
     const Py_ssize_t n = PyList_GET_SIZE(args[0]);
-    bool same = true;
-    for (Py_ssize_t i = 0; i < n && same; ++i) {
-        PyObject* o = PyList_GET_ITEM(args[0], i);
-        TORCH_CHECK_TYPE(THPVariable_Check(o), "expected tensors");
-        const Tensor& p = THPVariable_Unpack(o);
-        if (write) {
-            if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
-            versions[i] = version_of(p);
-        } else if (p.scalar_type() != at::kFloat) {
-            same = version_of(p) == versions[i];
-        }
+    for (Py_ssize_t i = 0; i < n; ++i)
+        TORCH_CHECK_TYPE(THPVariable_Check(PyList_GET_ITEM(args[0], i)), "expected tensors");
+    for (Py_ssize_t i = 0; i < n && write; ++i) {
+        const Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(args[0], i));
+        if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
     }
-    return PyBool_FromLong(same);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(args[0], i));
+        if (write)
+            versions[i] = version_of(p);
+        else if (p.scalar_type() != at::kFloat && version_of(p) != versions[i])
+            Py_RETURN_FALSE;
+    }
+    Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }
 

@@ -503,8 +503,12 @@ class _Versions:
         if self.ext is not None and len(entries) == len(self.params):
             self.ext.adamw_written(self.params, self.address)
         else:
+            # Views of one buffer share their counter, also with those that take no part.
+            before = [_version_of(p) for p in self.params]
+            agreed = self.values == before
+            agreed[[e.place[0] for e in entries]] = True
             increment_version([e.p for e in entries])
-            self.values[[e.place[0] for e in entries]] = [_version_of(e.p) for e in entries]
+            self.values[agreed] = np.array([_version_of(p) for p in self.params])[agreed]
 
 
 def _copied(value):
