@@ -184,8 +184,8 @@ PyObject* py_group_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 struct Place {
     int64_t address, type, numel, order;
     explicit Place(const Tensor& t)
-        : address((int64_t)t.data_ptr()),
-          type((int64_t)t.scalar_type() << 8 | (int64_t)t.layout()),
+        : address((int64_t)t.const_data_ptr()),
+          type((int64_t)t.scalar_type()),
           numel(t.numel()),
           order(0) {
         if (t.is_contiguous()) return;
@@ -199,6 +199,41 @@ struct Place {
         order = (int64_t)mix;
     }
 };
+
+// adamw_unchanged(groups, params, sizes, state, keys, values): whether the groups' lists
+// of parameters are `params`, one list after the other and sizes[k] of them each, and
+// the dict `state` has these keys and values, the same objects in the same order.
+PyObject* py_adamw_unchanged(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(nargs == 6 && PyDict_Check(args[3]), "adamw_unchanged: expected 6 arguments");
+    for (int k : {0, 1, 2, 4, 5})
+        TORCH_CHECK_TYPE(PyList_Check(args[k]), "adamw_unchanged: expected lists");
+    PyObject *params = args[1], *sizes = args[2], *keys = args[4], *values = args[5];
+    const Py_ssize_t ngroups = PyList_GET_SIZE(args[0]), n = PyDict_Size(args[3]);
+    if (ngroups != PyList_GET_SIZE(sizes) || n != PyList_GET_SIZE(keys) ||
+        n != PyList_GET_SIZE(values))
+        Py_RETURN_FALSE;
+    Py_ssize_t at = 0;
+    for (Py_ssize_t k = 0; k < ngroups; ++k) {
+        PyObject* group = PyList_GET_ITEM(args[0], k);
+        PyObject* list = PyDict_Check(group) ? PyDict_GetItemString(group, "params") : nullptr;
+        if (!list || !PyList_Check(list)) Py_RETURN_FALSE;
+        const Py_ssize_t size = PyList_GET_SIZE(list);
+        if (PyLong_AsSsize_t(PyList_GET_ITEM(sizes, k)) != size ||
+            at + size > PyList_GET_SIZE(params))
+            Py_RETURN_FALSE;
+        for (Py_ssize_t i = 0; i < size; ++i, ++at)
+            if (PyList_GET_ITEM(list, i) != PyList_GET_ITEM(params, at)) Py_RETURN_FALSE;
+    }
+    if (at != PyList_GET_SIZE(params)) Py_RETURN_FALSE;
+    PyObject *key, *value;
+    Py_ssize_t pos = 0;
+    for (Py_ssize_t i = 0; PyDict_Next(args[3], &pos, &key, &value); ++i)
+        if (key != PyList_GET_ITEM(keys, i) || value != PyList_GET_ITEM(values, i))
+            Py_RETURN_FALSE;
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
 
 // adamw_place(tensors, places): writes each tensor's Place into the array by that
 // address; adamw_held(tensors, places): whether all still are what it holds.
@@ -298,11 +333,15 @@ PyObject* py_adamw_count(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // What autograd counts of a tensor's writes in place, for those that it counts.
-int64_t version_of(const Tensor& t) { return t.is_inference() ? 0 : (int64_t)t._version(); }
+int64_t version_of(const Tensor& t) {
+    return t.is_inference() ? 0
+                            : (int64_t)t.unsafeGetTensorImpl()->version_counter().current_version();
+}
 
 // adamw_unwritten(params, versions): whether each 16-bit parameter's version counter
 // is the one in the array (int64, by address); adamw_written(params, versions): raises
-// all counters and then puts them there (views of one buffer share theirs).
+// all counters and then puts those of the 16-bit parameters there (views of one buffer
+// share theirs).
 PyObject* with_versions(PyObject* const* args, Py_ssize_t nargs, bool write) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(nargs == 2 && PyList_Check(args[0]), "expected a list and an address");
@@ -317,9 +356,10 @@ PyObject* with_versions(PyObject* const* args, Py_ssize_t nargs, bool write) {
     }
     for (Py_ssize_t i = 0; i < n; ++i) {
         const Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(args[0], i));
+        if (p.scalar_type() == at::kFloat) continue;
         if (write)
             versions[i] = version_of(p);
-        else if (p.scalar_type() != at::kFloat && version_of(p) != versions[i])
+        else if (version_of(p) != versions[i])
             Py_RETURN_FALSE;
     }
     Py_RETURN_TRUE;
@@ -340,6 +380,7 @@ PyObject* py_signature_hash(PyObject*, PyObject*) {
 
 PyMethodDef methods[] = {
     {"group_norm", (PyCFunction)(void (*)(void))py_group_norm, METH_FASTCALL, nullptr},
+    {"adamw_unchanged", (PyCFunction)(void (*)(void))py_adamw_unchanged, METH_FASTCALL, nullptr},
     {"adamw_place", (PyCFunction)(void (*)(void))py_adamw_place, METH_FASTCALL, nullptr},
     {"adamw_held", (PyCFunction)(void (*)(void))py_adamw_held, METH_FASTCALL, nullptr},
     {"adamw_current", (PyCFunction)(void (*)(void))py_adamw_current, METH_FASTCALL, nullptr},

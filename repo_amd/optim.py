@@ -518,9 +518,10 @@ def _copied(value):
 def _refuse_options(groups):
     """Options of torch's AdamW that change its update, wherever a group has them from."""
     for group in groups:
-        for option in ("amsgrad", "maximize", "differentiable"):
-            if group.get(option):
-                raise NotImplementedError(f"repo_amd.optim.AdamW implements {option}=False")
+        get = group.get
+        if get("amsgrad") or get("maximize") or get("differentiable"):
+            option = next(o for o in ("amsgrad", "maximize", "differentiable") if get(o))
+            raise NotImplementedError(f"repo_amd.optim.AdamW implements {option}=False")
 
 
 class _AdamWEntry:
@@ -861,7 +862,10 @@ class AdamW(torch.optim.Optimizer):
     def _entries(self):
         """The entries in the parameters' order, None where a parameter has none.
         An entry that is there may still have to be remade (`fresh`)."""
-        groups = self.param_groups
+        groups, ext = self.param_groups, torchcall.module()
+        if ext is not None and ext.adamw_unchanged(groups, self._params, self._sizes, self.state,
+                                                   self._keys, self._values):
+            return self._order
         params = [p for group in groups for p in group["params"]]
         sizes = [len(group["params"]) for group in groups]
         keys, values = list(self.state), list(self.state.values())

@@ -165,6 +165,35 @@ def test_places_of_tensors():
             ext.adamw_held(*bad)
 
 
+def test_what_counts_as_unchanged():
+    """The extension's look at the groups and the states, and its refusals."""
+    from repo_amd import torchcall
+    ext = torchcall.module()
+    if ext is None:
+        pytest.skip("extension not built (run __graft_entry__.build())")
+    a, b, c = (torch.zeros(1) for _ in range(3))
+    x, y = {}, {}
+
+    def now(groups=((a, b), (c,)), params=(a, b, c), sizes=(2, 1), state=((a, x), (c, y)),
+            keys=(a, c), values=(x, y)):
+        return ext.adamw_unchanged([{"params": list(g)} for g in groups], list(params),
+                                   list(sizes), dict(state), list(keys), list(values))
+
+    assert now() is True
+    assert now(groups=(), params=(), sizes=(), state=(), keys=(), values=()) is True
+    for other in (dict(groups=((a,), (b, c))), dict(groups=((b, a), (c,))),
+                  dict(groups=((a, b), ())), dict(groups=((a, b),)), dict(groups=((a, b, c), ())),
+                  dict(groups=((a, b), (c, c))), dict(params=(a, b)), dict(params=(a, b, c, c)),
+                  dict(sizes=(2,)), dict(state=((a, x),)), dict(state=((c, y), (a, x))),
+                  dict(state=((a, x), (c, {}))), dict(state=((a, x), (b, y))),
+                  dict(state=((a, x), (c, y), (b, {}))), dict(keys=(a,)), dict(values=(x,))):
+        assert now(**other) is False, other
+    assert ext.adamw_unchanged([{}], [], [0], {}, [], []) is False
+    for bad in ((), ([], [], [], [], [], []), ([], (), [], {}, [], [])):
+        with pytest.raises(TypeError):
+            ext.adamw_unchanged(*bad)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("how", EXTENSION)
 @pytest.mark.parametrize("state_bits", [32, 8])
