@@ -430,6 +430,8 @@ def _same_layout(a, b):
 def _memory_order(t):
     """The dimensions of a dense tensor from the outermost in memory to the innermost,
     without those of size one; () for the logical order."""
+    if t.is_contiguous():
+        return ()
     dims = [d for d in range(t.dim()) if t.shape[d] != 1]
     order = sorted(dims, key=lambda d: -t.stride(d))
     return () if t.numel() < 2 or order == dims else tuple(order)
@@ -464,8 +466,8 @@ class _Held:
         if ext is None:
             self.places = [self.place(t) for t in self.tensors]
         else:
-            self.places = np.empty((len(self.tensors), 4), dtype=np.int64)
-            self.address = self.places.ctypes.data
+            self.places = (ctypes.c_int64 * (4 * len(self.tensors)))()
+            self.address = ctypes.addressof(self.places)
             ext.adamw_place(self.tensors, self.address)
 
     @staticmethod
