@@ -35,9 +35,11 @@
 // launch takes up to 56 tensors, whose pointers travel in its arguments, so nothing
 // of the step is uploaded; a workgroup takes one pass of 2048 elements of one tensor,
 // found by one ballot over the tensors' first workgroups, and its loads go out
-// together.  Measured: fp32 states 890 us of 197M bf16 weights (6.2 TB/s), 67 us of
-// 16.3M fp32 (6.8 TB/s); 8-bit states 139 us of 54.5M bf16 (6.3 TB/s), 45 us of 16.3M
-// fp32 (5.8 TB/s).
+// together.  Measured (means of a kernel trace): fp32 states 897 us of 197M bf16 weights
+// (6.1 TB/s), 69 us of 16.3M fp32 (6.6 TB/s); 8-bit states 525 us of 197M bf16 (6.0
+// TB/s), 165 us of 60.0M bf16 (5.8 TB/s), 45 us of 16.3M fp32 (5.8 TB/s).  Tensors off 16
+// bytes are read and written value by value: 16.7M, most of them off, 137 us fp32 and
+// 153 us bf16 with fp32 states, where aligned ones take 70 and 74.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -483,9 +485,9 @@ __global__ __launch_bounds__(kAwThreads) void k_adamw_pack(AwArgs a) {
 }
 
 // What the states stand for, in T.  Bound: HBM, 6 bytes an element from 8 bits to
-// bf16: 206 us of 197M (5.7 TB/s).  16-bit values go past the caches (bf16, us
-// without and with: 54.5M values of each moment 63 and 50, 16.3M 21.9 and 16.9, 3.5M
-// 6.7 and 5.4); fp32 values lie 32 bytes a lane, in two stores that only the cache
+// bf16: 226 us of 197M (5.2 TB/s), 17 us of 16.3M.  16-bit values go past the caches
+// (bf16, us without and with: 54.5M values of each moment 63 and 50, 16.3M 21.9 and 16.9,
+// 3.5M 6.7 and 5.4); fp32 values lie 32 bytes a lane, in two stores that only the cache
 // joins.
 template <typename T>
 __device__ inline void aw_unpack(const AwTensor& t, int64_t begin, int64_t end) {
@@ -531,8 +533,9 @@ __global__ __launch_bounds__(kAwThreads) void k_adamw_unpack(AwArgs a) {
 // ---- the gradients' norm
 
 // One launch sums squares, up to 2048 workgroups over all tensors, and a workgroup
-// of its own joins them in fp64.  Bound: HBM, reads the gradients: 69 us of 197M bf16
-// (5.7 TB/s), 14 us of 16.3M fp32 (4.6 TB/s), and 4 us for the joining launch.
+// of its own joins them in fp64.  Bound: HBM, reads the gradients: 68 us of 197M bf16
+// (5.8 TB/s; 78 after the values of 8-bit states were written), 14 us of 16.3M fp32 (4.6
+// TB/s), and 4 us for the joining launch.
 struct NormTensor {
     const void* grad;
     int64_t n;
@@ -657,11 +660,14 @@ enum AwOp { kStep, kPack, kUnpack };
 constexpr int64_t kAwBlocks = (int64_t)1 << 21;
 
 // The moments go past the caches where a step moves more than the memory-side cache
-// holds (fp32, us with and without: 10.1M weights, 283 MB, 43.8 and 47.6; 6.4M, 179
-// MB, 29.8 and 28.4); the weights and gradients too where they alone are more than
-// it holds (bf16, 197M, us: nothing 1027, the moments 1010, all 920; fp32, 16.3M:
-// 87, 68, 75).  With 8-bit states the weights and gradients: 197M 580 and 539, 16.3M
-// (261 MB) 49.7 and 46.4, 6.4M (102 MB) 21.4 and 21.8.
+// holds (three states in turn, us without and with: fp32, 3.2M weights, 85 MB, 15.6 and
+// 16.6; 6.4M, 171 MB, 30.7 and 29.2; 10.1M, 270 MB, 55.9 and 46.1); the weights and
+// gradients too where they alone are more than it holds (us: nothing, the moments, all:
+// fp32 16.3M 84.6, 76.0, 75.9; 36M 190, 180, 169; bf16 54.5M 286, 278, 257; 197M 1045,
+// 1020, 987).  With 8-bit states the weights and gradients go past them above the first
+// limit: bf16 197M 569 and 521, fp32 16.3M (249 MB) 51.9 and 46.9; below it the step
+// gains little (10.1M, 154 MB, 32.6 and 30.9; 6.4M, 98 MB, 22.6 and 22.4), and what
+// reads the weights next finds them in the caches.
 constexpr int64_t kAwPastBytes = (int64_t)224 << 20;
 constexpr int64_t kAwPastWeights = (int64_t)256 << 20;
 

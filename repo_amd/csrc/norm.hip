@@ -26,6 +26,9 @@
 // The variance is not formed from a sum of squares: each thread sums x and x^2
 // relative to its first value per channel, and (count, mean, sum of squared
 // deviations) are what is joined, so a mean far from zero costs nothing.
+//
+// Times at the kernels are means of a kernel trace; pairs that a rule is chosen by are
+// whole passes, both sides in turn.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -157,7 +160,12 @@ __device__ inline float gn_sigmoid(float z) {
 }
 
 // The normal distribution's tail below -|z| and e = exp(-z^2 / 2): erfc(x) = t P(t)
-// exp(-x^2), t = 1 / (1 + p x), Abramowitz and Stegun 7.1.26, within 1.5e-7.
+// exp(-x^2), t = 1 / (1 + p x), Abramowitz and Stegun 7.1.26, within 1.5e-7 of it, and
+// the exponential is the slope's too.  GELU is within 2.1e-7 for z < 0, relative to its
+// value 3e-6 at -2, 5e-5 at -3 and 5e-4 at -4, where z (1 + erf) / 2 in fp32 has 9e-7,
+// 1e-5 and 5e-4 (beyond that it loses all, and this does not).  With the library's erfc
+// a pass forward and backward takes 427 us for 239 (24x24576x128 bf16) and 470 for 397
+// (fp32).
 __device__ inline float gn_tail(float z, float* e) {
     const float x = __builtin_fabsf(z);
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(x, 0.3275911f * 0.70710678f, 1.0f));
@@ -304,7 +312,9 @@ __device__ inline void gn_groups_sum(const float* buf, float* out, const GnPlace
 // ---- forward
 
 // Mean and squared deviations of a slice's groups over a chunk.  Reads x once: 32 us
-// of 24x24576x128 bf16 (4.7 TB/s), 64 us of 2766240x32 fp32 (5.5 TB/s).
+// of 24x24576x128 bf16 (4.7 TB/s), 67 us of 2766240x32 fp32 (5.3 TB/s).  Small tensors
+// (8x6144x128 bf16, 12.6 MB: 10.6 us, 1.2 TB/s) wait for its four sums over the
+// workgroup, which has four rows a thread to read.
 template <typename T, int V>
 __global__ __launch_bounds__(kGnThreads) void k_gn_stats(GnArgs a) {
     __shared__ float buf[kGnThreads * V];
@@ -465,8 +475,8 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_join_stats(GnArgs a) {
     }
 }
 
-// y from x and the joined statistics.  Reads x, writes y: 50 us of 24x24576x128 bf16
-// (6.0 TB/s), 104 us of 2766240x32 fp32 (6.8 TB/s).  PAST: 1 stores past the caches,
+// y from x and the joined statistics.  Reads x, writes y: 51 us of 24x24576x128 bf16
+// (6.0 TB/s), 105 us of 2766240x32 fp32 (6.7 TB/s).  PAST: 1 stores past the caches,
 // 2 loads too.
 template <typename T, int V, int ACT, int PAST>
 __global__ __launch_bounds__(kGnThreads) void k_gn_apply(GnArgs a) {
@@ -529,8 +539,9 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_apply(GnArgs a) {
 // ---- backward
 
 // Sums of dz and dz xh per channel and, weighted, per group over a chunk.  Reads x and
-// dy: 60 us of 24x24576x128 bf16 silu (5.0 TB/s; its arithmetic takes some 40 of
-// them at the VALU's full rate), 122 us of 2766240x32 fp32 (5.8 TB/s).
+// dy: 61 us of 24x24576x128 bf16 silu (5.0 TB/s; its arithmetic takes some 40 of
+// them at the VALU's full rate), 81 with gelu, 126 us of 2766240x32 fp32 silu (5.6 TB/s);
+// 13.3 us of 8x6144x128 bf16 (25 MB, 1.9 TB/s: as k_gn_stats).
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_sums(GnArgs a) {
     __shared__ float buf[kGnThreads * V], chan_sums[2][kGnThreads * V], gsum[kGnThreads * V];
@@ -696,7 +707,7 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_join_sums(GnArgs a) {
 }
 
 // dx from x, dy and the joined sums.  Reads x and dy, writes dx: 74 us of 24x24576x128
-// bf16 silu (6.1 TB/s), 153 us of 2766240x32 fp32 (6.9 TB/s).  PAST as above.  The
+// bf16 silu (6.1 TB/s), 155 us of 2766240x32 fp32 (6.8 TB/s).  PAST as above.  The
 // first workgroups join dw and db where no launch in between has done so.
 template <typename T, int V, int ACT, int PAST>
 __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_apply(GnArgs a) {
@@ -771,8 +782,9 @@ __global__ __launch_bounds__(kGnThreads) void k_gn_bwd_apply(GnArgs a) {
 // ---- one launch: a workgroup keeps its slice of a sample in registers
 
 // At most kGnWholeThreads threads with P vectors each; x (and dy) are read once.
-// Bound: latency, of the launch, one reading and two to four sums over the workgroup
-// (1x384x256 bf16: 8.5 us of kernel where the two launches took 15).
+// Bound: latency, of the launch (some 4 us of any kernel in a trace), one reading and
+// two to four sums over the workgroup (1x384x256 bf16: 8.7 us forward and 10.6 backward,
+// the two launches forward took 15; 4x1024x128 bf16: 9.8 and 13.5).
 constexpr int kGnWholeThreads = 1024;
 
 extern __shared__ float gn_lds[];
@@ -1029,6 +1041,8 @@ static GnShape gn_shape(int64_t n, int64_t s, int32_t c, int32_t groups, int* ve
 // second launch would read more of them than this, and a group has more than one.
 constexpr int64_t kGnInline = 1024;
 
+// (8192x8x2048 bf16, a channel a group, one partial result each: joined all the same, in
+// 4 million workgroups, 9620 us forward and backward, 590 not.)
 static bool gn_joined(const GnShape& h) {
     return (int64_t)h.chunks * h.parts > 1 && (int64_t)h.chunks * h.parts * h.gs > kGnInline;
 }

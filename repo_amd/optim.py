@@ -592,8 +592,9 @@ class _AdamWPlan:
 
 class _AdamWBulk:
     """All parameters at once, where each has a state and is contiguous, and all
-    are on one device: one call of the extension looks at every parameter, state
-    and gradient (53 of them: 4 us, where the entries' own checks take 30)."""
+    are on one device: a few calls of the extension look at every parameter, state
+    and gradient (a step of 53 of them: 12 us of host time, where 53 that are not
+    contiguous take 98 by their entries' own checks)."""
 
     def __init__(self, version, entries, ngroups):
         self.version, self.device, self.n = version, entries[0].device, len(entries)
