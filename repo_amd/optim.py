@@ -432,9 +432,8 @@ def _memory_order(t):
     without those of size one; () for the logical order."""
     if t.is_contiguous():
         return ()
-    dims = [d for d in range(t.dim()) if t.shape[d] != 1]
-    order = sorted(dims, key=lambda d: -t.stride(d))
-    return () if t.numel() < 2 or order == dims else tuple(order)
+    return tuple(sorted((d for d in range(t.dim()) if t.shape[d] != 1),
+                        key=lambda d: -t.stride(d)))
 
 
 def _in_order(flat, shape, order):
@@ -1124,7 +1123,7 @@ class AdamW(torch.optim.Optimizer):
             if any(c.dtype is not torch.uint8 or c.numel() != _codes_numel(p.numel())
                    for c in codes):
                 raise ValueError("8-bit AdamW states of another size than the parameter's")
-            order = given.get(_ORDER8, ())
+            order = given.get(_ORDER8) or ()
             if order and not (isinstance(order, (tuple, list)) and sorted(order) == [
                     d for d in range(p.dim()) if p.shape[d] != 1]):
                 raise ValueError(f"8-bit AdamW states in an order {order} of the dimensions of "
