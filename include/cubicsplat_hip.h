@@ -762,6 +762,49 @@ int cs_group_norm_backward(const void* x, const void* dy, int64_t n, int64_t s, 
                            const float* rstd, float* workspace, void* dx, void* dweight,
                            void* dbias, hipStream_t stream);
 
+/* ---------------- log-probabilities of tokens, policy loss ---------------- */
+
+/* New (the reference has no tokens).  Row t of sequence b holds vocab logits
+ * (contiguous) at logits + b * batch_stride + t * row_stride elements, of dtype 0
+ * fp32, 1 bf16, 2 fp16, at any element's address; tokens [batch, length], mask
+ * [batch, length] bytes or NULL (all rows count), logprobs [batch, length].  A row
+ * that the mask leaves out is not read: its log-probability is 0 and its gradients are
+ * zeros.  A token outside the vocabulary gives NaN.  stats [batch, length, 2]: what
+ * the backward reads of each row's sum.  batch * length * vocab is at most 2^44.
+ *
+ * The backward writes grad [batch, length, vocab] (contiguous, of dtype) for upstream
+ * [batch, length], multiplied with the device scalar *factor where it is not NULL;
+ * with unless_one it writes nothing where *factor is 1. */
+int cs_token_logprobs_forward(const void* logits, int64_t batch, int64_t length, int64_t vocab,
+                              int64_t batch_stride, int64_t row_stride, int32_t dtype,
+                              const int64_t* tokens, const uint8_t* mask, double temperature,
+                              float* stats, float* logprobs, hipStream_t stream);
+int cs_token_logprobs_backward(const void* logits, int64_t batch, int64_t length, int64_t vocab,
+                               int64_t batch_stride, int64_t row_stride, int32_t dtype,
+                               const int64_t* tokens, const uint8_t* mask, double temperature,
+                               const float* stats, const float* upstream, const float* factor,
+                               int32_t unless_one, void* grad, hipStream_t stream);
+
+/* The clipped policy loss with a KL term, on rows as above:
+ *   scale * sum_t w_t (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
+ *                      + kl_weight (exp(d) - d - 1)),   r = exp(l - old), d = ref - l
+ * over the rows that count, w_t = 1 / (their number) (reduction 0), 1 / (their number
+ * in the sequence) / (sequences with such rows) (1), or 1 (2).  advantages at b *
+ * adv_batch_stride + t * adv_stride (0: broadcast); old_logprobs and ref_logprobs
+ * (NULL: no KL term) [batch, length].  out: the loss, the KL estimate (weighted by w) and
+ * the weight of the rows whose ratio was clipped.  slopes [batch, length]: the loss's
+ * derivatives by the log-probabilities (for cs_token_logprobs_backward); grad (may be NULL):
+ * by the logits.  workspace: cs_policy_loss_workspace_elems floats, 8-byte aligned, of
+ * which nothing is kept between calls. */
+size_t cs_policy_loss_workspace_elems(int64_t batch, int64_t length);
+int cs_policy_loss(const void* logits, int64_t batch, int64_t length, int64_t vocab,
+                   int64_t batch_stride, int64_t row_stride, int32_t dtype, const int64_t* tokens,
+                   const uint8_t* mask, double temperature, const float* advantages,
+                   int64_t adv_batch_stride, int64_t adv_stride, const float* old_logprobs,
+                   const float* ref_logprobs, double clip_low, double clip_high, double kl_weight,
+                   int32_t reduction, double scale, float* workspace, float* stats, float* slopes,
+                   float* logprobs, float* out, void* grad, hipStream_t stream);
+
 /* ---------------- 2D Gaussian splats (GsRenderFunction) ---------------- */
 
 /* project_gaussians_2d_scale_rot_forward_kernel (ops/forward2d.py:14-164):

@@ -1,6 +1,7 @@
 """Float64 restatements of the operators for networks in front of the renderer
 (numpy, from the formulas): group norm with an activation and its gradients,
-the AdamW step, and what the 8-bit optimizer states hold."""
+the AdamW step, what the 8-bit optimizer states hold, Newton-Schulz steps and the
+Muon step, log-probabilities of tokens and the clipped policy loss."""
 from __future__ import annotations
 
 import math
@@ -118,3 +119,76 @@ def hold8(x, mantissa, r, floor=False):
         whole = np.where((a > 0) & (whole == 0), 1.0, whole)
     held = np.where(finite, np.copysign(whole * spacing * unit, rows), np.nan)
     return held.reshape(-1)[:n], e.reshape(-1)
+
+
+# ---------------------------------------------------------------------- Muon
+
+
+def newton_schulz64(x, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """x [..., m, n] after the steps x <- a x + (b g + c g^2) x, g = x x^T."""
+    x = np.asarray(x, np.float64)
+    if x.shape[-2] > x.shape[-1]:
+        return np.swapaxes(newton_schulz64(np.swapaxes(x, -1, -2), steps, coefficients, eps), -1, -2)
+    a, b, c = coefficients
+    x = x / np.maximum(np.sqrt((x * x).sum((-1, -2), keepdims=True)), eps)
+    for _ in range(steps):
+        g = x @ np.swapaxes(x, -1, -2)
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x
+
+
+def muon_step64(p, g, momentum_buffer, *, lr, weight_decay=0.1, momentum=0.95, nesterov=True,
+                adjust=None, **newton_schulz):
+    """(p, momentum_buffer) after one step."""
+    p, g, m = (np.asarray(a, np.float64) for a in (p, g, momentum_buffer))
+    m = m + (1 - momentum) * (g - m)
+    u = (g + momentum * (m - g) if nesterov else m).reshape(p.shape[0], -1)
+    rows, cols = u.shape
+    by = (0.2 * math.sqrt(max(rows, cols)) if adjust == "match_rms_adamw"
+          else math.sqrt(max(1.0, rows / cols)))
+    o = newton_schulz64(u, **newton_schulz).reshape(p.shape)
+    return p * (1 - lr * weight_decay) - lr * by * o, m
+
+
+# -------------------------------------------------------------------- tokens
+
+
+def token_logprobs64(z, tokens, mask=None, temperature=1.0, upstream=None):
+    """z [..., V]: the chosen tokens' log-probabilities, or with upstream (they, dz)."""
+    z = np.asarray(z, np.float64) / temperature
+    mask = np.ones(tokens.shape, bool) if mask is None else np.asarray(mask, bool)
+    z = np.where(mask[..., None], z, 0.0)
+    at = np.where(mask, tokens, 0)[..., None]
+    top = z.max(-1, keepdims=True)
+    e = np.exp(z - top)
+    total = e.sum(-1, keepdims=True)
+    lp = np.where(mask, (np.take_along_axis(z - top, at, -1) - np.log(total))[..., 0], 0.0)
+    if upstream is None:
+        return lp
+    slope = np.where(mask, upstream, 0.0)[..., None] / temperature
+    dz = -slope * (e / total)
+    np.put_along_axis(dz, at, np.take_along_axis(dz, at, -1) + slope, -1)
+    return lp, dz
+
+
+def policy_terms64(lp, old, adv, ref=None, clip=(0.2, 0.2), kl_weight=0.0):
+    """(loss, derivative by lp, KL estimate, clipped) of each token."""
+    r = np.exp(lp - old)
+    low, high = 1 - clip[0], 1 + clip[1]
+    gain = np.minimum(r * adv, np.clip(r, low, high) * adv)
+    clipped = np.where(adv >= 0, r > high, r < low)
+    slope = np.where(clipped, 0.0, -adv * r)
+    d = np.zeros_like(lp) if ref is None else ref - lp
+    kl = np.expm1(d) - d
+    return -gain + kl_weight * kl, slope - kl_weight * np.expm1(d), kl, clipped & (adv != 0)
+
+
+def policy_weights64(mask, reduction):
+    """The weight of each token; the last dimension is a sequence's."""
+    m = np.asarray(mask, np.float64)
+    if reduction == "sum":
+        return m
+    if reduction == "token":
+        return m / max(1.0, m.sum())
+    n = m.sum(-1, keepdims=True)
+    return m / np.maximum(n, 1.0) / max(1.0, float((n > 0).sum()))

@@ -142,6 +142,14 @@ _SIGNATURES = {
                                              _I32, _P, _P, _P, _P, _P]),
     "cs_group_norm_backward": (ctypes.c_int, [_P, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _I32,
                                               _I32, _P, _P, _P, _P, _P, _P, _P]),
+    "cs_policy_loss_workspace_elems": (_SZ, [_I64, _I64]),
+    "cs_token_logprobs_forward": (ctypes.c_int, [_P, _I64, _I64, _I64, _I64, _I64, _I32, _P, _P,
+                                                 _D, _P, _P, _P]),
+    "cs_token_logprobs_backward": (ctypes.c_int, [_P, _I64, _I64, _I64, _I64, _I64, _I32, _P, _P,
+                                                  _D, _P, _P, _P, _I32, _P, _P]),
+    "cs_policy_loss": (ctypes.c_int, [_P, _I64, _I64, _I64, _I64, _I64, _I32, _P, _P, _D, _P, _I64,
+                                      _I64, _P, _P, _D, _D, _D, _I32, _D, _P, _P, _P, _P, _P, _P,
+                                      _P]),
     "cs_gs_project_forward": (ctypes.c_int, [_P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P,
                                              _P, _P, _P]),
     "cs_gs_bin_prepare": (ctypes.c_int, [_P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P,

@@ -1,0 +1,104 @@
+"""What repo_amd.policy refuses, before anything reaches the device, and the C entries'
+own checks of sizes (host only)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from repo_amd.policy import policy_loss, token_logprobs
+
+
+def _args(shape=(2, 3), vocab=5, dtype=torch.float32):
+    return dict(logits=torch.zeros(*shape, vocab, dtype=dtype),
+                tokens=torch.zeros(shape, dtype=torch.int64), advantages=torch.zeros(shape),
+                old_logprobs=torch.zeros(shape))
+
+
+BAD = [
+    (dict(logits=torch.zeros(2, 3, 5, dtype=torch.float64)), "logits must be"),
+    (dict(logits=torch.zeros(())), "logits must be"),
+    (dict(logits=torch.zeros(2, 3, 0)), "empty vocabulary"),
+    (dict(tokens=torch.zeros(2, 3)), "tokens must be"),
+    (dict(tokens=torch.zeros(2, 4, dtype=torch.int64)), "tokens must have shape"),
+    (dict(mask=torch.ones(2, 3)), "mask must be bool"),
+    (dict(mask=torch.ones(2, 1, dtype=torch.bool)), "mask must have shape"),
+    (dict(temperature=0.0), "Invalid temperature"),
+    (dict(temperature=float("nan")), "Invalid temperature"),
+    (dict(temperature=float("inf")), "Invalid temperature"),
+    (dict(temperature=1e-40), "Invalid temperature"),
+]
+BAD_LOSS = [
+    (dict(reduction="mean"), "reduction must be"),
+    (dict(clip=(-0.1, 0.2)), "Invalid clip"),
+    (dict(clip=(0.1, float("nan"))), "Invalid clip"),
+    (dict(kl_weight=-1.0), "Invalid kl_weight"),
+    (dict(scale=float("inf")), "Invalid scale"),
+    (dict(kl_weight=0.1), "needs ref_logprobs"),
+    (dict(advantages=torch.zeros(2, 3, dtype=torch.float64)), "advantages must be"),
+    (dict(advantages=torch.zeros(3)), "advantages must have shape"),
+    (dict(advantages=torch.zeros(1, 3)), "advantages must have shape"),
+    (dict(old_logprobs=torch.zeros(2, 1)), "old_logprobs must have shape"),
+    (dict(ref_logprobs=torch.zeros(2)), "ref_logprobs must have shape"),
+    (dict(old_logprobs=torch.zeros(2, 3, requires_grad=True)), "no gradient for old_logprobs"),
+    (dict(advantages=torch.zeros(2, 3, requires_grad=True)), "no gradient for advantages"),
+]
+
+
+@pytest.mark.parametrize("change,message", BAD + BAD_LOSS)
+def test_policy_loss_refuses(change, message):
+    args = {**_args(), **change}
+    with pytest.raises(ValueError, match=message):
+        policy_loss(args.pop("logits"), args.pop("tokens"), args.pop("advantages"),
+                    args.pop("old_logprobs"), **args)
+
+
+@pytest.mark.parametrize("change,message", BAD)
+def test_token_logprobs_refuses(change, message):
+    args = {**_args(), **change}
+    args.pop("advantages"), args.pop("old_logprobs")
+    with pytest.raises(ValueError, match=message):
+        token_logprobs(args.pop("logits"), args.pop("tokens"), **args)
+
+
+def test_cpu_tensors_are_refused():
+    a = _args()
+    with pytest.raises(ValueError, match="logits must be a CUDA"):
+        token_logprobs(a["logits"], a["tokens"])
+    with pytest.raises(ValueError, match="logits must be a CUDA"):
+        policy_loss(a["logits"], a["tokens"], a["advantages"], a["old_logprobs"])
+
+
+def test_entries_check_their_sizes():
+    """None of these calls launches: the pointers are not looked at."""
+    from repo_amd import _native as N
+    big = 1 << 44
+
+    def rows(batch=1, length=1, vocab=8, bs=8, rs=8, dtype=0, tokens=256, t=1.0, logits=256):
+        return (logits, batch, length, vocab, bs, rs, dtype, tokens, None, t)
+
+    bad = [rows(batch=0), rows(length=0), rows(vocab=0), rows(vocab=big + 1),
+           rows(batch=1 << 30, length=1 << 30), rows(bs=-1), rows(rs=-1), rows(dtype=3),
+           rows(dtype=-1), rows(tokens=None), rows(logits=None), rows(t=0.0), rows(t=-1.0),
+           rows(t=float("nan")), rows(t=1e-31), rows(length=1 << 33)]
+    for head in bad:
+        for name, tail in (("cs_token_logprobs_forward", (256, 256)),
+                           ("cs_token_logprobs_backward", (256, 256, None, 0, 256)),
+                           ("cs_policy_loss", (256, 1, 1, 256, None, 0.2, 0.2, 0.0, 0, 1.0, 256, 256,
+                                               256, 256, 256, None))):
+            with pytest.raises(RuntimeError, match="invalid arguments"):
+                N.call(name, *head, *tail, None)
+    good = rows()
+    for tail in ((256, None), (None, 256)):
+        with pytest.raises(RuntimeError, match="invalid arguments"):
+            N.call("cs_token_logprobs_forward", *good, *tail, None)
+    for tail in ((256, 256, None, 1, 256), (None, 256, None, 0, 256), (256, 256, None, 0, None)):
+        with pytest.raises(RuntimeError, match="invalid arguments"):
+            N.call("cs_token_logprobs_backward", *good, *tail, None)
+    whole = [256, 1, 1, 256, None, 0.2, 0.2, 0.0, 0, 1.0, 256, 256, 256, 256, 256, None]
+    for at, value in ((0, None), (1, -1), (2, -1), (3, None), (5, -0.1), (6, float("nan")),
+                      (7, -1.0), (8, 3), (8, -1), (10, None), (10, 260), (11, None), (12, None),
+                      (13, None), (14, None)):
+        with pytest.raises(RuntimeError, match="invalid arguments"):
+            N.call("cs_policy_loss", *good, *whole[:at], value, *whole[at + 1:], None)
+    size = N.lib().cs_policy_loss_workspace_elems
+    assert size(0, 1) == 0 and size(1, 0) == 0 and size(1 << 30, 1 << 30) == 0 and size(3, 4) >= 72
