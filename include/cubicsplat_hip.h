@@ -762,6 +762,40 @@ int cs_group_norm_backward(const void* x, const void* dy, int64_t n, int64_t s, 
                            const float* rstd, float* workspace, void* dx, void* dweight,
                            void* dbias, hipStream_t stream);
 
+/* ---------------- orthogonalising matrices, Muon ---------------- */
+
+/* New (the reference has no such optimizer).  Newton-Schulz steps x <- a x + (b g + c g g) x,
+ * g = x x^T, on a matrix scaled to a Frobenius norm of one (the norm not below eps), with fp32's
+ * precision.  table is a host array of ntensors rows of eight int64:
+ *   [0] x, [1] y    of the type, contiguous; may be the same
+ *   [2] count       matrices of this shape behind each other
+ *   [4] rows  [5] columns  [6] type (0 fp32, 1 bf16, 2 fp16)
+ * steps 1 to 64; |a|, |b|, |c| at most 64, and such that no singular value in [0, 1] passes 64 on
+ * its way.  workspace: cs_orthogonalize_workspace_bytes bytes (-1: invalid arguments), 128-byte
+ * aligned, of which nothing is kept between calls.  count times the 64 x 64 patches of a matrix
+ * padded to whole tiles of 128 is at most CS_MUON_MAX_PATCHES. */
+#define CS_MUON_MAX_PATCHES 524288
+int64_t cs_orthogonalize_workspace_bytes(int32_t ntensors, const int64_t* table, int32_t steps,
+                                         double a, double b, double c);
+int cs_orthogonalize(int32_t ntensors, const int64_t* table, int32_t steps, double a, double b,
+                     double c, double eps, void* workspace, hipStream_t stream);
+
+/* The Muon step over any number of matrices.  Rows of the table as above but for
+ *   [0] parameter   updated in place
+ *   [1] gradient    of the parameter's type
+ *   [2] master      fp32 copy of a bf16 or fp16 parameter (0 for fp32); the update moves it and the
+ *                   parameter is it, rounded
+ *   [3] momentum    fp32, updated in place
+ * all of one element order; scalars: four floats a row, decay (1 - lr * weight_decay), lr (adjusted
+ * to the shape), mix (1 - momentum) and look:
+ *   momentum += mix (gradient - momentum),  u = momentum + look (gradient - momentum)
+ *   parameter = parameter * decay - lr * orthogonalized(u)
+ * look is 1 - momentum for Nesterov's form and 0 without. */
+int64_t cs_muon_workspace_bytes(int32_t ntensors, const int64_t* table, const float* scalars,
+                                int32_t steps, double a, double b, double c);
+int cs_muon_step(int32_t ntensors, const int64_t* table, const float* scalars, int32_t steps,
+                 double a, double b, double c, double eps, void* workspace, hipStream_t stream);
+
 /* ---------------- log-probabilities of tokens, policy loss ---------------- */
 
 /* New (the reference has no tokens).  Row t of sequence b holds vocab logits

@@ -27,6 +27,7 @@ RASTER_LOG_BLOCK_BYTES = 2048  # log pool reserved per wave at a time
 EDGE_AUX_INTS = 4        # 16-byte (segment, t0, t1) record of the adaptive flattening
 ADAMW_BLOCK = 128        # values that share an exponent in the 8-bit optimizer states
 GRAD_NORM_BLOCKS = 2048  # partial sums of the gradients' norm (and one a tensor)
+MUON_MAX_PATCHES = 524288  # 64 x 64 patches of one row of the Muon entry points' tables
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -142,6 +143,10 @@ _SIGNATURES = {
                                              _I32, _P, _P, _P, _P, _P]),
     "cs_group_norm_backward": (ctypes.c_int, [_P, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _I32,
                                               _I32, _P, _P, _P, _P, _P, _P, _P]),
+    "cs_orthogonalize_workspace_bytes": (_I64, [_I32, _P, _I32, _D, _D, _D]),
+    "cs_orthogonalize": (ctypes.c_int, [_I32, _P, _I32, _D, _D, _D, _D, _P, _P]),
+    "cs_muon_workspace_bytes": (_I64, [_I32, _P, _P, _I32, _D, _D, _D]),
+    "cs_muon_step": (ctypes.c_int, [_I32, _P, _P, _I32, _D, _D, _D, _D, _P, _P]),
     "cs_policy_loss_workspace_elems": (_SZ, [_I64, _I64]),
     "cs_token_logprobs_forward": (ctypes.c_int, [_P, _I64, _I64, _I64, _I64, _I64, _I32, _P, _P,
                                                  _D, _P, _P, _P]),

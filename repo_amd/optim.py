@@ -1,4 +1,4 @@
-"""Adam, Adan and AdamW with the step in one HIP launch for many parameters.
+"""Adam, Adan, AdamW and Muon over many parameters, in few HIP launches.
 
 The reference optimizes its primitives with ``torch.optim.Adam`` over
 per-group learning rates (gaussian_trace/model.py:172-189).  ``Adam`` here is
@@ -20,6 +20,10 @@ network) is for the weights of a network in front of the renderer: decoupled
 weight decay, fp32, bf16 and fp16 parameters of any dense layout, a global-norm
 clip without a host read, states in 32 or 8 bits, one launch for up to 56
 tensors.  ``global_grad_norm`` is the norm by itself.
+
+``Muon`` (new as well) is for those of the weights that are matrices: the momentum's
+direction, orthogonalised by Newton-Schulz steps, moves them.  ``orthogonalize`` is
+that by itself.
 """
 from __future__ import annotations
 
@@ -1161,3 +1165,310 @@ class AdamW(torch.optim.Optimizer):
         table = np.array([row], dtype=np.int64)
         with torch.cuda.device(p.device):
             N.call(name, 1, table.ctypes.data, *args, N.stream(p.device))
+
+
+# -------------------------------------------------------------------- Muon
+
+_NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _check_newton_schulz(steps, coefficients, eps):
+    """The steps' arguments, as the entry points take them."""
+    a, b, c = (float(v) for v in coefficients)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"Invalid epsilon value: {eps}")
+    if int(steps) != steps or not 1 <= steps <= 64:
+        raise ValueError(f"Newton-Schulz steps must be 1 to 64, got {steps}")
+    if N.lib().cs_orthogonalize_workspace_bytes(0, None, int(steps), a, b, c) < 0:
+        raise ValueError(f"Newton-Schulz coefficients {(a, b, c)} are no numbers up to 64, or let "
+                         "singular values in [0, 1] pass 64")
+    return int(steps), a, b, c
+
+
+def _padded(n):
+    """Patches along a dimension that is padded to whole tiles."""
+    return -(-n // 128) * 2
+
+
+def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=_NS_COEFFICIENTS,
+                  eps: float = 1e-7) -> torch.Tensor:
+    """The matrices x [..., m, n] with their singular values brought near one by Newton-Schulz
+    steps, as Muon does with its updates:
+
+        x <- x / max(|x|, eps) (Frobenius norm),  then ``steps`` times
+        x <- a x + (b g + c g g) x,  g = x x^T,  (a, b, c) = coefficients
+
+    x: fp32, bf16 or fp16 on the GPU; of a stack each matrix is scaled by its own norm.  The
+    result has x's type and shape.  Products are as exact as fp32's, whatever the type (of a norm far
+    below eps the result is exact to 1e-9, not to its own size), and sums are taken in a fixed
+    order.  Not differentiable: an x that requires a gradient is refused."""
+    steps, a, b, c = _check_newton_schulz(steps, coefficients, eps)
+    if x.dim() < 2:
+        raise ValueError(f"expected [..., m, n], got {tuple(x.shape)}")
+    if x.dtype not in _ADAMW_DTYPES:
+        raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("orthogonalize has no gradient: detach x")
+    m, n = x.shape[-2:]
+    patches = _padded(m) * _padded(n)
+    if patches > N.MUON_MAX_PATCHES:
+        raise ValueError(f"a matrix of {m} x {n} is too large for orthogonalize")
+    N.require_gpu(x, "x")
+    x = x.detach()
+    if x.device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(x.device):
+            return orthogonalize(x, steps, coefficients, eps)
+    if not x.is_contiguous() and x.mT.is_contiguous():
+        return orthogonalize(x.mT, steps, coefficients, eps).mT
+    x = x.contiguous()
+    y = torch.empty_like(x)
+    if x.numel() == 0:
+        return y
+    count, most = x.numel() // (m * n), N.MUON_MAX_PATCHES // patches
+    for k in range(0, count, most):
+        at = k * m * n * x.element_size()
+        table = np.array([[x.data_ptr() + at, y.data_ptr() + at, min(most, count - k), 0, m, n,
+                           _ADAMW_DTYPES[x.dtype], 0]], dtype=np.int64)
+        args = (1, table.ctypes.data, steps, a, b, c)
+        work = torch.empty(N.lib().cs_orthogonalize_workspace_bytes(*args), dtype=torch.uint8,
+                           device=x.device)
+        with N.prof("optim.orthogonalize"):
+            N.call("cs_orthogonalize", *args, float(eps), work.data_ptr(), N.stream(x.device))
+    return y
+
+
+def _as_matrix(p):
+    """(rows, columns) of a parameter [out, ...] as its values lie in memory: [out, the rest], or the
+    other way round (the order of the rest does not matter to its singular values).  None where
+    neither is so."""
+    rows, cols = p.shape[0], p.numel() // max(1, p.shape[0])
+    if not _is_dense(p):
+        return None
+    if p.numel() == 0 or rows == 1 or cols == 1 or p.stride(0) == cols:
+        return rows, cols
+    return (cols, rows) if p.stride(0) == 1 else None
+
+
+class Muon(torch.optim.Optimizer):
+    """Muon (torch.optim.Muon's arguments, groups and update) over the matrices of a network, for fp32,
+    bf16 and fp16 device parameters:
+
+        m <- m + (1 - momentum) (g - m),   u = g + momentum (m - g)  (nesterov; else m)
+        p <- p (1 - lr weight_decay) - lr' orthogonalize(u, ns_steps, ns_coefficients, eps)
+
+    lr' is lr sqrt(max(1, rows / columns)) (adjust_lr_fn None or "original") or
+    0.2 lr sqrt(max(rows, columns)) ("match_rms_adamw").  Parameters have two dimensions or more and
+    are taken as [shape[0], the rest] (a convolution's filters); those with one belong to AdamW.
+    Layouts: any dense one whose first dimension is the outermost in memory (contiguous,
+    ``channels_last``) or the innermost (a transposed matrix).
+
+    ``state`` holds ``momentum_buffer`` in fp32, and for a 16-bit parameter an fp32 copy ``master``,
+    which the update moves; the parameter is the copy rounded to nearest.  A parameter that is
+    written in place between steps is noticed by its version counter: where it is not the copy
+    rounded, the copy takes its values (writes through ``p.data`` are not noticed; whoever makes
+    such deletes ``state[p]["master"]``).
+
+    Up to 20 parameters share each launch.  A step can be captured in a graph, with the numbers of its
+    groups as they are then."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
+                 ns_coefficients=_NS_COEFFICIENTS, eps=1e-7, ns_steps=5, adjust_lr_fn=None):
+        self._written = {}
+        defaults = dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
+                        ns_coefficients=ns_coefficients, eps=eps, ns_steps=ns_steps,
+                        adjust_lr_fn=adjust_lr_fn)
+        self._check_group(defaults)
+        super().__init__(params, defaults)
+
+    @staticmethod
+    def _check_group(group):
+        if not 0.0 <= float(group["lr"]) < float("inf"):
+            raise ValueError(f"Invalid learning rate: {group['lr']}")
+        if not 0.0 <= group["weight_decay"] < float("inf"):
+            raise ValueError(f"Invalid weight_decay value: {group['weight_decay']}")
+        if not 0.0 <= group["momentum"] < 1.0:
+            raise ValueError(f"Invalid momentum value: {group['momentum']}")
+        if group["adjust_lr_fn"] not in (None, "original", "match_rms_adamw"):
+            raise ValueError("adjust_lr_fn must be None, 'original' or 'match_rms_adamw', got "
+                             f"{group['adjust_lr_fn']!r}")
+        return _check_newton_schulz(group["ns_steps"], group["ns_coefficients"], group["eps"])
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._written = {}
+
+    zero_grad = Adam.zero_grad
+
+    def add_param_group(self, param_group):
+        if isinstance(param_group, dict):
+            self._check_group({**self.defaults, **param_group})
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                shape = tuple(p.shape)
+                self.param_groups.pop()
+                raise ValueError(f"Muon is for matrices, got a parameter of shape {shape}")
+
+    def step(self, closure=None):
+        args, kwargs, closure = _run_pre_hooks(self, closure)
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        self._step()
+        self._optimizer_step_code()
+        _run_post_hooks(self, args, kwargs)
+        return loss
+
+    step.hooked = True   # as Adam's: the hooks are called above
+
+    @torch.no_grad()
+    def _step(self):
+        # Gathered first: nothing is launched if a tensor is refused.
+        work, stepped = {}, []
+        for group in self.param_groups:
+            key = (*self._check_group(group), float(group["eps"]))
+            lr, momentum = float(group["lr"]), float(group["momentum"])
+            decay, mix = 1.0 - lr * group["weight_decay"], 1.0 - momentum
+            look = mix if group["nesterov"] else 0.0
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                shape = self._check_param(p)
+                _check_grad(g, p)
+                if not (_is_dense(g) and _same_layout(g, p)):
+                    g = torch.empty_like(p).copy_(g.detach())
+                st = self._ready(p)
+                rows, cols = p.shape[0], p.numel() // max(1, p.shape[0])
+                if p.numel() == 0:
+                    continue
+                by = (0.2 * math.sqrt(max(rows, cols)) if group["adjust_lr_fn"] == "match_rms_adamw"
+                      else math.sqrt(max(1.0, rows / cols)))
+                tables, scalars, held = work.setdefault((p.device, key), ([], [], []))
+                master = st.get("master") if p.dtype is not torch.float32 else None
+                tables.append((p.data_ptr(), g.data_ptr(), 0 if master is None else
+                               master.data_ptr(), st["momentum_buffer"].data_ptr(), *shape,
+                               _ADAMW_DTYPES[p.dtype], 0))
+                scalars.append((decay, lr * by, mix, look))
+                held.append(g)
+                stepped.append(p)
+        for (device, key), (tables, scalars, _) in work.items():
+            if device.index == torch._C._cuda_getDevice():
+                self._launch(device, tables, scalars, *key)
+            else:
+                with torch.cuda.device(device):
+                    self._launch(device, tables, scalars, *key)
+        if stepped:
+            increment_version(stepped)
+            for p in stepped:
+                self._wrote(p)
+
+    @staticmethod
+    def _launch(device, rows, scalars, steps, a, b, c, eps):
+        table = np.array(rows, dtype=np.int64)
+        numbers = np.array(scalars, dtype=np.float32)
+        args = (len(rows), table.ctypes.data, numbers.ctypes.data, steps, a, b, c)
+        work = torch.empty(N.lib().cs_muon_workspace_bytes(*args), dtype=torch.uint8, device=device)
+        with N.prof("optim.muon"):
+            N.call("cs_muon_step", *args, eps, work.data_ptr(), N.stream(device))
+
+    # ---- state
+
+    @staticmethod
+    def _check_param(p):
+        if p.dtype not in _ADAMW_DTYPES or not p.is_cuda or p.layout is not torch.strided:
+            raise ValueError("repo_amd.optim.Muon needs float32, bfloat16 or float16 CUDA (ROCm) "
+                             f"parameters, got {p.dtype} on {p.device}")
+        shape = _as_matrix(p)
+        if shape is None:
+            raise ValueError("repo_amd.optim.Muon needs parameters that fill their memory, with the "
+                             "first dimension outermost or innermost, got shape "
+                             f"{tuple(p.shape)} with strides {p.stride()}")
+        if _padded(shape[0]) * _padded(shape[1]) > N.MUON_MAX_PATCHES:
+            raise ValueError(f"a matrix of {shape[0]} x {shape[1]} is too large for Muon")
+        return shape
+
+    def _wrote(self, p):
+        """The master agrees with p as it is now."""
+        master = self.state[p].get("master")
+        if master is not None:
+            self._written[p] = (_version_of(p), p.data_ptr(), master)
+
+    def _ready(self, p):
+        """p's state, made where there is none, and in step with p."""
+        st = self.state[p]
+        if "momentum_buffer" not in st:
+            st["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32,
+                                                     memory_format=torch.preserve_format)
+        names = ["momentum_buffer"]
+        if p.dtype is not torch.float32:
+            names.append("master")
+            if "master" not in st:
+                st["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
+                self._wrote(p)
+        for t in (st[name] for name in names):
+            if (t.dtype is not torch.float32 or t.device != p.device or t.shape != p.shape
+                    or not _is_dense(t) or not _same_layout(t, p)):
+                raise ValueError("a Muon state does not fit its parameter: "
+                                 f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device} "
+                                 f"beside {tuple(p.shape)} with strides {p.stride()} on {p.device}")
+        if len(names) > 1:
+            master, known = st["master"], self._written.get(p)
+            if (known is not None and known[2] is master
+                    and known[:2] != (_version_of(p), p.data_ptr())):
+                q = p.detach()
+                master.copy_(torch.where(master.to(q.dtype) == q, master, q.float()))
+            self._wrote(p)
+        return st
+
+    def load_state_dict(self, state_dict):
+        """Takes states in fp32, bf16 and fp16 (as torch's optimizers keep them beside 16-bit
+        parameters) and holds them in fp32.  torch's own loading would cast every state to its
+        parameter's type, so only the groups go through it."""
+        pre, post = (self._optimizer_load_state_dict_pre_hooks,
+                     self._optimizer_load_state_dict_post_hooks)
+        state_dict = state_dict.copy()
+        for hook in pre.values():
+            got = hook(self, state_dict)
+            if got is not None:
+                state_dict = got
+        ids = [k for group in state_dict["param_groups"] for k in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for group in state_dict["param_groups"]:
+            self._check_group({**self.defaults, **group})
+        taken = {}
+        for k, p in zip(ids, params):
+            if k in state_dict["state"]:
+                taken[p] = self._taken(p, state_dict["state"][k])
+        self._optimizer_load_state_dict_pre_hooks = type(pre)()
+        self._optimizer_load_state_dict_post_hooks = type(post)()
+        try:
+            super().load_state_dict({**state_dict, "state": {}})
+        finally:
+            self._optimizer_load_state_dict_pre_hooks = pre
+            self._optimizer_load_state_dict_post_hooks = post
+        self._written = {}
+        for p, st in taken.items():
+            self.state[p] = st
+            self._wrote(p)   # from here on writes to p are told from what its master was loaded for
+        for hook in post.values():
+            hook(self)
+
+    @staticmethod
+    @torch.no_grad()
+    def _taken(p, given):
+        st = {}
+        for name, value in given.items():
+            if name == "master" and p.dtype is torch.float32:
+                continue
+            if name in ("momentum_buffer", "master"):
+                if value.shape != p.shape:   # copy_ would broadcast it
+                    raise ValueError(f"a Muon state does not fit its parameter: {tuple(value.shape)} "
+                                     f"beside {tuple(p.shape)}")
+                value = torch.empty_like(p, dtype=torch.float32,
+                                         memory_format=torch.preserve_format).copy_(value)
+            else:
+                value = _copied(value)
+            st[name] = value
+        return st
