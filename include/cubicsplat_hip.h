@@ -773,7 +773,7 @@ int cs_group_norm_backward(const void* x, const void* dy, int64_t n, int64_t s, 
  * steps 1 to 64; |a|, |b|, |c| at most 64, and such that no singular value in [0, 1] passes 64 on
  * its way.  workspace: cs_orthogonalize_workspace_bytes bytes (-1: invalid arguments), 128-byte
  * aligned, of which nothing is kept between calls.  count times the 64 x 64 patches of a matrix
- * padded to whole tiles of 128 is at most CS_MUON_MAX_PATCHES. */
+ * padded to whole tiles of 256 is at most CS_MUON_MAX_PATCHES. */
 #define CS_MUON_MAX_PATCHES 524288
 int64_t cs_orthogonalize_workspace_bytes(int32_t ntensors, const int64_t* table, int32_t steps,
                                          double a, double b, double c);
@@ -790,9 +790,8 @@ int cs_orthogonalize(int32_t ntensors, const int64_t* table, int32_t steps, doub
  * to the shape), mix (1 - momentum) and look:
  *   momentum += mix (gradient - momentum),  u = momentum + look (gradient - momentum)
  *   parameter = parameter * decay - lr * orthogonalized(u)
- * look is 1 - momentum for Nesterov's form and 0 without. */
-int64_t cs_muon_workspace_bytes(int32_t ntensors, const int64_t* table, const float* scalars,
-                                int32_t steps, double a, double b, double c);
+ * look is 1 - momentum for Nesterov's form and 0 without.  workspace: as large as
+ * cs_orthogonalize_workspace_bytes says of matrices of these sizes, in this order. */
 int cs_muon_step(int32_t ntensors, const int64_t* table, const float* scalars, int32_t steps,
                  double a, double b, double c, double eps, void* workspace, hipStream_t stream);
 

@@ -145,7 +145,6 @@ _SIGNATURES = {
                                               _I32, _P, _P, _P, _P, _P, _P, _P]),
     "cs_orthogonalize_workspace_bytes": (_I64, [_I32, _P, _I32, _D, _D, _D]),
     "cs_orthogonalize": (ctypes.c_int, [_I32, _P, _I32, _D, _D, _D, _D, _P, _P]),
-    "cs_muon_workspace_bytes": (_I64, [_I32, _P, _P, _I32, _D, _D, _D]),
     "cs_muon_step": (ctypes.c_int, [_I32, _P, _P, _I32, _D, _D, _D, _D, _P, _P]),
     "cs_policy_loss_workspace_elems": (_SZ, [_I64, _I64]),
     "cs_token_logprobs_forward": (ctypes.c_int, [_P, _I64, _I64, _I64, _I64, _I64, _I32, _P, _P,

@@ -8,9 +8,10 @@
 // X <- Q X at the phase's end.  All of these are polynomials of one symmetric matrix, so
 // they commute and are symmetric: half of each product is computed and mirrored.  A step
 // then costs 4 m^3 instead of 3 m^2 n + m^3.  A's rounding grows by a^2 a step where
-// singular values are small (X's own by a), so a phase ends after three steps: relative
-// to float64, 1.0 to 1.4 times the error of the steps on X (fp32 products, spectra flat
-// to 1 / k^2), where one phase of five steps has 5 to 80 times.
+// singular values are small (X's own by a), so phases are of two steps and one in turn for a
+// = 3.4445: relative to float64 the result has 0.8 to 1.3 times the error of the steps on X in
+// fp32 (spectra flat to 1 / k^2), where phases of three steps have up to 4.7 times and one of
+// five up to 100 times.
 //
 // Products.  A value v is held as two halves of 16 bits, h = fp16(v 2^e) and l =
 // fp16(v 2^e - h), together 23 bits of v where h is normal: as much as fp32 has.  A
@@ -26,6 +27,7 @@
 #include <algorithm>
 #include <memory>
 #include <new>
+#include <vector>
 
 #include "../../include/cubicsplat_hip.h"
 
@@ -35,13 +37,14 @@ enum { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
 constexpr int kMuMaxEntries = 20;  // of one chunk: a launch has at most two jobs of each
 constexpr int kMuMaxJobs = 2 * kMuMaxEntries;
-constexpr int kMuTile = 128;
-constexpr int kMuThreads = 256;
+constexpr int kMuThreads = 256;   // of all launches but the products'
 constexpr int kMuPatch = 64;       // of the launch that makes pairs
 constexpr int kMuParts = 256;      // partial sums of a matrix's norm
 constexpr int kMuPass = 2048;
-constexpr int kMuPhase = 3;        // steps of a phase
+constexpr int kMuPhase = 3;        // most steps of a phase
+constexpr int kMuUnit = 4096;      // halves, or floats of partial sums, that offsets count
 constexpr int kMuMaxSteps = 64;
+constexpr int kMuMostTile = 256;
 constexpr int64_t kMuMaxPatches = CS_MUON_MAX_PATCHES;
 static_assert(kMuMaxPatches * kMuMaxEntries * kMuThreads < ((int64_t)1 << 32), "a launch's threads");
 
@@ -53,18 +56,20 @@ typedef float Float4 __attribute__((ext_vector_type(4)));
 
 enum { kGram = 0, kPoly = 1, kApply = 2 };
 
-// out[i][j] = scale * sum_k left[i][k] right[j][k] (+ poly_b A_ij + poly_a (i == j)).
-// Offsets are in halves from the workspace's beginning; matrix b of a stack lies
-// b * stride further.
+// out[i][j] = scale * sum_k left[i][k] right[j][k] (+ poly_b A_ij + poly_a (i == j)), A at
+// `other`.  Offsets are from the workspace's beginning, in units; matrix b of a stack lies
+// b * stride further.  A sum over a long k is cut into pieces, whose partial sums a launch
+// of its own joins.
 struct MuJob {
-    int64_t left, right, out, other, stride;
+    int32_t left, right, out, other, stride;
+    int32_t partial;      // pieces > 1: [matrix][tile][piece][T][T] floats
+    int32_t pieces, piece_stages;
     int32_t k;            // padded, in values
-    int32_t rows, cols;   // of tiles; cols 0: symmetric, the lower triangle's tiles
+    int32_t cols;         // of tiles; 0: symmetric, the lower triangle's tiles
     int32_t ld_out, ld_other;
     uint32_t first;       // workgroup
     int32_t tiles;        // of a matrix
-    int32_t mode;
-    int32_t m;
+    int32_t mode, m;
     float scale, poly_a, poly_b;
 };
 
@@ -78,10 +83,9 @@ static_assert(sizeof(MuJobs) <= 4096, "kernel arguments");
 // Where the last product goes: y of a type, or the Muon step on fp32 weights.
 struct MuLast {
     MuJob job;
+    int32_t rows, cols;   // of out, as it lies in memory
     void* out;            // y or the parameter
     float* master;        // Muon: fp32 weights of a 16-bit parameter
-    int64_t out_stride;   // of a stack, in elements
-    int32_t rows, cols;   // of out, as it lies in memory
     int32_t tall;         // out is n x m
     int32_t dtype, muon;
     float decay, lr;
@@ -126,127 +130,342 @@ __device__ inline void mu_to_lds(const _Float16* from, char* to) {
                                      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
-// One tile's sums.  A fragment (16 rows, 32 values, h or l) lies in LDS in its lanes'
-// order: lane r + 16 q holds row r's values 8 q to 8 q + 7.  acc[i][j] of wave (w >> 1, w & 1):
-// lane's left row 16 i + (lane & 15), right rows 16 j + 4 (lane >> 4) + 0..3.
-__device__ inline void mu_tile(const _Float16* left, const _Float16* right, int k, char* lds,
-                               Float4 (&acc)[4][4]) {
+// Tiles of T x T by WR x WC waves, each of I x J blocks of 16 x 16; a stage brings 32 KS
+// values of k of every row, and ST stages are there or on their way.
+template <int TILE> struct MuShape;
+template <> struct MuShape<256> { enum { T = 256, WR = 2, WC = 4, KS = 1, ST = 2 }; };
+template <> struct MuShape<128> { enum { T = 128, WR = 2, WC = 2, KS = 1, ST = 2 }; };
+template <> struct MuShape<64> { enum { T = 64, WR = 2, WC = 2, KS = 2, ST = 3 }; };
+
+template <typename S> struct MuSizes {
+    enum {
+        kWaves = S::WR * S::WC,
+        kThreads = kWaves * 64,
+        I = S::T / S::WR / 16,
+        J = S::T / S::WC / 16,
+        kSide = S::T / 16 * S::KS * 2048,   // bytes of a stage's left or right rows
+        kStage = 2 * kSide,
+        kLds = kStage * S::ST,
+        kBlocks = S::T / 16 / (kWaves / 2),   // of 16 rows, that a wave brings
+        kLoads = kBlocks * S::KS * 2
+    };
+};
+
+template <int N> __device__ inline void mu_wait_barrier() {
+    // What this wave has asked for up to its N newest loads is there, and what it reads is read.
+    __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+}
+
+__device__ inline Float4 mu_mfma(Half8 a, Half8 b, Float4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// One tile's sums over stages [from, to).  acc[i][j]: the lane's left row 16 i + (lane & 15) of
+// its wave's, right rows 16 j + 4 (lane >> 4) + 0..3.  16 rows' 32 values lie in LDS row by row, 128
+// bytes each, as in memory, so that eight lanes bring a whole line; a row's eight parts of 16
+// bytes change places by its number, so that lanes that read the same part of different rows
+// find it in different banks.  (Brought in the order in which lanes read it, 16 bytes here and there,
+// a 4096 x 4096 matrix took 6.45 ms for 4.12 with tiles of 128.)
+template <typename S>
+__device__ inline void mu_tile(const _Float16* left, const _Float16* right, int k, int from, int to,
+                               char* lds, Float4 (&acc)[MuSizes<S>::I][MuSizes<S>::J]) {
+    typedef MuSizes<S> Z;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t ld = 2 * (int64_t)k;
-    // Waves 0 and 1 bring the left rows, 2 and 3 the right: 4 blocks of 16 each.
-    const _Float16* from = (wave < 2 ? left : right) +
-                           ((wave & 1) * 64 + (lane & 15)) * ld + (lane >> 4) * 8;
-    char* to = lds + wave * 8192;
-    const int stages = k >> 5;
-    auto bring = [&](int s) {
-        char* at = to + (s & 1) * 32768;
+    // The first half of the waves brings the left rows, the other the right ones.
+    const int mine = (wave & (Z::kWaves / 2 - 1)) * Z::kBlocks;
+    const _Float16* src = (wave < Z::kWaves / 2 ? left : right) + (mine * 16 + (lane >> 3)) * ld +
+                          ((lane & 7) ^ (lane >> 3)) * 8;
+    char* dst = lds + (wave < Z::kWaves / 2 ? 0 : Z::kSide) + mine * (S::KS * 2048);
+    auto bring = [&](int s, int slot) {
+        char* at = dst + slot * Z::kStage;
+        const _Float16* p = src + (int64_t)s * (S::KS * 64);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < Z::kBlocks; ++i)
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
-                mu_to_lds(from + i * 16 * ld + (int64_t)s * 64 + p * 32, at + (i * 2 + p) * 1024);
+            for (int c = 0; c < S::KS * 2; ++c)
+                mu_to_lds(p + (i * 16 + (c & 1) * 8) * ld + (c >> 1) * 64,
+                          at + (i * S::KS * 2 + c) * 1024);
     };
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < Z::I; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = Float4{0.0f, 0.0f, 0.0f, 0.0f};
-    bring(0);
-    for (int s = 0; s < stages; ++s) {
-        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();   // this stage is there, and the last one read
-        if (s + 1 < stages) bring(s + 1);
-        const char* at = lds + (s & 1) * 32768;
-        const char* a = at + (wave >> 1) * 8192 + lane * 16;
-        const char* b = at + 16384 + (wave & 1) * 8192 + lane * 16;
-        Half8 ah[4], al[4], bh[4], bl[4];
+        for (int j = 0; j < Z::J; ++j) acc[i][j] = Float4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < S::ST - 1; ++s)
+        if (from + s < to) bring(from + s, s);
+    const int high = (lane & 15) * 128 + ((lane >> 4) ^ (lane & 7)) * 16, low = high ^ 64;
+    const char* a0 = lds + (wave / S::WC) * (Z::I * S::KS * 2048);
+    const char* b0 = lds + Z::kSide + (wave % S::WC) * (Z::J * S::KS * 2048);
+    int slot = 0;
+    if constexpr (S::KS == 1 && S::ST == 2) {
+        // The barrier comes before a step's last blocks, whose operands then are in registers:
+        // the next step's first reads go out between their products.
+        constexpr int kTail = 3, kMain = Z::I - kTail;
+        Half8 bh[Z::J], bl[Z::J], ah[2], al[2], th[kTail], tl[kTail];
+        mu_wait_barrier<0>();
+        if (from + 1 < to) bring(from + 1, 1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            ah[i] = *(const Half8*)(a + i * 2048);
-            al[i] = *(const Half8*)(a + i * 2048 + 1024);
-            bh[i] = *(const Half8*)(b + i * 2048);
-            bl[i] = *(const Half8*)(b + i * 2048 + 1024);
+        for (int j = 0; j < Z::J; ++j) {
+            bh[j] = *(const Half8*)(b0 + j * 2048 + high);
+            bl[j] = *(const Half8*)(b0 + j * 2048 + low);
         }
+        ah[0] = *(const Half8*)(a0 + high);
+        al[0] = *(const Half8*)(a0 + low);
+        for (int s = from; s < to; ++s) {
+            const char* a = a0 + slot * Z::kStage;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < kMain; ++i) {
+                if (i + 1 < kMain) {
+                    ah[(i + 1) & 1] = *(const Half8*)(a + (i + 1) * 2048 + high);
+                    al[(i + 1) & 1] = *(const Half8*)(a + (i + 1) * 2048 + low);
+                } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bl[j], ah[i], acc[i][j], 0, 0, 0);
+                    for (int t = 0; t < kTail; ++t) {
+                        th[t] = *(const Half8*)(a + (kMain + t) * 2048 + high);
+                        tl[t] = *(const Half8*)(a + (kMain + t) * 2048 + low);
+                    }
+                }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+                for (int j = 0; j < Z::J; ++j)
+                    acc[i][j] = mu_mfma(bl[j], ah[i & 1], acc[i][j]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh[j], al[i], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < Z::J; ++j)
+                    acc[i][j] = mu_mfma(bh[j], al[i & 1], acc[i][j]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+                for (int j = 0; j < Z::J; ++j)
+                    acc[i][j] = mu_mfma(bh[j], ah[i & 1], acc[i][j]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            mu_wait_barrier<0>();
+            __builtin_amdgcn_sched_barrier(0);
+            if (s + 2 < to) bring(s + 2, slot);
+            slot ^= 1;
+            // Behind the last stage this reads what was there before it, for nothing.
+            const char* an = a0 + slot * Z::kStage;
+            const char* bn = b0 + slot * Z::kStage;
+            ah[0] = *(const Half8*)(an + high);
+            al[0] = *(const Half8*)(an + low);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh[j], ah[i], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < Z::J; ++j) {
+#pragma unroll
+                for (int t = 0; t < kTail; ++t)
+                    acc[kMain + t][j] = mu_mfma(bl[j], th[t], acc[kMain + t][j]);
+#pragma unroll
+                for (int t = 0; t < kTail; ++t)
+                    acc[kMain + t][j] = mu_mfma(bh[j], tl[t], acc[kMain + t][j]);
+#pragma unroll
+                for (int t = 0; t < kTail; ++t)
+                    acc[kMain + t][j] = mu_mfma(bh[j], th[t], acc[kMain + t][j]);
+                bh[j] = *(const Half8*)(bn + j * 2048 + high);
+                bl[j] = *(const Half8*)(bn + j * 2048 + low);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        return;
     }
+    for (int s = from; s < to; ++s) {
+        // This stage is there; the one read last has been read, and is brought anew.
+        if (s + S::ST - 1 <= to)
+            mu_wait_barrier<(S::ST - 2) * Z::kLoads>();
+        else
+            mu_wait_barrier<0>();
+        if (s + S::ST - 1 < to) bring(s + S::ST - 1, slot == 0 ? S::ST - 1 : slot - 1);
+        const char* a = a0 + slot * Z::kStage;
+        const char* b = b0 + slot * Z::kStage;
+#pragma unroll
+        for (int c = 0; c < S::KS; ++c) {
+            Half8 bh[Z::J], bl[Z::J];
+#pragma unroll
+            for (int j = 0; j < Z::J; ++j) {
+                bh[j] = *(const Half8*)(b + (j * S::KS + c) * 2048 + high);
+                bl[j] = *(const Half8*)(b + (j * S::KS + c) * 2048 + low);
+            }
+#pragma unroll
+            for (int i = 0; i < Z::I; ++i) {
+                const Half8 ah = *(const Half8*)(a + (i * S::KS + c) * 2048 + high);
+                const Half8 al = *(const Half8*)(a + (i * S::KS + c) * 2048 + low);
+#pragma unroll
+                for (int j = 0; j < Z::J; ++j) acc[i][j] = mu_mfma(bl[j], ah, acc[i][j]);
+#pragma unroll
+                for (int j = 0; j < Z::J; ++j) acc[i][j] = mu_mfma(bh[j], al, acc[i][j]);
+#pragma unroll
+                for (int j = 0; j < Z::J; ++j) acc[i][j] = mu_mfma(bh[j], ah, acc[i][j]);
+            }
+        }
+        slot = slot == S::ST - 1 ? 0 : slot + 1;
+    }
+}
+
+// A workgroup's place: matrix b of the stack, tile (ti, tj), its number, its piece.
+struct MuPlace { int b, t, ti, tj, piece; };
+
+__device__ inline MuPlace mu_place(const MuJob& job, uint32_t at) {
+    MuPlace p;
+    p.piece = at % job.pieces;
+    at /= job.pieces;
+    p.b = at / job.tiles;
+    p.t = at - p.b * job.tiles;
+    if (job.cols == 0) {
+        mu_triangle(p.t, &p.ti, &p.tj);
+    } else {
+        p.ti = p.t / job.cols;
+        p.tj = p.t - p.ti * job.cols;
+    }
+    return p;
+}
+
+// N times four neighbours of a row, 16 columns apart, into `out`, and mirrored: the other tile of
+// a symmetric product, or X beside its transpose.
+template <int N>
+__device__ inline void mu_store(const MuJob& job, _Float16* ws, int row, int col, Float4 (&v)[N],
+                                bool mirror) {
+    Half4 h[N], l[N];
+    if (job.mode == kPoly) {
+        const _Float16* a = ws + (int64_t)job.other * kMuUnit;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int64_t o = mu_at(row, job.ld_out, col + 16 * j);
+            h[j] = *(const Half4*)(a + o);
+            l[j] = *(const Half4*)(a + o + 32);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float x = v[j][e] * job.scale;
+            if (job.mode == kPoly) {
+                x += job.poly_b * ((float)h[j][e] + (float)l[j][e]);
+                if (row == col + 16 * j + e && row < job.m) x += job.poly_a;
+            }
+            _Float16 y, z;
+            mu_split(x, &y, &z);
+            h[j][e] = y;
+            l[j][e] = z;
+        }
+    }
+    _Float16* out = ws + (int64_t)job.out * kMuUnit;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int64_t o = mu_at(row, job.ld_out, col + 16 * j);
+        *(Half4*)(out + o) = h[j];
+        *(Half4*)(out + o + 32) = l[j];
+    }
+    if (!mirror) return;
+    const bool sym = job.cols == 0;
+    const int ld = sym ? job.ld_out : job.ld_other;
+    if (!sym) out = ws + (int64_t)job.other * kMuUnit;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t q = mu_at(col + 16 * j + e, ld, row);
+            out[q] = h[j][e];
+            out[q + 32] = l[j][e];
+        }
 }
 
 __device__ inline uint32_t mu_first_job(const MuJobs& a, int k) { return a.j[k].first; }
 __device__ inline uint32_t mu_first_last(const MuLasts& a, int k) { return a.j[k].job.first; }
 
-__global__ __launch_bounds__(kMuThreads, 2) void k_mu_product(MuJobs a) {
-    __shared__ __attribute__((aligned(16))) char lds[65536];
+template <int TILE>
+__global__ __launch_bounds__(MuSizes<MuShape<TILE>>::kThreads, 2) void k_mu_product(MuJobs a) {
+    typedef MuShape<TILE> S;
+    typedef MuSizes<S> Z;
+    __shared__ __attribute__((aligned(16))) char lds[Z::kLds];
+    const MuJob& job = a.j[mu_find(a, a.n, mu_first_job)];
+    const MuPlace p = mu_place(job, blockIdx.x - job.first);
+    _Float16* ws = a.ws + (int64_t)p.b * job.stride * kMuUnit;
+    const int64_t ld = 2 * (int64_t)job.k;
+    const int stages = job.k / (32 * S::KS), from = p.piece * job.piece_stages;
+    const int to = from + job.piece_stages < stages ? from + job.piece_stages : stages;
+    Float4 acc[Z::I][Z::J];
+    mu_tile<S>(ws + (int64_t)job.left * kMuUnit + p.ti * S::T * ld,
+               ws + (int64_t)job.right * kMuUnit + p.tj * S::T * ld, job.k, from, to, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row0 = (wave / S::WC) * (Z::I * 16) + (lane & 15);
+    const int col0 = (wave % S::WC) * (Z::J * 16) + (lane >> 4) * 4;
+    if (job.pieces > 1) {
+        float* part = (float*)a.ws + (int64_t)job.partial * kMuUnit +
+                      (((int64_t)p.b * job.tiles + p.t) * job.pieces + p.piece) * (S::T * S::T);
+#pragma unroll
+        for (int i = 0; i < Z::I; ++i)
+#pragma unroll
+            for (int j = 0; j < Z::J; ++j)
+                *(Float4*)(part + (row0 + 16 * i) * S::T + col0 + 16 * j) = acc[i][j];
+        return;
+    }
+    const bool mirror = job.cols == 0 ? p.ti != p.tj : job.other >= 0;
+#pragma unroll
+    for (int i = 0; i < Z::I; ++i)
+        mu_store(job, ws, p.ti * S::T + row0 + 16 * i, p.tj * S::T + col0, acc[i], mirror);
+}
+
+// The pieces' sums, in their order: a workgroup takes 64 x 64 values of a tile, a thread eight
+// neighbours of a row, and for the mirrored tile of a column.
+template <int TILE>
+__global__ __launch_bounds__(kMuThreads) void k_mu_join(MuJobs a) {
+    constexpr int kSide = TILE / kMuPatch;
+    __shared__ float patch[kMuPatch][kMuPatch + 1];
     const MuJob& job = a.j[mu_find(a, a.n, mu_first_job)];
     const uint32_t at = blockIdx.x - job.first;
-    const int b = at / job.tiles, t = at - b * job.tiles;
-    int ti, tj;
-    if (job.cols == 0) {
-        mu_triangle(t, &ti, &tj);
-    } else {
-        ti = t / job.cols;
-        tj = t - ti * job.cols;
-    }
-    _Float16* ws = a.ws + b * job.stride;
-    const int64_t ld = 2 * (int64_t)job.k;
-    Float4 acc[4][4];
-    mu_tile(ws + job.left + ti * kMuTile * ld, ws + job.right + tj * kMuTile * ld, job.k, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row0 = ti * kMuTile + (wave >> 1) * 64 + (lane & 15);
-    const int col0 = tj * kMuTile + (wave & 1) * 64 + (lane >> 4) * 4;
-    // The mirrored tile of a symmetric product; X beside its transpose.
-    const bool mirror = job.cols == 0 ? ti != tj : job.other >= 0;
-    const int64_t mirrored = job.cols == 0 ? job.out : job.other;
-    const int ld_mirrored = job.cols == 0 ? job.ld_out : job.ld_other;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = row0 + 16 * i;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int col = col0 + 16 * j;
-            const int64_t o = mu_at(row, job.ld_out, col);
-            Float4 v = acc[i][j] * job.scale;
-            if (job.mode == kPoly) {
-                const Half4 h = *(const Half4*)(ws + job.other + o);
-                const Half4 l = *(const Half4*)(ws + job.other + o + 32);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[e] += job.poly_b * ((float)h[e] + (float)l[e]);
-                    if (row == col + e && row < job.m) v[e] += job.poly_a;
-                }
-            }
-            Half4 h, l;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                _Float16 x, y;
-                mu_split(v[e], &x, &y);
-                h[e] = x;
-                l[e] = y;
-            }
-            *(Half4*)(ws + job.out + o) = h;
-            *(Half4*)(ws + job.out + o + 32) = l;
-            if (mirror) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int64_t q = mirrored + mu_at(col + e, ld_mirrored, row);
-                    ws[q] = h[e];
-                    ws[q + 32] = l[e];
-                }
-            }
+    MuJob whole = job;
+    whole.pieces = 1;
+    const MuPlace p = mu_place(whole, at / (kSide * kSide));
+    const int r0 = at % (kSide * kSide) / kSide * kMuPatch, c0 = at % kSide * kMuPatch;
+    _Float16* ws = a.ws + (int64_t)p.b * job.stride * kMuUnit;
+    _Float16* out = ws + (int64_t)job.out * kMuUnit;
+    const float* part = (const float*)a.ws + (int64_t)job.partial * kMuUnit +
+                        ((int64_t)p.b * job.tiles + p.t) * job.pieces * (TILE * TILE);
+    const int c8 = (threadIdx.x & 7) * 8;
+    for (int r = threadIdx.x >> 3; r < kMuPatch; r += kMuThreads / 8) {
+        const float* from = part + (r0 + r) * TILE + c0 + c8;
+        Float4 x = *(const Float4*)from, y = *(const Float4*)(from + 4);
+#pragma unroll 4
+        for (int q = 1; q < job.pieces; ++q) {
+            x += *(const Float4*)(from + (int64_t)q * (TILE * TILE));
+            y += *(const Float4*)(from + (int64_t)q * (TILE * TILE) + 4);
         }
+        const int row = p.ti * TILE + r0 + r, col = p.tj * TILE + c0 + c8;
+        const int64_t o = mu_at(row, job.ld_out, col);
+        Half8 h, l;
+        if (job.mode == kPoly) {
+            h = *(const Half8*)(ws + (int64_t)job.other * kMuUnit + o);
+            l = *(const Half8*)(ws + (int64_t)job.other * kMuUnit + o + 32);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float v = (e < 4 ? x[e & 3] : y[e & 3]) * job.scale;
+            if (job.mode == kPoly) {
+                v += job.poly_b * ((float)h[e] + (float)l[e]);
+                if (row == col + e && row < job.m) v += job.poly_a;
+            }
+            patch[r][c8 + e] = v;
+            _Float16 f, g;
+            mu_split(v, &f, &g);
+            h[e] = f;
+            l[e] = g;
+        }
+        *(Half8*)(out + o) = h;
+        *(Half8*)(out + o + 32) = l;
+    }
+    if (p.ti == p.tj) return;
+    __syncthreads();
+    for (int c = threadIdx.x >> 3; c < kMuPatch; c += kMuThreads / 8) {
+        Half8 h, l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            _Float16 f, g;
+            mu_split(patch[c8 + e][c], &f, &g);
+            h[e] = f;
+            l[e] = g;
+        }
+        const int64_t o = mu_at(p.tj * TILE + c0 + c, job.ld_out, p.ti * TILE + r0 + c8);
+        *(Half8*)(out + o) = h;
+        *(Half8*)(out + o + 32) = l;
     }
 }
 
@@ -263,41 +482,54 @@ __device__ inline float mu_get(const void* p, int dtype, int64_t at) {
 }
 
 // The last X, into y or the weights.
-__global__ __launch_bounds__(kMuThreads, 2) void k_mu_last(MuLasts a) {
-    __shared__ __attribute__((aligned(16))) char lds[65536];
+template <int TILE>
+__global__ __launch_bounds__(MuSizes<MuShape<TILE>>::kThreads, 2) void k_mu_last(MuLasts a) {
+    typedef MuShape<TILE> S;
+    typedef MuSizes<S> Z;
+    __shared__ __attribute__((aligned(16))) char lds[Z::kLds];
     const MuLast& l = a.j[mu_find(a, a.n, mu_first_last)];
     const MuJob& job = l.job;
-    const uint32_t at = blockIdx.x - job.first;
-    const int b = at / job.tiles, t = at - b * job.tiles;
-    const int ti = t / job.cols, tj = t - ti * job.cols;
-    const _Float16* ws = a.ws + b * job.stride;
+    const MuPlace p = mu_place(job, blockIdx.x - job.first);
+    const _Float16* ws = a.ws + (int64_t)p.b * job.stride * kMuUnit;
     const int64_t ld = 2 * (int64_t)job.k;
-    Float4 acc[4][4];
-    mu_tile(ws + job.left + ti * kMuTile * ld, ws + job.right + tj * kMuTile * ld, job.k, lds, acc);
+    Float4 acc[Z::I][Z::J];
+    mu_tile<S>(ws + (int64_t)job.left * kMuUnit + p.ti * S::T * ld,
+               ws + (int64_t)job.right * kMuUnit + p.tj * S::T * ld, job.k, 0,
+               job.k / (32 * S::KS), lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row0 = ti * kMuTile + (wave >> 1) * 64 + (lane & 15);
-    const int col0 = tj * kMuTile + (wave & 1) * 64 + (lane >> 4) * 4;
+    const int row0 = p.ti * S::T + (wave / S::WC) * (Z::I * 16) + (lane & 15);
+    const int col0 = p.tj * S::T + (wave % S::WC) * (Z::J * 16) + (lane >> 4) * 4;
+    const int64_t first = (int64_t)p.b * l.rows * l.cols;
+    float* weights = l.dtype == kF32 ? (float*)l.out : l.master;
+    // Row `row0 + 16 i` of X's transpose; its weights are asked for together.
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < Z::I; ++i) {
+        int64_t at[Z::J][4];
+        float w[Z::J][4] = {};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < Z::J; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                // Row `row0 + 16 i` of X's transpose.
                 const int r = l.tall ? row0 + 16 * i : col0 + 16 * j + e;
                 const int c = l.tall ? col0 + 16 * j + e : row0 + 16 * i;
-                if (r >= l.rows || c >= l.cols) continue;
-                const int64_t o = b * l.out_stride + (int64_t)r * l.cols + c;
-                const float v = acc[i][j][e] * job.scale;
-                if (!l.muon) {
-                    mu_put(l.out, l.dtype, o, v);
-                    continue;
-                }
-                float* w = l.dtype == kF32 ? (float*)l.out : l.master;
-                const float moved = __builtin_fmaf(-l.lr, v, w[o] * l.decay);
-                w[o] = moved;
-                if (l.dtype != kF32) mu_put(l.out, l.dtype, o, moved);
+                const bool in = r < l.rows && c < l.cols;
+                at[j][e] = in ? first + (int64_t)r * l.cols + c : -1;
+                if (l.muon && in) w[j][e] = weights[at[j][e]];
             }
+#pragma unroll
+        for (int j = 0; j < Z::J; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (at[j][e] < 0) continue;
+                float v = acc[i][j][e] * job.scale;
+                if (l.muon) {
+                    v = __builtin_fmaf(-l.lr, v, w[j][e] * l.decay);
+                    weights[at[j][e]] = v;
+                    if (l.dtype == kF32) continue;
+                }
+                mu_put(l.out, l.dtype, at[j][e], v);
+            }
+    }
 }
 
 // ------------------------------------------------------- what goes into them
@@ -308,11 +540,10 @@ struct MuSource {
     const void* x;
     float* momentum;
     double* parts;         // [count][kMuParts]
-    int64_t x_stride;      // of a stack, in elements
-    int64_t pairs, flipped; // offsets of X and its transpose, or the other way round: pairs in
-                           // the source's orientation
-    int64_t stride;        // of a stack, in halves
     int64_t chunk;         // elements of a partial sum
+    int32_t pairs, flipped; // X and its transpose, or the other way round: `pairs` has the source's
+                           // orientation
+    int32_t stride;        // of a stack, in units
     int32_t rows, cols;
     int32_t padded_rows, padded_cols;
     uint32_t first_sum, first_patch;
@@ -338,24 +569,66 @@ __device__ inline float mu_update(float g, float m, float look) {
     return __builtin_fmaf(look, g - m, m);
 }
 
+typedef Float4 MuAny4 __attribute__((aligned(4)));    // at any element
+typedef Float4 MuAny2 __attribute__((aligned(2)));
+
+// Eight neighbours, at any element's address.
+__device__ inline void mu_get8(const void* p, int dtype, int64_t at, float (&v)[8]) {
+    if (dtype == kF32) {
+        const Float4 x = *(const MuAny4*)((const float*)p + at);
+        const Float4 y = *(const MuAny4*)((const float*)p + at + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[i] = x[i]; v[4 + i] = y[i]; }
+    } else if (dtype == kBF16) {
+        typedef __bf16 B8 __attribute__((ext_vector_type(8)));
+        const B8 x = __builtin_bit_cast(B8, (Float4) * (const MuAny2*)((const __bf16*)p + at));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+    } else {
+        const Half8 x = __builtin_bit_cast(Half8, (Float4) * (const MuAny2*)((const _Float16*)p + at));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+    }
+}
+
 // The momentum's move, and partial sums of the squares of each matrix, in fp64.
 __global__ __launch_bounds__(kMuThreads) void k_mu_sums(MuSources a) {
     __shared__ double lds[kMuThreads / 64];
     const MuSource& s = a.s[mu_find(a, a.n, mu_first_sum)];
     const uint32_t at = blockIdx.x - s.first_sum;
     const int b = at / s.nparts, part = at - b * s.nparts;
-    const int64_t size = (int64_t)s.rows * s.cols, from = part * s.chunk;
+    const int64_t size = (int64_t)s.rows * s.cols, from = part * s.chunk, base = b * size;
     const int64_t to = from + s.chunk < size ? from + s.chunk : size;
     double sum = 0.0;
-    for (int64_t i = from + threadIdx.x; i < to; i += kMuThreads) {
-        float u = mu_get(s.x, s.dtype, b * s.x_stride + i);
-        if (s.momentum) {
-            float m = s.momentum[i];
-            m = __builtin_fmaf(s.mix, u - m, m);
-            s.momentum[i] = m;
-            u = mu_update(u, m, s.look);
+    for (int64_t i = from + threadIdx.x * 8; i < to; i += kMuThreads * 8) {
+        if (i + 8 <= to) {
+            float u[8];
+            mu_get8(s.x, s.dtype, base + i, u);
+            if (s.momentum) {
+                float m[8];
+                mu_get8(s.momentum, kF32, i, m);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    m[e] = __builtin_fmaf(s.mix, u[e] - m[e], m[e]);
+                    u[e] = mu_update(u[e], m[e], s.look);
+                }
+                *(MuAny4*)(s.momentum + i) = Float4{m[0], m[1], m[2], m[3]};
+                *(MuAny4*)(s.momentum + i + 4) = Float4{m[4], m[5], m[6], m[7]};
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = __builtin_fma((double)u[e], (double)u[e], sum);
+        } else {
+            for (int64_t e = i; e < to; ++e) {
+                float u = mu_get(s.x, s.dtype, base + e);
+                if (s.momentum) {
+                    float m = s.momentum[e];
+                    m = __builtin_fmaf(s.mix, u - m, m);
+                    s.momentum[e] = m;
+                    u = mu_update(u, m, s.look);
+                }
+                sum = __builtin_fma((double)u, (double)u, sum);
+            }
         }
-        sum = __builtin_fma((double)u, (double)u, sum);
     }
     for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = sum;
@@ -366,7 +639,8 @@ __global__ __launch_bounds__(kMuThreads) void k_mu_sums(MuSources a) {
     }
 }
 
-// X and its transpose as pairs, scaled to a norm of one (times 2^e), patch by patch.
+// X and its transpose as pairs, scaled to a norm of one (times 2^e), patch by patch: a
+// thread takes eight neighbours of a row, and then of a column.
 __global__ __launch_bounds__(kMuThreads) void k_mu_pairs(MuSources a) {
     __shared__ float tile[kMuPatch][kMuPatch + 1];
     __shared__ double lds[kMuThreads / 64];
@@ -374,43 +648,67 @@ __global__ __launch_bounds__(kMuThreads) void k_mu_pairs(MuSources a) {
     const uint32_t at = blockIdx.x - s.first_patch;
     const int b = at / s.patches, t = at - b * s.patches;
     const int r0 = t / s.patch_cols * kMuPatch, c0 = t % s.patch_cols * kMuPatch;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     static_assert(kMuParts == kMuThreads, "one partial sum a thread");
     double sum = (int)threadIdx.x < s.nparts ? s.parts[(int64_t)b * kMuParts + threadIdx.x] : 0.0;
     for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
-    if (lane == 0) lds[wave] = sum;
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = sum;
     __syncthreads();
     sum = 0.0;
     for (int w = 0; w < kMuThreads / 64; ++w) sum += lds[w];
     const double norm = sqrt(sum);
     const double by = (double)a.scale / (norm < a.eps ? a.eps : norm);   // NaN stays
-    const int c = c0 + lane;
-    for (int r = wave; r < kMuPatch; r += kMuThreads / 64) {
-        float u = 0.0f;
-        if (r0 + r < s.rows && c < s.cols) {
-            const int64_t i = (int64_t)(r0 + r) * s.cols + c;
-            u = mu_get(s.x, s.dtype, b * s.x_stride + i);
-            if (s.momentum) u = mu_update(u, s.momentum[i], s.look);
-            u = (float)((double)u * by);
+    const int64_t base = (int64_t)b * s.rows * s.cols;
+    _Float16* ws = a.ws + (int64_t)b * s.stride * kMuUnit;
+    const int c8 = (threadIdx.x & 7) * 8;
+    for (int r = threadIdx.x >> 3; r < kMuPatch; r += kMuThreads / 8) {
+        float u[8] = {};
+        const int row = r0 + r, col = c0 + c8;
+        if (row < s.rows && col < s.cols) {
+            const int64_t i = (int64_t)row * s.cols + col;
+            if (col + 8 <= s.cols) {
+                mu_get8(s.x, s.dtype, base + i, u);
+                if (s.momentum) {
+                    float m[8];
+                    mu_get8(s.momentum, kF32, i, m);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) u[e] = mu_update(u[e], m[e], s.look);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (col + e < s.cols) {
+                        u[e] = mu_get(s.x, s.dtype, base + i + e);
+                        if (s.momentum) u[e] = mu_update(u[e], s.momentum[i + e], s.look);
+                    }
+            }
         }
-        tile[r][lane] = u;
+        Half8 h, l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = (float)((double)u[e] * by);
+            tile[r][c8 + e] = v;
+            _Float16 x, y;
+            mu_split(v, &x, &y);
+            h[e] = x;
+            l[e] = y;
+        }
+        _Float16* o = ws + (int64_t)s.pairs * kMuUnit + mu_at(row, s.padded_cols, col);
+        *(Half8*)o = h;
+        *(Half8*)(o + 32) = l;
     }
     __syncthreads();
-    _Float16* ws = a.ws + b * s.stride;
-    for (int r = wave; r < kMuPatch; r += kMuThreads / 64) {
-        _Float16 h, l;
-        if (r0 + r < s.padded_rows) {
-            mu_split(tile[r][lane], &h, &l);
-            const int64_t o = s.pairs + mu_at(r0 + r, s.padded_cols, c);
-            ws[o] = h;
-            ws[o + 32] = l;
+    for (int c = threadIdx.x >> 3; c < kMuPatch; c += kMuThreads / 8) {
+        Half8 h, l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            _Float16 x, y;
+            mu_split(tile[c8 + e][c], &x, &y);
+            h[e] = x;
+            l[e] = y;
         }
-        if (c0 + r < s.padded_cols) {
-            mu_split(tile[lane][r], &h, &l);
-            const int64_t o = s.flipped + mu_at(c0 + r, s.padded_rows, r0 + lane);
-            ws[o] = h;
-            ws[o + 32] = l;
-        }
+        _Float16* o = ws + (int64_t)s.flipped * kMuUnit + mu_at(c0 + c, s.padded_rows, r0 + c8);
+        *(Half8*)o = h;
+        *(Half8*)(o + 32) = l;
     }
 }
 
@@ -459,7 +757,7 @@ bool mu_plan(MuPlan* p, int steps, double a, double b, double c) {
         if (!(p->x[k + 1] <= 64.0)) return false;   // values that grow without end
     }
     // The rounding of A grows by a^2 a step of a phase.
-    while (p->phase < kMuPhase && pow(fabs(a), 2.0 * p->phase) <= 200.0) ++p->phase;
+    while (p->phase < kMuPhase && pow(fabs(a), 2.0 * p->phase) <= 14.0) ++p->phase;
     return true;
 }
 
@@ -473,34 +771,42 @@ struct MuEntry {
 
     bool tall;
     int64_t m, n, mp, np;        // m <= n, and padded
-    int phase;
-    int64_t base, stride;        // halves
+    int phase;                   // most steps of a phase
+    int64_t stride;              // in units, as the offsets
     int64_t X, XT[2], A, T, P, Q[2];
 };
 
 int64_t mu_round(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// The products of one matrix by steps on X, or by phases, in m^3.
+// Phases: the longest, one shorter, the longest, ...
+int mu_len(int phase, int number, int left) {
+    const int len = number & 1 ? std::max(1, phase - 1) : phase;
+    return std::min(len, left);
+}
+
+// The products of one matrix, in m^3.
 double mu_cost(int steps, int phase, double ratio) {
     double cost = 0.0;
-    for (int k = 0; k < steps; k += phase) {
-        const int len = std::min(phase, steps - k);
+    for (int k = 0, number = 0; k < steps; ++number) {
+        const int len = mu_len(phase, number, steps - k);
         cost += 3.0 * ratio + 4.0 * len - 3.0;
+        k += len;
     }
     return cost;
 }
 
-// Where an entry's matrices lie; their size in halves.
-int64_t mu_layout(MuEntry* e, const MuPlan& p, int64_t base) {
+// Where an entry's matrices lie for a tile, from `base` on; the units that it takes.
+int64_t mu_layout(MuEntry* e, const MuPlan& p, int tile, int64_t base) {
     e->tall = e->rows > e->cols;
     e->m = e->tall ? e->cols : e->rows;
     e->n = e->tall ? e->rows : e->cols;
-    e->mp = mu_round(e->m, kMuTile);
-    e->np = mu_round(e->n, kMuTile);
+    e->mp = mu_round(e->m, tile);
+    e->np = mu_round(e->n, tile);
     const double ratio = (double)e->np / (double)e->mp;
     e->phase = mu_cost(p.steps, p.phase, ratio) < mu_cost(p.steps, 1, ratio) ? p.phase : 1;
-    const int64_t wide = 2 * e->mp * e->np, square = 2 * e->mp * e->mp;
+    const int64_t wide = 2 * e->mp * e->np / kMuUnit, square = 2 * e->mp * e->mp / kMuUnit;
     int64_t at = 0;
+    // Each an even number of units, as partial sums behind them need it.
     auto take = [&](int64_t size) { const int64_t o = base + at; at += size; return o; };
     e->X = take(wide);
     e->XT[0] = take(wide);
@@ -512,35 +818,25 @@ int64_t mu_layout(MuEntry* e, const MuPlan& p, int64_t base) {
         e->P = take(square);
         e->Q[1] = take(square);
     }
-    e->base = base;
     e->stride = at;
     return at * e->count;
 }
 
-int64_t mu_chunk_bytes(MuEntry* e, int n, const MuPlan& p) {
-    int64_t halves = 0, parts = 0;
-    for (int k = 0; k < n; ++k) {
-        halves += mu_layout(e + k, p, halves);
-        parts += e[k].count * kMuParts;
-    }
-    return halves * 2 + parts * 8;
-}
+// A product: rows x cols values, or the lower triangle of a square (cols 0).
+struct MuOp { MuJob job; int64_t rows, cols; int slot; };
 
-struct MuOp { MuJob job; int slot; };
-
-// The products of an entry, each with the launch that it goes into (up to two of them a launch),
-// without the last.
+// The products of an entry, each with the launch that it goes into (up to two of them a
+// launch), without the last.
 struct MuSchedule {
     MuOp ops[8 * kMuMaxSteps];
-    int n = 0, slots = 0;
-    MuJob last;
+    int n, slots;
+    MuOp last;
 
     void make(const MuEntry& e, const MuPlan& p) {
         n = slots = 0;
-        const double xs = p.x[0];
-        int ex = mu_exponent(xs), xt = 0;
-        for (int k = 0; k < p.steps; k += e.phase) {
-            const int len = std::min(e.phase, p.steps - k);
+        int ex = mu_exponent(p.x[0]), xt = 0;
+        for (int k = 0, number = 0;; ++number) {
+            const int len = mu_len(e.phase, number, p.steps - k);
             int ea = mu_exponent(p.x[k] * p.x[k]), eq = 0, q = 0;
             double pq = 1.0;
             sym(e, e.X, e.X, e.A, e.np, ea - 2 * ex);
@@ -551,17 +847,17 @@ struct MuSchedule {
                 const int64_t P = i == 0 ? e.Q[0] : e.P;
                 MuJob* j = sym(e, e.A, e.A, P, e.mp, 0);
                 j->mode = kPoly;
-                j->other = e.A;
+                j->other = (int32_t)e.A;
                 j->scale = (float)ldexp(p.c, ep - 2 * ea);
                 j->poly_b = (float)ldexp(p.b, ep - ea);
                 j->poly_a = (float)ldexp(p.a, ep);
                 ++slots;
                 pq *= bound;
-                const int next = mu_exponent(pq);
                 if (i == 0) eq = ep;
                 const bool more = i + 1 < len;
                 const int et = mu_exponent(x * x * bound);
                 if (i > 0) {
+                    const int next = mu_exponent(pq);
                     sym(e, P, e.Q[q], e.Q[q ^ 1], e.mp, next - ep - eq);
                     q ^= 1;
                     eq = next;
@@ -575,33 +871,31 @@ struct MuSchedule {
                     ++slots;
                 }
             }
-            const bool end = k + e.phase >= p.steps;
-            const int ex2 = end ? 0 : mu_exponent(p.x[k + len]);
+            k += len;
+            const bool end = k >= p.steps;
+            const int ex2 = end ? 0 : mu_exponent(p.x[k]);
             MuJob j = job(e, e.XT[xt], e.Q[q], e.mp, ex2 - ex - eq);
             j.mode = kApply;
-            j.rows = (int32_t)(e.np / kMuTile);
-            j.cols = (int32_t)(e.mp / kMuTile);
-            j.tiles = j.rows * j.cols;
             j.ld_out = (int32_t)e.mp;
             j.ld_other = (int32_t)e.np;
             if (end) {
-                last = j;
+                last = MuOp{j, e.np, e.mp, slots};
                 return;
             }
-            j.out = e.XT[xt ^ 1];
-            j.other = e.X;
-            ops[n++] = MuOp{j, slots++};
+            j.out = (int32_t)e.XT[xt ^ 1];
+            j.other = (int32_t)e.X;
+            ops[n++] = MuOp{j, e.np, e.mp, slots++};
             xt ^= 1;
             ex = ex2;
         }
     }
 
   private:
-    static MuJob job(const MuEntry& e, int64_t left, int64_t right, int64_t k, int exponent) {
+    MuJob job(const MuEntry& e, int64_t left, int64_t right, int64_t k, int exponent) {
         MuJob j{};
-        j.left = left;
-        j.right = right;
-        j.stride = e.stride;
+        j.left = (int32_t)left;
+        j.right = (int32_t)right;
+        j.stride = (int32_t)e.stride;
         j.k = (int32_t)k;
         j.m = (int32_t)e.m;
         j.scale = (float)ldexp(1.0, exponent);
@@ -611,28 +905,213 @@ struct MuSchedule {
     MuJob* sym(const MuEntry& e, int64_t left, int64_t right, int64_t out, int64_t k,
                int exponent) {
         MuJob j = job(e, left, right, k, exponent);
-        const int t = (int)(e.mp / kMuTile);
-        j.out = out;
-        j.tiles = t * (t + 1) / 2;
+        j.out = (int32_t)out;
         j.ld_out = (int32_t)e.mp;
-        ops[n] = MuOp{j, slots};
+        ops[n] = MuOp{j, e.mp, 0, slots};
         return &ops[n++].job;
     }
 };
 
 bool mu_launched() { return hipGetLastError() == hipSuccess; }
 
-int mu_chunk(MuEntry* e, int n, const MuPlan& p, double eps, void* workspace, MuSchedule* sched,
+int64_t mu_tiles(const MuOp& o, int tile) {
+    const int64_t r = o.rows / tile;
+    return o.cols ? r * (o.cols / tile) : r * (r + 1) / 2;
+}
+
+// What a launch of products costs with a tile, in us, from measurements: `stage` values of k
+// take `us` where the CU's `resident` workgroups share it, and at least `alone`; a workgroup's
+// beginning and end take `ends`.
+struct MuTileCost { int tile, stage, resident; double us, alone, ends; };
+const MuTileCost kMuTiles[] = {{64, 64, 1, 0.75, 0.65, 1.5}, {128, 32, 2, 1.4, 0.75, 4.0},
+                               {256, 32, 1, 2.1, 2.1, 10.0}};
+constexpr int kMuCus = 256;
+constexpr double kMuLaunch = 4.0;       // a launch more
+constexpr double kMuBytesPerUs = 4e6;   // of partial sums
+
+// How a launch's sums are cut: its tile, the most stages of a piece, and what it costs.
+struct MuCut {
+    const MuTileCost* tile;
+    int64_t piece;
+    double us;
+    int64_t partials;   // units
+
+    int64_t stages(const MuJob& j) const { return j.k / tile->stage; }
+    int64_t pieces(const MuOp& o) const {
+        return o.cols ? 1 : (stages(o.job) + piece - 1) / piece;
+    }
+};
+
+MuCut mu_cut(const MuOp* const* ops, const int64_t* counts, int n, int most_tile, bool may_split) {
+    MuCut best{nullptr, 0, 1e30, 0};
+    for (const MuTileCost& t : kMuTiles) {
+        if (t.tile > most_tile) continue;
+        MuCut c{&t, (int64_t)1 << 40, 0.0, 0};
+        const double slots = kMuCus * t.resident;
+        int64_t longest = 0;
+        double work = 0.0;
+        for (int i = 0; i < n; ++i) {
+            work += (double)mu_tiles(*ops[i], t.tile) * counts[i] * c.stages(ops[i]->job);
+            longest = std::max(longest, c.stages(ops[i]->job));
+        }
+        for (int cuts = 1; cuts <= (may_split ? 32 : 1); cuts += 1 + cuts / 8) {
+            // Pieces as long as these cuts of the longest sum.
+            c.piece = (longest + cuts - 1) / cuts;
+            if (cuts > 1 && c.piece < 4) break;
+            double blocks = 0.0;
+            int64_t piece = 0;
+            c.partials = 0;
+            for (int i = 0; i < n; ++i) {
+                const int64_t pieces = c.pieces(*ops[i]), st = c.stages(ops[i]->job);
+                piece = std::max(piece, (st + pieces - 1) / pieces);
+                blocks += (double)mu_tiles(*ops[i], t.tile) * counts[i] * pieces;
+                if (pieces > 1)
+                    c.partials += mu_tiles(*ops[i], t.tile) * counts[i] * pieces * t.tile *
+                                  t.tile / kMuUnit;
+            }
+            // Rounds of the longest pieces; pieces of all lengths fill the last round better.
+            double rounds = work / (double)piece / slots, last = 0.0;
+            if (blocks * (double)piece < 1.1 * work) {
+                last = rounds - floor(rounds);
+                rounds = std::max(1.0, floor(rounds) + (last > 0.02 ? 1.0 : 0.0));
+            } else {
+                last = std::min(1.0, rounds);
+                rounds = std::max(1.0, rounds + 0.5);
+            }
+            c.us = t.ends * std::max(1.0, blocks / slots) +
+                   (double)piece * ((rounds - 1.0) * t.us + t.alone + (t.us - t.alone) * last);
+            if (c.partials) c.us += kMuLaunch + c.partials * (kMuUnit * 8.0) / kMuBytesPerUs;
+            if (c.us < best.us && c.partials < (int64_t)1 << 17) best = c;
+            if (cuts > 1 && !c.partials) break;
+        }
+    }
+    return best;
+}
+
+// The products of a launch.
+struct MuLaunch {
+    const MuOp* op[kMuMaxJobs];
+    int64_t count[kMuMaxJobs];
+    int n = 0;
+    MuCut cut;
+
+    void add(const MuOp& o, int64_t c) {
+        op[n] = &o;
+        count[n++] = c;
+    }
+    // Of the same sizes: cut alike.
+    bool like(const MuLaunch& o) const {
+        if (n != o.n) return false;
+        for (int i = 0; i < n; ++i)
+            if (op[i]->rows != o.op[i]->rows || op[i]->cols != o.op[i]->cols ||
+                op[i]->job.k != o.op[i]->job.k || count[i] != o.count[i])
+                return false;
+        return true;
+    }
+    void place(MuJob* j, int i, int64_t* blocks, int64_t* partial) const {
+        *j = op[i]->job;
+        const int tile = cut.tile->tile;
+        j->cols = (int32_t)(op[i]->cols / tile);
+        j->tiles = (int32_t)mu_tiles(*op[i], tile);
+        j->pieces = (int32_t)cut.pieces(*op[i]);
+        const int64_t stages = cut.stages(*j);
+        j->piece_stages = (int32_t)((stages + j->pieces - 1) / j->pieces);
+        // Rounded up, some pieces fewer may do.
+        j->pieces = (int32_t)((stages + j->piece_stages - 1) / j->piece_stages);
+        j->first = (uint32_t)*blocks;
+        *blocks += j->tiles * count[i] * j->pieces;
+        if (j->pieces > 1) {
+            j->partial = (int32_t)*partial;
+            *partial += j->tiles * count[i] * j->pieces * (tile * tile / kMuUnit);
+        }
+    }
+};
+
+template <int TILE>
+bool mu_products(const MuJobs& a, int64_t blocks, const MuJobs& joins, int64_t join_blocks,
+                 hipStream_t stream) {
+    hipLaunchKernelGGL(k_mu_product<TILE>, dim3((unsigned)blocks),
+                       dim3(MuSizes<MuShape<TILE>>::kThreads), 0, stream, a);
+    if (!mu_launched()) return false;
+    if (join_blocks == 0) return true;
+    hipLaunchKernelGGL(k_mu_join<TILE>, dim3((unsigned)join_blocks), dim3(kMuThreads), 0, stream,
+                       joins);
+    return mu_launched();
+}
+
+template <int TILE>
+bool mu_last(const MuLasts& a, int64_t blocks, hipStream_t stream) {
+    hipLaunchKernelGGL(k_mu_last<TILE>, dim3((unsigned)blocks),
+                       dim3(MuSizes<MuShape<TILE>>::kThreads), 0, stream, a);
+    return mu_launched();
+}
+
+// Entries whose launches are shared: what they are padded to, and their launches.
+struct MuChunk {
+    MuEntry* e;
+    int n, pad;
+    double us;
+    int64_t units;      // of halves; behind them the partial sums of products, and of norms
+    int64_t partials, parts;
+    std::unique_ptr<MuSchedule[]> sched;
+    std::vector<MuLaunch> launches;   // the last one is the last product's
+
+    int64_t bytes() const { return (units * 2 + partials * 4) * kMuUnit + parts * 8; }
+
+    void lay(const MuPlan& p, int pad_of) {
+        pad = pad_of;
+        units = partials = parts = 0;
+        int slots = 0;
+        us = 0.0;
+        for (int k = 0; k < n; ++k) {
+            units += mu_layout(e + k, p, pad, units);
+            parts += e[k].count * kMuParts;
+            sched[k].make(e[k], p);
+            slots = std::max(slots, sched[k].slots);
+        }
+        launches.assign(slots + 1, MuLaunch());
+        for (int k = 0; k < n; ++k) {
+            for (int i = 0; i < sched[k].n; ++i)
+                launches[sched[k].ops[i].slot].add(sched[k].ops[i], e[k].count);
+            launches[slots].add(sched[k].last, e[k].count);
+        }
+        for (int i = 0; i <= slots; ++i) {
+            MuLaunch& l = launches[i];
+            int same = 0;
+            while (same < i && !l.like(launches[same])) ++same;
+            l.cut = same < i && i < slots ? launches[same].cut
+                                          : mu_cut(l.op, l.count, l.n, pad, i < slots);
+            us += l.cut.us + kMuLaunch;
+            partials = std::max(partials, l.cut.partials);
+        }
+    }
+
+    // The padding that costs least.
+    void choose(const MuPlan& p) {
+        int best = 0;
+        double least = 1e30;
+        for (const MuTileCost& t : kMuTiles) {
+            lay(p, t.tile);
+            if (us < least) {
+                least = us;
+                best = t.tile;
+            }
+        }
+        if (best != pad) lay(p, best);
+    }
+};
+
+int mu_chunk(const MuChunk& chunk, const MuPlan& p, double eps, void* workspace,
              hipStream_t stream) {
+    const MuEntry* e = chunk.e;
+    const int n = chunk.n;
     MuSources src{};
     src.ws = (_Float16*)workspace;
     src.eps = eps;
     src.scale = (float)ldexp(1.0, mu_exponent(p.x[0]));
     src.n = n;
-    int64_t sums = 0, patches = 0, halves = 0;
-    for (int k = 0; k < n; ++k) halves += e[k].stride * e[k].count;
-    double* parts = (double*)((char*)workspace + halves * 2);
-    int slots = 0;
+    int64_t sums = 0, patches = 0;
+    double* parts = (double*)((char*)workspace + (chunk.units * 2 + chunk.partials * 4) * kMuUnit);
     for (int k = 0; k < n; ++k) {
         MuSource& s = src.s[k];
         const int64_t size = e[k].rows * e[k].cols;
@@ -640,10 +1119,9 @@ int mu_chunk(MuEntry* e, int n, const MuPlan& p, double eps, void* workspace, Mu
         s.momentum = e[k].momentum;
         s.parts = parts;
         parts += e[k].count * kMuParts;
-        s.x_stride = size;
-        s.pairs = e[k].tall ? e[k].XT[0] : e[k].X;
-        s.flipped = e[k].tall ? e[k].X : e[k].XT[0];
-        s.stride = e[k].stride;
+        s.pairs = (int32_t)(e[k].tall ? e[k].XT[0] : e[k].X);
+        s.flipped = (int32_t)(e[k].tall ? e[k].X : e[k].XT[0]);
+        s.stride = (int32_t)e[k].stride;
         s.chunk = mu_round((size + kMuParts - 1) / kMuParts, kMuPass);
         s.nparts = (int32_t)((size + s.chunk - 1) / s.chunk);
         s.rows = (int32_t)e[k].rows;
@@ -659,42 +1137,45 @@ int mu_chunk(MuEntry* e, int n, const MuPlan& p, double eps, void* workspace, Mu
         s.first_patch = (uint32_t)patches;
         sums += s.nparts * e[k].count;
         patches += s.patches * e[k].count;
-        sched[k].make(e[k], p);
-        slots = std::max(slots, sched[k].slots);
     }
     const dim3 block(kMuThreads);
     hipLaunchKernelGGL(k_mu_sums, dim3((unsigned)sums), block, 0, stream, src);
     if (!mu_launched()) return CS_ERR_HIP;
     hipLaunchKernelGGL(k_mu_pairs, dim3((unsigned)patches), block, 0, stream, src);
     if (!mu_launched()) return CS_ERR_HIP;
-    int at[kMuMaxEntries] = {};
-    for (int slot = 0; slot < slots; ++slot) {
-        MuJobs a{};
-        a.ws = (_Float16*)workspace;
-        int64_t blocks = 0;
-        for (int k = 0; k < n; ++k)
-            for (; at[k] < sched[k].n && sched[k].ops[at[k]].slot == slot; ++at[k]) {
-                MuJob& j = a.j[a.n++];
-                j = sched[k].ops[at[k]].job;
-                if (j.mode != kApply) j.cols = 0;
-                j.first = (uint32_t)blocks;
-                blocks += j.tiles * e[k].count;
+    // Partial sums lie behind the pairs; offsets count units of 4096 halves there, and of as many
+    // floats here, so they begin at an even unit.
+    for (size_t i = 0; i + 1 < chunk.launches.size(); ++i) {
+        const MuLaunch& l = chunk.launches[i];
+        MuJobs a{}, joins{};
+        a.ws = joins.ws = (_Float16*)workspace;
+        a.n = l.n;
+        int64_t blocks = 0, partial = chunk.units / 2, join_blocks = 0;
+        const int tile = l.cut.tile->tile;
+        for (int k = 0; k < l.n; ++k) {
+            l.place(&a.j[k], k, &blocks, &partial);
+            if (a.j[k].pieces > 1) {
+                MuJob& j = joins.j[joins.n++];
+                j = a.j[k];
+                j.first = (uint32_t)join_blocks;
+                join_blocks += j.tiles * l.count[k] * (tile * tile / kMuUnit);
             }
-        hipLaunchKernelGGL(k_mu_product, dim3((unsigned)blocks), block, 0, stream, a);
-        if (!mu_launched()) return CS_ERR_HIP;
+        }
+        const bool ok = tile == 256 ? mu_products<256>(a, blocks, joins, join_blocks, stream)
+                        : tile == 128 ? mu_products<128>(a, blocks, joins, join_blocks, stream)
+                                      : mu_products<64>(a, blocks, joins, join_blocks, stream);
+        if (!ok) return CS_ERR_HIP;
     }
-    MuLasts l{};
-    l.ws = (_Float16*)workspace;
-    l.n = n;
-    int64_t blocks = 0;
+    const MuLaunch& l = chunk.launches.back();
+    MuLasts last{};
+    last.ws = (_Float16*)workspace;
+    last.n = n;
+    int64_t blocks = 0, none = 0;
     for (int k = 0; k < n; ++k) {
-        MuLast& y = l.j[k];
-        y.job = sched[k].last;
-        y.job.first = (uint32_t)blocks;
-        blocks += y.job.tiles * e[k].count;
+        MuLast& y = last.j[k];
+        l.place(&y.job, k, &blocks, &none);
         y.out = e[k].out;
         y.master = e[k].master;
-        y.out_stride = e[k].rows * e[k].cols;
         y.rows = (int32_t)e[k].rows;
         y.cols = (int32_t)e[k].cols;
         y.tall = e[k].tall;
@@ -703,8 +1184,11 @@ int mu_chunk(MuEntry* e, int n, const MuPlan& p, double eps, void* workspace, Mu
         y.decay = e[k].decay;
         y.lr = e[k].lr;
     }
-    hipLaunchKernelGGL(k_mu_last, dim3((unsigned)blocks), block, 0, stream, l);
-    return mu_launched() ? CS_OK : CS_ERR_HIP;
+    const int tile = l.cut.tile->tile;
+    const bool ok = tile == 256 ? mu_last<256>(last, blocks, stream)
+                    : tile == 128 ? mu_last<128>(last, blocks, stream)
+                                  : mu_last<64>(last, blocks, stream);
+    return ok ? CS_OK : CS_ERR_HIP;
 }
 
 // Rows of the tables, checked: how many entries have anything, or -1.
@@ -725,8 +1209,8 @@ int mu_entries(int32_t ntensors, const int64_t* table, const float* scalars, boo
             return -1;
         if (x.count == 0 || x.rows == 0 || x.cols == 0) continue;
         // A launch has fewer than 2^32 threads.
-        const int64_t rt = mu_round(x.rows, kMuTile) / kMuPatch,
-                      ct = mu_round(x.cols, kMuTile) / kMuPatch;
+        const int64_t rt = mu_round(x.rows, kMuMostTile) / kMuPatch,
+                      ct = mu_round(x.cols, kMuMostTile) / kMuPatch;
         if (x.count * rt > kMuMaxPatches / ct) return -1;
         if (!row[0] || !row[1]) return -1;
         if (muon) {
@@ -757,54 +1241,48 @@ int mu_run(int32_t ntensors, const int64_t* table, const float* scalars, bool mu
         !mu_plan(&p, steps, a, b, c))
         return CS_ERR_ARGS;
     if (!bytes && ntensors > 0 && (!workspace || ((uintptr_t)workspace & 127))) return CS_ERR_ARGS;
-    std::unique_ptr<MuEntry[]> e(new (std::nothrow) MuEntry[ntensors + 1]);
-    std::unique_ptr<MuSchedule[]> sched(bytes ? nullptr
-                                              : new (std::nothrow) MuSchedule[kMuMaxEntries]);
-    if (!e || (!bytes && !sched)) return CS_ERR_ARGS;
-    const int n = mu_entries(ntensors, table, scalars, muon, e.get());
-    if (n < 0) return CS_ERR_ARGS;
-    for (int k = 0; k < n; ++k) mu_layout(&e[k], p, 0);
-    // The longest sums first: they end last.
-    std::stable_sort(e.get(), e.get() + n,
-                     [](const MuEntry& x, const MuEntry& y) { return x.np > y.np; });
-    if (bytes) *bytes = 0;
-    for (int k = 0; k < n; k += kMuMaxEntries) {
-        const int many = std::min(kMuMaxEntries, n - k);
-        const int64_t need = mu_chunk_bytes(&e[k], many, p);
-        if (bytes) {
-            *bytes = std::max(*bytes, need);
-        } else {
-            const int rc = mu_chunk(&e[k], many, p, eps, workspace, sched.get(), stream);
-            if (rc != CS_OK) return rc;
+    try {
+        std::vector<MuEntry> e(ntensors + 1);
+        const int n = mu_entries(ntensors, table, scalars, muon, e.data());
+        if (n < 0) return CS_ERR_ARGS;
+        // The longest sums first: they end last.
+        std::stable_sort(e.begin(), e.begin() + n, [](const MuEntry& x, const MuEntry& y) {
+            return std::max(x.rows, x.cols) > std::max(y.rows, y.cols);
+        });
+        if (bytes) *bytes = 0;
+        MuChunk chunk;
+        chunk.sched.reset(new MuSchedule[kMuMaxEntries]);
+        for (int k = 0; k < n; k += kMuMaxEntries) {
+            chunk.e = &e[k];
+            chunk.n = std::min(kMuMaxEntries, n - k);
+            chunk.choose(p);
+            if (chunk.units + 2 * chunk.partials > 0x7FFFFFFF) return CS_ERR_ARGS;
+            if (bytes) {
+                *bytes = std::max(*bytes, chunk.bytes());
+            } else {
+                const int rc = mu_chunk(chunk, p, eps, workspace, stream);
+                if (rc != CS_OK) return rc;
+            }
         }
+    } catch (const std::bad_alloc&) {
+        return CS_ERR_ARGS;
     }
     return CS_OK;
-}
-
-int64_t mu_bytes(int32_t ntensors, const int64_t* table, const float* scalars, bool muon,
-                 int32_t steps, double a, double b, double c) {
-    int64_t bytes = 0;
-    return mu_run(ntensors, table, scalars, muon, steps, a, b, c, 0.0, nullptr, &bytes, nullptr) ==
-                   CS_OK ? bytes : -1;
 }
 
 }  // namespace
 
 extern "C" int64_t cs_orthogonalize_workspace_bytes(int32_t ntensors, const int64_t* table,
                                                     int32_t steps, double a, double b, double c) {
-    return mu_bytes(ntensors, table, nullptr, false, steps, a, b, c);
+    int64_t bytes = 0;
+    return mu_run(ntensors, table, nullptr, false, steps, a, b, c, 0.0, nullptr, &bytes,
+                  nullptr) == CS_OK ? bytes : -1;
 }
 
 extern "C" int cs_orthogonalize(int32_t ntensors, const int64_t* table, int32_t steps, double a,
                                 double b, double c, double eps, void* workspace,
                                 hipStream_t stream) {
     return mu_run(ntensors, table, nullptr, false, steps, a, b, c, eps, workspace, nullptr, stream);
-}
-
-extern "C" int64_t cs_muon_workspace_bytes(int32_t ntensors, const int64_t* table,
-                                           const float* scalars, int32_t steps, double a, double b,
-                                           double c) {
-    return mu_bytes(ntensors, table, scalars, true, steps, a, b, c);
 }
 
 extern "C" int cs_muon_step(int32_t ntensors, const int64_t* table, const float* scalars,

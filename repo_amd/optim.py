@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from functools import lru_cache
 from itertools import chain
 from operator import is_
 
@@ -1187,7 +1188,17 @@ def _check_newton_schulz(steps, coefficients, eps):
 
 def _padded(n):
     """Patches along a dimension that is padded to whole tiles."""
-    return -(-n // 128) * 2
+    return -(-n // 256) * 4
+
+
+@lru_cache(maxsize=256)
+def _muon_workspace(shapes, steps, a, b, c):
+    """Bytes for a table of (count, rows, columns)."""
+    table = np.full((len(shapes), 8), 128, dtype=np.int64)
+    table[:, 6:] = 0
+    for row, (count, m, n) in zip(table, shapes):
+        row[2], row[4], row[5] = count, m, n
+    return N.lib().cs_orthogonalize_workspace_bytes(len(shapes), table.ctypes.data, steps, a, b, c)
 
 
 def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=_NS_COEFFICIENTS,
@@ -1229,11 +1240,11 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=_NS_COEFFICIENTS
         at = k * m * n * x.element_size()
         table = np.array([[x.data_ptr() + at, y.data_ptr() + at, min(most, count - k), 0, m, n,
                            _ADAMW_DTYPES[x.dtype], 0]], dtype=np.int64)
-        args = (1, table.ctypes.data, steps, a, b, c)
-        work = torch.empty(N.lib().cs_orthogonalize_workspace_bytes(*args), dtype=torch.uint8,
-                           device=x.device)
+        work = torch.empty(_muon_workspace(((min(most, count - k), m, n),), steps, a, b, c),
+                           dtype=torch.uint8, device=x.device)
         with N.prof("optim.orthogonalize"):
-            N.call("cs_orthogonalize", *args, float(eps), work.data_ptr(), N.stream(x.device))
+            N.call("cs_orthogonalize", 1, table.ctypes.data, steps, a, b, c, float(eps),
+                   work.data_ptr(), N.stream(x.device))
     return y
 
 
@@ -1368,10 +1379,11 @@ class Muon(torch.optim.Optimizer):
     def _launch(device, rows, scalars, steps, a, b, c, eps):
         table = np.array(rows, dtype=np.int64)
         numbers = np.array(scalars, dtype=np.float32)
-        args = (len(rows), table.ctypes.data, numbers.ctypes.data, steps, a, b, c)
-        work = torch.empty(N.lib().cs_muon_workspace_bytes(*args), dtype=torch.uint8, device=device)
+        work = torch.empty(_muon_workspace(tuple((1, *row[4:6]) for row in rows), steps, a, b, c),
+                           dtype=torch.uint8, device=device)
         with N.prof("optim.muon"):
-            N.call("cs_muon_step", *args, eps, work.data_ptr(), N.stream(device))
+            N.call("cs_muon_step", len(rows), table.ctypes.data, numbers.ctypes.data, steps, a, b,
+                   c, eps, work.data_ptr(), N.stream(device))
 
     # ---- state
 
