@@ -1,7 +1,7 @@
 // `_cs_torch`, a CPython extension on torch's C++ tensors, for what costs the host
-// most in Python: the autograd node of group norm (its backward then runs in the
-// engine's thread without the interpreter), and the checks that an AdamW step
-// makes of every parameter and gradient.  The kernels are reached through the C
+// most in Python: the autograd nodes of group norm, tokens' log-probabilities and the
+// policy loss (their backward then runs in the engine's thread without the
+// interpreter), and the checks that an AdamW step makes of every parameter and gradient.  The kernels are reached through the C
 // ABI of libcubicsplat_hip.so, as everywhere.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -175,6 +175,239 @@ PyObject* py_group_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                     : forward(x, weight.value_or(Tensor()), bias.value_or(Tensor()), groups, eps,
                               act, nullptr);
     return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// A gradient under create_graph gets a node that refuses to be differentiated, rather
+// than none.
+Tensor once(Tensor grad, const char* what) {
+    if (!at::GradMode::is_enabled()) return grad;
+    auto refuse = std::make_shared<torch::autograd::DelayedError>(what, 1);
+    return (*refuse)(variable_list{grad.detach().set_requires_grad(true)})[0];
+}
+
+// Logits as [batch, length, vocab] rows that the entry points can read, and what belongs
+// to them: whole-number tokens and a mask, contiguous.
+struct Rows {
+    Tensor z, tokens, mask;
+    double temperature;
+
+    Rows(Tensor z_, Tensor tokens_, Tensor mask_, double t)
+        : z(std::move(z_)), tokens(std::move(tokens_)), mask(std::move(mask_)), temperature(t) {}
+
+    static Rows of(const Tensor& logits, const Tensor& tokens, const std::optional<Tensor>& mask,
+                   double temperature) {
+        Tensor z = logits.detach();
+        if (z.dim() < 3) z = z.reshape({1, z.dim() < 2 ? 1 : z.size(0), z.size(-1)});
+        else if (z.dim() > 3) z = z.reshape({-1, z.size(-2), z.size(-1)});
+        if (z.size(2) != 1 && z.stride(2) != 1) z = z.contiguous();
+        return Rows(z, tokens.detach().to(at::kLong).contiguous(),
+                    mask ? mask->detach().contiguous() : Tensor(), temperature);
+    }
+    int64_t batch() const { return z.size(0); }
+    int64_t length() const { return z.size(1); }
+    at::TensorOptions fp32() const { return z.options().dtype(at::kFloat); }
+    const uint8_t* mask_pointer() const { return (const uint8_t*)pointer(mask); }
+
+    // The gradient for slopes of the log-probabilities, times *factor; into `into`, which
+    // holds it for a factor of one, or a new tensor.
+    Tensor gradient(const Tensor& stats, const Tensor& slopes, const Tensor& factor, Tensor into,
+                    at::IntArrayRef shape) const {
+        const bool fresh = !into.defined();
+        if (fresh) into = at::empty(shape, z.options());
+        check(cs_token_logprobs_backward(z.data_ptr(), batch(), length(), z.size(2), z.stride(0),
+                                         z.stride(1), type_code(z), tokens.data_ptr<int64_t>(),
+                                         mask_pointer(), temperature, stats.data_ptr<float>(),
+                                         slopes.data_ptr<float>(), (const float*)pointer(factor),
+                                         fresh ? 0 : 1, into.data_ptr(), stream(z)),
+              "cs_token_logprobs_backward");
+        return into;
+    }
+};
+
+Tensor logprobs_forward(const Rows& a, Tensor* stats) {
+    *stats = at::empty({a.batch(), a.length(), 2}, a.fp32());
+    Tensor lp = at::empty(a.tokens.sizes(), a.fp32());
+    check(cs_token_logprobs_forward(a.z.data_ptr(), a.batch(), a.length(), a.z.size(2),
+                                    a.z.stride(0), a.z.stride(1), type_code(a.z),
+                                    a.tokens.data_ptr<int64_t>(), a.mask_pointer(), a.temperature,
+                                    stats->data_ptr<float>(), lp.data_ptr<float>(), stream(a.z)),
+          "cs_token_logprobs_forward");
+    return lp;
+}
+
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens,
+                          const std::optional<Tensor>& mask, double temperature) {
+        const Rows a = Rows::of(logits, tokens, mask, temperature);
+        Tensor stats, lp = logprobs_forward(a, &stats);
+        ctx->save_for_backward({a.z, a.tokens, a.mask, stats});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["shape"] = logits.sizes().vec();
+        return lp;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Rows a(saved[0], saved[1], saved[2], ctx->saved_data["temperature"].toDouble());
+        Tensor grad;
+        {
+            at::AutoGradMode off(false);
+            grad = a.gradient(saved[3], grads[0].contiguous(), Tensor(), Tensor(),
+                              ctx->saved_data["shape"].toIntVector());
+        }
+        return {once(grad, "token_logprobs is differentiable once"), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// What the loss takes besides the rows: constants, and numbers.
+struct LossArgs {
+    Tensor advantages, old_logprobs, ref_logprobs;
+    double clip_low, clip_high, kl_weight, scale;
+    int64_t reduction;
+};
+
+// [loss, KL, clipped], the log-probabilities; with `grad` the gradient for an incoming one.
+struct LossOut { Tensor out, logprobs, stats, slopes, grad; };
+
+LossOut loss_forward(const Rows& a, const LossArgs& f, at::IntArrayRef shape, bool with_grad) {
+    LossOut y;
+    y.out = at::empty({3}, a.fp32());
+    y.logprobs = at::empty(a.tokens.sizes(), a.fp32());
+    y.slopes = at::empty({a.batch(), a.length()}, a.fp32());
+    y.stats = at::empty({a.batch(), a.length(), 2}, a.fp32());
+    if (with_grad) y.grad = at::empty(shape, a.z.options());
+    const Tensor work = at::empty(
+        {(int64_t)cs_policy_loss_workspace_elems(a.batch(), a.length())}, a.fp32());
+    const Tensor adv = f.advantages.detach().to(at::kFloat).expand(a.tokens.sizes()).reshape(
+        {a.batch(), a.length()});
+    const Tensor old = f.old_logprobs.detach().to(at::kFloat).contiguous();
+    const Tensor ref = f.ref_logprobs.defined()
+                           ? f.ref_logprobs.detach().to(at::kFloat).contiguous() : Tensor();
+    check(cs_policy_loss(a.z.data_ptr(), a.batch(), a.length(), a.z.size(2), a.z.stride(0),
+                         a.z.stride(1), type_code(a.z), a.tokens.data_ptr<int64_t>(),
+                         a.mask_pointer(), a.temperature, adv.data_ptr<float>(), adv.stride(0),
+                         adv.stride(1), old.data_ptr<float>(), (const float*)pointer(ref),
+                         f.clip_low, f.clip_high, f.kl_weight, (int32_t)f.reduction, f.scale,
+                         work.data_ptr<float>(), y.stats.data_ptr<float>(),
+                         y.slopes.data_ptr<float>(), y.logprobs.data_ptr<float>(),
+                         y.out.data_ptr<float>(), pointer(y.grad), stream(a.z)),
+          "cs_policy_loss");
+    return y;
+}
+
+struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens,
+                                 const std::optional<Tensor>& mask, double temperature,
+                                 const LossArgs* f) {
+        const Rows a = Rows::of(logits, tokens, mask, temperature);
+        LossOut y = loss_forward(a, *f, logits.sizes(), true);
+        variable_list out{y.out[0], y.logprobs, y.out[1], y.out[2]};
+        ctx->mark_non_differentiable({out[1], out[2], out[3]});
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({a.z, a.tokens, a.mask, y.stats, y.slopes});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["shape"] = logits.sizes().vec();
+        ctx->saved_data["grad"] = y.grad;
+        return out;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        // The gradient for an incoming one is there; another one's is computed from the
+        // logits, not from that one's rounded values.  A second backward pass finds it given
+        // away.
+        const variable_list saved = ctx->get_saved_variables();
+        const Rows a(saved[0], saved[1], saved[2], ctx->saved_data["temperature"].toDouble());
+        Tensor grad;
+        auto held = ctx->saved_data.find("grad");
+        if (held != ctx->saved_data.end()) {
+            grad = held->second.toTensor();
+            ctx->saved_data.erase(held);
+        }
+        if (!grads[0].defined()) return variable_list(5);
+        {
+            at::AutoGradMode off(false);
+            grad = a.gradient(saved[3], saved[4], grads[0].to(at::kFloat).contiguous(), grad,
+                              ctx->saved_data["shape"].toIntVector());
+        }
+        return {once(grad, "policy_loss is differentiable once"), Tensor(), Tensor(), Tensor(),
+                Tensor()};
+    }
+};
+
+bool wants_node(const Tensor& t) {
+    return (at::GradMode::is_enabled() && t.requires_grad()) || has_tangent(t);
+}
+
+void check_rows(const char* what, PyObject* const* args) {
+    for (int k : {0, 1})
+        TORCH_CHECK_TYPE(THPVariable_Check(args[k]), what, ": expected tensors");
+    TORCH_CHECK_TYPE(args[2] == Py_None || THPVariable_Check(args[2]), what,
+                     ": mask must be a tensor or None");
+    const Tensor &z = THPVariable_Unpack(args[0]), &t = THPVariable_Unpack(args[1]);
+    TORCH_CHECK_VALUE(z.is_cuda() && type_code(z) >= 0 && z.dim() >= 1 && t.numel() > 0 &&
+                          z.numel() > 0 && z.numel() / z.size(-1) == t.numel() &&
+                          t.device() == z.device(),
+                      what, ": logits and tokens do not fit");
+    if (args[2] != Py_None) {
+        const Tensor& m = THPVariable_Unpack(args[2]);
+        TORCH_CHECK_VALUE(m.scalar_type() == at::kBool && m.sizes() == t.sizes() &&
+                              m.device() == z.device(), what, ": the mask does not fit");
+    }
+}
+
+// token_logprobs(logits, tokens, mask | None, temperature): all arguments checked by the caller.
+PyObject* py_token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(nargs == 4, "token_logprobs: expected 4 arguments");
+    check_rows("token_logprobs", args);
+    const Tensor &logits = THPVariable_Unpack(args[0]), &tokens = THPVariable_Unpack(args[1]);
+    const std::optional<Tensor> mask = optional_tensor(args[2]);
+    const double temperature = PyFloat_AsDouble(args[3]);
+    if (PyErr_Occurred()) return nullptr;
+    Tensor stats;
+    Tensor lp = wants_node(logits)
+                    ? TokenLogprobs::apply(logits, tokens, mask, temperature)
+                    : logprobs_forward(Rows::of(logits, tokens, mask, temperature), &stats);
+    return THPVariable_Wrap(std::move(lp));
+    END_HANDLE_TH_ERRORS
+}
+
+// policy_loss(logits, tokens, mask | None, temperature, advantages, old, ref | None, clip_low,
+// clip_high, kl_weight, reduction, scale) -> (loss, logprobs, kl, clipped): all arguments
+// checked by the caller.
+PyObject* py_policy_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(nargs == 12, "policy_loss: expected 12 arguments");
+    check_rows("policy_loss", args);
+    for (int k : {4, 5}) TORCH_CHECK_TYPE(THPVariable_Check(args[k]), "policy_loss: expected tensors");
+    TORCH_CHECK_TYPE(args[6] == Py_None || THPVariable_Check(args[6]),
+                     "policy_loss: ref must be a tensor or None");
+    const Tensor &logits = THPVariable_Unpack(args[0]), &tokens = THPVariable_Unpack(args[1]);
+    const std::optional<Tensor> mask = optional_tensor(args[2]);
+    LossArgs f{THPVariable_Unpack(args[4]), THPVariable_Unpack(args[5]),
+               optional_tensor(args[6]).value_or(Tensor()), PyFloat_AsDouble(args[7]),
+               PyFloat_AsDouble(args[8]), PyFloat_AsDouble(args[9]), PyFloat_AsDouble(args[11]),
+               PyLong_AsLongLong(args[10])};
+    const double temperature = PyFloat_AsDouble(args[3]);
+    if (PyErr_Occurred()) return nullptr;
+    for (const Tensor& t : {f.old_logprobs, f.ref_logprobs})
+        TORCH_CHECK_VALUE(!t.defined() || (t.sizes() == tokens.sizes() &&
+                                           t.device() == logits.device()),
+                          "policy_loss: the constants do not fit");
+    TORCH_CHECK_VALUE(f.advantages.device() == logits.device(),
+                      "policy_loss: the constants do not fit");
+    variable_list out;
+    if (wants_node(logits)) {
+        out = PolicyLoss::apply(logits, tokens, mask, temperature, &f);
+    } else {
+        LossOut y = loss_forward(Rows::of(logits, tokens, mask, temperature), f, {}, false);
+        out = {y.out[0], y.logprobs, y.out[1], y.out[2]};
+    }
+    PyObject* tuple = PyTuple_New(4);
+    if (!tuple) return nullptr;
+    for (int k = 0; k < 4; ++k) PyTuple_SET_ITEM(tuple, k, THPVariable_Wrap(std::move(out[k])));
+    return tuple;
     END_HANDLE_TH_ERRORS
 }
 
@@ -380,6 +613,8 @@ PyObject* py_signature_hash(PyObject*, PyObject*) {
 
 PyMethodDef methods[] = {
     {"group_norm", (PyCFunction)(void (*)(void))py_group_norm, METH_FASTCALL, nullptr},
+    {"token_logprobs", (PyCFunction)(void (*)(void))py_token_logprobs, METH_FASTCALL, nullptr},
+    {"policy_loss", (PyCFunction)(void (*)(void))py_policy_loss, METH_FASTCALL, nullptr},
     {"adamw_unchanged", (PyCFunction)(void (*)(void))py_adamw_unchanged, METH_FASTCALL, nullptr},
     {"adamw_place", (PyCFunction)(void (*)(void))py_adamw_place, METH_FASTCALL, nullptr},
     {"adamw_held", (PyCFunction)(void (*)(void))py_adamw_held, METH_FASTCALL, nullptr},

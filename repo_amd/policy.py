@@ -14,6 +14,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _native as N
+from . import torchcall
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _REDUCTIONS = {"token": 0, "sequence": 1, "sum": 2}
@@ -55,8 +56,7 @@ def _beside(t, name, logits):
 
 
 def _rows(logits):
-    """logits as [batch, length, vocab] with the vocabulary contiguous; autograd sees
-    how."""
+    """logits as [batch, length, vocab] with the vocabulary contiguous."""
     if logits.dim() < 3:
         logits = logits.reshape((1,) * (3 - logits.dim()) + logits.shape)
     elif logits.dim() > 3:
@@ -75,35 +75,87 @@ def _plain(t, dtype):
     return t.detach().to(dtype).contiguous()
 
 
+def _inputs(logits, tokens, mask):
+    return (_rows(logits.detach()), _plain(tokens, torch.int64),
+            None if mask is None else mask.contiguous())
+
+
+# The nodes below are for runs without the extension, and where each launch is bracketed by a
+# context manager; the extension's do the same.
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, tokens, mask, temperature):
-        lp = torch.empty(z.shape[:2], dtype=torch.float32, device=z.device)
+    def forward(ctx, logits, tokens, mask, temperature):
+        z, tokens, mask = _inputs(logits, tokens, mask)
+        lp = torch.empty(tokens.shape, dtype=torch.float32, device=z.device)
         stats = torch.empty((*z.shape[:2], 2), dtype=torch.float32, device=z.device)
         with N.prof("policy.logprobs"):
             N.call("cs_token_logprobs_forward", *_head(z, tokens, mask, temperature),
                    stats.data_ptr(), lp.data_ptr(), N.stream(z.device))
         ctx.save_for_backward(z, tokens, mask, stats)
-        ctx.temperature = temperature
+        ctx.temperature, ctx.shape = temperature, logits.shape
         return lp
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, upstream):
         z, tokens, mask, stats = ctx.saved_tensors
-        return (_gradient(z, tokens, mask, ctx.temperature, stats, upstream.contiguous()),
-                None, None, None)
+        return (_gradient(z, tokens, mask, ctx.temperature, stats, upstream.contiguous(),
+                          ctx.shape), None, None, None)
 
 
-def _gradient(z, tokens, mask, temperature, stats, slopes, factor=None, into=None):
+def _gradient(z, tokens, mask, temperature, stats, slopes, shape, factor=None, into=None):
     """The logits' gradient for slopes of the log-probabilities, times *factor; into
     `into`, which holds it for a factor of one, or a new tensor."""
-    grad = torch.empty(z.shape, dtype=z.dtype, device=z.device) if into is None else into
+    grad = torch.empty(shape, dtype=z.dtype, device=z.device) if into is None else into
     with N.prof("policy.logprobs_bwd"):
         N.call("cs_token_logprobs_backward", *_head(z, tokens, mask, temperature),
                stats.data_ptr(), slopes.data_ptr(), N.ptr(factor), 0 if into is None else 1,
                grad.data_ptr(), N.stream(z.device))
     return grad
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, mask, temperature, need, advantages, old, ref, *numbers):
+        z, tokens, mask = _inputs(logits, tokens, mask)
+        batch, length, _ = z.shape
+        dev = z.device
+        advantages = advantages.detach().float().expand(tokens.shape).reshape(batch, length)
+        old, ref = _plain(old, torch.float32), None if ref is None else _plain(ref, torch.float32)
+        grad = torch.empty(logits.shape, dtype=z.dtype, device=dev) if need else None
+        lp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+        slopes = torch.empty((batch, length), dtype=torch.float32, device=dev)
+        stats = torch.empty((batch, length, 2), dtype=torch.float32, device=dev)
+        out = torch.empty(3, dtype=torch.float32, device=dev)
+        work = torch.empty(int(N.lib().cs_policy_loss_workspace_elems(batch, length)),
+                           dtype=torch.float32, device=dev)
+        with N.prof("policy.loss"):
+            N.call("cs_policy_loss", *_head(z, tokens, mask, temperature), advantages.data_ptr(),
+                   advantages.stride(0), advantages.stride(1), old.data_ptr(), N.ptr(ref),
+                   *numbers, work.data_ptr(), stats.data_ptr(), slopes.data_ptr(), lp.data_ptr(),
+                   out.data_ptr(), N.ptr(grad), N.stream(dev))
+        loss, kl, clipped = out.unbind()
+        ctx.mark_non_differentiable(lp, kl, clipped)
+        if need:
+            ctx.save_for_backward(z, tokens, mask, stats, slopes)
+            ctx.grad, ctx.temperature, ctx.shape = grad, temperature, logits.shape
+        return loss, lp, kl, clipped
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, upstream, *_):
+        # The gradient for an incoming one is there; another one's is computed from the
+        # logits, not from that one's rounded values.  A second backward pass finds it given away.
+        z, tokens, mask, stats, slopes = ctx.saved_tensors
+        into, ctx.grad = ctx.grad, None
+        factor = upstream.to(torch.float32).contiguous()
+        return (_gradient(z, tokens, mask, ctx.temperature, stats, slopes, ctx.shape, factor,
+                          into), *(None,) * 12)
+
+
+def _extension():
+    return torchcall.module() if N._PROFILE_CTX_FACTORY is None else None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *,
@@ -124,45 +176,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *,
     if logits.device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(logits.device):
             return token_logprobs(logits, tokens, mask=mask, temperature=temperature)
-    return _TokenLogprobs.apply(_rows(logits), _plain(tokens, torch.int64),
-                                None if mask is None else mask.contiguous(),
-                                float(temperature)).view(tokens.shape)
-
-
-class _PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, tokens, mask, advantages, old, ref, numbers, temperature, need):
-        batch, length, _ = z.shape
-        dev = z.device
-        grad = torch.empty(z.shape, dtype=z.dtype, device=dev) if need else None
-        lp, slopes = torch.empty((2, batch, length), dtype=torch.float32, device=dev).unbind()
-        stats = torch.empty((batch, length, 2), dtype=torch.float32, device=dev)
-        out = torch.empty(3, dtype=torch.float32, device=dev)
-        work = torch.empty(int(N.lib().cs_policy_loss_workspace_elems(batch, length)),
-                           dtype=torch.float32, device=dev)
-        with N.prof("policy.loss"):
-            N.call("cs_policy_loss", *_head(z, tokens, mask, temperature), advantages.data_ptr(),
-                   advantages.stride(0), advantages.stride(1), old.data_ptr(), N.ptr(ref),
-                   *numbers, work.data_ptr(), stats.data_ptr(), slopes.data_ptr(), lp.data_ptr(),
-                   out.data_ptr(), N.ptr(grad), N.stream(dev))
-        loss, kl, clipped = out.unbind()
-        ctx.mark_non_differentiable(lp, kl, clipped)
-        if need:
-            ctx.save_for_backward(z, tokens, mask, stats, slopes)
-            ctx.grad, ctx.temperature = grad, temperature
-        return loss, lp, kl, clipped
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, upstream, *_):
-        # The gradient for an upstream of one is there; another one's is computed from
-        # the logits, not from that one's rounded values.  A second backward pass finds
-        # it given away.
-        z, tokens, mask, stats, slopes = ctx.saved_tensors
-        into, ctx.grad = ctx.grad, None
-        factor = upstream.to(torch.float32).contiguous()
-        return (_gradient(z, tokens, mask, ctx.temperature, stats, slopes, factor, into),
-                *(None,) * 8)
+    ext = _extension()
+    return (ext.token_logprobs if ext is not None else _TokenLogprobs.apply)(
+        logits, tokens, mask, float(temperature))
 
 
 def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Tensor,
@@ -227,12 +243,11 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Te
                                ref_logprobs=ref_logprobs, mask=mask, clip=clip,
                                kl_weight=kl_weight, temperature=temperature, reduction=reduction,
                                scale=scale)
-    z = _rows(logits)
-    advantages = advantages.detach().float().expand(shape).reshape(z.shape[:2])
-    loss, lp, kl, clipped = _PolicyLoss.apply(
-        z, _plain(tokens, torch.int64), None if mask is None else mask.contiguous(), advantages,
-        _plain(old_logprobs, torch.float32),
-        None if ref_logprobs is None else _plain(ref_logprobs, torch.float32),
-        (float(low), float(high), float(kl_weight), _REDUCTIONS[reduction], float(scale)),
-        float(temperature), torch.is_grad_enabled() and z.requires_grad)
-    return PolicyLoss(loss, lp.view(shape), kl, clipped)
+    constants = (advantages, old_logprobs, ref_logprobs, float(low), float(high),
+                 float(kl_weight), _REDUCTIONS[reduction], float(scale))
+    ext = _extension()
+    if ext is not None:
+        return PolicyLoss(*ext.policy_loss(logits, tokens, mask, float(temperature), *constants))
+    return PolicyLoss(*_PolicyLoss.apply(logits, tokens, mask, float(temperature),
+                                         torch.is_grad_enabled() and logits.requires_grad,
+                                         *constants))
