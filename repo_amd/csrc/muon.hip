@@ -131,15 +131,18 @@ __device__ inline void mu_to_lds(const _Float16* from, char* to) {
 }
 
 // Tiles of T x T by WR x WC waves, each of I x J blocks of 16 x 16; a stage brings 32 KS
-// values of k of every row, and ST stages are there or on their way.
+// values of k of every row, and ST stages are there or on their way.  KW groups of such waves
+// share a stage's k: a tile of 64 mostly has a CU to itself, where one group waits for its own
+// reads (a stage of one took 0.63 us, 1021 x 765 219 us).
 template <int TILE> struct MuShape;
-template <> struct MuShape<256> { enum { T = 256, WR = 2, WC = 4, KS = 1, ST = 2 }; };
-template <> struct MuShape<128> { enum { T = 128, WR = 2, WC = 2, KS = 1, ST = 2 }; };
-template <> struct MuShape<64> { enum { T = 64, WR = 2, WC = 2, KS = 2, ST = 3 }; };
+template <> struct MuShape<256> { enum { T = 256, WR = 2, WC = 4, KS = 1, KW = 1, ST = 2 }; };
+template <> struct MuShape<128> { enum { T = 128, WR = 2, WC = 2, KS = 1, KW = 1, ST = 2 }; };
+template <> struct MuShape<64> { enum { T = 64, WR = 2, WC = 2, KS = 2, KW = 2, ST = 3 }; };
 
 template <typename S> struct MuSizes {
     enum {
-        kWaves = S::WR * S::WC,
+        kGroup = S::WR * S::WC,
+        kWaves = kGroup * S::KW,
         kThreads = kWaves * 64,
         I = S::T / S::WR / 16,
         J = S::T / S::WC / 16,
@@ -197,8 +200,9 @@ __device__ inline void mu_tile(const _Float16* left, const _Float16* right, int 
     for (int s = 0; s < S::ST - 1; ++s)
         if (from + s < to) bring(from + s, s);
     const int high = (lane & 15) * 128 + ((lane >> 4) ^ (lane & 7)) * 16, low = high ^ 64;
-    const char* a0 = lds + (wave / S::WC) * (Z::I * S::KS * 2048);
-    const char* b0 = lds + Z::kSide + (wave % S::WC) * (Z::J * S::KS * 2048);
+    const int member = wave & (Z::kGroup - 1);
+    const char* a0 = lds + (member / S::WC) * (Z::I * S::KS * 2048);
+    const char* b0 = lds + Z::kSide + (member % S::WC) * (Z::J * S::KS * 2048);
     int slot = 0;
     if constexpr (S::KS == 1 && S::ST == 2) {
         // The barrier comes before a step's last blocks, whose operands then are in registers:
@@ -276,27 +280,62 @@ __device__ inline void mu_tile(const _Float16* left, const _Float16* right, int 
         const char* a = a0 + slot * Z::kStage;
         const char* b = b0 + slot * Z::kStage;
 #pragma unroll
-        for (int c = 0; c < S::KS; ++c) {
+        for (int q = 0; q < S::KS / S::KW; ++q) {
+            const int c = q * S::KW + wave / Z::kGroup;
             Half8 bh[Z::J], bl[Z::J];
 #pragma unroll
             for (int j = 0; j < Z::J; ++j) {
                 bh[j] = *(const Half8*)(b + (j * S::KS + c) * 2048 + high);
                 bl[j] = *(const Half8*)(b + (j * S::KS + c) * 2048 + low);
             }
+            Half8 ah[Z::I], al[Z::I];
 #pragma unroll
             for (int i = 0; i < Z::I; ++i) {
-                const Half8 ah = *(const Half8*)(a + (i * S::KS + c) * 2048 + high);
-                const Half8 al = *(const Half8*)(a + (i * S::KS + c) * 2048 + low);
-#pragma unroll
-                for (int j = 0; j < Z::J; ++j) acc[i][j] = mu_mfma(bl[j], ah, acc[i][j]);
-#pragma unroll
-                for (int j = 0; j < Z::J; ++j) acc[i][j] = mu_mfma(bh[j], al, acc[i][j]);
-#pragma unroll
-                for (int j = 0; j < Z::J; ++j) acc[i][j] = mu_mfma(bh[j], ah, acc[i][j]);
+                ah[i] = *(const Half8*)(a + (i * S::KS + c) * 2048 + high);
+                al[i] = *(const Half8*)(a + (i * S::KS + c) * 2048 + low);
             }
+            // A product waits for the last one into its sums: as many others between them as
+            // there are.
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+#pragma unroll
+                for (int i = 0; i < Z::I; ++i)
+#pragma unroll
+                    for (int j = 0; j < Z::J; ++j)
+                        acc[i][j] = mu_mfma(p == 0 ? bl[j] : bh[j], p == 1 ? al[i] : ah[i],
+                                            acc[i][j]);
         }
         slot = slot == S::ST - 1 ? 0 : slot + 1;
     }
+    if constexpr (S::KW == 2) {
+        // Each group ends with the whole sums of its half of the block rows.
+        constexpr int kHalf = Z::I / 2;
+        __syncthreads();
+        const int group = wave / Z::kGroup;
+        Float4* there = (Float4*)lds + (group * Z::kGroup + member) * (kHalf * Z::J * 64) + lane;
+        const Float4* here =
+            (Float4*)lds + ((group ^ 1) * Z::kGroup + member) * (kHalf * Z::J * 64) + lane;
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i)
+#pragma unroll
+            for (int j = 0; j < Z::J; ++j)
+                there[(i * Z::J + j) * 64] = group ? acc[i][j] : acc[i + kHalf][j];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i)
+#pragma unroll
+            for (int j = 0; j < Z::J; ++j) {
+                if (group) acc[i + kHalf][j] = here[(i * Z::J + j) * 64] + acc[i + kHalf][j];
+                else acc[i][j] += here[(i * Z::J + j) * 64];
+            }
+    }
+}
+
+// Whether block row i of a tile's sums is the wave's to store.
+template <typename S>
+__device__ inline bool mu_mine(int i) {
+    typedef MuSizes<S> Z;
+    return S::KW == 1 || i / (Z::I / S::KW) == (int)(threadIdx.x >> 6) / Z::kGroup;
 }
 
 // A workgroup's place: matrix b of the stack, tile (ti, tj), its number, its piece.
@@ -385,7 +424,7 @@ __global__ __launch_bounds__(MuSizes<MuShape<TILE>>::kThreads, 2) void k_mu_prod
     Float4 acc[Z::I][Z::J];
     mu_tile<S>(ws + (int64_t)job.left * kMuUnit + p.ti * S::T * ld,
                ws + (int64_t)job.right * kMuUnit + p.tj * S::T * ld, job.k, from, to, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & (Z::kGroup - 1);
     const int row0 = (wave / S::WC) * (Z::I * 16) + (lane & 15);
     const int col0 = (wave % S::WC) * (Z::J * 16) + (lane >> 4) * 4;
     if (job.pieces > 1) {
@@ -395,13 +434,15 @@ __global__ __launch_bounds__(MuSizes<MuShape<TILE>>::kThreads, 2) void k_mu_prod
         for (int i = 0; i < Z::I; ++i)
 #pragma unroll
             for (int j = 0; j < Z::J; ++j)
-                *(Float4*)(part + (row0 + 16 * i) * S::T + col0 + 16 * j) = acc[i][j];
+                if (mu_mine<S>(i))
+                    *(Float4*)(part + (row0 + 16 * i) * S::T + col0 + 16 * j) = acc[i][j];
         return;
     }
     const bool mirror = job.cols == 0 ? p.ti != p.tj : job.other >= 0;
 #pragma unroll
     for (int i = 0; i < Z::I; ++i)
-        mu_store(job, ws, p.ti * S::T + row0 + 16 * i, p.tj * S::T + col0, acc[i], mirror);
+        if (mu_mine<S>(i))
+            mu_store(job, ws, p.ti * S::T + row0 + 16 * i, p.tj * S::T + col0, acc[i], mirror);
 }
 
 // The pieces' sums, in their order: a workgroup takes 64 x 64 values of a tile, a thread eight
@@ -496,7 +537,7 @@ __global__ __launch_bounds__(MuSizes<MuShape<TILE>>::kThreads, 2) void k_mu_last
     mu_tile<S>(ws + (int64_t)job.left * kMuUnit + p.ti * S::T * ld,
                ws + (int64_t)job.right * kMuUnit + p.tj * S::T * ld, job.k, 0,
                job.k / (32 * S::KS), lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & (Z::kGroup - 1);
     const int row0 = p.ti * S::T + (wave / S::WC) * (Z::I * 16) + (lane & 15);
     const int col0 = p.tj * S::T + (wave % S::WC) * (Z::J * 16) + (lane >> 4) * 4;
     const int64_t first = (int64_t)p.b * l.rows * l.cols;
@@ -504,6 +545,7 @@ __global__ __launch_bounds__(MuSizes<MuShape<TILE>>::kThreads, 2) void k_mu_last
     // Row `row0 + 16 i` of X's transpose; its weights are asked for together.
 #pragma unroll
     for (int i = 0; i < Z::I; ++i) {
+        if (!mu_mine<S>(i)) continue;
         int64_t at[Z::J][4];
         float w[Z::J][4] = {};
 #pragma unroll
@@ -709,6 +751,399 @@ __global__ __launch_bounds__(kMuThreads) void k_mu_pairs(MuSources a) {
         _Float16* o = ws + (int64_t)s.flipped * kMuUnit + mu_at(c0 + c, s.padded_rows, r0 + c8);
         *(Half8*)o = h;
         *(Half8*)(o + 32) = l;
+    }
+}
+
+// ------------------------------------------------------------ small matrices
+
+// A matrix of at most 96 rows by one workgroup, all steps in one launch: X stays in registers.
+// A wave holds 32 C columns n, as operands whose lane is n and whose k is m: lane r + 16 g of
+// block b has n = 16 b + r, and of 32 values of m those with (m & 15) >> 2 = g, value i being
+// m = 16 (i >> 2) + 4 g + (i & 3).  In that order a product's sums lie as its operands do (four
+// neighbours of m in the lane of their n), so P X becomes the next X where it is.  For X X^T,
+// whose k is n, the wave's columns go through LDS and come back transposed.  A and P lie in LDS
+// as operands of the same order.
+struct MuSmall {
+    const void* x;
+    void* out;
+    float *master, *momentum;
+    int32_t rows, cols;
+    uint32_t first;
+    int32_t dtype, tall;
+    float decay, lr, mix, look;
+    int32_t pad;
+};
+
+constexpr int kMuSmallWaves = 8;
+constexpr int kMuSmallSteps = 32;   // whose numbers travel with the launch
+
+struct MuSmalls {
+    MuSmall s[kMuMaxEntries];
+    float gram[kMuSmallSteps], square[kMuSmallSteps], linear[kMuSmallSteps], one[kMuSmallSteps],
+        apply[kMuSmallSteps];
+    double eps;
+    float scale, unscale;
+    int32_t steps, n;
+};
+static_assert(sizeof(MuSmalls) <= 4096, "kernel arguments");
+
+__device__ inline uint32_t mu_first_small(const MuSmalls& a, int k) { return a.s[k].first; }
+
+template <int MB> struct MuSmallLds {
+    enum {
+        B = 2 * MB,                       // blocks of 16 rows
+        S = B * (B + 1) / 2,              // of the lower triangle
+        kRow = 64 * MB + 8,               // bytes of a column on its way through LDS
+        kTurn = 2 * 32 * kRow,            // h and l of a wave's 32 columns
+        kPair = B * MB * 2048,            // A or P
+        kTurns = kMuSmallWaves * kTurn,
+        kSums = kMuSmallWaves / 2 * S * 1024,
+        kWork = kTurns > kSums ? kTurns : kSums,
+    };
+};
+
+// Block (bi, bj) of a symmetric matrix, rows 16 bi + 4 g + e of column 16 bj + (lane & 15), into
+// the operands, and mirrored.
+template <int MB>
+__device__ inline void mu_small_put(char* pair, int bi, int bj, Float4 v) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    Half4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        _Float16 x, y;
+        mu_split(v[e], &x, &y);
+        h[e] = x;
+        l[e] = y;
+    }
+    char* to = pair + (bj * MB + (bi >> 1)) * 2048 + lane * 16 + (bi & 1) * 8;
+    *(Half4*)to = h;
+    *(Half4*)(to + 1024) = l;
+    if (bi == bj) return;
+    to = pair + (bi * MB + (bj >> 1)) * 2048 + (4 * g + 16 * (c >> 2)) * 16 +
+         (4 * (bj & 1) + (c & 3)) * 2;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        *(_Float16*)(to + e * 16) = h[e];
+        *(_Float16*)(to + e * 16 + 1024) = l[e];
+    }
+}
+
+// Four neighbours in LDS of each lane: of 16 lanes, lane j gives the place of four of the 16
+// columns of row j >> 2 and gets its column's values of the four rows.
+__device__ inline Half4 mu_turned(const char* at) {
+    typedef short Short4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(Half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) Short4*)at));
+}
+
+// Sixteen values by their places; the type is asked for once, so that the loads go out together.
+__device__ inline void mu_gather(const void* p, int dtype, int64_t first, const int (&at)[16],
+                                 float (&v)[16]) {
+    if (dtype == kF32) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = ((const float*)p)[first + at[e]];
+    } else if (dtype == kBF16) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = (float)((const __bf16*)p)[first + at[e]];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = (float)((const _Float16*)p)[first + at[e]];
+    }
+}
+
+__device__ inline void mu_scatter(void* p, int dtype, int64_t first, const int (&at)[16],
+                                  const bool (&in)[16], const float (&v)[16]) {
+    if (dtype == kF32) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (in[e]) ((float*)p)[first + at[e]] = v[e];
+    } else if (dtype == kBF16) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (in[e]) ((__bf16*)p)[first + at[e]] = (__bf16)v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (in[e]) ((_Float16*)p)[first + at[e]] = (_Float16)v[e];
+    }
+}
+
+template <int MB, int C>
+__global__ __launch_bounds__(kMuSmallWaves * 64, 2) void k_mu_small(MuSmalls a) {
+    typedef MuSmallLds<MB> Z;
+    constexpr int B = Z::B, S = Z::S;
+    __shared__ __attribute__((aligned(16))) char lds[Z::kPair + Z::kWork];
+    __shared__ double norms[kMuSmallWaves];
+    char* const mat = lds;                 // A
+    char* const work = lds + Z::kPair;     // columns on their way, sums, P
+    const MuSmall& s = a.s[mu_find(a, a.n, mu_first_small)];
+    const int64_t first = (int64_t)(blockIdx.x - s.first) * s.rows * s.cols;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m = s.tall ? s.cols : s.rows, n = s.tall ? s.rows : s.cols;
+    // A wave's columns through LDS, whose rows of memory its lanes read side by side, 16 at a
+    // time: 32 lanes take neighbours, columns, or rows where X is tall.
+    char* const turn = work + wave * Z::kTurn;
+    constexpr int kFar = 2 * Z::kRow;   // bytes of a column of floats
+    const int fast = lane & 31, slow = lane >> 5;
+    float u[C][2][MB][8];
+    double sum = 0.0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int n0 = (c * kMuSmallWaves + wave) * 32;
+        if (n0 < n) {
+            for (int i = 0; i < 32 * MB; i += 32) {
+                int at[16], to[16];
+                bool in[16];
+                float v[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = i + 2 * e + slow;
+                    const int col = s.tall ? j & 31 : fast, row = s.tall ? (j & ~31) + fast : j;
+                    in[e] = row < m && n0 + col < n;
+                    at[e] = !in[e] ? 0 : s.tall ? (n0 + col) * s.cols + row : row * s.cols + n0 + col;
+                    to[e] = col * kFar + row * 4;
+                }
+                mu_gather(s.x, s.dtype, first, at, v);
+                if (s.momentum) {
+                    float q[16];
+                    mu_gather(s.momentum, kF32, 0, at, q);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        q[e] = __builtin_fmaf(s.mix, v[e] - q[e], q[e]);
+                        v[e] = mu_update(v[e], q[e], s.look);
+                        if (in[e]) s.momentum[at[e]] = q[e];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    v[e] = in[e] ? v[e] : 0.0f;
+                    sum = __builtin_fma((double)v[e], (double)v[e], sum);
+                    *(float*)(turn + to[e]) = v[e];
+                }
+            }
+        }
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int k = 0; k < MB; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    Float4 x = *(const Float4*)(turn + (16 * b + r) * kFar +
+                                                (32 * k + 16 * e + 4 * g) * 4);
+                    if (n0 >= n) x = Float4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) u[c][b][k][4 * e + i] = x[i];
+                }
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    for (int q = 1; q < 64; q <<= 1) sum += __shfl_xor(sum, q);
+    if (lane == 0) norms[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < kMuSmallWaves; ++w) sum += norms[w];
+    const double norm = sqrt(sum);
+    const double by = (double)a.scale / (norm < a.eps ? a.eps : norm);   // NaN stays
+    Half8 h[C][2][MB], l[C][2][MB];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int k = 0; k < MB; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    _Float16 x, y;
+                    mu_split((float)((double)u[c][b][k][i] * by), &x, &y);
+                    h[c][b][k][i] = x;
+                    l[c][b][k][i] = y;
+                }
+
+    for (int step = 0; step < a.steps; ++step) {
+        // A = X X^T: each wave's columns, then the waves' sums.
+        Float4 acc[S];
+#pragma unroll
+        for (int t = 0; t < S; ++t) acc[t] = Float4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if ((c * kMuSmallWaves + wave) * 32 >= n) continue;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int k = 0; k < MB; ++k)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        char* to = turn + (16 * b + r) * Z::kRow + (32 * k + 16 * e + 4 * g) * 2;
+                        const Half8 x = h[c][b][k], y = l[c][b][k];
+                        *(Half4*)to = Half4{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]};
+                        *(Half4*)(to + Z::kTurn / 2) =
+                            Half4{y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]};
+                    }
+            __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            Half8 fh[B], fl[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const char* from = turn + (4 * g + (r >> 2)) * Z::kRow + (16 * b + 4 * (r & 3)) * 2;
+                const Half4 h0 = mu_turned(from), h1 = mu_turned(from + 16 * Z::kRow);
+                const Half4 l0 = mu_turned(from + Z::kTurn / 2),
+                            l1 = mu_turned(from + Z::kTurn / 2 + 16 * Z::kRow);
+                fh[b] = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
+                fl[b] = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+#pragma unroll
+                for (int bi = 0; bi < B; ++bi)
+#pragma unroll
+                    for (int bj = 0; bj <= bi; ++bj) {
+                        Float4& t = acc[bi * (bi + 1) / 2 + bj];
+                        t = mu_mfma(q == 0 ? fl[bi] : fh[bi], q == 1 ? fl[bj] : fh[bj], t);
+                    }
+        }
+        __syncthreads();   // nothing is on its way any more
+        char* const mine = work + (wave & (kMuSmallWaves / 2 - 1)) * (S * 1024) + lane * 16;
+        const bool half = C == 1 && n <= kMuSmallWaves / 2 * 32;   // of the waves have columns
+        if (!half) {
+            if (wave >= kMuSmallWaves / 2) {
+#pragma unroll
+                for (int t = 0; t < S; ++t) *(Float4*)(mine + t * 1024) = acc[t];
+            }
+            __syncthreads();
+        }
+        if (wave < kMuSmallWaves / 2) {
+#pragma unroll
+            for (int t = 0; t < S; ++t) {
+                if (!half) acc[t] += *(const Float4*)(mine + t * 1024);
+                *(Float4*)(mine + t * 1024) = acc[t];
+            }
+        }
+        __syncthreads();
+        for (int t = wave; t < S; t += kMuSmallWaves) {
+            int bi, bj;
+            mu_triangle(t, &bi, &bj);
+            Float4 v = *(const Float4*)(work + t * 1024 + lane * 16);
+            for (int w = 1; w < kMuSmallWaves / 2; ++w)
+                v += *(const Float4*)(work + (w * S + t) * 1024 + lane * 16);
+            mu_small_put<MB>(mat, bi, bj, v * a.gram[step]);
+        }
+        __syncthreads();   // A is there, and the sums read: P takes their place
+        for (int t = wave; t < S; t += kMuSmallWaves) {
+            int bi, bj;
+            mu_triangle(t, &bi, &bj);
+            Float4 v{0.0f, 0.0f, 0.0f, 0.0f}, v1 = v, v2 = v;
+#pragma unroll
+            for (int k = 0; k < MB; ++k) {
+                const char* x = mat + (bi * MB + k) * 2048 + lane * 16;
+                const char* y = mat + (bj * MB + k) * 2048 + lane * 16;
+                const Half8 xh = *(const Half8*)x, xl = *(const Half8*)(x + 1024);
+                const Half8 yh = *(const Half8*)y, yl = *(const Half8*)(y + 1024);
+                v1 = mu_mfma(xl, yh, v1);
+                v2 = mu_mfma(xh, yl, v2);
+                v = mu_mfma(xh, yh, v);
+            }
+            v += v1 + v2;
+            const char* own = mat + (bj * MB + (bi >> 1)) * 2048 + lane * 16 + (bi & 1) * 8;
+            const Half4 oh = *(const Half4*)own, ol = *(const Half4*)(own + 1024);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = 16 * bi + 4 * g + e;
+                v[e] = v[e] * a.square[step] + a.linear[step] * ((float)oh[e] + (float)ol[e]);
+                if (row == 16 * bj + r && row < m) v[e] += a.one[step];
+            }
+            mu_small_put<MB>(work, bi, bj, v);
+        }
+        __syncthreads();
+        // X <- P X, where it is.
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if ((c * kMuSmallWaves + wave) * 32 >= n) continue;
+            Float4 y[2][B];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int t = 0; t < B; ++t) y[b][t] = Float4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < MB; ++k)
+#pragma unroll
+                for (int t = 0; t < B; t += 2) {
+                    Half8 ph[2], pl[2];
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        const char* p = work + ((t + d) * MB + k) * 2048 + lane * 16;
+                        ph[d] = *(const Half8*)p;
+                        pl[d] = *(const Half8*)(p + 1024);
+                    }
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+#pragma unroll
+                        for (int d = 0; d < 2; ++d)
+#pragma unroll
+                            for (int b = 0; b < 2; ++b)
+                                y[b][t + d] = mu_mfma(q == 0 ? pl[d] : ph[d],
+                                                      q == 1 ? l[c][b][k] : h[c][b][k], y[b][t + d]);
+                }
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int t = 0; t < B; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        _Float16 x, z;
+                        mu_split(y[b][t][e] * a.apply[step], &x, &z);
+                        h[c][b][t >> 1][4 * (t & 1) + e] = x;
+                        l[c][b][t >> 1][4 * (t & 1) + e] = z;
+                    }
+        }
+        __syncthreads();   // P is read
+    }
+
+    // Out as it came: the two halves hold a value to 2^-24.
+    float* const weights = s.dtype == kF32 ? (float*)s.out : s.master;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int n0 = (c * kMuSmallWaves + wave) * 32;
+        if (n0 >= n) continue;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int k = 0; k < MB; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    Float4 x;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        x[i] = ((float)h[c][b][k][4 * e + i] + (float)l[c][b][k][4 * e + i]) *
+                               a.unscale;
+                    *(Float4*)(turn + (16 * b + r) * kFar + (32 * k + 16 * e + 4 * g) * 4) = x;
+                }
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int i = 0; i < 32 * MB; i += 32) {
+            int at[16];
+            bool in[16];
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int j = i + 2 * e + slow;
+                const int col = s.tall ? j & 31 : fast, row = s.tall ? (j & ~31) + fast : j;
+                in[e] = row < m && n0 + col < n;
+                at[e] = !in[e] ? 0 : s.tall ? (n0 + col) * s.cols + row : row * s.cols + n0 + col;
+                v[e] = *(const float*)(turn + col * kFar + row * 4);
+            }
+            if (s.momentum) {
+                float w[16];
+                mu_gather(weights, kF32, 0, at, w);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    v[e] = __builtin_fmaf(-s.lr, v[e], w[e] * s.decay);
+                    if (in[e]) weights[at[e]] = v[e];
+                }
+                if (s.dtype == kF32) continue;
+            }
+            mu_scatter(s.out, s.dtype, first, at, in, v);
+        }
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
@@ -1191,6 +1626,78 @@ int mu_chunk(const MuChunk& chunk, const MuPlan& p, double eps, void* workspace,
     return ok ? CS_OK : CS_ERR_HIP;
 }
 
+// The columns that a workgroup of small matrices holds are 256 C.
+int mu_small_blocks(const MuEntry& e) { return (int)((std::min(e.rows, e.cols) + 31) / 32); }
+
+int mu_small_columns(const MuEntry& e) {
+    const int64_t need = (std::max(e.rows, e.cols) + 255) / 256;
+    return need <= 4 ? (int)need : 8;
+}
+
+// Registers hold 16 blocks of 32 rows by 32 C columns, halves of it, and the sums.
+bool mu_is_small(const MuEntry& e, const MuPlan& p) {
+    const int mb = mu_small_blocks(e);
+    return p.steps <= kMuSmallSteps && mb <= 3 &&
+           std::max(e.rows, e.cols) <= (mb == 1 ? 2048 : mb == 2 ? 1024 : 512);
+}
+
+template <int MB, int C>
+bool mu_small_launch(const MuSmalls& a, int64_t blocks, hipStream_t stream) {
+    hipLaunchKernelGGL((k_mu_small<MB, C>), dim3((unsigned)blocks), dim3(kMuSmallWaves * 64), 0,
+                       stream, a);
+    return mu_launched();
+}
+
+// All entries are small: a launch for each kind, of up to 20.
+int mu_small(const std::vector<MuEntry>& e, int n, const MuPlan& p, double eps,
+             hipStream_t stream) {
+    MuSmalls a{};
+    a.eps = eps;
+    a.steps = p.steps;
+    a.scale = (float)ldexp(1.0, mu_exponent(p.x[0]));
+    for (int k = 0; k < p.steps; ++k) {
+        const int ex = mu_exponent(p.x[k]), ea = mu_exponent(p.x[k] * p.x[k]);
+        const int ep = mu_exponent(mu_bound(p, p.x[k], false));
+        const int next = mu_exponent(p.x[k + 1]);
+        a.unscale = (float)ldexp(1.0, -next);
+        a.gram[k] = (float)ldexp(1.0, ea - 2 * ex);
+        a.square[k] = (float)ldexp(p.c, ep - 2 * ea);
+        a.linear[k] = (float)ldexp(p.b, ep - ea);
+        a.one[k] = (float)ldexp(p.a, ep);
+        a.apply[k] = (float)ldexp(1.0, next - ep - ex);
+    }
+    for (int mb = 1; mb <= 3; ++mb)
+        for (int c : {1, 2, 3, 4, 8}) {
+            int64_t blocks = 0;
+            a.n = 0;
+            for (int k = 0; k <= n; ++k) {
+                if (a.n == kMuMaxEntries || (k == n && a.n > 0)) {
+                    const bool ok =
+                        mb == 1 ? (c == 1   ? mu_small_launch<1, 1>(a, blocks, stream)
+                                   : c == 2 ? mu_small_launch<1, 2>(a, blocks, stream)
+                                   : c <= 4 ? mu_small_launch<1, 4>(a, blocks, stream)
+                                            : mu_small_launch<1, 8>(a, blocks, stream))
+                        : mb == 2 ? (c == 1   ? mu_small_launch<2, 1>(a, blocks, stream)
+                                     : c == 2 ? mu_small_launch<2, 2>(a, blocks, stream)
+                                     : c == 3 ? mu_small_launch<2, 3>(a, blocks, stream)
+                                              : mu_small_launch<2, 4>(a, blocks, stream))
+                                  : (c == 1 ? mu_small_launch<3, 1>(a, blocks, stream)
+                                            : mu_small_launch<3, 2>(a, blocks, stream));
+                    if (!ok) return CS_ERR_HIP;
+                    a.n = 0;
+                    blocks = 0;
+                }
+                if (k == n || mu_small_blocks(e[k]) != mb || mu_small_columns(e[k]) != c) continue;
+                MuSmall& s = a.s[a.n++];
+                s = MuSmall{e[k].x, e[k].out, e[k].master, e[k].momentum, (int32_t)e[k].rows,
+                            (int32_t)e[k].cols, (uint32_t)blocks, e[k].dtype,
+                            e[k].rows > e[k].cols, e[k].decay, e[k].lr, e[k].mix, e[k].look, 0};
+                blocks += e[k].count;
+            }
+        }
+    return CS_OK;
+}
+
 // Rows of the tables, checked: how many entries have anything, or -1.
 int mu_entries(int32_t ntensors, const int64_t* table, const float* scalars, bool muon,
                MuEntry* e) {
@@ -1240,7 +1747,6 @@ int mu_run(int32_t ntensors, const int64_t* table, const float* scalars, bool mu
     if (ntensors < 0 || (ntensors > 0 && (!table || (muon && !scalars))) || !(eps >= 0.0) ||
         !mu_plan(&p, steps, a, b, c))
         return CS_ERR_ARGS;
-    if (!bytes && ntensors > 0 && (!workspace || ((uintptr_t)workspace & 127))) return CS_ERR_ARGS;
     try {
         std::vector<MuEntry> e(ntensors + 1);
         const int n = mu_entries(ntensors, table, scalars, muon, e.data());
@@ -1250,6 +1756,10 @@ int mu_run(int32_t ntensors, const int64_t* table, const float* scalars, bool mu
             return std::max(x.rows, x.cols) > std::max(y.rows, y.cols);
         });
         if (bytes) *bytes = 0;
+        if (std::all_of(e.begin(), e.begin() + n,
+                        [&](const MuEntry& x) { return mu_is_small(x, p); }))
+            return bytes ? CS_OK : mu_small(e, n, p, eps, stream);
+        if (!bytes && (!workspace || ((uintptr_t)workspace & 127))) return CS_ERR_ARGS;
         MuChunk chunk;
         chunk.sched.reset(new MuSchedule[kMuMaxEntries]);
         for (int k = 0; k < n; k += kMuMaxEntries) {

@@ -22,7 +22,9 @@ HALF = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11
 SHAPES = [
     (1, 1), (1, 2), (2, 1), (1, 700), (700, 1), (2, 3), (5, 5), (31, 33), (63, 64), (64, 65),
     (96, 97), (127, 127), (128, 128), (129, 128), (128, 129), (130, 131), (64, 576), (576, 64),
-    (40, 3001), (3001, 40), (255, 257), (256, 512), (300, 1000), (1000, 130), (513, 520), (641, 2000),
+    (40, 3001), (3001, 40), (32, 256), (33, 257), (16, 500), (700, 20), (31, 1030), (2048, 30),
+    (2049, 30), (64, 512), (60, 768), (64, 769), (1024, 64), (64, 1025), (96, 256), (96, 257), (512, 90),
+    (96, 513), (97, 96), (255, 257), (256, 512), (300, 1000), (1000, 130), (513, 520), (641, 2000),
 ]
 
 

@@ -103,7 +103,7 @@ def test_checkpoints_are_taken_in_fp32_and_checked():
 
 def test_entries_check_their_tables():
     """None of these calls launches: the pointers are not looked at."""
-    good = [4096, 4096, 1, 0, 8, 8, 0, 0]
+    good = [4096, 4096, 1, 0, 200, 200, 0, 0]
     coeffs = (3.4445, -4.7750, 2.0315)
     lib = N.lib()
 
@@ -130,10 +130,10 @@ def test_entries_check_their_tables():
     N.call("cs_orthogonalize", 0, None, 5, *coeffs, 1e-7, None, None)
     call([0, 0, 0, 0, 8, 8, 0, 0])
     call([0, 0, 1, 0, 0, 8, 0, 0])
-    row = [4096, 4096, 0, 4096, 8, 8, 1, 0]
+    row = [4096, 4096, 0, 4096, 200, 200, 1, 0]
     numbers = np.zeros(4, np.float32)
-    for rows, scalars in ((row, numbers), ([4096, 4096, 0, 0, 8, 8, 0, 0], numbers),
-                          ([4096, 4096, 4096, 4096, 8, 8, 1, 0], None)):
+    for rows, scalars in ((row, numbers), ([4096, 4096, 0, 0, 200, 200, 0, 0], numbers),
+                          ([4096, 4096, 4096, 4096, 200, 200, 1, 0], None)):
         t = np.array([rows], dtype=np.int64)
         with pytest.raises(RuntimeError, match="invalid arguments"):
             N.call("cs_muon_step", 1, t.ctypes.data, None if scalars is None else scalars.ctypes.data,
@@ -143,3 +143,5 @@ def test_entries_check_their_tables():
     one = lib.cs_orthogonalize_workspace_bytes(1, t.ctypes.data, 5, *coeffs)
     two = lib.cs_orthogonalize_workspace_bytes(2, t.ctypes.data, 5, *coeffs)
     assert 0 < one < two
+    t = np.array([[4096, 4096, 5, 0, 64, 576, 0, 0]], dtype=np.int64)
+    assert lib.cs_orthogonalize_workspace_bytes(1, t.ctypes.data, 5, *coeffs) == 0
