@@ -20,6 +20,14 @@
 // computes from the coefficients alone, so that nothing leaves fp16's range.
 // A "pair" matrix holds, for 32 values of a row, their 32 h and then their 32 l (128
 // bytes), and is padded with zeros to whole tiles.
+//
+// Bound: three matrix instructions for each pair of 32 values. Measured (means of a kernel
+// trace): a 4096 x 4096 product 1.3 PFLOP/s of fp16 instructions with tiles of 256 (the matrix
+// cores are busy 68% of the clock that they leave, 1.8 to 2.05 GHz; an instruction loop without
+// operands' traffic reaches 2.3), a symmetric one 210 us with its sums cut in three, 272 whole.
+// The 18 matrices of an encoder 256 to 2048 wide take 12.0 ms a step, those of one 64 to 512 wide
+// 0.59 ms; a matrix of 1021 x 765 185 us, 17 launches of some 11 us, of which its products are
+// about half.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -1155,6 +1163,7 @@ struct MuPlan {
     int steps, phase;
     double a, b, c;
     double x[kMuMaxSteps + 1];
+    double p[kMuMaxSteps];   // bounds of P's
 };
 
 double mu_poly(const MuPlan& p, double s) { return p.a + s * s * (p.b + s * s * p.c); }
@@ -1179,15 +1188,20 @@ double mu_bound(const MuPlan& p, double s, bool odd) {
     return most * 1.01;   // the steps' own roundings
 }
 
-// What is below `bound` is held times 2^e: below 2^14, where fp16 ends at 2^16.
-int mu_exponent(double bound) { return 14 - (int)ceil(log2(std::max(bound, 1e-3))); }
+// What is below `bound` is held times 2^e: at most 2^14, where fp16 ends at 2^16.
+int mu_exponent(double bound) {
+    int e;
+    frexp(std::max(bound, 1e-3), &e);   // below 2^e
+    return 14 - e;
+}
 
 bool mu_plan(MuPlan* p, int steps, double a, double b, double c) {
     if (steps < 1 || steps > kMuMaxSteps || !(fabs(a) <= 64.0) || !(fabs(b) <= 64.0) ||
         !(fabs(c) <= 64.0))
         return false;
-    *p = MuPlan{steps, 1, a, b, c, {1.01}};
+    *p = MuPlan{steps, 1, a, b, c, {1.01}, {}};
     for (int k = 0; k < steps; ++k) {
+        p->p[k] = mu_bound(*p, p->x[k], false);
         p->x[k + 1] = mu_bound(*p, p->x[k], true);
         if (!(p->x[k + 1] <= 64.0)) return false;   // values that grow without end
     }
@@ -1230,15 +1244,16 @@ double mu_cost(int steps, int phase, double ratio) {
     return cost;
 }
 
-// Where an entry's matrices lie for a tile, from `base` on; the units that it takes.
-int64_t mu_layout(MuEntry* e, const MuPlan& p, int tile, int64_t base) {
+// Where an entry's matrices lie for a tile and phases of so many steps (where they save work),
+// from `base` on; the units that it takes.
+int64_t mu_layout(MuEntry* e, const MuPlan& p, int tile, int phase, int64_t base) {
     e->tall = e->rows > e->cols;
     e->m = e->tall ? e->cols : e->rows;
     e->n = e->tall ? e->rows : e->cols;
     e->mp = mu_round(e->m, tile);
     e->np = mu_round(e->n, tile);
     const double ratio = (double)e->np / (double)e->mp;
-    e->phase = mu_cost(p.steps, p.phase, ratio) < mu_cost(p.steps, 1, ratio) ? p.phase : 1;
+    e->phase = mu_cost(p.steps, phase, ratio) < mu_cost(p.steps, 1, ratio) ? phase : 1;
     const int64_t wide = 2 * e->mp * e->np / kMuUnit, square = 2 * e->mp * e->mp / kMuUnit;
     int64_t at = 0;
     // Each an even number of units, as partial sums behind them need it.
@@ -1277,7 +1292,7 @@ struct MuSchedule {
             sym(e, e.X, e.X, e.A, e.np, ea - 2 * ex);
             ++slots;
             for (int i = 0; i < len; ++i) {
-                const double x = p.x[k + i], bound = mu_bound(p, x, false);
+                const double x = p.x[k + i], bound = p.p[k + i];
                 const int ep = mu_exponent(bound);
                 const int64_t P = i == 0 ? e.Q[0] : e.P;
                 MuJob* j = sym(e, e.A, e.A, P, e.mp, 0);
@@ -1356,7 +1371,9 @@ int64_t mu_tiles(const MuOp& o, int tile) {
 
 // What a launch of products costs with a tile, in us, from measurements: `stage` values of k
 // take `us` where the CU's `resident` workgroups share it, and at least `alone`; a workgroup's
-// beginning and end take `ends`.
+// beginning and end take `ends`.  (Measured with one tile for all launches, 64 / 128 / 256:
+// 1021 x 765 216 / 449 / 1165 us; 4096 x 4096 6.9 / 4.1 / 4.0 ms; the encoder 64 wide 0.96 / 1.24
+// / 2.66 ms, 256 wide 21.9 / 13.8 / 13.0 ms; by these costs 0.22, 3.8, 0.59 and 12.0.)
 struct MuTileCost { int tile, stage, resident; double us, alone, ends; };
 const MuTileCost kMuTiles[] = {{64, 64, 1, 0.75, 0.65, 1.5}, {128, 32, 2, 1.4, 0.75, 4.0},
                                {256, 32, 1, 2.1, 2.1, 10.0}};
@@ -1383,13 +1400,14 @@ MuCut mu_cut(const MuOp* const* ops, const int64_t* counts, int n, int most_tile
         if (t.tile > most_tile) continue;
         MuCut c{&t, (int64_t)1 << 40, 0.0, 0};
         const double slots = kMuCus * t.resident;
-        int64_t longest = 0;
+        int64_t longest = 0, tiles[kMuMaxJobs];
         double work = 0.0;
         for (int i = 0; i < n; ++i) {
-            work += (double)mu_tiles(*ops[i], t.tile) * counts[i] * c.stages(ops[i]->job);
+            tiles[i] = mu_tiles(*ops[i], t.tile) * counts[i];
+            work += (double)(tiles[i] * c.stages(ops[i]->job));
             longest = std::max(longest, c.stages(ops[i]->job));
         }
-        for (int cuts = 1; cuts <= (may_split ? 32 : 1); cuts += 1 + cuts / 8) {
+        for (int cuts = 1; cuts <= (may_split ? 32 : 1); cuts += 1 + cuts / 4) {
             // Pieces as long as these cuts of the longest sum.
             c.piece = (longest + cuts - 1) / cuts;
             if (cuts > 1 && c.piece < 4) break;
@@ -1399,10 +1417,8 @@ MuCut mu_cut(const MuOp* const* ops, const int64_t* counts, int n, int most_tile
             for (int i = 0; i < n; ++i) {
                 const int64_t pieces = c.pieces(*ops[i]), st = c.stages(ops[i]->job);
                 piece = std::max(piece, (st + pieces - 1) / pieces);
-                blocks += (double)mu_tiles(*ops[i], t.tile) * counts[i] * pieces;
-                if (pieces > 1)
-                    c.partials += mu_tiles(*ops[i], t.tile) * counts[i] * pieces * t.tile *
-                                  t.tile / kMuUnit;
+                blocks += (double)(tiles[i] * pieces);
+                if (pieces > 1) c.partials += tiles[i] * pieces * (t.tile * t.tile / kMuUnit);
             }
             // Rounds of the longest pieces; pieces of all lengths fill the last round better.
             double rounds = work / (double)piece / slots, last = 0.0;
@@ -1484,7 +1500,7 @@ bool mu_last(const MuLasts& a, int64_t blocks, hipStream_t stream) {
 // Entries whose launches are shared: what they are padded to, and their launches.
 struct MuChunk {
     MuEntry* e;
-    int n, pad;
+    int n, pad, phase;
     double us;
     int64_t units;      // of halves; behind them the partial sums of products, and of norms
     int64_t partials, parts;
@@ -1493,13 +1509,14 @@ struct MuChunk {
 
     int64_t bytes() const { return (units * 2 + partials * 4) * kMuUnit + parts * 8; }
 
-    void lay(const MuPlan& p, int pad_of) {
+    void lay(const MuPlan& p, int pad_of, int phase_of) {
         pad = pad_of;
+        phase = phase_of;
         units = partials = parts = 0;
         int slots = 0;
         us = 0.0;
         for (int k = 0; k < n; ++k) {
-            units += mu_layout(e + k, p, pad, units);
+            units += mu_layout(e + k, p, pad, phase, units);
             parts += e[k].count * kMuParts;
             sched[k].make(e[k], p);
             slots = std::max(slots, sched[k].slots);
@@ -1521,18 +1538,21 @@ struct MuChunk {
         }
     }
 
-    // The padding that costs least.
+    // The padding that costs least, and phases or steps on X: phases save work where X is long,
+    // steps on X launches.
     void choose(const MuPlan& p) {
-        int best = 0;
+        int best_pad = 0, best_phase = p.phase;
         double least = 1e30;
-        for (const MuTileCost& t : kMuTiles) {
-            lay(p, t.tile);
-            if (us < least) {
-                least = us;
-                best = t.tile;
-            }
-        }
-        if (best != pad) lay(p, best);
+        auto look = [&](int tile, int by) {
+            lay(p, tile, by);
+            if (us >= least) return;
+            least = us;
+            best_pad = tile;
+            best_phase = by;
+        };
+        for (const MuTileCost& t : kMuTiles) look(t.tile, p.phase);
+        if (p.phase > 1) look(best_pad, 1);
+        if (best_pad != pad || best_phase != phase) lay(p, best_pad, best_phase);
     }
 };
 
@@ -1634,7 +1654,8 @@ int mu_small_columns(const MuEntry& e) {
     return need <= 4 ? (int)need : 8;
 }
 
-// Registers hold 16 blocks of 32 rows by 32 C columns, halves of it, and the sums.
+// What the registers hold beside the sums.  (64 x 576 takes 60 us for 96 in launches of products,
+// 24 x 96 x 97 45 for 105.)
 bool mu_is_small(const MuEntry& e, const MuPlan& p) {
     const int mb = mu_small_blocks(e);
     return p.steps <= kMuSmallSteps && mb <= 3 &&
@@ -1657,7 +1678,7 @@ int mu_small(const std::vector<MuEntry>& e, int n, const MuPlan& p, double eps,
     a.scale = (float)ldexp(1.0, mu_exponent(p.x[0]));
     for (int k = 0; k < p.steps; ++k) {
         const int ex = mu_exponent(p.x[k]), ea = mu_exponent(p.x[k] * p.x[k]);
-        const int ep = mu_exponent(mu_bound(p, p.x[k], false));
+        const int ep = mu_exponent(p.p[k]);
         const int next = mu_exponent(p.x[k + 1]);
         a.unscale = (float)ldexp(1.0, -next);
         a.gram[k] = (float)ldexp(1.0, ea - 2 * ex);
