@@ -7,7 +7,8 @@ each with ``repo_amd.norm.GroupNorm`` and its SiLU behind it.  Its head gives
 eight rings of ten control points, with colours and opacities, for each 16 x 16
 pixels; the renderer turns them into an image, and the loss (MSE and SSIM) goes
 back through it into the weights, which ``repo_amd.optim.AdamW`` moves with a global-norm clip and
-8-bit states.  The images are synthetic: discs of random places and colours.
+8-bit states; with ``--muon`` the filters and the head's matrix are moved by ``repo_amd.optim.Muon``
+instead.  The images are synthetic: discs of random places and colours.
 """
 from __future__ import annotations
 
@@ -25,7 +26,7 @@ if ROOT not in sys.path:
 import manbo  # noqa: E402
 from repo_amd import fused  # noqa: E402
 from repo_amd.norm import GroupNorm  # noqa: E402
-from repo_amd.optim import AdamW  # noqa: E402
+from repo_amd.optim import AdamW, Muon  # noqa: E402
 
 POINTS, SUBDIV, SAMPLES = 10, 2, 8
 
@@ -102,25 +103,30 @@ def render(points, colours, opacities, size):
 
 
 def train(steps=200, size=128, batch=4, width=32, state_bits=8, lr=2e-3, seed=0,
-          device="cuda", report=None):
-    """The trained encoder, its optimizer and the loss of each step."""
+          device="cuda", report=None, muon=False):
+    """The trained encoder, its optimizer (AdamW's part of it) and the loss of each step."""
     torch.manual_seed(seed)
     generator = torch.Generator(device).manual_seed(seed)
     encoder = Encoder(width).to(device)
     decay = [p for p in encoder.parameters() if p.dim() > 1]
     keep = [p for p in encoder.parameters() if p.dim() <= 1]
-    opt = AdamW([{"params": decay}, {"params": keep, "weight_decay": 0.0}], lr=lr,
-                state_bits=state_bits, max_grad_norm=1.0, seed=seed)
+    groups = [{"params": decay}, {"params": keep, "weight_decay": 0.0}]
+    opt = AdamW(groups[1:] if muon else groups, lr=lr, state_bits=state_bits, max_grad_norm=1.0,
+                seed=seed)
+    # An update as long as AdamW's, so that one learning rate does for both.
+    matrices = Muon(decay, lr=lr, weight_decay=1e-2, adjust_lr_fn="match_rms_adamw") if muon else None
     losses = []
     for step in range(steps):
         images = discs(batch, size, generator, device)
-        opt.zero_grad()
+        encoder.zero_grad()
         total = 0.0
         for image, *answer in zip(images, *encoder(images)):
             loss, _ = fused.clamp_mse_ssim_loss(render(*answer, size), image.unsqueeze(0))
             total = total + loss / batch
         total.backward()
         opt.step()
+        if muon:
+            matrices.step()
         losses.append(total.detach())
         if report and (step + 1) % report == 0:
             print(f"step {step + 1}: loss {losses[-1].item():.4f}, gradient norm "
@@ -137,8 +143,9 @@ def main():
     ap.add_argument("--state-bits", type=int, default=8, choices=(8, 32))
     ap.add_argument("--lr", type=float, default=2e-3)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--muon", action="store_true")
     a = ap.parse_args()
-    train(a.steps, a.size, a.batch, a.width, a.state_bits, a.lr, a.seed, report=20)
+    train(a.steps, a.size, a.batch, a.width, a.state_bits, a.lr, a.seed, report=20, muon=a.muon)
 
 
 if __name__ == "__main__":
