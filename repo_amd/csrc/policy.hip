@@ -10,8 +10,9 @@
 //   dL/dz_j = dL/dl (delta_ja - exp(z_j / T) / sum) / T
 // The loss is the sum of w L over the rows that the mask leaves.
 //
-// Exponentials are powers of two: with k = log2(e) / T and c = max(z) k, both
-// rounded to fp32, s = sum_j 2^(z_j k - c), each difference one fused operation.
+// Exponentials are powers of two: with k = log2(e) / T in fp32 and c = max(z),
+// s = sum_j 2^((z_j - c) k).  The difference comes first: z k of a type's lowest value, which
+// masks use, has no fp32 value.
 // What follows once a row (l, the ratio, the KL term, the slopes) is in fp64: d and
 // l - old are differences of numbers of size 10, and exp(d) - d - 1 of a small d
 // has no digits left in fp32.  Sums over rows are in fp64 and of a fixed order.
@@ -90,14 +91,18 @@ __device__ inline void pl_put(T* p, const PlVec<T>& x) {
     *reinterpret_cast<PlAny*>(p) = __builtin_bit_cast(PlFour, x);
 }
 
-struct PlSum { float c, s; };   // sum of 2^(z k - c), c the largest z k
+struct PlSum { float c, s; };   // sum of 2^((z - c) k), c the largest z
 
-__device__ inline PlSum pl_join(PlSum a, PlSum b) {
-    // No value seen yet: c = -inf and s = 0.
+__device__ inline float pl_power(float z, float c, float k) {
+    return __builtin_amdgcn_exp2f((z - c) * k);
+}
+
+__device__ inline PlSum pl_join(PlSum a, PlSum b, float k) {
+    // No value seen yet, or -inf alone: c = -inf and s = 0.
     if (a.s == 0.0f && a.c == -INFINITY) return b;
     if (b.s == 0.0f && b.c == -INFINITY) return a;
     const float c = __builtin_fmaxf(a.c, b.c);
-    return {c, a.s * __builtin_amdgcn_exp2f(a.c - c) + b.s * __builtin_amdgcn_exp2f(b.c - c)};
+    return {c, a.s * pl_power(a.c, c, k) + b.s * pl_power(b.c, c, k)};
 }
 
 // N values more.  While -inf alone has been seen the sum stays empty: a row of it has
@@ -107,14 +112,13 @@ __device__ inline void pl_add(PlSum& a, const float (&z)[N], float k) {
     float most = z[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) most = __builtin_fmaxf(most, z[i]);
-    most *= k;
     if (most > a.c) {
-        a.s *= __builtin_amdgcn_exp2f(a.c - most);
+        a.s *= pl_power(a.c, most, k);
         a.c = most;
     }
     const float c = a.c == -INFINITY ? 0.0f : a.c;
 #pragma unroll
-    for (int i = 0; i < N; ++i) a.s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], k, -c));
+    for (int i = 0; i < N; ++i) a.s += pl_power(z[i], c, k);
 }
 
 // The THREADS threads of a row: a wave, or a whole workgroup.
@@ -159,9 +163,9 @@ struct PlTeam {
         }
         return x;
     }
-    __device__ PlSum join(PlSum a) const {
+    __device__ PlSum join(PlSum a, float k) const {
         for (int m = 1; m < 64; m <<= 1)
-            a = pl_join(a, {__shfl_xor(a.c, m), __shfl_xor(a.s, m)});
+            a = pl_join(a, {__shfl_xor(a.c, m), __shfl_xor(a.s, m)}, k);
         if (THREADS > 64) {
             if ((threadIdx.x & 63) == 0) {
                 lds->c[threadIdx.x >> 6] = a.c;
@@ -169,7 +173,7 @@ struct PlTeam {
             }
             __syncthreads();
             a = {lds->c[0], lds->s[0]};
-            for (int w = 1; w < THREADS / 64; ++w) a = pl_join(a, {lds->c[w], lds->s[w]});
+            for (int w = 1; w < THREADS / 64; ++w) a = pl_join(a, {lds->c[w], lds->s[w]}, k);
         }
         return a;
     }
@@ -219,7 +223,7 @@ __device__ inline double pl_log(float s) {
 
 // l of a row, of whose token `chosen` is the logit (NaN for a token outside the vocabulary).
 __device__ inline double pl_logprob(const PlRows& a, float chosen, PlSum sum) {
-    const double l = ((double)chosen * (double)a.k - (double)sum.c) * kLn2 - pl_log(sum.s);
+    const double l = ((double)chosen - (double)sum.c) * a.inv_t - pl_log(sum.s);
     return l > 0.0 ? 0.0 : l;   // s is rounded, a probability is at most 1
 }
 
@@ -250,7 +254,7 @@ struct PlRow {
     }
 };
 
-// What a row's gradient slope (delta_ja - p_j) / T is made of: q 2^(z_j k - c), and `own` at its
+// What a row's gradient slope (delta_ja - p_j) / T is made of: q 2^((z_j - c) k), and `own` at its
 // token, 1 - p without the difference.  none: zeros, and nothing of the row is read.
 struct PlSlope {
     float q, own, c;
@@ -269,7 +273,7 @@ __device__ inline PlVec<T> pl_slopes(const PlVec<T>& x, const PlSlope& g, float 
     PlVec<T> y;
 #pragma unroll
     for (int i = 0; i < PlVec<T>::n; ++i)
-        y.v[i] = (T)(g.q * __builtin_amdgcn_exp2f(__builtin_fmaf((float)x.v[i], k, -g.c)));
+        y.v[i] = (T)(g.q * pl_power((float)x.v[i], g.c, k));
     return y;
 }
 
@@ -277,7 +281,7 @@ template <typename T>
 __device__ inline T pl_slope_of(float z, const PlSlope& g, float k, bool own) {
     return (T)(own ? g.own
                : g.none ? 0.0f
-                        : g.q * __builtin_amdgcn_exp2f(__builtin_fmaf(z, k, -g.c)));
+                        : g.q * pl_power(z, g.c, k));
 }
 
 // A row is whole vectors and less than one of single values, which the first threads take.
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(PlTeam<THREADS>::kBlock, THREADS == 1024 ? 8 : 4) v
                 const float v[1] = {(float)z[tail.at()]};
                 pl_add(sum, v, a.k);
             }
-            sum = team.join(sum);
+            sum = team.join(sum, a.k);
         }
         const PlSlope g = pl_row_done<THREADS, LOSS>(a, f, o, team, r, row, sum);
         if (LOSS && o.grad) pl_gradient<T, THREADS>(a, z, (T*)o.grad + r * a.vocab, row.token, g);
@@ -466,15 +470,15 @@ __global__ __launch_bounds__(PlTeam<THREADS>::kBlock, 4) void k_rows_held(PlRows
 #pragma unroll
                 for (int i = 0; i < V; ++i) most = __builtin_fmaxf(most, (float)v.v[i]);
             }
-            sum.c = team.most(most) * a.k;
+            sum.c = team.most(most);
             const float c = sum.c == -INFINITY ? 0.0f : sum.c;
-            sum.s = __builtin_amdgcn_exp2f(__builtin_fmaf(last, a.k, -c));
+            sum.s = pl_power(last, c, a.k);
 #pragma unroll
             for (int n = 0; n < N; ++n) {
                 const PlVec<T> v = pl_anew<T>(x[n]);
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    sum.s += __builtin_amdgcn_exp2f(__builtin_fmaf((float)v.v[i], a.k, -c));
+                    sum.s += pl_power((float)v.v[i], c, a.k);
             }
             sum.s = team.sum(sum.s);
         }

@@ -4,7 +4,7 @@ sizes, strides, masks that leave a row or everything out, values that are not fi
 tokens outside the vocabulary, extreme ratios, other streams, graphs, far offsets.
 
 Tolerances, with u = 2^-24.  A term 2^(z k - c) of the sum has a relative error of at most
-  u |z k - c| ln 2  (its argument's rounding) + 3 u  (the hardware's exponential, 1 ulp),
+  2 u |z - c| / T  (its argument's roundings) + 3 u  (the hardware's exponential, 1 ulp),
 rescaled at most 40 times (2 u each) and added at most V / 64 + 40 times (u each); k is
 rounded, which stands for another temperature: u (max z - min z) / T.  With R = (max z -
 min z) / T over the finite logits
@@ -319,6 +319,35 @@ def test_infinite_logits(vocab, dtype):
         assert torch.isnan(lp[r]) and torch.isnan(grad[r]).any()
     assert float(lp[4]) == float("-inf")
     assert float(lp[5]) == 0.0 and not grad[5].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [9, 515, 3001, 70001, 140001])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_a_types_lowest_values(dtype, vocab):
+    """Masks of the vocabulary by the type's lowest value: those tokens have no probability, and a
+    row of them alone has one distribution, the uniform."""
+    from repo_amd.policy import token_logprobs
+    z, tokens, _, up = _inputs((4,), vocab, DTYPES[dtype], seed=31)
+    low = torch.finfo(DTYPES[dtype]).min
+    z[0, 1::2] = low
+    tokens[0] = 0
+    z[1] = low
+    z[2] = -low
+    z[3, tokens[3]] = low
+    for temperature in (1.0, 0.5):
+        leaf = z.detach().requires_grad_()
+        lp = token_logprobs(leaf, tokens, temperature=temperature)
+        grad, = torch.autograd.grad(lp, leaf, up)
+        assert torch.isfinite(grad).all() and torch.isfinite(lp[:3]).all()
+        keep = z[:1, ::2].contiguous()
+        want = O.token_logprobs64(_np(keep), np.zeros(1, np.int64), None, temperature)
+        assert abs(float(lp[0]) - want[0]) <= _lp_bound(keep, want, temperature)[0]
+        assert not grad[0, 1::2].any()
+        even = -np.log(vocab)
+        for r in (1, 2):
+            assert abs(float(lp[r]) - even) <= U * (130 + vocab / 64 + abs(even))
+        assert float(lp[3]) < -1e4
 
 
 @pytest.mark.gpu
