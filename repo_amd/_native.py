@@ -27,7 +27,7 @@ RASTER_LOG_BLOCK_BYTES = 2048  # log pool reserved per wave at a time
 EDGE_AUX_INTS = 4        # 16-byte (segment, t0, t1) record of the adaptive flattening
 ADAMW_BLOCK = 128        # values that share an exponent in the 8-bit optimizer states
 GRAD_NORM_BLOCKS = 2048  # partial sums of the gradients' norm (and one a tensor)
-MUON_MAX_PATCHES = 524288  # 64 x 64 patches of one row of the Muon entry points' tables
+MUON_MAX_PATCHES = 262144  # 64 x 64 patches of one row of the Muon entry points' tables
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32

@@ -54,7 +54,7 @@ constexpr int kMuUnit = 4096;      // halves, or floats of partial sums, that of
 constexpr int kMuMaxSteps = 64;
 constexpr int kMuMostTile = 256;
 constexpr int64_t kMuMaxPatches = CS_MUON_MAX_PATCHES;
-static_assert(kMuMaxPatches * kMuMaxEntries * kMuThreads < ((int64_t)1 << 32), "a launch's threads");
+static_assert(kMuMaxPatches * kMuMaxEntries * 512 < ((int64_t)1 << 32), "a launch's threads");
 
 typedef _Float16 Half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 Half4 __attribute__((ext_vector_type(4)));

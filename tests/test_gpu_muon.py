@@ -134,6 +134,17 @@ def test_stacks(shape, dtype):
 
 
 @pytest.mark.gpu
+def test_more_matrices_than_a_call_takes():
+    """16384 of up to 256 x 256 are as many as a call may have."""
+    from repo_amd.optim import orthogonalize
+    for shape in ((20000, 2, 3), (16400, 100, 40)):
+        x = _random(shape, torch.bfloat16, seed=11)
+        y = orthogonalize(x)
+        for k in (0, 16383, 16384, shape[0] - 1):
+            _check(x[k], y[k])
+
+
+@pytest.mark.gpu
 def test_layouts():
     from repo_amd.optim import orthogonalize
     wide = _random((5, 140, 150), seed=6)
