@@ -33,8 +33,8 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <exception>
 #include <memory>
-#include <new>
 #include <vector>
 
 #include "../../include/cubicsplat_hip.h"
@@ -1769,7 +1769,7 @@ int mu_run(int32_t ntensors, const int64_t* table, const float* scalars, bool mu
         !mu_plan(&p, steps, a, b, c))
         return CS_ERR_ARGS;
     try {
-        std::vector<MuEntry> e(ntensors + 1);
+        std::vector<MuEntry> e((size_t)ntensors + 1);
         const int n = mu_entries(ntensors, table, scalars, muon, e.data());
         if (n < 0) return CS_ERR_ARGS;
         // The longest sums first: they end last.
@@ -1795,7 +1795,7 @@ int mu_run(int32_t ntensors, const int64_t* table, const float* scalars, bool mu
                 if (rc != CS_OK) return rc;
             }
         }
-    } catch (const std::bad_alloc&) {
+    } catch (const std::exception&) {   // of memory or lengths
         return CS_ERR_ARGS;
     }
     return CS_OK;

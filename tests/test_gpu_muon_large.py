@@ -93,3 +93,13 @@ def test_steps_over_lists(shapes, dtype):
         _check(p.grad, master.double() / -by, 4 * U)
         assert torch.equal(p.detach(), master.to(dtype))
         assert torch.equal(opt.state[p]["momentum_buffer"], p.grad.float())
+
+
+@pytest.mark.gpu
+def test_the_largest_matrix():
+    """As many values as a call takes: their pairs' addresses and the halves' numbers pass 2^31."""
+    from repo_amd.optim import orthogonalize
+    x = _random((1 << 20, 1024), torch.bfloat16, 0)
+    _check(x, orthogonalize(x), HALF[x.dtype])
+    with pytest.raises(ValueError, match="too large"):
+        orthogonalize(torch.empty((1 << 20, 1025), dtype=torch.bfloat16, device="cuda"))
