@@ -1280,7 +1280,7 @@ class Muon(torch.optim.Optimizer):
     such deletes ``state[p]["master"]``).
 
     Up to 20 parameters share each launch.  A step can be captured in a graph, with the numbers of its
-    groups as they are then."""
+    groups as they are then, once an eager step has made the states."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
                  ns_coefficients=_NS_COEFFICIENTS, eps=1e-7, ns_steps=5, adjust_lr_fn=None):
@@ -1410,12 +1410,16 @@ class Muon(torch.optim.Optimizer):
     def _ready(self, p):
         """p's state, made where there is none, and in step with p."""
         st = self.state[p]
-        if "momentum_buffer" not in st:
-            st["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32,
-                                                     memory_format=torch.preserve_format)
         names = ["momentum_buffer"]
         if p.dtype is not torch.float32:
             names.append("master")
+        if any(n not in st for n in names) and torch._C._cuda_isCurrentStreamCapturing():
+            raise RuntimeError("a captured Muon step would make its states anew in each replay: "
+                               "make one step before")
+        if "momentum_buffer" not in st:
+            st["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32,
+                                                     memory_format=torch.preserve_format)
+        if len(names) > 1:
             if "master" not in st:
                 st["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
                 self._wrote(p)

@@ -447,6 +447,24 @@ def test_captured_graphs_follow_their_inputs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_a_captured_step_makes_no_states(dtype, monkeypatch):
+    """They would be made anew, momentum zero, in each replay."""
+    from repo_amd.optim import Muon
+    p = _random((70, 90), DTYPES[dtype]).requires_grad_()
+    p.grad = _random((70, 90), DTYPES[dtype], seed=1)
+    opt = Muon([p])
+    kept = p.detach().clone()
+    with monkeypatch.context() as m:
+        m.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: True)
+        with pytest.raises(RuntimeError, match="make one step before"):
+            opt.step()
+    assert torch.equal(p, kept)
+    opt.step()
+    assert not torch.equal(p, kept)
+
+
+@pytest.mark.gpu
 def test_profile_labels():
     from contextlib import contextmanager
     from repo_amd import _native as N
