@@ -24,10 +24,10 @@
 // Bound: three matrix instructions for each pair of 32 values. Measured (means of a kernel
 // trace): a 4096 x 4096 product 1.3 PFLOP/s of fp16 instructions with tiles of 256 (the matrix
 // cores are busy 68% of the clock that they leave, 1.8 to 2.05 GHz; an instruction loop without
-// operands' traffic reaches 2.3), a symmetric one 210 us with its sums cut in three, 272 whole.
-// The 18 matrices of an encoder 256 to 2048 wide take 12.0 ms a step, those of one 64 to 512 wide
-// 0.59 ms; a matrix of 1021 x 765 185 us, 17 launches of some 11 us, of which its products are
-// about half.
+// operands' traffic reaches 2.3), a symmetric one 191 us and 34 to join its sums, cut in three, 272
+// whole.  The 18 matrices of an encoder 256 to 2048 wide take 12.0 ms a step, those of one 64 to 512
+// wide 0.6 ms; a matrix of 1021 x 765 185 us, 17 launches of some 11 us, of which loads alone and
+// products alone take 9 to 10 each.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
