@@ -20,10 +20,10 @@
 // Bound: HBM, the logits read once and the gradient written once.  The loss makes the
 // gradient for an incoming one while the row is in registers (a second launch in the
 // backward pass finds that one and ends, or makes another's from the logits): a wave holds
-// rows up to 4 KB, a workgroup up to 128 KB.  Longer rows are read twice, by workgroups of
-// 1024 threads, so that the rows in flight stay in the memory-side cache (of 256 threads:
-// 1008 us for 890).  Measured: 16x512x32768 bf16, 0.7 of the rows counting, loss and
-// gradient 194 us (913 MB at 4.7 TB/s), 8x1024x131072 914 us (3.65 GB, 4.0 TB/s); scoring
+// rows up to 8 KB, a workgroup up to 64 KB.  Longer rows are read twice, those above 160 KB by
+// workgroups of 1024 threads, so that the rows in flight stay in the memory-side cache (8192 of 256
+// KB: 1008 us of 256 threads for 890).  Measured: 16x512x32768 bf16, 0.7 of the rows counting, loss
+// and gradient 194 us (913 MB at 4.7 TB/s), 8x1024x131072 914 us (3.65 GB, 4.0 TB/s); scoring
 // 16x511x32768 67 us (375 MB, 5.6 TB/s).  Writing past the caches was slower (by 16 and 36 us).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -646,19 +646,33 @@ bool pl_rows_held(const PlRows& a, const PlLoss& f, const PlOut& o, hipStream_t 
     return true;
 }
 
-// The fewest threads that hold a row: a wave, or a workgroup.
+template <typename T, bool LOSS, int THREADS>
+void pl_rows_twice(const PlRows& a, const PlLoss& f, const PlOut& o, hipStream_t stream) {
+    hipLaunchKernelGGL((k_rows<T, THREADS, LOSS>), pl_grid<THREADS>(a), dim3(THREADS), 0, stream, a,
+                       f, o);
+}
+
+// The fewest threads that hold a row, as what a row costs besides its values (its arithmetic, the
+// workgroup's barriers) is theirs: bf16, 32768 rows of 4096, loss / scoring, us: a wave 107 / 40, 128
+// threads 106 / 41, 256 131 / 55, 512 by the longer rows' kernel 244 / 168.  Two to four thousand
+// vectors, 10920 rows of 24576: 512 threads that hold them 199 / 96, 256 that read twice 201 / 92
+// (13416 of 20000: 223 / 113, 207 / 93; 8192 of 32768: 186 / 86, 197 / 93).  Longer rows, 5456 of
+// 49152: 512 threads that read twice 196 / 94, 1024 227 / 127, 1024 that hold them 237 / 162; 1336 of
+// 200000: 512 229 / 102, 1024 223 / 103.
 template <typename T, bool LOSS>
 void pl_run_rows(const PlRows& a, const PlLoss& f, const PlOut& o, hipStream_t stream) {
+    const int64_t vectors = a.vocab / PlVec<T>::n;
     if (pl_rows_held<T, LOSS, 64, 1>(a, f, o, stream) ||
         pl_rows_held<T, LOSS, 64, 2>(a, f, o, stream) ||
         pl_rows_held<T, LOSS, 64, 4>(a, f, o, stream) ||
-        pl_rows_held<T, LOSS, 256, 2>(a, f, o, stream) ||
-        pl_rows_held<T, LOSS, 256, 4>(a, f, o, stream) ||
-        pl_rows_held<T, LOSS, 512, 4>(a, f, o, stream) ||
-        pl_rows_held<T, LOSS, 512, 8>(a, f, o, stream) ||
-        pl_rows_held<T, LOSS, 1024, 8>(a, f, o, stream))
+        pl_rows_held<T, LOSS, 64, 8>(a, f, o, stream) ||
+        pl_rows_held<T, LOSS, 128, 8>(a, f, o, stream) ||
+        pl_rows_held<T, LOSS, 256, 8>(a, f, o, stream))
         return;
-    hipLaunchKernelGGL((k_rows<T, 1024, LOSS>), pl_grid<1024>(a), dim3(1024), 0, stream, a, f, o);
+    if (vectors <= 3000) pl_rows_twice<T, LOSS, 256>(a, f, o, stream);
+    else if (pl_rows_held<T, LOSS, 512, 8>(a, f, o, stream)) return;
+    else if (!LOSS || vectors <= 10240) pl_rows_twice<T, LOSS, 512>(a, f, o, stream);
+    else pl_rows_twice<T, LOSS, 1024>(a, f, o, stream);
 }
 
 template <typename T, int THREADS>

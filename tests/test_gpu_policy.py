@@ -30,7 +30,7 @@ SHAPES = [
     ((), 7), ((1,), 1), ((3,), 2), ((2, 3), 3), ((5, 7), 8), ((1, 1), 9), ((2, 2), 63), ((2, 2), 64),
     ((3, 2), 65), ((2, 3), 255), ((3, 5), 257), ((12, 33), 515), ((4, 9), 1037), ((2, 2, 3), 1024),
     ((2, 3), 2047), ((2, 3), 2048), ((2, 3), 2049), ((1, 3), 4097), ((3, 3), 8192), ((2, 3), 8200),
-    ((1, 5), 16384), ((1, 3), 16391), ((1, 3), 32768), ((2, 2), 32771), ((1, 2), 65536),
+    ((1, 5), 16384), ((1, 3), 16391), ((2, 3), 20011), ((1, 3), 25003), ((1, 3), 32768), ((2, 2), 32771), ((1, 2), 65536),
     ((1, 2), 65543), ((1, 2), 131072), ((1, 2), 131075), ((1, 2), 200001), ((300, 2), 40),
 ]
 
