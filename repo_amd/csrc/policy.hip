@@ -23,8 +23,8 @@
 // rows up to 8 KB, a workgroup up to 64 KB.  Longer rows are read twice, those above 160 KB by
 // workgroups of 1024 threads, so that the rows in flight stay in the memory-side cache (8192 of 256
 // KB: 1008 us of 256 threads for 890).  Measured: 16x512x32768 bf16, 0.7 of the rows counting, loss
-// and gradient 194 us (913 MB at 4.7 TB/s), 8x1024x131072 914 us (3.65 GB, 4.0 TB/s); scoring
-// 16x511x32768 67 us (375 MB, 5.6 TB/s).  Writing past the caches was slower (by 16 and 36 us).
+// and gradient 194 us (913 MB at 4.7 TB/s), 8x1024x131072 914 to 949 us (3.65 GB, 3.9 TB/s); scoring
+// 16x511x32768 68 us (375 MB, 5.6 TB/s).  Writing past the caches was slower (by 16 and 36 us).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -13,6 +13,15 @@ U = 2.0 ** -24
 HALF = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 
 
+@pytest.fixture(scope="module", autouse=True)
+def _memory_given_back():
+    """The tests behind these find the allocator as they would without them."""
+    yield
+    if torch.cuda.is_available():
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+
+
 def _steps(x, dtype, steps=5, coefficients=(3.4445, -4.7750, 2.0315)):
     """The steps with torch's products, matrix by matrix; the scale from float64."""
     if x.dim() > 2:
