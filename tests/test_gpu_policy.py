@@ -35,6 +35,15 @@ SHAPES = [
 ]
 
 
+@pytest.fixture(scope="module", autouse=True)
+def _memory_given_back():
+    """The tests behind these find the allocator as they would without them."""
+    yield
+    if torch.cuda.is_available():
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+
+
 def _np(t):
     return t.detach().double().cpu().numpy()
 
@@ -196,6 +205,24 @@ def test_other_forms():
 def test_other_incoming_gradients_are_not_rounded_twice(factor):
     z, tokens, mask, adv, old, ref = _policy_inputs((4, 6), 517, torch.bfloat16, seed=11)
     _check_policy(z, tokens, mask, adv, old, ref, factor=factor)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(9001, 41), (2100, 5003), (1030, 16400), (530, 65600)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_more_rows_than_the_backward_launches_workgroups_for(rows, vocab, dtype):
+    """It takes rows in turns where its factor most likely is one.  Half a gradient is half of every
+    number that it is made of, as with a scale of a half."""
+    from repo_amd.policy import policy_loss
+    z, tokens, mask, _ = _inputs((rows, 1), vocab, DTYPES[dtype], seed=5)
+    z.requires_grad_()
+    adv = torch.randn(rows, 1, device="cuda")
+    old = -torch.rand(rows, 1, device="cuda") * 3
+    grads = []
+    for scale, factor in ((0.5, 1.0), (1.0, 0.5)):
+        loss = policy_loss(z, tokens, adv, old, mask=mask, reduction="sum", scale=scale).loss
+        grads.append(torch.autograd.grad(loss * factor if factor != 1.0 else loss, z)[0])
+    assert torch.equal(*grads) and bool(grads[0].any())
 
 
 @pytest.mark.gpu
