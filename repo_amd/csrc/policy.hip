@@ -186,9 +186,10 @@ __device__ inline const T* pl_row(const PlRows& a, int64_t r) {
 
 // e^x - 1: x = n ln 2 + r with |r| <= ln 2 / 2, the exponential's series to r^14 / 14! (2^-63 of r),
 // then 2^n (e^r - 1) + (2^n - 1).  Within 2^-50 of it, relative; the library's function keeps
-// 95 registers beside those that hold a row.
+// 95 registers beside those that hold a row.  From 709.79 on e^x is beyond fp64: n is at most 1024,
+// and half of the sum is taken first, whose terms then are finite, so that its double is infinity.
 __device__ inline double pl_expm1(double x) {
-    x = x > 800.0 ? 800.0 : x < -800.0 ? -800.0 : x;   // infinity and -1; NaN stays
+    x = x > 710.0 ? 710.0 : x < -800.0 ? -800.0 : x;   // infinity and -1; NaN stays
     const double n = __builtin_rint(x * 1.4426950408889634074);
     // ln 2 as its first 32 bits, which n of 11 bits multiplies exactly, and the rest.
     constexpr double kHead = 2977044471.0 / 4294967296.0;
@@ -208,8 +209,8 @@ __device__ inline double pl_expm1(double x) {
     p = __builtin_fma(p, r, 1.0 / 6.0);
     p = __builtin_fma(p, r, 0.5);
     p = __builtin_fma(p * r, r, r);
-    const int e = (int)n;
-    return __builtin_ldexp(p, e) + (__builtin_ldexp(1.0, e) - 1.0);
+    const int e = (int)n - 1;
+    return 2.0 * (__builtin_ldexp(p, e) + (__builtin_ldexp(1.0, e) - 0.5));
 }
 
 // log s from the hardware's logarithm y (22 bits): log s = y + log(1 + d), d = s e^-y - 1.
