@@ -296,13 +296,20 @@ LossOut loss_forward(const Rows& a, const LossArgs& f, at::IntArrayRef shape, bo
     return y;
 }
 
+// Loss, log-probabilities, KL estimate and clipped share: tensors of their own, which callers may write
+// in place, and not views of one.
+variable_list results(const LossOut& y) {
+    return {y.out[0].variable_data(), y.logprobs, y.out[1].variable_data(),
+            y.out[2].variable_data()};
+}
+
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens,
                                  const std::optional<Tensor>& mask, double temperature,
                                  const LossArgs* f) {
         const Rows a = Rows::of(logits, tokens, mask, temperature);
         LossOut y = loss_forward(a, *f, logits.sizes(), true);
-        variable_list out{y.out[0], y.logprobs, y.out[1], y.out[2]};
+        variable_list out = results(y);
         ctx->mark_non_differentiable({out[1], out[2], out[3]});
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({a.z, a.tokens, a.mask, y.stats, y.slopes});
@@ -401,8 +408,7 @@ PyObject* py_policy_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (wants_node(logits)) {
         out = PolicyLoss::apply(logits, tokens, mask, temperature, &f);
     } else {
-        LossOut y = loss_forward(Rows::of(logits, tokens, mask, temperature), f, {}, false);
-        out = {y.out[0], y.logprobs, y.out[1], y.out[2]};
+        out = results(loss_forward(Rows::of(logits, tokens, mask, temperature), f, {}, false));
     }
     PyObject* tuple = PyTuple_New(4);
     if (!tuple) return nullptr;

@@ -135,7 +135,8 @@ class _PolicyLoss(torch.autograd.Function):
                    advantages.stride(0), advantages.stride(1), old.data_ptr(), N.ptr(ref),
                    *numbers, work.data_ptr(), stats.data_ptr(), slopes.data_ptr(), lp.data_ptr(),
                    out.data_ptr(), N.ptr(grad), N.stream(dev))
-        loss, kl, clipped = out.unbind()
+        # Tensors of their own, which callers may write in place, and not views of one.
+        loss, kl, clipped = (t.data for t in out.unbind())
         ctx.mark_non_differentiable(lp, kl, clipped)
         if need:
             ctx.save_for_backward(z, tokens, mask, stats, slopes)
@@ -235,8 +236,8 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Te
                          f"{tuple(advantages.shape)}")
     N.require_gpu(logits, "logits")
     if tokens.numel() == 0:
-        zero = torch.zeros((), dtype=torch.float32, device=logits.device)
-        return PolicyLoss(logits.sum(dtype=torch.float32), zero.expand(shape), zero, zero)
+        return PolicyLoss(logits.sum(dtype=torch.float32), *(
+            torch.zeros(s, dtype=torch.float32, device=logits.device) for s in (shape, (), ())))
     if logits.device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(logits.device):
             return policy_loss(logits, tokens, advantages, old_logprobs,

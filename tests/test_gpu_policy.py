@@ -640,3 +640,39 @@ def test_ratios_and_kl_terms_beyond_fp64(vocab):
         e = float(_lp_bound(args[0], _np(lp[one]), 1.0).max())
         # The reference's value is rounded to fp32 too, and so is the term.
         assert abs(float(below) - (d - 1.0)) <= 2 * e + 2 * U * (d + 20.0) + U * d, d
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extension", [True, False])
+def test_results_can_be_written_in_place(extension, monkeypatch):
+    """As a training loop does (loss += other, loss /= n): each result is a tensor of its own."""
+    from repo_amd import policy
+    if not extension:
+        monkeypatch.setattr(policy, "_extension", lambda: None)
+    z, tokens, mask, adv, old, ref = _policy_inputs((4, 6), 131, torch.bfloat16, seed=32)
+
+    def make(x):
+        return policy.policy_loss(x, tokens, adv, old, ref_logprobs=ref, mask=mask, kl_weight=0.1)
+    leaf = z.detach().requires_grad_()
+    plain = make(leaf)
+    want, = torch.autograd.grad(plain.loss * 0.5, leaf)
+    got = make(leaf)
+    loss = got.loss
+    loss += 1.0
+    loss *= 0.5
+    assert torch.equal(loss, (plain.loss + 1.0) * 0.5)
+    for name in ("logprobs", "kl", "clipped"):
+        assert torch.equal(getattr(got, name), getattr(plain, name))
+        getattr(got, name).fill_(7.0)
+    assert torch.equal(loss, (plain.loss + 1.0) * 0.5)
+    loss.backward()
+    assert torch.equal(leaf.grad, want)
+    for x in (z, leaf, torch.zeros(0, 3, 5, device="cuda")):   # without gradients and without tokens too
+        args = () if x.dim() == 3 and len(x) else (torch.zeros(0, 3),) * 2
+        got = make(x) if args == () else policy.policy_loss(
+            x, torch.zeros(0, 3, dtype=torch.int64, device="cuda"), *(a.cuda() for a in args))
+        before = [t.detach().clone() for t in got]
+        got.kl.add_(3.0)
+        assert torch.equal(got.clipped, before[3]) and torch.equal(got.loss.detach(), before[0])
+        got.clipped.add_(3.0)
+        assert torch.equal(got.kl, before[2] + 3.0)
