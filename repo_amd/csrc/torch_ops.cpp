@@ -54,6 +54,17 @@ Tensor workspace(const Tensor& x, const Sizes& z, int64_t groups, int backward) 
 
 hipStream_t stream(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.device().index()); }
 
+// The capture that x's current stream belongs to, 0 for none, -1 where it cannot be told.
+int64_t capture_of(const Tensor& x) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(stream(x), &status, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        return -1;
+    }
+    return status == hipStreamCaptureStatusNone ? 0 : (int64_t)id;
+}
+
 // t if its channels lie together without gaps, else a copy that does.
 Tensor channels_last(const Tensor& t) {
     const Tensor last = t.movedim(1, -1);
@@ -316,20 +327,24 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         ctx->saved_data["temperature"] = temperature;
         ctx->saved_data["shape"] = logits.sizes().vec();
         ctx->saved_data["grad"] = y.grad;
+        ctx->saved_data["capture"] = capture_of(a.z);
         return out;
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         // The gradient for an incoming one is there; another one's is computed from the
         // logits, not from that one's rounded values.  A second backward pass finds it given
-        // away.
+        // away.  Of a loss that is in another graph than this pass, or of which one is in none, it
+        // is left: replays of one without the other would find what the last has made of it.
         const variable_list saved = ctx->get_saved_variables();
         const Rows a(saved[0], saved[1], saved[2], ctx->saved_data["temperature"].toDouble());
         Tensor grad;
         auto held = ctx->saved_data.find("grad");
         if (held != ctx->saved_data.end()) {
-            grad = held->second.toTensor();
-            ctx->saved_data.erase(held);
+            const int64_t capture = capture_of(a.z);
+            if (capture >= 0 && capture == ctx->saved_data["capture"].toInt())
+                grad = held->second.toTensor();
+            ctx->saved_data.erase("grad");
         }
         if (!grads[0].defined()) return variable_list(5);
         {

@@ -123,7 +123,10 @@ class _PolicyLoss(torch.autograd.Function):
         dev = z.device
         advantages = advantages.detach().float().expand(tokens.shape).reshape(batch, length)
         old, ref = _plain(old, torch.float32), None if ref is None else _plain(ref, torch.float32)
-        grad = torch.empty(logits.shape, dtype=z.dtype, device=dev) if need else None
+        # A loss in a graph leaves its gradient to the backward pass, which may be in none or
+        # in another one: replays of one without the other would find what the last has made of it.
+        hold = need and not torch._C._cuda_isCurrentStreamCapturing()
+        grad = torch.empty(logits.shape, dtype=z.dtype, device=dev) if hold else None
         lp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
         slopes = torch.empty((batch, length), dtype=torch.float32, device=dev)
         stats = torch.empty((batch, length, 2), dtype=torch.float32, device=dev)
@@ -147,9 +150,12 @@ class _PolicyLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, upstream, *_):
         # The gradient for an incoming one is there; another one's is computed from the
-        # logits, not from that one's rounded values.  A second backward pass finds it given away.
+        # logits, not from that one's rounded values.  A second backward pass finds it given away,
+        # and one in a graph leaves it.
         z, tokens, mask, stats, slopes = ctx.saved_tensors
         into, ctx.grad = ctx.grad, None
+        if torch._C._cuda_isCurrentStreamCapturing():
+            into = None
         factor = upstream.to(torch.float32).contiguous()
         return (_gradient(z, tokens, mask, ctx.temperature, stats, slopes, ctx.shape, factor,
                           into), *(None,) * 12)
