@@ -13,6 +13,7 @@ from contextlib import nullcontext
 from typing import Callable, ContextManager, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcubicsplat_hip.so")
@@ -356,6 +357,11 @@ def prof(label: str):
     if _PROFILE_CTX_FACTORY is None:
         return nullcontext()
     return _PROFILE_CTX_FACTORY(label)
+
+
+def has_tangent(t: torch.Tensor) -> bool:
+    """Whether t carries a tangent of forward-mode differentiation."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
 def require_gpu(t: torch.Tensor, name: str) -> None:

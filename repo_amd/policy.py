@@ -227,7 +227,7 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Te
             continue
         if t.dtype not in _DTYPES:
             raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-        if t.requires_grad and torch.is_grad_enabled():
+        if (t.requires_grad and torch.is_grad_enabled()) or N.has_tangent(t):
             raise ValueError(f"policy_loss has no gradient for {name}: detach it")
         if name != "advantages":
             _beside(t, name, logits)

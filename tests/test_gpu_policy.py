@@ -747,3 +747,23 @@ def test_an_eager_gradient_of_a_captured_loss_is_its_own(extension, monkeypatch)
             assert torch.equal(a, b)
         side.synchronize()
     torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extension", [True, False])
+def test_tangents_of_the_constants_are_refused(extension, monkeypatch):
+    """A loss without a tangent would be a derivative of zero."""
+    from repo_amd import policy
+    from torch.autograd import forward_ad
+    if not extension:
+        monkeypatch.setattr(policy, "_extension", lambda: None)
+    z, tokens, _, adv, old, ref = _policy_inputs((2, 3), 64, torch.float32, seed=34)
+    for which in ("advantages", "old_logprobs", "ref_logprobs"):
+        for leaf in (z, z.detach().requires_grad_()):
+            with forward_ad.dual_level():
+                c = dict(advantages=adv, old_logprobs=old, ref_logprobs=ref)
+                c[which] = forward_ad.make_dual(c[which], torch.ones_like(c[which]))
+                with pytest.raises(ValueError, match=f"no gradient for {which}: detach it"):
+                    policy.policy_loss(leaf, tokens, **c)
+                c[which] = c[which].detach()
+                assert torch.isfinite(policy.policy_loss(leaf, tokens, **c).loss)
