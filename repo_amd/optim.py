@@ -1212,13 +1212,13 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=_NS_COEFFICIENTS
     x: fp32, bf16 or fp16 on the GPU; of a stack each matrix is scaled by its own norm.  The
     result has x's type and shape.  Products are as exact as fp32's, whatever the type (of a norm far
     below eps the result is exact to 1e-9, not to its own size), and sums are taken in a fixed
-    order.  Not differentiable: an x that requires a gradient is refused."""
+    order.  Not differentiable: an x that requires a gradient or has a tangent is refused."""
     steps, a, b, c = _check_newton_schulz(steps, coefficients, eps)
     if x.dim() < 2:
         raise ValueError(f"expected [..., m, n], got {tuple(x.shape)}")
     if x.dtype not in _ADAMW_DTYPES:
         raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    if x.requires_grad and torch.is_grad_enabled():
+    if (x.requires_grad and torch.is_grad_enabled()) or N.has_tangent(x):
         raise ValueError("orthogonalize has no gradient: detach x")
     m, n = x.shape[-2:]
     patches = _padded(m) * _padded(n)

@@ -7,6 +7,7 @@ import copy
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from repo_amd import _native as N
 from repo_amd.optim import Muon, orthogonalize
@@ -145,3 +146,14 @@ def test_entries_check_their_tables():
     assert 0 < one < two
     t = np.array([[4096, 4096, 5, 0, 64, 576, 0, 0]], dtype=np.int64)
     assert lib.cs_orthogonalize_workspace_bytes(1, t.ctypes.data, 5, *coeffs) == 0
+
+
+def test_orthogonalize_refuses_tangents():
+    """A result without a tangent would be a derivative of zero."""
+    for grad in (True, False):
+        with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+            x = forward_ad.make_dual(torch.zeros(3, 3), torch.ones(3, 3))
+            with pytest.raises(ValueError, match="no gradient"):
+                orthogonalize(x)
+            with pytest.raises(ValueError, match="x must be a CUDA"):
+                orthogonalize(x.detach())
