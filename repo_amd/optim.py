@@ -627,9 +627,9 @@ class _AdamWBulk:
         return None
 
 
-def _check_grad(g, p):
+def _check_grad(g, p, name="AdamW"):
     if g.layout is not torch.strided:
-        raise RuntimeError("AdamW does not support sparse gradients")
+        raise RuntimeError(f"{name} does not support sparse gradients")
     if g.dtype is not p.dtype or g.device != p.device or g.shape != p.shape:
         raise ValueError(f"a gradient of {g.dtype} {tuple(g.shape)} on {g.device} beside a "
                          f"parameter of {p.dtype} {tuple(p.shape)} on {p.device}")
@@ -1347,7 +1347,7 @@ class Muon(torch.optim.Optimizer):
                 if g is None:
                     continue
                 shape = self._check_param(p)
-                _check_grad(g, p)
+                _check_grad(g, p, "Muon")
                 if not (_is_dense(g) and _same_layout(g, p)):
                     g = torch.empty_like(p).copy_(g.detach())
                 st = self._ready(p)

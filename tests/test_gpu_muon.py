@@ -484,3 +484,14 @@ def test_profile_labels():
     finally:
         N.set_profile_ctx_factory(None)
     assert seen == ["optim.orthogonalize", "optim.muon"]
+
+
+@pytest.mark.gpu
+def test_sparse_gradients_are_refused_by_name():
+    from repo_amd.optim import Muon
+    p = torch.nn.Parameter(torch.ones(4, 3, device="cuda"))
+    opt = Muon([p])
+    p.grad = torch.ones(4, 3, device="cuda").to_sparse()
+    with pytest.raises(RuntimeError, match="Muon does not support sparse gradients"):
+        opt.step()
+    assert torch.equal(p.detach(), torch.ones(4, 3, device="cuda"))
