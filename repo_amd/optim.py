@@ -1307,6 +1307,8 @@ class Muon(torch.optim.Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self._written = {}
+        for p in self.state:
+            self._wrote(p)   # a copy tells writes to p from here on
 
     zero_grad = Adam.zero_grad
 

@@ -495,3 +495,24 @@ def test_sparse_gradients_are_refused_by_name():
     with pytest.raises(RuntimeError, match="Muon does not support sparse gradients"):
         opt.step()
     assert torch.equal(p.detach(), torch.ones(4, 3, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_copies_notice_writes_before_their_first_step():
+    import copy
+    import pickle
+    from repo_amd.optim import Muon
+    params = _params([(20, 30), (30, 20)], torch.bfloat16)
+    opt = Muon(params, lr=0.0)
+    _grads(params, 3)
+    opt.step()
+    for copied in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        p, q = copied.param_groups[0]["params"]
+        with torch.no_grad():
+            p.add_(1.0)
+        want, kept = p.detach().clone(), copied.state[q]["master"].clone()
+        _grads([p, q], 4)
+        copied.param_groups[0]["weight_decay"] = 0.0
+        copied.step()
+        assert torch.equal(p, want) and torch.equal(copied.state[p]["master"], want.float())
+        assert torch.equal(copied.state[q]["master"], kept)
