@@ -772,8 +772,8 @@ int cs_group_norm_backward(const void* x, const void* dy, int64_t n, int64_t s, 
  *   [4] rows  [5] columns  [6] type (0 fp32, 1 bf16, 2 fp16)
  * steps 1 to 64; |a|, |b|, |c| at most 64, and such that no singular value in [0, 1] passes 64 on
  * its way.  workspace: cs_orthogonalize_workspace_bytes bytes (-1: invalid arguments; 0 where all
- * matrices are small), 128-byte aligned, of which nothing is kept between calls.  count times the 64 x 64 patches of a matrix
- * padded to whole tiles of 256 is at most CS_MUON_MAX_PATCHES. */
+ * matrices are small), 128-byte aligned, of which nothing is kept between calls.  count times the
+ * 64 x 64 patches of a matrix padded to whole tiles of 256 is at most CS_MUON_MAX_PATCHES. */
 #define CS_MUON_MAX_PATCHES 262144
 int64_t cs_orthogonalize_workspace_bytes(int32_t ntensors, const int64_t* table, int32_t steps,
                                          double a, double b, double c);

@@ -20,10 +20,11 @@
 // Bound: HBM, the logits read once and the gradient written once.  The loss makes the
 // gradient for an incoming one while the row is in registers (a second launch in the
 // backward pass finds that one and ends, or makes another's from the logits): a wave holds
-// rows up to 8 KB, a workgroup up to 64 KB.  Longer rows are read twice, those above 160 KB by
-// workgroups of 1024 threads, so that the rows in flight stay in the memory-side cache (8192 of 256
-// KB: 1008 us of 256 threads for 890).  Measured: 16x512x32768 bf16, 0.7 of the rows counting, loss
-// and gradient 194 us (913 MB at 4.7 TB/s), 8x1024x131072 914 to 949 us (3.65 GB, 3.9 TB/s); scoring
+// rows up to 8 KB, a workgroup up to 32 KB, and of 512 threads those of 47 to 64 KB.  Rows of 32 to
+// 47 KB and above 64 KB are read twice, for the loss those above 160 KB by workgroups of 1024 threads,
+// so that the rows in flight stay in the memory-side cache (8192 of 256 KB: 1008 us of 256 threads for
+// 890).  Measured: 16x512x32768 bf16, 0.7 of the rows counting, loss
+// and gradient 194 us (913 MB at 4.7 TB/s), 8x1024x131072 914 to 966 us (3.65 GB, 3.9 TB/s); scoring
 // 16x511x32768 68 us (375 MB, 5.6 TB/s).  Writing past the caches was slower (by 16 and 36 us).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -381,7 +382,8 @@ __device__ inline PlSlope pl_row_done(const PlRows& a, const PlLoss& f, const Pl
 // Rows of any length: an online sum, two vectors ahead; with LOSS the gradient from a second
 // reading.
 template <typename T, int THREADS, bool LOSS>
-__global__ __launch_bounds__(PlTeam<THREADS>::kBlock, THREADS == 1024 ? 8 : 4) void k_rows(PlRows a, PlLoss f, PlOut o) {
+__global__ __launch_bounds__(PlTeam<THREADS>::kBlock, THREADS == 1024 ? 8 : 4) void k_rows(
+    PlRows a, PlLoss f, PlOut o) {
     constexpr int V = PlVec<T>::n, U = 2;
     __shared__ typename PlTeam<THREADS>::Lds lds;
     const PlTeam<THREADS> team{&lds};

@@ -1,8 +1,9 @@
 // `_cs_torch`, a CPython extension on torch's C++ tensors, for what costs the host
 // most in Python: the autograd nodes of group norm, tokens' log-probabilities and the
 // policy loss (their backward then runs in the engine's thread without the
-// interpreter), and the checks that an AdamW step makes of every parameter and gradient.  The kernels are reached through the C
-// ABI of libcubicsplat_hip.so, as everywhere.
+// interpreter), and the checks that an AdamW step makes of every parameter and
+// gradient.  The kernels are reached through the C ABI of libcubicsplat_hip.so, as
+// everywhere.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>

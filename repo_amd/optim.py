@@ -1280,7 +1280,8 @@ class Muon(torch.optim.Optimizer):
     such deletes ``state[p]["master"]``).
 
     Up to 20 parameters share each launch.  A step can be captured in a graph, with the numbers of its
-    groups as they are then, once an eager step has made the states."""
+    groups as they are then, once an eager step has made the states.  Replays look at no counters:
+    whoever writes a 16-bit parameter between them writes its master too."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
                  ns_coefficients=_NS_COEFFICIENTS, eps=1e-7, ns_steps=5, adjust_lr_fn=None):
